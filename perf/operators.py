@@ -73,7 +73,7 @@ def _pitch(frames):
 
 
 def _words(frames):
-    p = (frames + 511) // 512 * 16
+    p = (frames + 2047) // 2048 * 64
     return p + 96 if p % 512 == 0 else p
 
 

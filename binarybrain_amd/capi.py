@@ -106,6 +106,16 @@ _SIGNATURES = {
     "bbhip_Shuffle_Forward": (C.c_int, [_vp, _vp] + [_u] * 4 + [_vp]),
     "bbhip_Shuffle_Backward": (C.c_int, [_vp, _vp] + [_u] * 4 + [_vp]),
     "bbhip_fp32_ConvBitToReal": (C.c_int, [_vp, _vp, _f, _f, _i, _i, _i, _i, _vp]),
+    "bbhip_LayerNormalization_WorkspaceBytes": (C.c_size_t, [_i, _i]),
+    "bbhip_fp32_LayerNormalization_Forward": (C.c_int, [_vp] * 6 + [_f] + [_i] * 4 + [_vp, C.c_size_t, _vp]),
+    "bbhip_bit_fp32_LayerNormalization_Forward": (C.c_int, [_vp] * 6 + [_f] + [_i] * 4 + [_vp, C.c_size_t, _vp]),
+    "bbhip_fp32_LayerNormalization_Backward": (C.c_int, [_vp] * 8 + [_i] * 5 + [_vp, C.c_size_t, _vp]),
+    "bbhip_bit_fp32_LayerNormalization_Backward": (C.c_int, [_vp] * 8 + [_i] * 5 + [_vp, C.c_size_t, _vp]),
+    "bbhip_TopLogits_WorkspaceBytes": (C.c_size_t, [_i] * 4),
+    "bbhip_fp32_TopLogits": (C.c_int, [_vp, _vp, _vp] + [_i] * 6 + [_vp, C.c_size_t, _vp]),
+    "bbhip_LossDistillation_WorkspaceBytes": (C.c_size_t, [_i] * 3),
+    "bbhip_fp32_LossDistillation": (C.c_int, [_vp] * 6 + [_f, _f] + [_i] * 6 + [_vp, C.c_size_t, _vp]),
+    "bbhip_fp32_CategoricalSampling": (C.c_int, [_vp] * 4 + [_f, _i, _f, _f] + [_i] * 4 + [_vp, C.c_size_t, _vp]),
     "bbhip_fp32_StochasticLut_Forward": (C.c_int, [_i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _f, _vp]),
     "bbhip_fp32_StochasticLut_Forward_NoAlloc": (C.c_int, [_i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _f, _vp]),
     "bbhip_fp32_StochasticLut_ForwardClampW": (C.c_int, [_i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _f, _f, _f, _vp]),

@@ -29,6 +29,9 @@
 #include "bn_kernels.hpp"
 #include "modulation_kernels.hpp"
 #include "pooling_kernels.hpp"
+#include "layer_norm_kernels.hpp"
+#include "distillation_kernels.hpp"
+#include "top_logits_kernels.hpp"
 
 using namespace bbhip;
 
@@ -2404,6 +2407,310 @@ int bbhip_fp32_StochasticBatchNormalization_Backward(float const *dev_x_buf, flo
     a.gamma = gamma; a.reciprocal_frame_size = reciprocal_frame_size;
     a.frame_size = frame_size; a.x_stride = x_frame_stride; a.out_stride = frame_stride;
     return launch_bn_rows(a, node_size, true, stream);
+}
+
+// ---- operators down the columns: LayerNormalization, LossDistillation, TopLogits, CategoricalSampling ----
+// How a call divides `pix_size * frame_size` columns of `rows` rows among workgroups.  `wide`: units of four frames.  `batch`: rows that a thread reads at a time.
+static int column_space(ColumnSpace &c, TileDivisor &tiles, bool wide, int pix_size, int frame_size, int rows, int batch, char const *name)
+{
+    int const per_row = ceil_div(frame_size, wide ? 4 : 1);
+    if ((long long)pix_size * per_row > (1 << 28)) { return fail("%s: too many frames", name); }
+    c.units_per_row = make_tile_divisor(per_row);
+    c.units = pix_size * per_row;
+    c.frame_size = frame_size;
+    c.rows = rows;
+    column_split(c.units, rows, wide, batch, c.log_tx, c.tiles, c.slab_rows, c.slabs);
+    if ((long long)c.tiles * c.slabs > 0x3fffffffLL) { return fail("%s: grid too large", name); }
+    tiles = make_tile_divisor(c.tiles);
+    return 0;
+}
+
+// an entry's workspace, as its ...WorkspaceBytes counts it
+static int check_workspace(void const *workspace, size_t size, size_t needed, char const *name)
+{
+    if (size < needed || (needed > 0 && workspace == nullptr)) { return fail("%s: a workspace of %zu bytes is needed, %zu given", name, needed, workspace ? size : (size_t)0); }
+    if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0)  { return fail("%s: the workspace must be aligned to 256 bytes", name); }
+    return 0;
+}
+
+static bool starts_on_16_bytes(void const *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+static size_t layer_norm_partial_bytes(ColumnSpace const &c, bool wide) { return align256((size_t)c.slabs * c.units * (wide ? 4 : 1) * sizeof(float2)); }
+
+size_t bbhip_LayerNormalization_WorkspaceBytes(int node_size, int frame_size)
+{
+    if (node_size <= 0 || frame_size <= 0) { return 0; }
+    size_t most = 0;
+    for (int form = 0; form < 4; ++form) {
+        bool const wide = (form & 1) != 0, backward = (form & 2) != 0;
+        ColumnSpace c;
+        TileDivisor tiles;
+        if (column_space(c, tiles, wide, 1, frame_size, node_size, backward ? kLayerNormBatch / 2 : kLayerNormBatch, __func__)) { return 0; }
+        size_t const bytes = layer_norm_partial_bytes(c, wide) + (backward ? (size_t)c.tiles * node_size * sizeof(float2) : 0);
+        most = bytes > most ? bytes : most;
+    }
+    return align256(most);
+}
+
+static int layer_norm_forward(void const *x, bool bit, float *y, float const *gamma, float const *beta, float *mean, float *rstd, float eps, int node_size,
+                              int frame_size, int x_stride, int y_stride, void *workspace, size_t workspace_size, void *stream, char const *name)
+{
+    if (!(x && y)) { return fail("%s: null buffer", name); }
+    if (!(node_size > 0 && frame_size > 0)) { return fail("%s: sizes must be positive", name); }
+    if ((bit ? (long long)x_stride * 32 : x_stride) < frame_size || y_stride < frame_size) { return fail("%s: frame stride shorter than the frames", name); }
+    if (!(eps >= 0.0f)) { return fail("%s: eps must not be negative", name); }
+    bool const wide = frame_size >= 4 && starts_on_16_bytes(y) && y_stride % 4 == 0 && (bit || (starts_on_16_bytes(x) && x_stride % 4 == 0)) &&
+                      starts_on_16_bytes(mean) && starts_on_16_bytes(rstd);
+    LayerNormArgs a{};
+    if (column_space(a.c, a.tiles, wide, 1, frame_size, node_size, kLayerNormBatch, name)) { return 1; }
+    if (check_workspace(workspace, workspace_size, layer_norm_partial_bytes(a.c, wide), name)) { return 1; }
+    a.x = x; a.out = y; a.gamma = gamma; a.beta = beta; a.mean = mean; a.rstd = rstd; a.eps = eps;
+    a.partial = static_cast<float2 *>(workspace);
+    a.x_stride = x_stride; a.out_stride = y_stride;
+    hipStream_t const st = static_cast<hipStream_t>(stream);
+    ScopedTimer tm(kTimeOther, st);
+    dim3 const grid((unsigned)(a.c.tiles * a.c.slabs)), block(kColBlock);
+#define BBHIP_LAYER_NORM(W, BIT)                                                                        \
+    do {                                                                                                \
+        launch((layer_norm_stats_kernel<W, BIT>), grid, block, 0, st, a);                               \
+        launch((layer_norm_apply_kernel<W, BIT>), grid, block, 0, st, a);                               \
+    } while (0)
+    if (wide) { if (bit) { BBHIP_LAYER_NORM(4, true); } else { BBHIP_LAYER_NORM(4, false); } }
+    else      { if (bit) { BBHIP_LAYER_NORM(1, true); } else { BBHIP_LAYER_NORM(1, false); } }
+#undef BBHIP_LAYER_NORM
+    BBHIP_LAUNCH_CHECK();
+    return 0;
+}
+
+int bbhip_fp32_LayerNormalization_Forward(float const *dev_x_buf, float *dev_y_buf, float const *dev_gamma, float const *dev_beta, float *dev_mean_buf,
+                                          float *dev_rstd_buf, float eps, int node_size, int frame_size, int x_frame_stride, int y_frame_stride,
+                                          void *dev_workspace, size_t workspace_size, void *stream)
+{
+    clear_hints();
+    return layer_norm_forward(dev_x_buf, false, dev_y_buf, dev_gamma, dev_beta, dev_mean_buf, dev_rstd_buf, eps, node_size, frame_size, x_frame_stride,
+                              y_frame_stride, dev_workspace, workspace_size, stream, __func__);
+}
+
+int bbhip_bit_fp32_LayerNormalization_Forward(int const *dev_x_buf, float *dev_y_buf, float const *dev_gamma, float const *dev_beta, float *dev_mean_buf,
+                                              float *dev_rstd_buf, float eps, int node_size, int frame_size, int x_frame_stride, int y_frame_stride,
+                                              void *dev_workspace, size_t workspace_size, void *stream)
+{
+    clear_hints();
+    return layer_norm_forward(dev_x_buf, true, dev_y_buf, dev_gamma, dev_beta, dev_mean_buf, dev_rstd_buf, eps, node_size, frame_size, x_frame_stride,
+                              y_frame_stride, dev_workspace, workspace_size, stream, __func__);
+}
+
+static int layer_norm_backward(void const *x, bool bit, float const *dy, float *dx, float const *gamma, float const *mean, float const *rstd, float *dgamma,
+                               float *dbeta, int accumulate, int node_size, int frame_size, int x_stride, int stride, void *workspace, size_t workspace_size,
+                               void *stream, char const *name)
+{
+    if (!(x && dy && dx && mean && rstd)) { return fail("%s: null buffer", name); }
+    if (!(node_size > 0 && frame_size > 0)) { return fail("%s: sizes must be positive", name); }
+    if ((bit ? (long long)x_stride * 32 : x_stride) < frame_size || stride < frame_size) { return fail("%s: frame stride shorter than the frames", name); }
+    bool const wide = frame_size >= 4 && starts_on_16_bytes(dy) && starts_on_16_bytes(dx) && stride % 4 == 0 &&
+                      (bit || (starts_on_16_bytes(x) && x_stride % 4 == 0)) && starts_on_16_bytes(mean) && starts_on_16_bytes(rstd);
+    LayerNormArgs a{};
+    if (column_space(a.c, a.tiles, wide, 1, frame_size, node_size, kLayerNormBatch / 2, name)) { return 1; }
+    bool const weights = dgamma != nullptr || dbeta != nullptr;
+    size_t const partial = layer_norm_partial_bytes(a.c, wide);
+    if (check_workspace(workspace, workspace_size, partial + (weights ? (size_t)a.c.tiles * node_size * sizeof(float2) : 0), name)) { return 1; }
+    a.x = x; a.dy = dy; a.out = dx; a.gamma = gamma; a.mean = const_cast<float *>(mean); a.rstd = const_cast<float *>(rstd);
+    a.dgamma = dgamma; a.dbeta = dbeta; a.accumulate = accumulate; a.reciprocal_rows = 1.0f / (float)node_size;
+    a.partial = static_cast<float2 *>(workspace);
+    a.row_partial = weights ? reinterpret_cast<float2 *>(static_cast<char *>(workspace) + partial) : nullptr;
+    a.x_stride = x_stride; a.out_stride = stride;
+    a.main_blocks = a.c.tiles * a.c.slabs;
+    hipStream_t const st = static_cast<hipStream_t>(stream);
+    ScopedTimer tm(kTimeOther, st);
+    dim3 const grid((unsigned)a.main_blocks), apply((unsigned)(a.main_blocks + (weights ? ceil_div(node_size, kWave) : 0))), block(kColBlock);
+#define BBHIP_LAYER_NORM(W, BIT)                                                                        \
+    do {                                                                                                \
+        launch((layer_norm_backward_sums_kernel<W, BIT>), grid, block, 0, st, a);                       \
+        launch((layer_norm_backward_apply_kernel<W, BIT>), apply, block, 0, st, a);                     \
+    } while (0)
+    if (wide) { if (bit) { BBHIP_LAYER_NORM(4, true); } else { BBHIP_LAYER_NORM(4, false); } }
+    else      { if (bit) { BBHIP_LAYER_NORM(1, true); } else { BBHIP_LAYER_NORM(1, false); } }
+#undef BBHIP_LAYER_NORM
+    BBHIP_LAUNCH_CHECK();
+    return 0;
+}
+
+int bbhip_fp32_LayerNormalization_Backward(float const *dev_x_buf, float const *dev_dy_buf, float *dev_dx_buf, float const *dev_gamma, float const *dev_mean_buf,
+                                           float const *dev_rstd_buf, float *dev_dgamma, float *dev_dbeta, int accumulate, int node_size, int frame_size,
+                                           int x_frame_stride, int frame_stride, void *dev_workspace, size_t workspace_size, void *stream)
+{
+    clear_hints();
+    return layer_norm_backward(dev_x_buf, false, dev_dy_buf, dev_dx_buf, dev_gamma, dev_mean_buf, dev_rstd_buf, dev_dgamma, dev_dbeta, accumulate, node_size,
+                               frame_size, x_frame_stride, frame_stride, dev_workspace, workspace_size, stream, __func__);
+}
+
+int bbhip_bit_fp32_LayerNormalization_Backward(int const *dev_x_buf, float const *dev_dy_buf, float *dev_dx_buf, float const *dev_gamma, float const *dev_mean_buf,
+                                               float const *dev_rstd_buf, float *dev_dgamma, float *dev_dbeta, int accumulate, int node_size, int frame_size,
+                                               int x_frame_stride, int frame_stride, void *dev_workspace, size_t workspace_size, void *stream)
+{
+    clear_hints();
+    return layer_norm_backward(dev_x_buf, true, dev_dy_buf, dev_dx_buf, dev_gamma, dev_mean_buf, dev_rstd_buf, dev_dgamma, dev_dbeta, accumulate, node_size,
+                               frame_size, x_frame_stride, frame_stride, dev_workspace, workspace_size, stream, __func__);
+}
+
+// what the operators on logits ask of their sizes
+static int check_logits(int top_size, int pix_size, int ch_size, int frame_size, int frame_stride, int list_stride, char const *name)
+{
+    if (!(top_size > 0 && pix_size > 0 && ch_size > 0 && frame_size > 0)) { return fail("%s: sizes must be positive", name); }
+    if (frame_stride < frame_size || list_stride < frame_size) { return fail("%s: frame stride shorter than the frames", name); }
+    if (top_size > kTopMost) { return fail("%s: top_size=%d: at most %d", name, top_size, kTopMost); }
+    if ((long long)pix_size * ch_size > 0x7fffffffLL || (long long)pix_size * frame_size > 0x3fffffffLL) { return fail("%s: node count too large", name); }
+    return 0;
+}
+
+// ---- LossDistillation ----
+static size_t distillation_partial_bytes(ColumnSpace const &c, bool wide) { return align256((size_t)c.slabs * c.units * (wide ? 4 : 1) * sizeof(float2)); }
+
+size_t bbhip_LossDistillation_WorkspaceBytes(int pix_size, int ch_size, int frame_size)
+{
+    if (pix_size <= 0 || ch_size <= 0 || frame_size <= 0) { return 0; }
+    size_t most = 0;
+    for (int wide = 0; wide < 2; ++wide) {
+        ColumnSpace c;
+        TileDivisor tiles;
+        if (column_space(c, tiles, wide != 0, pix_size, frame_size, ch_size, 8, __func__)) { return 0; }
+        size_t const bytes = distillation_partial_bytes(c, wide != 0) + (size_t)c.units * (wide ? 4 : 1) * sizeof(float4);
+        most = bytes > most ? bytes : most;
+    }
+    return align256(most);
+}
+
+int bbhip_fp32_LossDistillation(float const *dev_y_buf, int const *dev_index_buf, float const *dev_logit_buf, float const *dev_weight_buf, float *dev_dy_buf,
+                                float *dev_loss_buf, float temperature, float weight_sum, int top_size, int pix_size, int ch_size, int frame_size,
+                                int frame_stride, int list_frame_stride, void *dev_workspace, size_t workspace_size, void *stream)
+{
+    clear_hints();
+    if (!(dev_y_buf && dev_index_buf && dev_logit_buf && dev_dy_buf && dev_loss_buf)) { return fail("%s: null buffer", __func__); }
+    if (check_logits(top_size, pix_size, ch_size, frame_size, frame_stride, list_frame_stride, __func__)) { return 1; }
+    if (!(temperature > 0.0f && temperature < __builtin_inff())) { return fail("%s: the temperature must be positive", __func__); }
+    bool const wide = frame_size >= 4 && frame_stride % 4 == 0 && starts_on_16_bytes(dev_y_buf) && starts_on_16_bytes(dev_dy_buf) && starts_on_16_bytes(dev_loss_buf);
+    DistillArgs a{};
+    if (column_space(a.c, a.tiles, wide, pix_size, frame_size, ch_size, 8, __func__)) { return 1; }
+    size_t const partial = distillation_partial_bytes(a.c, wide);
+    if (check_workspace(dev_workspace, workspace_size, partial + (size_t)a.c.units * (wide ? 4 : 1) * sizeof(float4), __func__)) { return 1; }
+    a.frames = make_tile_divisor(frame_size);
+    a.y = dev_y_buf; a.index = dev_index_buf; a.logit = dev_logit_buf; a.weight = dev_weight_buf; a.dy = dev_dy_buf; a.loss = dev_loss_buf;
+    a.partial = static_cast<float2 *>(dev_workspace);
+    a.lists   = reinterpret_cast<float4 *>(static_cast<char *>(dev_workspace) + partial);
+    a.scale = (float)(1.4426950408889634 / (double)temperature);
+    a.reciprocal_t = (float)(1.0 / (double)temperature);
+    a.t_square = (float)((double)temperature * (double)temperature);
+    a.coefficient = (float)((double)temperature / (double)weight_sum);
+    a.top_size = top_size; a.pix_size = pix_size; a.frame_stride = frame_stride; a.list_stride = list_frame_stride;
+    a.main_blocks = a.c.tiles * a.c.slabs; a.unit_width = wide ? 4 : 1;
+    hipStream_t const st = static_cast<hipStream_t>(stream);
+    ScopedTimer tm(kTimeOther, st);
+    dim3 const grid((unsigned)a.main_blocks), sums((unsigned)(a.main_blocks + ceil_div(pix_size * frame_size, kListColumns))), block(kColBlock);
+    if (wide) {
+        launch((distillation_sums_kernel<4>), sums, block, 0, st, a);
+        launch((distillation_gradient_kernel<4>), grid, block, 0, st, a);
+    }
+    else {
+        launch((distillation_sums_kernel<1>), sums, block, 0, st, a);
+        launch((distillation_gradient_kernel<1>), grid, block, 0, st, a);
+    }
+    BBHIP_LAUNCH_CHECK();
+    return 0;
+}
+
+// ---- TopLogits, CategoricalSampling ----
+// four frames per thread or one, and how many threads side by side
+static int top_space(TopArgs &a, bool wide, int top_size, int pix_size, int ch_size, int frame_size, char const *name)
+{
+    int const per_row = ceil_div(frame_size, wide ? 4 : 1);
+    a.c.units_per_row = make_tile_divisor(per_row);
+    a.c.units = pix_size * per_row;
+    a.c.frame_size = frame_size;
+    a.c.rows = ch_size;
+    top_split(a.c.units, ch_size, top_size, a.c.log_tx, a.c.tiles, a.c.slab_rows, a.c.slabs);
+    if ((long long)a.c.tiles * a.c.slabs > 0x3fffffffLL) { return fail("%s: grid too large", name); }
+    a.tiles = make_tile_divisor(a.c.tiles);
+    return 0;
+}
+
+static size_t top_candidate_bytes(TopArgs const &a, bool wide, int top_size)
+{
+    return a.c.slabs > 1 ? align256((size_t)a.c.slabs * a.c.units * (wide ? 4 : 1) * (size_t)top_size * sizeof(uint2)) : 0;
+}
+
+size_t bbhip_TopLogits_WorkspaceBytes(int top_size, int pix_size, int ch_size, int frame_size)
+{
+    if (check_logits(top_size, pix_size, ch_size, frame_size, frame_size, frame_size, __func__)) { return 0; }
+    size_t most = 0;
+    for (int wide = 0; wide < 2; ++wide) {
+        TopArgs a{};
+        if (top_space(a, wide != 0, top_size, pix_size, ch_size, frame_size, __func__)) { return 0; }
+        size_t const bytes = top_candidate_bytes(a, wide != 0, top_size);
+        most = bytes > most ? bytes : most;
+    }
+    return most;
+}
+
+static int run_top(TopArgs &a, bool draw, int ch_size, int frame_size, void *workspace, size_t workspace_size, void *stream, char const *name)
+{
+    bool const wide = frame_size >= 4 && a.frame_stride % 4 == 0 && starts_on_16_bytes(a.y);
+    if (a.top_size > ch_size) { return fail("%s: top_size=%d of %d channels", name, a.top_size, ch_size); }
+    if (top_space(a, wide, a.top_size, a.pix_size, ch_size, frame_size, name)) { return 1; }
+    if (check_workspace(workspace, workspace_size, top_candidate_bytes(a, wide, a.top_size), name)) { return 1; }
+    a.candidates = static_cast<uint2 *>(workspace);
+    hipStream_t const st = static_cast<hipStream_t>(stream);
+    ScopedTimer tm(kTimeOther, st);
+    dim3 const grid((unsigned)(a.c.tiles * a.c.slabs)), block((unsigned)(kTopChunk << a.c.log_tx));
+    dim3 const join((unsigned)ceil_div(a.c.units * (wide ? 4 : 1), kColWaves)), join_block(kColBlock);
+#define BBHIP_TOP(W, TX)                                                                                \
+    do {                                                                                                \
+        if (draw) { launch((top_logits_scan_kernel<W, TX, true>), grid, block, 0, st, a); }             \
+        else      { launch((top_logits_scan_kernel<W, TX, false>), grid, block, 0, st, a); }            \
+    } while (0)
+    if (wide) { if (a.c.log_tx) { BBHIP_TOP(4, 4); } else { BBHIP_TOP(4, 1); } }
+    else      { if (a.c.log_tx) { BBHIP_TOP(1, 4); } else { BBHIP_TOP(1, 1); } }
+#undef BBHIP_TOP
+    BBHIP_LAUNCH_CHECK();
+    if (a.c.slabs > 1) {
+        if (wide) {
+            if (draw) { launch((top_logits_join_kernel<4, true>), join, join_block, 0, st, a); }
+            else      { launch((top_logits_join_kernel<4, false>), join, join_block, 0, st, a); }
+        }
+        else {
+            if (draw) { launch((top_logits_join_kernel<1, true>), join, join_block, 0, st, a); }
+            else      { launch((top_logits_join_kernel<1, false>), join, join_block, 0, st, a); }
+        }
+        BBHIP_LAUNCH_CHECK();
+    }
+    return 0;
+}
+
+int bbhip_fp32_TopLogits(float const *dev_y_buf, int *dev_index_buf, float *dev_logit_buf, int top_size, int pix_size, int ch_size, int frame_size,
+                         int frame_stride, int list_frame_stride, void *dev_workspace, size_t workspace_size, void *stream)
+{
+    clear_hints();
+    if (!(dev_y_buf && dev_index_buf && dev_logit_buf)) { return fail("%s: null buffer", __func__); }
+    if (check_logits(top_size, pix_size, ch_size, frame_size, frame_stride, list_frame_stride, __func__)) { return 1; }
+    TopArgs a{};
+    a.y = dev_y_buf; a.index = dev_index_buf; a.logit = dev_logit_buf;
+    a.top_size = top_size; a.pix_size = pix_size; a.frame_stride = frame_stride; a.list_stride = list_frame_stride;
+    return run_top(a, false, ch_size, frame_size, dev_workspace, workspace_size, stream, __func__);
+}
+
+int bbhip_fp32_CategoricalSampling(float const *dev_y_buf, float const *dev_u_buf, int *dev_category_buf, float *dev_share_buf, float temperature, int top_size,
+                                   float top_p, float min_p, int pix_size, int ch_size, int frame_size, int frame_stride, void *dev_workspace,
+                                   size_t workspace_size, void *stream)
+{
+    clear_hints();
+    if (!(dev_y_buf && dev_u_buf && dev_category_buf)) { return fail("%s: null buffer", __func__); }
+    if (check_logits(top_size, pix_size, ch_size, frame_size, frame_stride, frame_stride, __func__)) { return 1; }
+    if (!(temperature > 0.0f && temperature < __builtin_inff())) { return fail("%s: the temperature must be positive (the largest logit: top_size 1)", __func__); }
+    if (!(top_p > 0.0f && top_p <= 1.0f && min_p >= 0.0f && min_p <= 1.0f)) { return fail("%s: top_p must lie in (0, 1], min_p in [0, 1]", __func__); }
+    TopArgs a{};
+    a.y = dev_y_buf; a.u = dev_u_buf; a.category = dev_category_buf; a.share = dev_share_buf;
+    a.temperature = temperature; a.top_p = top_p; a.min_p = min_p;
+    a.top_size = top_size; a.pix_size = pix_size; a.frame_stride = frame_stride; a.list_stride = frame_stride;
+    return run_top(a, true, ch_size, frame_size, dev_workspace, workspace_size, stream, __func__);
 }
 
 // ---- RealToBinary, BinaryToReal, Binarize, HardTanh ----

@@ -1,0 +1,86 @@
+// Sums and maxima down the columns of node-major, frame-minor buffers: a column is one (pixel, frame), its elements lie one row pitch (times
+// the pixels) apart.  Shared by the operators that work frame by frame over all nodes: layer normalisation and what reads the logits.
+//
+// A unit is W consecutive frames of one row (W = 4: one 128-bit access where rows start on 16 bytes, else W = 1).  A workgroup owns a tile
+// of `tx` consecutive units (a power of two up to the wavefront) and a slab of rows; lane l of a wavefront takes unit l % tx and
+// row l / tx of the 64 / tx rows that the wavefront reads at once, so a load covers segments of 16 * tx bytes.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "lut_kernels.hpp"
+
+namespace bbhip {
+
+constexpr int kColBlock = 256;
+constexpr int kColWaves = kColBlock / kWave;
+
+struct ColumnSpace {
+    TileDivisor units_per_row;      // units of one (pixel) row: ceil(frame_size / W)
+    int units;                      // pix_size * units_per_row
+    int frame_size;
+    int log_tx;                     // tile width, log2
+    int tiles;                      // ceil(units / tx)
+    int rows, slab_rows, slabs;     // rows = nodes or channels
+};
+
+// the unit of a lane: where it lies in its row block and how many of its W frames exist (0: no such unit)
+template <int W>
+struct ColumnUnit {
+    int pix, f0, live, column;      // column: of its first frame, in the compact order of units
+    __device__ __forceinline__ ColumnUnit(ColumnSpace const &c, int unit)
+    {
+        bool const in = unit < c.units;
+        int const u = in ? unit : 0;
+        int q;
+        split_tile(u, c.units_per_row, pix, q);
+        f0     = q * W;
+        live   = in ? (c.frame_size - f0 < W ? c.frame_size - f0 : W) : 0;
+        column = u * W;
+    }
+};
+
+// W frames at p, the absent ones 0 (nothing behind the last frame is read)
+template <int W, class E>
+__device__ __forceinline__ void column_load(E const *__restrict__ p, int live, E (&v)[W])
+{
+    if constexpr (W == 4) {
+        if (live == 4) {
+            using V = std::conditional_t<std::is_same_v<E, float>, float4, int4>;
+            V const t = *reinterpret_cast<V const *>(p);
+            v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
+            return;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < W; ++j) { v[j] = j < live ? p[j] : E(0); }
+}
+
+template <int W>
+__device__ __forceinline__ void column_store(float *__restrict__ p, int live, float const (&v)[W])
+{
+    if constexpr (W == 4) {
+        if (live == 4) {
+            *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
+            return;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < W; ++j) { if (j < live) { p[j] = v[j]; } }
+}
+
+// v of the lane `o` lanes away (o a power of two, wave-uniform)
+__device__ __forceinline__ float lane_xor_any(float v, int o)
+{
+    switch (o) {
+    case 1:  return lane_xor(v, 1);
+    case 2:  return lane_xor(v, 2);
+    case 4:  return lane_xor(v, 4);
+    case 8:  return lane_xor(v, 8);
+    case 16: return lane_xor(v, 16);
+    default: return lane_xor(v, 32);
+    }
+}
+
+}  // namespace bbhip

@@ -255,4 +255,33 @@ inline int pool_shared_rows(int lanes, long long nodes)
     return (lanes > 32 && (nodes <= 256 || (nodes > 16384 && full))) ? 1 : 256 / lanes;
 }
 
+// How the operators down the columns divide `units` (of four frames, or of one) and `rows` among workgroups of 256 threads: tiles of 2^log_tx units, slabs of rows.
+// Sixteen units of four frames are a segment of 256 bytes of a row, 64 of one frame likewise; fewer where there are fewer.  Slabs until the launch has
+// 2048 workgroups, of at least `batch` rows per thread, at most 64 (every workgroup of the second launch adds its columns' slabs up).
+inline void column_split(int units, int rows, bool wide, int batch, int &log_tx, int &tiles, int &slab_rows, int &slabs)
+{
+    log_tx = 0;
+    while ((1 << log_tx) < units && log_tx < (wide ? 4 : 6)) { ++log_tx; }
+    tiles = ceil_div(units, 1 << log_tx);
+    int const step = (4 * 64 >> log_tx) * batch;                        // rows that a workgroup reads at a time
+    int want = ceil_div(2048, tiles);
+    if (want > 64) { want = 64; }
+    int const steps = ceil_div(rows, step);
+    slab_rows = ceil_div(steps, want < steps ? want : steps) * step;
+    slabs = ceil_div(rows, slab_rows);
+}
+
+// The same for the selection of the largest logits: tiles of four units or of one, slabs of whole chunks of 256 channels, of which the second launch can
+// select from 1024 / top_size at most.
+inline void top_split(int units, int channels, int top_size, int &log_tx, int &tiles, int &slab_rows, int &slabs)
+{
+    log_tx = units > 1 ? 2 : 0;
+    tiles = ceil_div(units, 1 << log_tx);
+    int want = ceil_div(512, tiles);
+    if (want > 1024 / top_size) { want = 1024 / top_size; }
+    int const chunks = ceil_div(channels, 256);
+    slab_rows = ceil_div(chunks, want < chunks ? want : chunks) * 256;
+    slabs = ceil_div(channels, slab_rows);
+}
+
 }  // namespace bbhip

@@ -1,0 +1,399 @@
+// LayerNormalization: every frame is normalised over all nodes of its layer, then each node is mapped by its own gamma and beta:
+//   mean = sum_n x / N,  var = sum_n (x - mean)^2 / N,  rstd = 1 / sqrt(var + eps),  y = ((x - mean) rstd) gamma_n + beta_n
+// and backward, with xh = (x - mean) rstd and g = dy gamma_n:
+//   dgamma_n = sum_f dy xh,  dbeta_n = sum_f dy,  dx = rstd (g - sum_n g / N - xh (sum_n g xh) / N).
+// The statistics are sums down the columns of the buffer (column_tiles.hpp), the weights' gradients sums along its rows.
+//
+// Means and squared deviations are formed over eight rows at a time and merged pairwise with their counts (the update of Chan, Golub and
+// LeVeque), so a mean that is large against the deviation costs no digits; packed bits are counted, and their squared deviation is
+// ones * zeros / N.  All sums are taken in a fixed order: the same input gives the same bits on every run.
+//
+// Any size goes in two launches: the sums of a slab of rows per workgroup (forward: mean and squared deviation; backward: the two sums per
+// frame and, of the same reading, the two sums per node over the tile's frames), then every workgroup adds up the slabs of its frames and writes.
+#pragma once
+
+#include "column_tiles.hpp"
+
+namespace bbhip {
+
+struct LayerNormArgs {
+    ColumnSpace c;
+    TileDivisor tiles;              // of one slab
+    void const  *x;                 // fp32 frames or packed words
+    float const *dy;                // backward
+    float       *out;               // y or dx
+    float const *gamma, *beta;      // NULL: 1 and 0
+    float       *mean, *rstd;       // forward: written unless NULL; backward: read
+    float2      *partial;           // [slabs][units * W]: forward (mean, squared deviation) or (ones, -), backward (sum g, sum g xh)
+    float2      *row_partial;       // [tiles][rows]: (sum dy xh, sum dy)
+    float       *dgamma, *dbeta;    // backward
+    float eps, reciprocal_rows;
+    int   x_stride, out_stride;     // (dy has the pitch of dx)
+    int   accumulate;               // dgamma, dbeta: added to
+    int   main_blocks;              // backward's second launch: workgroups that write dx, behind them those that close the rows' sums
+};
+
+// W values of row `r` of a unit
+template <int W, bool BIT>
+__device__ __forceinline__ void layer_norm_load(void const *__restrict__ x, int stride, int r, int f0, int live, float (&v)[W])
+{
+    if constexpr (BIT) {
+        uint32_t const word = live > 0 ? static_cast<uint32_t const *>(x)[(size_t)r * stride + (f0 >> 5)] >> (f0 & 31) : 0u;
+#pragma unroll
+        for (int j = 0; j < W; ++j) { v[j] = (float)((word >> j) & 1u); }
+    }
+    else { column_load<W, float>(static_cast<float const *>(x) + (size_t)r * stride + f0, live, v); }
+}
+
+// count, mean and squared deviation of W columns
+template <int W>
+struct Moments {
+    float n = 0.0f, mean[W] = {}, m2[W] = {};
+    // (the other's share of the count is 0 where both are empty)
+    __device__ __forceinline__ void merge(float on, float const (&omean)[W], float const (&om2)[W])
+    {
+        float const total = n + on, share = total > 0.0f ? on / total : 0.0f, weight = n * share;
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+            float const d = omean[j] - mean[j];
+            mean[j] = __builtin_fmaf(d, share, mean[j]);
+            m2[j]   = __builtin_fmaf(d * d, weight, m2[j] + om2[j]);
+        }
+        n = total;
+    }
+};
+
+constexpr int kColShareMax = kColWaves * kWave * 4;     // floats: one value per wavefront and column of the widest tile
+
+// over the lanes and wavefronts of a workgroup that hold the same unit; the result is wavefront 0's.  share: 2 * kColShareMax + kColWaves * kWave floats
+template <int W>
+__device__ __forceinline__ void merge_workgroup(Moments<W> &m, int log_tx, float *share)
+{
+    int const lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, tx = lane & ((1 << log_tx) - 1);
+    for (int o = 1 << log_tx; o < kWave; o <<= 1) {
+        float om[W], o2[W];
+        float const on = lane_xor_any(m.n, o);
+#pragma unroll
+        for (int j = 0; j < W; ++j) { om[j] = lane_xor_any(m.mean[j], o); o2[j] = lane_xor_any(m.m2[j], o); }
+        m.merge(on, om, o2);
+    }
+    float *const s_mean = share, *const s_m2 = share + kColShareMax, *const s_n = share + 2 * kColShareMax;
+    if (lane < (1 << log_tx)) {
+        s_n[wave * kWave + tx] = m.n;
+#pragma unroll
+        for (int j = 0; j < W; ++j) { s_mean[(wave * kWave + tx) * W + j] = m.mean[j]; s_m2[(wave * kWave + tx) * W + j] = m.m2[j]; }
+    }
+    __syncthreads();
+    if (wave == 0) {
+        for (int w = 1; w < kColWaves; ++w) {
+            float om[W], o2[W];
+#pragma unroll
+            for (int j = 0; j < W; ++j) { om[j] = s_mean[(w * kWave + tx) * W + j]; o2[j] = s_m2[(w * kWave + tx) * W + j]; }
+            m.merge(s_n[w * kWave + tx], om, o2);
+        }
+    }
+}
+
+// the same for two plain sums
+template <int W>
+__device__ __forceinline__ void add_workgroup(float (&a)[W], float (&b)[W], int log_tx, float *share)
+{
+    int const lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, tx = lane & ((1 << log_tx) - 1);
+    for (int o = 1 << log_tx; o < kWave; o <<= 1) {
+#pragma unroll
+        for (int j = 0; j < W; ++j) { a[j] += lane_xor_any(a[j], o); b[j] += lane_xor_any(b[j], o); }
+    }
+    float *const s_a = share, *const s_b = share + kColShareMax;
+    if (lane < (1 << log_tx)) {
+#pragma unroll
+        for (int j = 0; j < W; ++j) { s_a[(wave * kWave + tx) * W + j] = a[j]; s_b[(wave * kWave + tx) * W + j] = b[j]; }
+    }
+    __syncthreads();
+    if (wave == 0) {
+        for (int w = 1; w < kColWaves; ++w) {
+#pragma unroll
+            for (int j = 0; j < W; ++j) { a[j] += s_a[(w * kWave + tx) * W + j]; b[j] += s_b[(w * kWave + tx) * W + j]; }
+        }
+    }
+}
+
+// where a thread of a workgroup stands: rows first, first + step, ... below end of its slab, one unit
+template <int W>
+struct ColumnThread {
+    int slab, tile, tx, first, step, end;
+    __device__ __forceinline__ ColumnThread(ColumnSpace const &c, TileDivisor const &tiles, int block, int blocks)
+    {
+        int const lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+        split_tile(xcd_remap(block, blocks), tiles, slab, tile);
+        tx = lane & ((1 << c.log_tx) - 1);
+        int const at_once = kWave >> c.log_tx, begin = slab * c.slab_rows;
+        first = begin + wave * at_once + (lane >> c.log_tx);
+        step  = kColWaves * at_once;
+        end   = begin + c.slab_rows < c.rows ? begin + c.slab_rows : c.rows;
+    }
+};
+
+constexpr int kLayerNormBatch = 8;      // rows that a thread has in flight
+
+// mean and squared deviation (packed bits: the ones) of every column over a slab
+template <int W, bool BIT>
+__global__ __launch_bounds__(kColBlock) void layer_norm_stats_kernel(LayerNormArgs a)
+{
+    __shared__ float share[2 * kColShareMax + kColWaves * kWave];
+    ColumnThread<W> const t(a.c, a.tiles, blockIdx.x, gridDim.x);
+    ColumnUnit<W> const u(a.c, (t.tile << a.c.log_tx) + t.tx);
+    constexpr int B = kLayerNormBatch;
+    float2 *const partial = a.partial + (size_t)t.slab * (a.c.units * W) + u.column;
+    bool const writes = threadIdx.x < (1u << a.c.log_tx) && u.live > 0;
+
+    if constexpr (BIT) {
+        float ones[W] = {}, none[W] = {};
+        for (int r = t.first; r < t.end; r += B * t.step) {
+            float v[B][W];
+#pragma unroll
+            for (int i = 0; i < B; ++i) {
+                int const row = r + i * t.step;
+                layer_norm_load<W, true>(a.x, a.x_stride, row < t.end ? row : r, u.f0, row < t.end ? u.live : 0, v[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < B; ++i) {
+#pragma unroll
+                for (int j = 0; j < W; ++j) { ones[j] += v[i][j]; }
+            }
+        }
+        add_workgroup<W>(ones, none, a.c.log_tx, share);
+        if (writes) {
+#pragma unroll
+            for (int j = 0; j < W; ++j) { partial[j] = make_float2(ones[j], 0.0f); }
+        }
+    }
+    else {
+        Moments<W> m;
+        for (int r = t.first; r < t.end; r += B * t.step) {
+            float v[B][W], n = 0.0f;
+#pragma unroll
+            for (int i = 0; i < B; ++i) {
+                int const row = r + i * t.step;
+                bool const in = row < t.end;
+                layer_norm_load<W, false>(a.x, a.x_stride, in ? row : r, u.f0, u.live, v[i]);      // (an absent row: another again, which counts for nothing)
+                n += in ? 1.0f : 0.0f;
+            }
+            float const rn = 1.0f / n;
+            float mean[W], m2[W];
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                float s = 0.0f, q = 0.0f;
+#pragma unroll
+                for (int i = 0; i < B; ++i) { s += r + i * t.step < t.end ? v[i][j] : 0.0f; }
+                mean[j] = s * rn;
+#pragma unroll
+                for (int i = 0; i < B; ++i) {
+                    float const d = r + i * t.step < t.end ? v[i][j] - mean[j] : 0.0f;
+                    q = __builtin_fmaf(d, d, q);
+                }
+                m2[j] = q;
+            }
+            m.merge(n, mean, m2);
+        }
+        merge_workgroup<W>(m, a.c.log_tx, share);
+        if (writes) {
+#pragma unroll
+            for (int j = 0; j < W; ++j) { partial[j] = make_float2(m.mean[j], m.m2[j]); }
+        }
+    }
+}
+
+// y, from the slabs' sums; the workgroups of the first slab write mean and rstd
+template <int W, bool BIT>
+__global__ __launch_bounds__(kColBlock) void layer_norm_apply_kernel(LayerNormArgs a)
+{
+    __shared__ float share[2 * kColShareMax + kColWaves * kWave];
+    ColumnThread<W> const t(a.c, a.tiles, blockIdx.x, gridDim.x);
+    ColumnUnit<W> const u(a.c, (t.tile << a.c.log_tx) + t.tx);
+    int const part = (int)threadIdx.x >> a.c.log_tx, parts = kColBlock >> a.c.log_tx;
+    Moments<W> m;
+    float ones[W] = {}, none[W] = {};
+    for (int s = part; s < a.c.slabs; s += parts) {
+        float2 const *const p = a.partial + (size_t)s * (a.c.units * W) + u.column;
+        int const left = a.c.rows - s * a.c.slab_rows;
+        float mean[W], m2[W];
+#pragma unroll
+        for (int j = 0; j < W; ++j) { float2 const v = p[j]; mean[j] = v.x; m2[j] = v.y; }
+        if constexpr (BIT) {
+#pragma unroll
+            for (int j = 0; j < W; ++j) { ones[j] += mean[j]; }
+        }
+        else { m.merge((float)(left < a.c.slab_rows ? left : a.c.slab_rows), mean, m2); }
+    }
+    if constexpr (BIT) { add_workgroup<W>(ones, none, a.c.log_tx, share); }
+    else               { merge_workgroup<W>(m, a.c.log_tx, share); }
+    __syncthreads();                                                            // (the partial sums in `share` have been read)
+    if (threadIdx.x < (1u << a.c.log_tx)) {
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+            float mean, var;
+            if constexpr (BIT) {
+                float const rows = (float)a.c.rows;
+                mean = ones[j] / rows;
+                var  = mean * ((rows - ones[j]) / rows);
+            }
+            else { mean = m.mean[j]; var = fmaxf(0.0f, m.m2[j] / (float)a.c.rows); }
+            share[t.tx * W + j] = mean;
+            share[kColShareMax + t.tx * W + j] = 1.0f / sqrtf(var + a.eps);
+        }
+    }
+    __syncthreads();
+    float mean[W], rstd[W];
+#pragma unroll
+    for (int j = 0; j < W; ++j) { mean[j] = share[t.tx * W + j]; rstd[j] = share[kColShareMax + t.tx * W + j]; }
+    if (t.slab == 0 && threadIdx.x < (1u << a.c.log_tx)) {
+        if (a.mean != nullptr) { column_store<W>(a.mean + u.f0, u.live, mean); }
+        if (a.rstd != nullptr) { column_store<W>(a.rstd + u.f0, u.live, rstd); }
+    }
+    constexpr int B = 4;
+    for (int r = t.first; r < t.end; r += B * t.step) {
+        float v[B][W], g[B], b[B];
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+            int const row = r + i * t.step < t.end ? r + i * t.step : r;
+            layer_norm_load<W, BIT>(a.x, a.x_stride, row, u.f0, u.live, v[i]);
+            g[i] = a.gamma != nullptr ? a.gamma[row] : 1.0f;
+            b[i] = a.beta != nullptr ? a.beta[row] : 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+            int const row = r + i * t.step;
+            if (row < t.end) {
+#pragma unroll
+                for (int j = 0; j < W; ++j) { v[i][j] = __builtin_fmaf((v[i][j] - mean[j]) * rstd[j], g[i], b[i]); }
+                column_store<W>(a.out + (size_t)row * a.out_stride + u.f0, u.live, v[i]);
+            }
+        }
+    }
+}
+
+// backward, first launch: per column of the slab sum g and sum g xh, per row of the tile sum dy xh and sum dy
+template <int W, bool BIT>
+__global__ __launch_bounds__(kColBlock) void layer_norm_backward_sums_kernel(LayerNormArgs a)
+{
+    __shared__ float share[2 * kColShareMax];
+    ColumnThread<W> const t(a.c, a.tiles, blockIdx.x, gridDim.x);
+    ColumnUnit<W> const u(a.c, (t.tile << a.c.log_tx) + t.tx);
+    constexpr int B = 4;
+    float mean[W], rstd[W], c1[W] = {}, c2[W] = {};
+    column_load<W>(a.mean + u.f0, u.live, mean);
+    column_load<W>(a.rstd + u.f0, u.live, rstd);
+    for (int r = t.first - ((int)(threadIdx.x % kWave) >> a.c.log_tx); r < t.end; r += B * t.step) {        // wave-uniform: lanes exchange their sums
+        float x[B][W], d[B][W], g[B], s1[B], s2[B];
+        int const mine = r + ((int)(threadIdx.x % kWave) >> a.c.log_tx);
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+            int const row = mine + i * t.step, from = row < t.end ? row : t.end - 1, live = row < t.end ? u.live : 0;
+            layer_norm_load<W, BIT>(a.x, a.x_stride, from, u.f0, u.live, x[i]);
+            column_load<W>(a.dy + (size_t)from * a.out_stride + u.f0, live, d[i]);                  // (0 in an absent row: it adds nothing)
+            g[i] = a.gamma != nullptr ? a.gamma[from] : 1.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+            s1[i] = 0.0f; s2[i] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                float const xh = (x[i][j] - mean[j]) * rstd[j], gd = d[i][j] * g[i];
+                c1[j] += gd;
+                c2[j] = __builtin_fmaf(gd, xh, c2[j]);
+                s1[i] = __builtin_fmaf(d[i][j], xh, s1[i]);
+                s2[i] += d[i][j];
+            }
+        }
+        if (a.row_partial != nullptr) {
+            for (int o = 1; o < (1 << a.c.log_tx); o <<= 1) {
+#pragma unroll
+                for (int i = 0; i < B; ++i) { s1[i] += lane_xor_any(s1[i], o); s2[i] += lane_xor_any(s2[i], o); }
+            }
+            if (t.tx == 0) {
+#pragma unroll
+                for (int i = 0; i < B; ++i) {
+                    int const row = mine + i * t.step;
+                    if (row < t.end) { a.row_partial[(size_t)t.tile * a.c.rows + row] = make_float2(s1[i], s2[i]); }
+                }
+            }
+        }
+    }
+    add_workgroup<W>(c1, c2, a.c.log_tx, share);
+    if (threadIdx.x < (1u << a.c.log_tx) && u.live > 0) {
+        float2 *const partial = a.partial + (size_t)t.slab * (a.c.units * W) + u.column;
+#pragma unroll
+        for (int j = 0; j < W; ++j) { partial[j] = make_float2(c1[j], c2[j]); }
+    }
+}
+
+// backward, second launch: dx; the workgroups behind main_blocks add up the tiles' sums of 64 rows each
+template <int W, bool BIT>
+__global__ __launch_bounds__(kColBlock) void layer_norm_backward_apply_kernel(LayerNormArgs a)
+{
+    __shared__ float share[2 * kColShareMax];
+    int const lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    if ((int)blockIdx.x >= a.main_blocks) {                                      // workgroup-uniform
+        int const row = ((int)blockIdx.x - a.main_blocks) * kWave + lane, from = row < a.c.rows ? row : a.c.rows - 1;
+        float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll 8
+        for (int tile = wave; tile < a.c.tiles; tile += kColWaves) {
+            float2 const p = a.row_partial[(size_t)tile * a.c.rows + from];
+            s1 += p.x; s2 += p.y;
+        }
+        share[wave * kWave + lane] = s1;
+        share[kColShareMax + wave * kWave + lane] = s2;
+        __syncthreads();
+        if (wave == 0 && row < a.c.rows) {
+            for (int w = 1; w < kColWaves; ++w) { s1 += share[w * kWave + lane]; s2 += share[kColShareMax + w * kWave + lane]; }
+            if (a.dgamma != nullptr) { a.dgamma[row] = a.accumulate ? a.dgamma[row] + s1 : s1; }
+            if (a.dbeta != nullptr)  { a.dbeta[row]  = a.accumulate ? a.dbeta[row] + s2 : s2; }
+        }
+        return;
+    }
+    ColumnThread<W> const t(a.c, a.tiles, blockIdx.x, a.main_blocks);
+    ColumnUnit<W> const u(a.c, (t.tile << a.c.log_tx) + t.tx);
+    int const part = (int)threadIdx.x >> a.c.log_tx, parts = kColBlock >> a.c.log_tx;
+    float mean[W], rstd[W], c1[W] = {}, c2[W] = {};
+    column_load<W>(a.mean + u.f0, u.live, mean);
+    column_load<W>(a.rstd + u.f0, u.live, rstd);
+    for (int s = part; s < a.c.slabs; s += parts) {
+        float2 const *const p = a.partial + (size_t)s * (a.c.units * W) + u.column;
+#pragma unroll
+        for (int j = 0; j < W; ++j) { float2 const v = p[j]; c1[j] += v.x; c2[j] += v.y; }
+    }
+    add_workgroup<W>(c1, c2, a.c.log_tx, share);
+    __syncthreads();
+    if (threadIdx.x < (1u << a.c.log_tx)) {
+#pragma unroll
+        for (int j = 0; j < W; ++j) { share[t.tx * W + j] = c1[j] * a.reciprocal_rows; share[kColShareMax + t.tx * W + j] = c2[j] * a.reciprocal_rows; }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < W; ++j) { c1[j] = share[t.tx * W + j]; c2[j] = share[kColShareMax + t.tx * W + j]; }
+    constexpr int B = 4;
+    for (int r = t.first; r < t.end; r += B * t.step) {
+        float x[B][W], d[B][W], g[B];
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+            int const row = r + i * t.step < t.end ? r + i * t.step : r;
+            layer_norm_load<W, BIT>(a.x, a.x_stride, row, u.f0, u.live, x[i]);
+            column_load<W>(a.dy + (size_t)row * a.out_stride + u.f0, u.live, d[i]);
+            g[i] = a.gamma != nullptr ? a.gamma[row] : 1.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+            int const row = r + i * t.step;
+            if (row < t.end) {
+#pragma unroll
+                for (int j = 0; j < W; ++j) {
+                    float const xh = (x[i][j] - mean[j]) * rstd[j];
+                    d[i][j] = rstd[j] * (__builtin_fmaf(d[i][j], g[i], -c1[j]) - xh * c2[j]);
+                }
+                column_store<W>(a.out + (size_t)row * a.out_stride + u.f0, u.live, d[i]);
+            }
+        }
+    }
+}
+
+}  // namespace bbhip

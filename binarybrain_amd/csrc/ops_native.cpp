@@ -15,6 +15,7 @@
 #include <ATen/ATen.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/DeviceGuard.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
@@ -442,6 +443,165 @@ classifier_tail(T x, T idx, T t, int frames, float t_sum, bool input_binary, boo
     return {std::move(y), std::move(dx), std::move(loss), std::move(accuracy), std::move(category), std::move(dy)};
 }
 
+// ---- operators at the head of a network --------------------------------------------------------------------------------------------
+// The launch goes to the device that the tensors are on, whichever is current; every tensor of a call is on it, of the type and with the rows that the call asks for.
+// The workspace comes from torch's allocator: a graph that captures the call keeps its own.
+struct HeadCall {
+    c10::DeviceGuard guard;
+    at::Device device;
+    char const *name;
+    HeadCall(T first, char const *name_) : guard(first.device()), device(first.device()), name(name_) {}
+    [[noreturn]] void refuse(std::string const &what) const { throw Failed((std::string(name) + ": " + what).c_str()); }
+    void rows(char const *what, T t, at::ScalarType type, int64_t rows, int64_t pitch_at_least) const
+    {
+        if (t.device() != device)       { refuse(std::string(what) + " is on another device"); }
+        if (t.scalar_type() != type)    { refuse(std::string(what) + (type == at::kFloat ? " must be float32" : " must be int32")); }
+        if (t.dim() != 2 || t.size(0) != rows || t.size(1) < pitch_at_least) {
+            refuse(std::string(what) + " must be [" + std::to_string(rows) + ", at least " + std::to_string(pitch_at_least) + "]");
+        }
+        if (rows > 2147483647LL || t.size(1) > 2147483647LL) { refuse(std::string(what) + " is too large"); }
+    }
+    void line(char const *what, T t, int64_t n) const
+    {
+        if (t.device() != device)                { refuse(std::string(what) + " is on another device"); }
+        if (t.scalar_type() != at::kFloat)       { refuse(std::string(what) + " must be float32"); }
+        if (t.dim() != 1 || t.size(0) != n)      { refuse(std::string(what) + " must be [" + std::to_string(n) + "]"); }
+    }
+    void line(char const *what, OptTensor t, int64_t n) const { if (t) { line(what, *t, n); } }
+    void sizes(int a, int b = 1, int c = 1, int d = 1) const
+    {
+        if (a <= 0 || b <= 0 || c <= 0 || d <= 0)       { refuse("sizes must be positive"); }
+        if ((int64_t)a * b * c > 2147483647LL)          { refuse("too many nodes"); }
+    }
+    at::Tensor workspace(T like, size_t bytes) const { return bytes ? new_tensor(like, {(int64_t)bytes}, at::kByte) : at::Tensor(); }
+    void *stream(void) const { return at::hip::getCurrentHIPStreamMasqueradingAsCUDA(device.index()).stream(); }
+};
+void *address(at::Tensor const &t) { return t.defined() ? t.data_ptr() : nullptr; }
+size_t bytes_of(at::Tensor const &t) { return t.defined() ? (size_t)t.numel() : 0; }
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor>
+layer_normalization_forward_as(bool bit, char const *name, T x, OptTensor gamma, OptTensor beta, int frames, int y_stride, float eps, bool want_statistics)
+{
+    HeadCall const c(x, name);
+    if (x.dim() != 2) { c.refuse("x must have rows"); }
+    c.sizes(frames, 1); c.sizes((int)x.size(0), 1);
+    c.rows("x", x, bit ? at::kInt : at::kFloat, x.size(0), bit ? (frames - 1) / 32 + 1 : frames);
+    if (y_stride < frames) { c.refuse("the output's rows are shorter than the frames"); }
+    c.line("gamma", gamma, x.size(0)); c.line("beta", beta, x.size(0));
+    int const nodes = rows_of(x);
+    at::Tensor y = rows_f32(x, nodes, y_stride), mean, rstd;
+    if (want_statistics) { mean = line_f32(x, frames); rstd = line_f32(x, frames); }
+    at::Tensor const work = c.workspace(x, bbhip_LayerNormalization_WorkspaceBytes(nodes, frames));
+    if (bit) {
+        call(bbhip_bit_fp32_LayerNormalization_Forward, data<int const>(x), data<float>(y), data<float const>(gamma), data<float const>(beta), (float *)address(mean),
+             (float *)address(rstd), eps, nodes, frames, stride_of(x), y_stride, address(work), bytes_of(work), c.stream());
+    }
+    else {
+        call(bbhip_fp32_LayerNormalization_Forward, data<float const>(x), data<float>(y), data<float const>(gamma), data<float const>(beta), (float *)address(mean),
+             (float *)address(rstd), eps, nodes, frames, stride_of(x), y_stride, address(work), bytes_of(work), c.stream());
+    }
+    return {std::move(y), std::move(mean), std::move(rstd)};
+}
+std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_normalization_forward(T x, OptTensor gamma, OptTensor beta, int frames, float eps, bool want_statistics)
+{
+    return layer_normalization_forward_as(false, "layer_normalization_forward", x, gamma, beta, frames, x.dim() == 2 ? stride_of(x) : 0, eps, want_statistics);
+}
+std::tuple<at::Tensor, at::Tensor, at::Tensor> bit_layer_normalization_forward(T x, OptTensor gamma, OptTensor beta, int frames, int y_stride, float eps, bool want_statistics)
+{
+    return layer_normalization_forward_as(true, "bit_layer_normalization_forward", x, gamma, beta, frames, y_stride, eps, want_statistics);
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor>
+layer_normalization_backward_as(bool bit, char const *name, T x, T dy, OptTensor gamma, T mean, T rstd, int frames, OptTensor dgamma_in, OptTensor dbeta_in, bool want_weights)
+{
+    HeadCall const c(x, name);
+    if (x.dim() != 2) { c.refuse("x must have rows"); }
+    c.sizes(frames, 1); c.sizes((int)x.size(0), 1);
+    int const nodes = rows_of(x);
+    c.rows("x", x, bit ? at::kInt : at::kFloat, nodes, bit ? (frames - 1) / 32 + 1 : frames);
+    c.rows("dy", dy, at::kFloat, nodes, frames);
+    c.line("gamma", gamma, nodes); c.line("mean", mean, frames); c.line("rstd", rstd, frames);
+    c.line("dgamma", dgamma_in, nodes); c.line("dbeta", dbeta_in, nodes);
+    if ((bool)dgamma_in != (bool)dbeta_in) { c.refuse("dgamma and dbeta come together"); }
+    bool const accumulate = (bool)dgamma_in;
+    at::Tensor dx = rows_f32(dy, nodes, stride_of(dy)), dgamma, dbeta;
+    if (accumulate)        { dgamma = *dgamma_in; dbeta = *dbeta_in; }
+    else if (want_weights) { dgamma = line_f32(x, nodes); dbeta = line_f32(x, nodes); }
+    at::Tensor const work = c.workspace(x, bbhip_LayerNormalization_WorkspaceBytes(nodes, frames));
+    if (bit) {
+        call(bbhip_bit_fp32_LayerNormalization_Backward, data<int const>(x), data<float const>(dy), data<float>(dx), data<float const>(gamma), data<float const>(mean),
+             data<float const>(rstd), (float *)address(dgamma), (float *)address(dbeta), (int)accumulate, nodes, frames, stride_of(x), stride_of(dy), address(work), bytes_of(work), c.stream());
+    }
+    else {
+        call(bbhip_fp32_LayerNormalization_Backward, data<float const>(x), data<float const>(dy), data<float>(dx), data<float const>(gamma), data<float const>(mean),
+             data<float const>(rstd), (float *)address(dgamma), (float *)address(dbeta), (int)accumulate, nodes, frames, stride_of(x), stride_of(dy), address(work), bytes_of(work), c.stream());
+    }
+    return {std::move(dx), std::move(dgamma), std::move(dbeta)};
+}
+std::tuple<at::Tensor, at::Tensor, at::Tensor>
+layer_normalization_backward(T x, T dy, OptTensor gamma, T mean, T rstd, int frames, OptTensor dgamma, OptTensor dbeta, bool want_weights)
+{
+    return layer_normalization_backward_as(false, "layer_normalization_backward", x, dy, gamma, mean, rstd, frames, dgamma, dbeta, want_weights);
+}
+std::tuple<at::Tensor, at::Tensor, at::Tensor>
+bit_layer_normalization_backward(T x, T dy, OptTensor gamma, T mean, T rstd, int frames, OptTensor dgamma, OptTensor dbeta, bool want_weights)
+{
+    return layer_normalization_backward_as(true, "bit_layer_normalization_backward", x, dy, gamma, mean, rstd, frames, dgamma, dbeta, want_weights);
+}
+
+std::tuple<at::Tensor, at::Tensor> top_logits(T y, int top, int ch, int pix, int frames)
+{
+    HeadCall const c(y, "top_logits");
+    c.sizes(top, 1); c.sizes(ch, pix); c.sizes(frames, 1); c.sizes(top, pix);
+    c.rows("y", y, at::kFloat, (int64_t)ch * pix, frames);
+    if (top > ch) { c.refuse("more logits than channels are asked for"); }
+    int const S = stride_of(y);
+    at::Tensor const work = c.workspace(y, bbhip_TopLogits_WorkspaceBytes(top, pix, ch, frames));
+    at::Tensor index = rows_i32(y, (int64_t)top * pix, S), logit = rows_f32(y, (int64_t)top * pix, S);
+    call(bbhip_fp32_TopLogits, data<float const>(y), data<int>(index), data<float>(logit), top, pix, ch, frames, S, S, address(work), bytes_of(work), c.stream());
+    return {std::move(index), std::move(logit)};
+}
+
+std::tuple<at::Tensor, at::Tensor>
+loss_distillation(T y, T index, T logit, int ch, int pix, int frames, float temperature, OptTensor weight, float weight_sum)
+{
+    HeadCall const c(y, "loss_distillation");
+    c.sizes(ch, pix); c.sizes(frames, 1);
+    c.rows("y", y, at::kFloat, (int64_t)ch * pix, frames);
+    if (index.dim() != 2 || index.size(0) < pix || index.size(0) % pix != 0) { c.refuse("index must have as many rows for each pixel"); }
+    c.rows("index", index, at::kInt, index.size(0), frames);
+    c.rows("logit", logit, at::kFloat, index.size(0), frames);
+    int const S = stride_of(y), L = stride_of(index), top = (int)(index.size(0) / pix);
+    if (stride_of(logit) != L) { c.refuse("index and logit must have the same row pitch"); }
+    if (weight) {
+        c.rows("weight", *weight, at::kFloat, pix, frames);
+        if (stride_of(*weight) != S) { c.refuse("weight must have the row pitch of y"); }
+    }
+    at::Tensor dy = rows_f32(y, (int64_t)ch * pix, S), loss = rows_f32(y, pix, S);
+    at::Tensor const work = c.workspace(y, bbhip_LossDistillation_WorkspaceBytes(pix, ch, frames));
+    call(bbhip_fp32_LossDistillation, data<float const>(y), data<int const>(index), data<float const>(logit), data<float const>(weight), data<float>(dy), data<float>(loss),
+         temperature, weight_sum, top, pix, ch, frames, S, L, address(work), bytes_of(work), c.stream());
+    return {std::move(dy), std::move(loss)};
+}
+
+std::tuple<at::Tensor, at::Tensor>
+categorical_sampling(T y, T u, int ch, int pix, int frames, float temperature, int top, float top_p, float min_p, bool want_share)
+{
+    HeadCall const c(y, "categorical_sampling");
+    c.sizes(ch, pix); c.sizes(frames, 1); c.sizes(top, 1);
+    c.rows("y", y, at::kFloat, (int64_t)ch * pix, frames);
+    c.rows("u", u, at::kFloat, pix, frames);
+    int const S = stride_of(y);
+    if (stride_of(u) != S) { c.refuse("u must have the row pitch of y"); }
+    if (top > ch) { c.refuse("more logits than channels are asked for"); }
+    at::Tensor category = rows_i32(y, pix, S), share;
+    if (want_share) { share = rows_f32(y, pix, S); }
+    at::Tensor const work = c.workspace(y, bbhip_TopLogits_WorkspaceBytes(top, pix, ch, frames));
+    call(bbhip_fp32_CategoricalSampling, data<float const>(y), data<float const>(u), data<int>(category), (float *)address(share), temperature, top, top_p, min_p, pix, ch,
+         frames, S, address(work), bytes_of(work), c.stream());
+    return {std::move(category), std::move(share)};
+}
+
 // ---- Adam ------------------------------------------------------------------------------------------------------------------------
 // the bias-corrected rate (AdamState.lr_t), every operation rounded to float: 0.1 us where numpy's scalars take 1.0
 double adam_rate(float lr, float b1, float b2)
@@ -469,6 +629,8 @@ PyMethodDef methods[] = {
     BBHIP_FUNCTION(differentiable_lut_forward_inference), BBHIP_FUNCTION(bit_differentiable_lut_forward_inference),
     BBHIP_FUNCTION(differentiable_lut_forward_nobn), BBHIP_FUNCTION(differentiable_lut_backward), BBHIP_FUNCTION(bit_differentiable_lut_backward),
     BBHIP_FUNCTION(binary_lut_forward), BBHIP_FUNCTION(classifier_tail), BBHIP_FUNCTION(adam_rate),
+    BBHIP_FUNCTION(layer_normalization_forward), BBHIP_FUNCTION(bit_layer_normalization_forward), BBHIP_FUNCTION(layer_normalization_backward),
+    BBHIP_FUNCTION(bit_layer_normalization_backward), BBHIP_FUNCTION(top_logits), BBHIP_FUNCTION(loss_distillation), BBHIP_FUNCTION(categorical_sampling),
     BBHIP_FUNCTION(new_rows), BBHIP_FUNCTION(new_bits), BBHIP_FUNCTION(new_padded_bits), BBHIP_FUNCTION(new_zero_bits), BBHIP_FUNCTION(new_line),
     BBHIP_ENTRY(fp32_Vector_set), BBHIP_ENTRY(fp32_Vector_clamp), BBHIP_ENTRY(fp32_Vector_add_ex), BBHIP_ENTRY(fp32_Vector_mul_ex),
     BBHIP_ENTRY(fp32_Vector_div_ex), BBHIP_ENTRY(fp32_Vector_sqrt), BBHIP_ENTRY(fp32_Vector_exp), BBHIP_ENTRY(fp32_Vector_min),

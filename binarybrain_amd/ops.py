@@ -449,6 +449,49 @@ def classifier_tail(x, idx, t, frame_size, t_sum=None, binarize_input=False, mea
     return native.classifier_tail(x, idx, t, frame_size, t_sum, binarize_input, mean, want_y, want_dy, want_accuracy)
 
 
+def layer_normalization_forward(x, gamma, beta, frame_size, eps=1e-5, want_statistics=True):
+    """Every frame normalised over all nodes, each node mapped by its gamma and beta ([nodes], None: 1 and 0): fp32 x [nodes, stride] ->
+    (y, mean, rstd), the last two [frames] for the backward pass (None without want_statistics)."""
+    return native.layer_normalization_forward(x, gamma, beta, frame_size, eps, want_statistics)
+
+
+def bit_layer_normalization_forward(xbits, gamma, beta, frame_size, y_stride, eps=1e-5, want_statistics=True):
+    """The same over packed bits [nodes, words], read as 0 and 1: fp32 y [nodes, y_stride]."""
+    return native.bit_layer_normalization_forward(xbits, gamma, beta, frame_size, y_stride, eps, want_statistics)
+
+
+def layer_normalization_backward(x, dy, gamma, mean, rstd, frame_size, dgamma=None, dbeta=None, want_weights=True):
+    """-> (dx, dgamma, dbeta).  dgamma and dbeta given: added to in place; else new tensors (None without want_weights)."""
+    return native.layer_normalization_backward(x, dy, gamma, mean, rstd, frame_size, dgamma, dbeta, want_weights)
+
+
+def bit_layer_normalization_backward(xbits, dy, gamma, mean, rstd, frame_size, dgamma=None, dbeta=None, want_weights=True):
+    """The same for a forward pass over packed bits; dx is the gradient of the bits' values."""
+    return native.bit_layer_normalization_backward(xbits, dy, gamma, mean, rstd, frame_size, dgamma, dbeta, want_weights)
+
+
+def top_logits(y, top_size, ch_size, pix_size, frame_size):
+    """Of every pixel and frame the top_size (at most 256) largest logits of y [ch*pix, stride], descending, equal ones by ascending channel:
+    (index int32, logit float32), both [top*pix, stride] — what a teacher keeps for `loss_distillation`."""
+    return native.top_logits(y, top_size, ch_size, pix_size, frame_size)
+
+
+def loss_distillation(y, index, logit, ch_size, pix_size, frame_size, temperature=1.0, weight=None, weight_sum=None):
+    """Distillation from a teacher's kept logits ([top*pix, stride] channels and values, channel -1: no entry): (dy, loss [pix, stride]).  The loss of the
+    batch is loss[:, :frame_size].sum() / weight_sum, whose gradient dy is.  weight [pix, stride]: of each pixel and frame (None: 1);
+    weight_sum defaults to the sum of the weights of the frames in use, taken in float64."""
+    if weight_sum is None:
+        weight_sum = float(pix_size * frame_size) if weight is None else float(weight[:, :frame_size].sum(dtype=torch.float64).item())
+    return native.loss_distillation(y, index, logit, ch_size, pix_size, frame_size, temperature, weight, weight_sum)
+
+
+def categorical_sampling(y, u, ch_size, pix_size, frame_size, temperature=1.0, top_size=50, top_p=1.0, min_p=0.0, want_share=True):
+    """A channel of every pixel and frame drawn from softmax(y / temperature) by the given u in [0, 1) ([pix, stride]), among the top_size (at most 256) largest
+    logits, of them the shortest prefix that holds top_p of their probability, of it those of at least min_p times the largest probability:
+    (category int32 [pix, stride], -1 where nothing can be drawn, share float32 or None)."""
+    return native.categorical_sampling(y, u, ch_size, pix_size, frame_size, temperature, top_size, top_p, min_p, want_share)
+
+
 def conv_bit_to_real(xbits, frame_size, y_stride, value0=0.0, value1=1.0):
     y = native.new_rows(xbits, xbits.shape[0], y_stride)
     native.fp32_ConvBitToReal(xbits, y, value0, value1, xbits.shape[0], frame_size, xbits.shape[1], y_stride)

@@ -460,6 +460,61 @@ int bbhip_fp32_StochasticBatchNormalization_Backward(float const *dev_x_buf, flo
                                                      float reciprocal_frame_size, int node_size, int frame_size, int frame_stride,
                                                      int x_frame_stride, void *stream);
 
+/* ---- operators at the head of a network (no counterparts in the reference) ----
+ * They take what scratch they need from the caller: dev_workspace, 256-byte aligned, of at least as many bytes as the ..._WorkspaceBytes of the same sizes says
+ * (NULL where that is 0).  It needs no clearing, holds nothing between calls and may be shared by calls that follow one another on a stream; calls that may
+ * overlap (two streams, two graphs) take one each.  Every sum is taken in a fixed order: the same input gives the same bits on every run.  Padding behind the
+ * last frame of a row is neither read nor written.  Rows that start on 16 bytes (buffers and strides) are read four frames at a time. */
+
+/* LayerNormalization: every frame is normalised over all nodes, then each node is mapped by its own gamma and beta (NULL: 1 and 0):
+ *     mean = sum x / N, var = sum (x - mean)^2 / N, rstd = 1 / sqrt(var + eps), y = ((x - mean) * rstd) * gamma[node] + beta[node].
+ * dev_mean_buf and dev_rstd_buf ([frame_size], what the backward pass needs) may be NULL.  The bit entry reads packed bits as 0 and 1; x_frame_stride counts
+ * words there.  y may be x (fp32). */
+size_t bbhip_LayerNormalization_WorkspaceBytes(int node_size, int frame_size);
+int bbhip_fp32_LayerNormalization_Forward(float const *dev_x_buf, float *dev_y_buf, float const *dev_gamma, float const *dev_beta, float *dev_mean_buf,
+                                          float *dev_rstd_buf, float eps, int node_size, int frame_size, int x_frame_stride, int y_frame_stride,
+                                          void *dev_workspace, size_t workspace_size, void *stream);
+int bbhip_bit_fp32_LayerNormalization_Forward(int const *dev_x_buf, float *dev_y_buf, float const *dev_gamma, float const *dev_beta, float *dev_mean_buf,
+                                              float *dev_rstd_buf, float eps, int node_size, int frame_size, int x_frame_stride, int y_frame_stride,
+                                              void *dev_workspace, size_t workspace_size, void *stream);
+/* With xh = (x - mean) * rstd and g = dy * gamma:  dgamma = sum over frames of dy * xh, dbeta = sum of dy (each may be NULL; added to what they hold with
+ * accumulate, as dW of the LUT layers, else written),  dx = rstd * (g - (sum over nodes of g) / N - xh * (sum over nodes of g * xh) / N).  dy and dx have rows of
+ * frame_stride, x of x_frame_stride.  dx may be dy. */
+int bbhip_fp32_LayerNormalization_Backward(float const *dev_x_buf, float const *dev_dy_buf, float *dev_dx_buf, float const *dev_gamma, float const *dev_mean_buf,
+                                           float const *dev_rstd_buf, float *dev_dgamma, float *dev_dbeta, int accumulate, int node_size, int frame_size,
+                                           int x_frame_stride, int frame_stride, void *dev_workspace, size_t workspace_size, void *stream);
+int bbhip_bit_fp32_LayerNormalization_Backward(int const *dev_x_buf, float const *dev_dy_buf, float *dev_dx_buf, float const *dev_gamma, float const *dev_mean_buf,
+                                               float const *dev_rstd_buf, float *dev_dgamma, float *dev_dbeta, int accumulate, int node_size, int frame_size,
+                                               int x_frame_stride, int frame_stride, void *dev_workspace, size_t workspace_size, void *stream);
+
+/* TopLogits: of every pixel and frame the top_size (1 .. 256, at most ch_size) largest logits of the [ch][pix] nodes, descending, of equal ones the lowest channel
+ * first; what is not a number comes before all numbers; -0 counts and is returned as +0.  dev_index_buf (channels) and dev_logit_buf are [top][pix] nodes with
+ * rows of list_frame_stride: the record that a teacher leaves for LossDistillation. */
+size_t bbhip_TopLogits_WorkspaceBytes(int top_size, int pix_size, int ch_size, int frame_size);
+int bbhip_fp32_TopLogits(float const *dev_y_buf, int *dev_index_buf, float *dev_logit_buf, int top_size, int pix_size, int ch_size, int frame_size,
+                         int frame_stride, int list_frame_stride, void *dev_workspace, size_t workspace_size, void *stream);
+
+/* LossDistillation: forward and gradient of the cross entropy against a teacher's kept logits z_j of the channels i_j (top_size <= 256 of them per pixel and frame;
+ * entries whose channel is negative or not below ch_size are none; a channel named twice has both shares), less the entropy of the teacher's distribution:
+ *     q = softmax(z / T) over the entries, p = softmax(y / T) over the channels, w the place's weight (dev_weight_buf [pix] rows of frame_stride, NULL: 1)
+ *     dev_loss_buf[pix][frame] = w * T^2 * sum_j q_j * (log q_j - log p_{i_j}),   dy[c] = w * T * (p_c - q_c) / weight_sum.
+ * The caller passes weight_sum = the sum of the weights and reports sum(dev_loss_buf) / weight_sum, whose gradient dy is.  A place without entries, or whose entries are all
+ * minus infinity, or with weight 0 has loss 0 and gradient 0 whatever its logits are.  dev_loss_buf has rows of frame_stride too. */
+size_t bbhip_LossDistillation_WorkspaceBytes(int pix_size, int ch_size, int frame_size);
+int bbhip_fp32_LossDistillation(float const *dev_y_buf, int const *dev_index_buf, float const *dev_logit_buf, float const *dev_weight_buf, float *dev_dy_buf,
+                                float *dev_loss_buf, float temperature, float weight_sum, int top_size, int pix_size, int ch_size, int frame_size,
+                                int frame_stride, int list_frame_stride, void *dev_workspace, size_t workspace_size, void *stream);
+
+/* CategoricalSampling: a channel of every pixel and frame drawn from softmax(y / temperature) by the given number u in [0, 1) of its place (dev_u_buf [pix] rows of
+ * frame_stride).  Kept are the top_size (1 .. 256) largest logits in the order of TopLogits; of them, with top_p below 1, the shortest prefix whose sum of probabilities
+ * reaches top_p of theirs; of it those with at least min_p times the largest probability.  Drawn is the first whose probability together with those before it exceeds
+ * u times the sum of the kept; top_size 1 is the largest logit.  dev_category_buf [pix][frame_stride] receives the channel, dev_share_buf (NULL: not wanted) its share of the
+ * kept.  Sums are in 64 bits.  Where the largest logit is minus infinity or not a number nothing is drawn: category -1, share 0.
+ * The workspace is that of TopLogits. */
+int bbhip_fp32_CategoricalSampling(float const *dev_y_buf, float const *dev_u_buf, int *dev_category_buf, float *dev_share_buf, float temperature, int top_size,
+                                   float top_p, float min_p, int pix_size, int ch_size, int frame_size, int frame_stride, void *dev_workspace,
+                                   size_t workspace_size, void *stream);
+
 /* ---- StochasticLut ---- */
 /* bbcu_fp32_StochasticLut_Forward<N>, include/bbcu/bbcu.h:667-681 */
 int bbhip_fp32_StochasticLut_Forward(int n, float const *dev_x_buf, float *dev_y_buf, int const *dev_input_index,

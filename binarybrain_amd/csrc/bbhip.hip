@@ -2635,7 +2635,7 @@ static int top_space(TopArgs &a, bool wide, int top_size, int pix_size, int ch_s
 
 static size_t top_candidate_bytes(TopArgs const &a, bool wide, int top_size)
 {
-    return a.c.slabs > 1 ? align256((size_t)a.c.slabs * a.c.units * (wide ? 4 : 1) * (size_t)top_size * sizeof(uint2)) : 0;
+    return a.c.slabs > 1 ? align256((size_t)a.c.slabs * a.c.units * (wide ? 4 : 1) * (size_t)top_size * sizeof(uint64_t)) : 0;
 }
 
 size_t bbhip_TopLogits_WorkspaceBytes(int top_size, int pix_size, int ch_size, int frame_size)
@@ -2651,16 +2651,39 @@ size_t bbhip_TopLogits_WorkspaceBytes(int top_size, int pix_size, int ch_size, i
     return most;
 }
 
-static int run_top(TopArgs &a, bool draw, int ch_size, int frame_size, void *workspace, size_t workspace_size, void *stream, char const *name)
+static int run_top_few(TopArgs &a, bool draw, int ch_size, int frame_size, void *stream)
 {
-    bool const wide = frame_size >= 4 && a.frame_stride % 4 == 0 && starts_on_16_bytes(a.y);
-    if (a.top_size > ch_size) { return fail("%s: top_size=%d of %d channels", name, a.top_size, ch_size); }
-    if (top_space(a, wide, a.top_size, a.pix_size, ch_size, frame_size, name)) { return 1; }
-    if (check_workspace(workspace, workspace_size, top_candidate_bytes(a, wide, a.top_size), name)) { return 1; }
-    a.candidates = static_cast<uint2 *>(workspace);
+    a.c.units_per_row = make_tile_divisor(frame_size);
+    a.c.units = a.pix_size * frame_size;
+    a.c.frame_size = frame_size;
+    a.c.rows = ch_size;
     hipStream_t const st = static_cast<hipStream_t>(stream);
     ScopedTimer tm(kTimeOther, st);
-    dim3 const grid((unsigned)(a.c.tiles * a.c.slabs)), block((unsigned)(kTopChunk << a.c.log_tx));
+    dim3 const grid((unsigned)ceil_div(a.c.units, kWave)), block(kWave);
+#define BBHIP_TOP_FEW(MOST)                                                                             \
+    do {                                                                                                \
+        if (draw) { launch((top_logits_few_kernel<MOST, true>), grid, block, 0, st, a); }               \
+        else      { launch((top_logits_few_kernel<MOST, false>), grid, block, 0, st, a); }              \
+    } while (0)
+    if (ch_size <= 8)       { BBHIP_TOP_FEW(8); }
+    else if (ch_size <= 16) { BBHIP_TOP_FEW(16); }
+    else                    { BBHIP_TOP_FEW(32); }
+#undef BBHIP_TOP_FEW
+    BBHIP_LAUNCH_CHECK();
+    return 0;
+}
+
+static int run_top(TopArgs &a, bool draw, int ch_size, int frame_size, void *workspace, size_t workspace_size, void *stream, char const *name)
+{
+    if (a.top_size > ch_size) { return fail("%s: top_size=%d of %d channels", name, a.top_size, ch_size); }
+    if (ch_size <= kTopFew) { return run_top_few(a, draw, ch_size, frame_size, stream); }
+    bool const wide = frame_size >= 4 && a.frame_stride % 4 == 0 && starts_on_16_bytes(a.y);
+    if (top_space(a, wide, a.top_size, a.pix_size, ch_size, frame_size, name)) { return 1; }
+    if (check_workspace(workspace, workspace_size, top_candidate_bytes(a, wide, a.top_size), name)) { return 1; }
+    a.candidates = static_cast<uint64_t *>(workspace);
+    hipStream_t const st = static_cast<hipStream_t>(stream);
+    ScopedTimer tm(kTimeOther, st);
+    dim3 const grid((unsigned)(a.c.tiles * a.c.slabs)), block((unsigned)(a.c.log_tx ? kTopRows<4> * 4 : kTopRows<1>));
     dim3 const join((unsigned)ceil_div(a.c.units * (wide ? 4 : 1), kColWaves)), join_block(kColBlock);
 #define BBHIP_TOP(W, TX)                                                                                \
     do {                                                                                                \

@@ -25,10 +25,10 @@ struct ColumnSpace {
     int rows, slab_rows, slabs;     // rows = nodes or channels
 };
 
-// the unit of a lane: where it lies in its row block and how many of its W frames exist (0: no such unit)
+// the unit of a lane: where it lies in its row block and how many of its W frames exist (live 0: no such unit; it may load the first one, whose `span` frames exist)
 template <int W>
 struct ColumnUnit {
-    int pix, f0, live, column;      // column: of its first frame, in the compact order of units
+    int pix, f0, live, span, column;        // column: of its first frame, in the compact order of units
     __device__ __forceinline__ ColumnUnit(ColumnSpace const &c, int unit)
     {
         bool const in = unit < c.units;
@@ -36,7 +36,8 @@ struct ColumnUnit {
         int q;
         split_tile(u, c.units_per_row, pix, q);
         f0     = q * W;
-        live   = in ? (c.frame_size - f0 < W ? c.frame_size - f0 : W) : 0;
+        span   = c.frame_size - f0 < W ? c.frame_size - f0 : W;
+        live   = in ? span : 0;
         column = u * W;
     }
 };
@@ -82,5 +83,30 @@ __device__ __forceinline__ float lane_xor_any(float v, int o)
     default: return lane_xor(v, 32);
     }
 }
+
+// where a thread of a workgroup stands: one unit, rows begin + lead, + step, ... below end of its slab
+template <int W>
+struct ColumnThread {
+    int slab, tile, tx, begin, lead, step, end;
+    __device__ __forceinline__ ColumnThread(ColumnSpace const &c, TileDivisor const &tiles, int block, int blocks)
+    {
+        int const lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+        split_tile(xcd_remap(block, blocks), tiles, slab, tile);
+        tx = lane & ((1 << c.log_tx) - 1);
+        int const at_once = kWave >> c.log_tx;
+        begin = slab * c.slab_rows;
+        lead  = wave * at_once + (lane >> c.log_tx);
+        step  = kColWaves * at_once;
+        end   = begin + c.slab_rows < c.rows ? begin + c.slab_rows : c.rows;
+    }
+    // body(base, whole) for every B rows of a thread, rows base + lead + i * step; whole (a compile-time truth): all of them exist
+    template <int B, class F>
+    __device__ __forceinline__ void each(F body) const
+    {
+        int base = begin;
+        for (; base + B * step <= end; base += B * step) { body(base, std::true_type()); }      // workgroup-uniform
+        if (base < end) { body(base, std::false_type()); }
+    }
+};
 
 }  // namespace bbhip

@@ -5,8 +5,10 @@
 // A place without entries (or whose kept logits are all minus infinity) and one with w = 0 has loss 0 and gradient 0 whatever its logits are.
 //
 // Two launches.  The first takes, per column and slab of channels, the running maximum m and the sum of exp((y - m) / T) in one pass; workgroups behind
-// those read the lists and leave per column the largest z, the reciprocal of their sum and  sum_j q_j ((z_j - z_max) - y_{i_j}) / T - log(sum),  to which the
-// second launch adds the student's log-sum-exp to have the loss.  The second launch joins the slabs and writes dy: first p for every channel of its slab, then, behind a
+// those read the lists and leave per column the largest z, the reciprocal of their sum E, the largest listed logit y_r of the student, and
+//   sum_j q_j ((z_j - z_max) - (y_{i_j} - y_r)) / T - log E,
+// to which the second launch adds  log sum_c exp((y_c - y_r) / T)  to have the loss: differences of nearby logits throughout.  A hash table in LDS tells
+// whether a list names a channel twice.  The second launch joins the slabs and writes dy: first p for every channel of its slab, then, behind a
 // barrier, the few channels of the lists.  Exponents are taken of differences to the maximum, (y - m) * (log2 e / T): the rounding of the product
 // grows with the distance from the maximum and weighs as little as the term itself.
 #pragma once
@@ -23,14 +25,19 @@ struct DistillArgs {
     int const   *index;
     float       *dy, *loss;
     float2      *partial;           // [slabs][units * W]: (m, sum)
-    float4      *lists;             // [units * W]: (z_max, 1 / sum, the loss without the student's log-sum-exp, entries or not)
+    float4      *lists;             // [units * W]: (z_max, 1 / E (0: no entries, negative: a channel is named twice), the lists' part of the loss, y_r)
     float scale;                    // log2(e) / T
     float reciprocal_t, t_square, coefficient;      // 1 / T, T^2, T / weight_sum
     int   top_size, pix_size, frame_stride, list_stride;
     int   main_blocks, unit_width;
 };
 
-constexpr int kListColumns = kWave;         // columns of a workgroup that reads lists; its wavefronts share the entries
+constexpr int kListColumns = 4;                                 // columns of a workgroup that reads lists; 64 threads share the entries of each
+constexpr int kListParts   = kColBlock / kListColumns;
+constexpr int kListHeld    = 256 / kListParts;                  // entries of a thread (lists of up to 256)
+constexpr int kListSlots   = 512;                               // hash table of a column: twice the longest list
+constexpr int kDistillShare = 4 * kColBlock + kListSlots * kListColumns;        // floats: the sums of a tile, or the lists' values and tables
+static_assert(kDistillShare >= 2 * kColShareMax, "both uses fit");
 
 __device__ __forceinline__ float exp_scaled(float d, float scale) { return __builtin_amdgcn_exp2f(d * scale); }
 // what sums of exponentials are taken against: a maximum of minus infinity (nothing there yet) is not subtracted
@@ -75,74 +82,115 @@ __device__ __forceinline__ void join_workgroup(float (&m)[W], float (&s)[W], int
     }
 }
 
-// the lists of 64 columns: four wavefronts share the entries of each
-__device__ __forceinline__ void distillation_lists(DistillArgs const &a, int block, float *share)
+// the lists of a few columns.  slots: kListSlots * kListColumns
+__device__ __forceinline__ void distillation_lists(DistillArgs const &a, int block, float *share, int *slots)
 {
-    int const lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-    int const column = block * kListColumns + lane, columns = a.pix_size * a.c.frame_size;
+    int const col = threadIdx.x % kListColumns, part = threadIdx.x / kListColumns;
+    int const column = block * kListColumns + col, columns = a.pix_size * a.c.frame_size;
     bool const in = column < columns;
     int pix, f;
     split_tile(in ? column : 0, a.frames, pix, f);
     size_t const at = (size_t)pix * a.list_stride + f, entry = (size_t)a.pix_size * a.list_stride;
     size_t const y_at = (size_t)pix * a.frame_stride + f, channel = (size_t)a.pix_size * a.frame_stride;
-    float top = -__builtin_inff();
-    int entries = 0;
-#pragma unroll 4
-    for (int j = wave; j < a.top_size; j += kColWaves) {
-        bool const valid = (unsigned)a.index[at + j * entry] < (unsigned)a.c.rows;
-        float const z = a.logit[at + j * entry];
-        entries += valid && !(z == -__builtin_inff()) ? 1 : 0;
-        top = fmaxf(top, valid ? z : top);
+    for (int s = threadIdx.x; s < kListSlots * kListColumns; s += kColBlock) { slots[s] = -1; }
+    float z[kListHeld], y[kListHeld];
+    int c[kListHeld];
+#pragma unroll
+    for (int i = 0; i < kListHeld; ++i) {
+        int const j = i * kListParts + part;
+        c[i] = -1; z[i] = 0.0f;
+        if (i * kListParts < a.top_size && j < a.top_size) { c[i] = a.index[at + j * entry]; z[i] = a.logit[at + j * entry]; }
     }
-    share[wave * kWave + lane] = top;
-    share[kColShareMax + wave * kWave + lane] = (float)entries;
-    __syncthreads();
-    float any = 0.0f;
-    for (int w = 0; w < kColWaves; ++w) { top = fmaxf(top, share[w * kWave + lane]); any += share[kColShareMax + w * kWave + lane]; }
-    __syncthreads();
-    float const r = reference_of(top);
-    float sum = 0.0f, part = 0.0f;
-#pragma unroll 4
-    for (int j = wave; j < a.top_size; j += kColWaves) {
-        int const c = a.index[at + j * entry];
-        float const z = a.logit[at + j * entry];
-        bool const valid = (unsigned)c < (unsigned)a.c.rows;
-        float const d = z == top ? 0.0f : z - r, e = valid ? exp_scaled(d, a.scale) : 0.0f;
-        if (!(e == 0.0f)) {                                                     // (not a number: counts)
-            sum += e;
-            part = __builtin_fmaf(e, d - a.y[y_at + c * channel], part);
+    float top = -__builtin_inff(), near = -__builtin_inff(), any = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kListHeld; ++i) {
+        y[i] = 0.0f;
+        if (i * kListParts < a.top_size) {                                      // workgroup-uniform
+            bool const valid = (unsigned)c[i] < (unsigned)a.c.rows && !(z[i] == -__builtin_inff());
+            c[i] = valid ? c[i] : -1;
+            if (valid) { y[i] = a.y[y_at + c[i] * channel]; any = 1.0f; }
         }
     }
-    share[wave * kWave + lane] = sum;
-    share[kColShareMax + wave * kWave + lane] = part;
+#pragma unroll
+    for (int i = 0; i < kListHeld; ++i) {
+        top  = c[i] >= 0 ? fmaxf(top, z[i]) : top;
+        near = c[i] >= 0 ? fmaxf(near, y[i]) : near;
+    }
+    __syncthreads();                                                            // (the table is empty)
+    float twice = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kListHeld; ++i) {
+        if (c[i] >= 0) {
+            unsigned slot = ((unsigned)c[i] * 2654435761u) >> 23;               // (of 512; at most 256 of them are ever taken, so the search ends)
+            for (;;) {
+                int const there = atomicCAS(&slots[slot * kListColumns + col], -1, c[i]);
+                if (there == -1) { break; }
+                if (there == c[i]) { twice = 1.0f; break; }
+                slot = (slot + 1) % kListSlots;
+            }
+        }
+    }
+    // over the threads of a column: its lanes of a wavefront, then the wavefronts
+    int const wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+#pragma unroll
+    for (int o = kListColumns; o < kWave; o <<= 1) {
+        top = fmaxf(top, lane_xor(top, o)); near = fmaxf(near, lane_xor(near, o));
+        any = fmaxf(any, lane_xor(any, o)); twice = fmaxf(twice, lane_xor(twice, o));
+    }
+    float4 *const of_wave = reinterpret_cast<float4 *>(share);                  // [kColWaves][kListColumns]
+    if (lane < kListColumns) { of_wave[wave * kListColumns + lane] = make_float4(top, near, any, twice); }
     __syncthreads();
-    if (wave == 0 && in) {
-        for (int w = 1; w < kColWaves; ++w) { sum += share[w * kWave + lane]; part += share[kColShareMax + w * kWave + lane]; }
-        a.lists[(size_t)pix * a.c.units_per_row.count * a.unit_width + f] =
-            any > 0.0f ? make_float4(top, 1.0f / sum, part * a.reciprocal_t / sum - logf(sum), 1.0f) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int w = 0; w < kColWaves; ++w) {
+        float4 const o = of_wave[w * kListColumns + col];
+        top = fmaxf(top, o.x); near = fmaxf(near, o.y); any = fmaxf(any, o.z); twice = fmaxf(twice, o.w);
+    }
+    float const r = reference_of(top), yr = reference_of(near);
+    float sum = 0.0f, loss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kListHeld; ++i) {
+        float const d = z[i] == top ? 0.0f : z[i] - r, e = c[i] >= 0 ? exp_scaled(d, a.scale) : 0.0f;
+        if (!(e == 0.0f)) {                                                     // (not a number: counts)
+            sum += e;
+            loss = __builtin_fmaf(e, d - (y[i] - yr), loss);
+        }
+    }
+#pragma unroll
+    for (int o = kListColumns; o < kWave; o <<= 1) { sum += lane_xor(sum, o); loss += lane_xor(loss, o); }
+    __syncthreads();
+    if (lane < kListColumns) { of_wave[wave * kListColumns + lane] = make_float4(sum, loss, 0.0f, 0.0f); }
+    __syncthreads();
+    if (part == 0 && in) {
+        sum = 0.0f; loss = 0.0f;
+        for (int w = 0; w < kColWaves; ++w) { sum += of_wave[w * kListColumns + col].x; loss += of_wave[w * kListColumns + col].y; }
+        float const q = any > 0.0f ? 1.0f / sum : 0.0f;
+        a.lists[(size_t)pix * a.c.units_per_row.count * a.unit_width + f] = make_float4(top, twice > 0.0f ? -q : q, loss * a.reciprocal_t / sum - logf(sum), yr);
     }
 }
 
 template <int W>
 __global__ __launch_bounds__(kColBlock) void distillation_sums_kernel(DistillArgs a)
 {
-    __shared__ float share[2 * kColShareMax];
-    if ((int)blockIdx.x >= a.main_blocks) { distillation_lists(a, (int)blockIdx.x - a.main_blocks, share); return; }       // workgroup-uniform
+    __shared__ __align__(16) float share[kDistillShare];
+    if ((int)blockIdx.x >= a.main_blocks) {                                     // workgroup-uniform
+        distillation_lists(a, (int)blockIdx.x - a.main_blocks, share, reinterpret_cast<int *>(share + 4 * kColBlock));
+        return;
+    }
     ColumnThread<W> const t(a.c, a.tiles, blockIdx.x, a.main_blocks);
     ColumnUnit<W> const u(a.c, (t.tile << a.c.log_tx) + t.tx);
     constexpr int B = 8;
     size_t const channel = (size_t)a.pix_size * a.frame_stride;
-    float const *const y = a.y + (size_t)u.pix * a.frame_stride + u.f0;
+    float const *const y = a.y + (size_t)u.pix * a.frame_stride + u.f0 + (size_t)t.lead * channel;
     float m[W], s[W] = {};
 #pragma unroll
     for (int j = 0; j < W; ++j) { m[j] = -__builtin_inff(); }
-    for (int r = t.first; r < t.end; r += B * t.step) {
+    t.template each<B>([&](int base, auto whole) {
         float v[B][W];
 #pragma unroll
         for (int i = 0; i < B; ++i) {
-            int const row = r + i * t.step;
-            column_load<W>(y + (size_t)(row < t.end ? row : r) * channel, u.live, v[i]);
-            if (row >= t.end) {
+            bool const in = whole || base + t.lead + i * t.step < t.end;
+            column_load<W>(y + (size_t)(base + i * t.step) * channel, in ? u.span : 0, v[i]);
+            if (!in) {
 #pragma unroll
                 for (int j = 0; j < W; ++j) { v[i][j] = -__builtin_inff(); }
             }
@@ -158,7 +206,7 @@ __global__ __launch_bounds__(kColBlock) void distillation_sums_kernel(DistillArg
 #pragma unroll
             for (int i = 0; i < B; ++i) { s[j] += exp_scaled(v[i][j] - ref, a.scale); }
         }
-    }
+    });
     join_workgroup<W>(m, s, a.c.log_tx, a.scale, share);
     if (threadIdx.x < (1u << a.c.log_tx) && u.live > 0) {
         float2 *const partial = a.partial + (size_t)t.slab * (a.c.units * W) + u.column;
@@ -193,8 +241,8 @@ __global__ __launch_bounds__(kColBlock) void distillation_gradient_kernel(Distil
         for (int j = 0; j < W; ++j) {
             float4 const l = a.lists[u.column + j];
             float const w = j < u.live ? (a.weight != nullptr ? a.weight[place + j] : 1.0f) : 0.0f;
-            bool const none = l.w == 0.0f || w == 0.0f;
-            loss[j] = none ? 0.0f : w * a.t_square * (l.z + (m[j] * a.reciprocal_t + logf(s[j])));
+            bool const none = l.y == 0.0f || w == 0.0f;
+            loss[j] = none ? 0.0f : w * a.t_square * (l.z + ((m[j] - l.w) * a.reciprocal_t + logf(s[j])));
             of_m[t.tx * W + j] = reference_of(m[j]);
             of_s[t.tx * W + j] = 1.0f / s[j];
             of_k[t.tx * W + j] = none ? 0.0f : w * a.coefficient;
@@ -202,8 +250,8 @@ __global__ __launch_bounds__(kColBlock) void distillation_gradient_kernel(Distil
         if (t.slab == 0) { column_store<W>(a.loss + place, u.live, loss); }
     }
     __syncthreads();
-    float const *const y = a.y + place;
-    float *const dy = a.dy + place;
+    float const *const y = a.y + place + (size_t)t.lead * channel;
+    float *const dy = a.dy + place + (size_t)t.lead * channel;
     float ref[W], gain[W];
     bool learns[W];
 #pragma unroll
@@ -212,46 +260,61 @@ __global__ __launch_bounds__(kColBlock) void distillation_gradient_kernel(Distil
         ref[j] = of_m[t.tx * W + j]; gain[j] = k * of_s[t.tx * W + j]; learns[j] = !(k == 0.0f);
     }
     constexpr int B = 4;
-    for (int r = t.first; r < t.end; r += B * t.step) {
+    t.template each<B>([&](int base, auto whole) {
         float v[B][W];
 #pragma unroll
-        for (int i = 0; i < B; ++i) { column_load<W>(y + (size_t)(r + i * t.step < t.end ? r + i * t.step : r) * channel, u.live, v[i]); }
+        for (int i = 0; i < B; ++i) {
+            bool const in = whole || base + t.lead + i * t.step < t.end;
+            column_load<W>(y + (size_t)(base + i * t.step) * channel, in ? u.span : 0, v[i]);
+        }
 #pragma unroll
         for (int i = 0; i < B; ++i) {
-            int const row = r + i * t.step;
-            if (row < t.end) {
+            if (whole || base + t.lead + i * t.step < t.end) {
 #pragma unroll
                 for (int j = 0; j < W; ++j) { v[i][j] = learns[j] ? exp_scaled(v[i][j] - ref[j], a.scale) * gain[j] : 0.0f; }
-                column_store<W>(dy + (size_t)row * channel, u.live, v[i]);
+                column_store<W>(dy + (size_t)(base + i * t.step) * channel, u.live, v[i]);
             }
         }
-    }
+    });
     __syncthreads();                                                            // the slab's p is written; the listed channels follow
     int const log_columns = a.c.log_tx + (W == 4 ? 2 : 0), columns = 1 << log_columns, begin = t.slab * a.c.slab_rows;
     size_t const entry = (size_t)a.pix_size * a.list_stride;
-    for (int e = threadIdx.x; e < columns * a.top_size; e += kColBlock) {
-        int const col = e & (columns - 1), j = e >> log_columns;
-        ColumnUnit<W> const at(a.c, (t.tile << a.c.log_tx) + col / W);
-        float const k = of_k[col];
-        if (col % W >= at.live || k == 0.0f) { continue; }
-        int const *const index = a.index + (size_t)at.pix * a.list_stride + at.f0 + col % W;
-        int const c = index[j * entry];
-        if (c < begin || c >= t.end) { continue; }
-        float const *const logit = a.logit + (size_t)at.pix * a.list_stride + at.f0 + col % W;
-        float4 const l = a.lists[at.column + col % W];
-        float q = 0.0f;
-        bool first = true;
-        for (int i = 0; i < a.top_size; ++i) {                                  // a channel that the list names twice has both shares, added in the list's order
-            if (index[i * entry] == c) {
-                first = first && i >= j;
-                float const z = logit[i * entry];
-                q += exp_scaled(z == l.x ? 0.0f : z - reference_of(l.x), a.scale);
-            }
+    constexpr int AHEAD = 8;                                                    // entries that a thread looks at at a time
+    for (int e0 = threadIdx.x; e0 < columns * a.top_size; e0 += AHEAD * kColBlock) {
+        int c[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            int const e = e0 + i * kColBlock, col = e & (columns - 1), j = e >> log_columns;
+            ColumnUnit<W> const at(a.c, (t.tile << a.c.log_tx) + col / W);
+            c[i] = -1;
+            if (e < columns * a.top_size && col % W < at.live) { c[i] = a.index[(size_t)at.pix * a.list_stride + at.f0 + col % W + j * entry]; }
         }
-        if (first) {
-            size_t const here = (size_t)at.pix * a.frame_stride + at.f0 + col % W + (size_t)c * channel;
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            if (c[i] < begin || c[i] >= t.end) { continue; }                    // (a slab holds few of a list's channels)
+            int const e = e0 + i * kColBlock, col = e & (columns - 1), j = e >> log_columns;
+            float const k = of_k[col];
+            if (k == 0.0f) { continue; }
+            ColumnUnit<W> const at(a.c, (t.tile << a.c.log_tx) + col / W);
+            float const *const logit = a.logit + (size_t)at.pix * a.list_stride + at.f0 + col % W;
+            float4 const l = a.lists[at.column + col % W];
+            auto weight = [&](float z) { return exp_scaled(z == l.x ? 0.0f : z - reference_of(l.x), a.scale); };
+            float q = 0.0f;
+            if (!(l.y < 0.0f)) { q = weight(logit[j * entry]); }
+            else {                                                              // a channel may be named twice: its shares are added in the list's order, by its first entry's thread
+                int const *const index = a.index + (size_t)at.pix * a.list_stride + at.f0 + col % W;
+                int first = a.top_size;
+                for (int o = 0; o < a.top_size; ++o) {
+                    if (index[o * entry] == c[i]) {
+                        first = first < o ? first : o;
+                        q += weight(logit[o * entry]);
+                    }
+                }
+                if (first != j) { continue; }
+            }
+            size_t const here = (size_t)at.pix * a.frame_stride + at.f0 + col % W + (size_t)c[i] * channel;
             float const p = exp_scaled(a.y[here] - of_m[col], a.scale) * of_s[col];
-            a.dy[here] = k * (p - q * l.y);
+            a.dy[here] = k * (p - q * fabsf(l.y));
         }
     }
 }

@@ -35,14 +35,14 @@ struct LayerNormArgs {
 
 // W values of row `r` of a unit
 template <int W, bool BIT>
-__device__ __forceinline__ void layer_norm_load(void const *__restrict__ x, int stride, int r, int f0, int live, float (&v)[W])
+__device__ __forceinline__ void layer_norm_load(void const *__restrict__ x, int stride, int r, int f0, int span, float (&v)[W])
 {
     if constexpr (BIT) {
-        uint32_t const word = live > 0 ? static_cast<uint32_t const *>(x)[(size_t)r * stride + (f0 >> 5)] >> (f0 & 31) : 0u;
+        uint32_t const word = static_cast<uint32_t const *>(x)[(size_t)r * stride + (f0 >> 5)] >> (f0 & 31);
 #pragma unroll
         for (int j = 0; j < W; ++j) { v[j] = (float)((word >> j) & 1u); }
     }
-    else { column_load<W, float>(static_cast<float const *>(x) + (size_t)r * stride + f0, live, v); }
+    else { column_load<W, float>(static_cast<float const *>(x) + (size_t)r * stride + f0, span, v); }
 }
 
 // count, mean and squared deviation of W columns
@@ -117,22 +117,6 @@ __device__ __forceinline__ void add_workgroup(float (&a)[W], float (&b)[W], int 
     }
 }
 
-// where a thread of a workgroup stands: rows first, first + step, ... below end of its slab, one unit
-template <int W>
-struct ColumnThread {
-    int slab, tile, tx, first, step, end;
-    __device__ __forceinline__ ColumnThread(ColumnSpace const &c, TileDivisor const &tiles, int block, int blocks)
-    {
-        int const lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-        split_tile(xcd_remap(block, blocks), tiles, slab, tile);
-        tx = lane & ((1 << c.log_tx) - 1);
-        int const at_once = kWave >> c.log_tx, begin = slab * c.slab_rows;
-        first = begin + wave * at_once + (lane >> c.log_tx);
-        step  = kColWaves * at_once;
-        end   = begin + c.slab_rows < c.rows ? begin + c.slab_rows : c.rows;
-    }
-};
-
 constexpr int kLayerNormBatch = 8;      // rows that a thread has in flight
 
 // mean and squared deviation (packed bits: the ones) of every column over a slab
@@ -148,19 +132,20 @@ __global__ __launch_bounds__(kColBlock) void layer_norm_stats_kernel(LayerNormAr
 
     if constexpr (BIT) {
         float ones[W] = {}, none[W] = {};
-        for (int r = t.first; r < t.end; r += B * t.step) {
+        t.template each<B>([&](int base, auto whole) {
             float v[B][W];
 #pragma unroll
             for (int i = 0; i < B; ++i) {
-                int const row = r + i * t.step;
-                layer_norm_load<W, true>(a.x, a.x_stride, row < t.end ? row : r, u.f0, row < t.end ? u.live : 0, v[i]);
+                int const row = base + t.lead + i * t.step;
+                layer_norm_load<W, true>(a.x, a.x_stride, whole || row < t.end ? row : t.begin, u.f0, u.span, v[i]);
             }
 #pragma unroll
             for (int i = 0; i < B; ++i) {
+                bool const in = whole || base + t.lead + i * t.step < t.end;
 #pragma unroll
-                for (int j = 0; j < W; ++j) { ones[j] += v[i][j]; }
+                for (int j = 0; j < W; ++j) { ones[j] += in ? v[i][j] : 0.0f; }
             }
-        }
+        });
         add_workgroup<W>(ones, none, a.c.log_tx, share);
         if (writes) {
 #pragma unroll
@@ -169,32 +154,32 @@ __global__ __launch_bounds__(kColBlock) void layer_norm_stats_kernel(LayerNormAr
     }
     else {
         Moments<W> m;
-        for (int r = t.first; r < t.end; r += B * t.step) {
+        t.template each<B>([&](int base, auto whole) {
             float v[B][W], n = 0.0f;
 #pragma unroll
             for (int i = 0; i < B; ++i) {
-                int const row = r + i * t.step;
-                bool const in = row < t.end;
-                layer_norm_load<W, false>(a.x, a.x_stride, in ? row : r, u.f0, u.live, v[i]);      // (an absent row: another again, which counts for nothing)
+                int const row = base + t.lead + i * t.step;
+                bool const in = whole || row < t.end;
+                layer_norm_load<W, false>(a.x, a.x_stride, in ? row : t.begin, u.f0, u.span, v[i]);      // (an absent row: another, which counts for nothing)
                 n += in ? 1.0f : 0.0f;
             }
-            float const rn = 1.0f / n;
+            float const rn = whole ? 1.0f / B : n > 0.0f ? 1.0f / n : 0.0f;
             float mean[W], m2[W];
 #pragma unroll
             for (int j = 0; j < W; ++j) {
                 float s = 0.0f, q = 0.0f;
 #pragma unroll
-                for (int i = 0; i < B; ++i) { s += r + i * t.step < t.end ? v[i][j] : 0.0f; }
+                for (int i = 0; i < B; ++i) { s += whole || base + t.lead + i * t.step < t.end ? v[i][j] : 0.0f; }
                 mean[j] = s * rn;
 #pragma unroll
                 for (int i = 0; i < B; ++i) {
-                    float const d = r + i * t.step < t.end ? v[i][j] - mean[j] : 0.0f;
+                    float const d = whole || base + t.lead + i * t.step < t.end ? v[i][j] - mean[j] : 0.0f;
                     q = __builtin_fmaf(d, d, q);
                 }
                 m2[j] = q;
             }
             m.merge(n, mean, m2);
-        }
+        });
         merge_workgroup<W>(m, a.c.log_tx, share);
         if (writes) {
 #pragma unroll
@@ -251,25 +236,25 @@ __global__ __launch_bounds__(kColBlock) void layer_norm_apply_kernel(LayerNormAr
         if (a.rstd != nullptr) { column_store<W>(a.rstd + u.f0, u.live, rstd); }
     }
     constexpr int B = 4;
-    for (int r = t.first; r < t.end; r += B * t.step) {
+    t.template each<B>([&](int base, auto whole) {
         float v[B][W], g[B], b[B];
 #pragma unroll
         for (int i = 0; i < B; ++i) {
-            int const row = r + i * t.step < t.end ? r + i * t.step : r;
-            layer_norm_load<W, BIT>(a.x, a.x_stride, row, u.f0, u.live, v[i]);
+            int const there = base + t.lead + i * t.step, row = whole || there < t.end ? there : t.begin;
+            layer_norm_load<W, BIT>(a.x, a.x_stride, row, u.f0, u.span, v[i]);
             g[i] = a.gamma != nullptr ? a.gamma[row] : 1.0f;
             b[i] = a.beta != nullptr ? a.beta[row] : 0.0f;
         }
 #pragma unroll
         for (int i = 0; i < B; ++i) {
-            int const row = r + i * t.step;
-            if (row < t.end) {
+            int const row = base + t.lead + i * t.step;
+            if (whole || row < t.end) {
 #pragma unroll
                 for (int j = 0; j < W; ++j) { v[i][j] = __builtin_fmaf((v[i][j] - mean[j]) * rstd[j], g[i], b[i]); }
                 column_store<W>(a.out + (size_t)row * a.out_stride + u.f0, u.live, v[i]);
             }
         }
-    }
+    });
 }
 
 // backward, first launch: per column of the slab sum g and sum g xh, per row of the tile sum dy xh and sum dy
@@ -281,28 +266,28 @@ __global__ __launch_bounds__(kColBlock) void layer_norm_backward_sums_kernel(Lay
     ColumnUnit<W> const u(a.c, (t.tile << a.c.log_tx) + t.tx);
     constexpr int B = 4;
     float mean[W], rstd[W], c1[W] = {}, c2[W] = {};
-    column_load<W>(a.mean + u.f0, u.live, mean);
-    column_load<W>(a.rstd + u.f0, u.live, rstd);
-    for (int r = t.first - ((int)(threadIdx.x % kWave) >> a.c.log_tx); r < t.end; r += B * t.step) {        // wave-uniform: lanes exchange their sums
+    column_load<W>(a.mean + u.f0, u.span, mean);
+    column_load<W>(a.rstd + u.f0, u.span, rstd);
+    t.template each<B>([&](int base, auto whole) {
         float x[B][W], d[B][W], g[B], s1[B], s2[B];
-        int const mine = r + ((int)(threadIdx.x % kWave) >> a.c.log_tx);
 #pragma unroll
         for (int i = 0; i < B; ++i) {
-            int const row = mine + i * t.step, from = row < t.end ? row : t.end - 1, live = row < t.end ? u.live : 0;
-            layer_norm_load<W, BIT>(a.x, a.x_stride, from, u.f0, u.live, x[i]);
-            column_load<W>(a.dy + (size_t)from * a.out_stride + u.f0, live, d[i]);                  // (0 in an absent row: it adds nothing)
-            g[i] = a.gamma != nullptr ? a.gamma[from] : 1.0f;
+            int const there = base + t.lead + i * t.step, row = whole || there < t.end ? there : t.begin;
+            layer_norm_load<W, BIT>(a.x, a.x_stride, row, u.f0, u.span, x[i]);
+            column_load<W>(a.dy + (size_t)row * a.out_stride + u.f0, u.span, d[i]);
+            g[i] = a.gamma != nullptr ? a.gamma[row] : 1.0f;
         }
 #pragma unroll
         for (int i = 0; i < B; ++i) {
+            bool const in = u.live > 0 && (whole || base + t.lead + i * t.step < t.end);     // (what is not there adds nothing)
             s1[i] = 0.0f; s2[i] = 0.0f;
 #pragma unroll
             for (int j = 0; j < W; ++j) {
-                float const xh = (x[i][j] - mean[j]) * rstd[j], gd = d[i][j] * g[i];
+                float const dj = in ? d[i][j] : 0.0f, xh = in ? (x[i][j] - mean[j]) * rstd[j] : 0.0f, gd = dj * g[i];
                 c1[j] += gd;
                 c2[j] = __builtin_fmaf(gd, xh, c2[j]);
-                s1[i] = __builtin_fmaf(d[i][j], xh, s1[i]);
-                s2[i] += d[i][j];
+                s1[i] = __builtin_fmaf(dj, xh, s1[i]);
+                s2[i] += dj;
             }
         }
         if (a.row_partial != nullptr) {
@@ -313,12 +298,12 @@ __global__ __launch_bounds__(kColBlock) void layer_norm_backward_sums_kernel(Lay
             if (t.tx == 0) {
 #pragma unroll
                 for (int i = 0; i < B; ++i) {
-                    int const row = mine + i * t.step;
-                    if (row < t.end) { a.row_partial[(size_t)t.tile * a.c.rows + row] = make_float2(s1[i], s2[i]); }
+                    int const row = base + t.lead + i * t.step;
+                    if (whole || row < t.end) { a.row_partial[(size_t)t.tile * a.c.rows + row] = make_float2(s1[i], s2[i]); }
                 }
             }
         }
-    }
+    });
     add_workgroup<W>(c1, c2, a.c.log_tx, share);
     if (threadIdx.x < (1u << a.c.log_tx) && u.live > 0) {
         float2 *const partial = a.partial + (size_t)t.slab * (a.c.units * W) + u.column;
@@ -355,8 +340,8 @@ __global__ __launch_bounds__(kColBlock) void layer_norm_backward_apply_kernel(La
     ColumnUnit<W> const u(a.c, (t.tile << a.c.log_tx) + t.tx);
     int const part = (int)threadIdx.x >> a.c.log_tx, parts = kColBlock >> a.c.log_tx;
     float mean[W], rstd[W], c1[W] = {}, c2[W] = {};
-    column_load<W>(a.mean + u.f0, u.live, mean);
-    column_load<W>(a.rstd + u.f0, u.live, rstd);
+    column_load<W>(a.mean + u.f0, u.span, mean);
+    column_load<W>(a.rstd + u.f0, u.span, rstd);
     for (int s = part; s < a.c.slabs; s += parts) {
         float2 const *const p = a.partial + (size_t)s * (a.c.units * W) + u.column;
 #pragma unroll
@@ -372,19 +357,19 @@ __global__ __launch_bounds__(kColBlock) void layer_norm_backward_apply_kernel(La
 #pragma unroll
     for (int j = 0; j < W; ++j) { c1[j] = share[t.tx * W + j]; c2[j] = share[kColShareMax + t.tx * W + j]; }
     constexpr int B = 4;
-    for (int r = t.first; r < t.end; r += B * t.step) {
+    t.template each<B>([&](int base, auto whole) {
         float x[B][W], d[B][W], g[B];
 #pragma unroll
         for (int i = 0; i < B; ++i) {
-            int const row = r + i * t.step < t.end ? r + i * t.step : r;
-            layer_norm_load<W, BIT>(a.x, a.x_stride, row, u.f0, u.live, x[i]);
-            column_load<W>(a.dy + (size_t)row * a.out_stride + u.f0, u.live, d[i]);
+            int const there = base + t.lead + i * t.step, row = whole || there < t.end ? there : t.begin;
+            layer_norm_load<W, BIT>(a.x, a.x_stride, row, u.f0, u.span, x[i]);
+            column_load<W>(a.dy + (size_t)row * a.out_stride + u.f0, u.span, d[i]);
             g[i] = a.gamma != nullptr ? a.gamma[row] : 1.0f;
         }
 #pragma unroll
         for (int i = 0; i < B; ++i) {
-            int const row = r + i * t.step;
-            if (row < t.end) {
+            int const row = base + t.lead + i * t.step;
+            if (whole || row < t.end) {
 #pragma unroll
                 for (int j = 0; j < W; ++j) {
                     float const xh = (x[i][j] - mean[j]) * rstd[j];
@@ -393,7 +378,7 @@ __global__ __launch_bounds__(kColBlock) void layer_norm_backward_apply_kernel(La
                 column_store<W>(a.out + (size_t)row * a.out_stride + u.f0, u.live, d[i]);
             }
         }
-    }
+    });
 }
 
 }  // namespace bbhip

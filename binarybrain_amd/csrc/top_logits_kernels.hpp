@@ -3,11 +3,11 @@
 // Order: descending, equal values by ascending channel, anything that is not a number before all numbers, -0 equal to +0 (and returned as +0).  A value
 // becomes a 32-bit key that orders as an unsigned number; with the channel behind it no two entries of a column are equal, so the result is unique.
 //
-// One pass over the logits.  A workgroup owns the columns of a tile and a slab of channels and reads 256 channels of each column at a time.  What is not above the
-// column's bound (the k-th largest so far) is dropped by one comparison; the rest is appended to the column's list in LDS, in any order, and when a
-// list could overflow with the next 256 channels, one wavefront per column cuts it to its k largest and raises the bound.  With random logits a column appends
-// about k (1 + ln(channels / 256)) entries and is cut a few times.  Few columns are shared by several workgroups, a slab of channels each; a second launch
-// selects from their lists.
+// One pass over the logits.  A workgroup owns the columns of a tile and a slab of channels; its threads hold 16 channels of their columns in registers at a time.  Of the
+// first ones each thread gives the maxima of a group or two per column, 256 groups in all: the k-th largest of those bounds the k-th largest logit from below, and with random logits
+// 74 of 2048 reach the bound of k = 64.  What is below is dropped by one comparison, the rest is appended to the column's list in LDS, in any order, and the lists are cut to
+// their k largest before the next channels.  Logits that defeat the bound (ascending ones, ties) make a list overflow: those channels are appended again, a few at a
+// time.  Few columns are shared by several workgroups, a slab of channels each; a second launch selects from their lists.
 //
 // The k-th largest of a list is found bit by bit from the top: the count of keys that reach a candidate is the number of bits of a few ballots.
 #pragma once
@@ -17,10 +17,16 @@
 
 namespace bbhip {
 
-constexpr int kTopMost  = 256;                  // largest k
-constexpr int kTopChunk = 256;                  // channels that a workgroup reads at a time, of each column
-constexpr int kTopList  = kTopMost + kTopChunk; // entries of a column's list: cut to k <= kTopMost before each chunk that might not fit
-constexpr int kTopJoin  = 1024;                 // entries that the second launch selects from
+constexpr int kTopMost = 256;                   // largest k
+constexpr int kTopJoin = 1024;                  // entries that the second launch selects from
+constexpr int kTopFew  = 32;                    // channels up to which a lane takes a column by itself
+
+// TX threads side by side: a workgroup reads this many channels of each column with one load per thread ...
+template <int TX> constexpr int kTopRows = TX == 1 ? 256 : 128;
+// ... of which it holds so many at a time (128 registers let two workgroups share a compute unit) ...
+constexpr int kTopHeld = 12;
+// ... and a column's list holds these besides the kTopMost that it is cut to
+template <int TX> constexpr int kTopList = kTopMost + kTopRows<TX>;
 
 struct TopArgs {
     ColumnSpace c;                  // rows = channels
@@ -31,7 +37,7 @@ struct TopArgs {
     float const *u;                 // sampling: [pix][frame_stride], and so are
     int         *category;
     float       *share;             // the drawn category's share, or NULL
-    uint2       *candidates;        // [slabs][units * W][top]: (key, channel), where several slabs share a column
+    uint64_t    *candidates;        // [slabs][units * W][top], where several slabs share a column
     float temperature, top_p, min_p;
     int   top_size, pix_size, frame_stride, list_stride;
 };
@@ -49,14 +55,19 @@ __device__ __forceinline__ int bits_below_lane(uint64_t mask)
     return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u));
 }
 
-// The k largest of n > k entries, entry i * 64 + lane in register i, to the front of key_out / index_out in any order; returns a lower bound of their keys.
-// rows: above every channel.  A whole wavefront calls this.
+// an entry of a list: of two, the larger number comes first
+__device__ __forceinline__ uint64_t entry_of(uint32_t key, int channel) { return ((uint64_t)key << 32) | (uint32_t)~channel; }
+__device__ __forceinline__ uint32_t key_of(uint64_t entry)              { return (uint32_t)(entry >> 32); }
+__device__ __forceinline__ int      channel_of(uint64_t entry)          { return (int)~(uint32_t)entry; }
+
+// The k-th largest of n >= k keys, key i * 64 + lane in register i: bit by bit from the top, the keys that reach a candidate counted by ballots.  `reach`: how many keys
+// reach the returned bound; k where the search could stop early, and then the bound itself need not be a key.  A whole wavefront calls this.
 template <int PER>
-__device__ __forceinline__ uint32_t select_largest(uint32_t const (&key)[PER], int const (&index)[PER], int n, int k, int rows, uint32_t *key_out, int *index_out)
+__device__ __forceinline__ uint32_t kth_key(uint32_t const (&key)[PER], int n, int k, int &reach)
 {
     int const lane = threadIdx.x % kWave;
     uint32_t bound = 0u;
-    int reach = n;
+    reach = n;
     for (int bit = 31; bit >= 0 && reach != k; --bit) {
         uint32_t const candidate = bound | (1u << bit);
         int count = 0;
@@ -64,6 +75,24 @@ __device__ __forceinline__ uint32_t select_largest(uint32_t const (&key)[PER], i
         for (int i = 0; i < PER; ++i) { count += __popcll(__ballot(i * kWave + lane < n && key[i] >= candidate)); }
         if (count >= k) { bound = candidate; reach = count; }
     }
+    return bound;
+}
+
+// The k largest of n > k entries of `list`, to its front in any order; returns a lower bound of their keys.  rows: above every channel.  A whole wavefront calls this.
+template <int PER>
+__device__ __forceinline__ uint32_t cut_list_of(uint64_t *list, int n, int k, int rows)
+{
+    int const lane = threadIdx.x % kWave;
+    uint32_t key[PER];
+    int channel[PER], reach;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        int const e = i * kWave + lane;
+        uint64_t const v = e < n ? list[e] : 0u;
+        key[i] = key_of(v); channel[i] = channel_of(v);
+    }
+    wave_fence();
+    uint32_t const bound = kth_key<PER>(key, n, k, reach);
     int last = rows;                                                            // of the entries that equal the bound, those up to here
     if (reach != k) {                                                           // (bound is the k-th largest key, and more than k entries reach it)
         int above = 0;
@@ -75,73 +104,77 @@ __device__ __forceinline__ uint32_t select_largest(uint32_t const (&key)[PER], i
             int const candidate = last | (1 << bit);
             int count = 0;
 #pragma unroll
-            for (int i = 0; i < PER; ++i) { count += __popcll(__ballot(i * kWave + lane < n && key[i] == bound && index[i] < candidate)); }
+            for (int i = 0; i < PER; ++i) { count += __popcll(__ballot(i * kWave + lane < n && key[i] == bound && channel[i] < candidate)); }
             if (count < wanted) { last = candidate; }
         }
     }
     int base = 0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-        bool const taken = i * kWave + lane < n && (key[i] > bound || (key[i] == bound && index[i] <= last));
+        bool const taken = i * kWave + lane < n && (key[i] > bound || (key[i] == bound && channel[i] <= last));
         uint64_t const mask = __ballot(taken);
-        if (taken) {
-            int const at = base + bits_below_lane(mask);
-            key_out[at] = key[i]; index_out[at] = index[i];
-        }
+        if (taken) { list[base + bits_below_lane(mask)] = entry_of(key[i], channel[i]); }
         base += __popcll(mask);
     }
+    wave_fence();
     return bound;
+}
+// with as many registers as the list needs
+template <int MOST>
+__device__ __forceinline__ uint32_t cut_list(uint64_t *list, int n, int k, int rows)
+{
+    if (n <= 2 * kWave) { return cut_list_of<2>(list, n, k, rows); }
+    if (n <= 4 * kWave) { return cut_list_of<4>(list, n, k, rows); }
+    if constexpr (MOST > 8 * kWave) { if (n > 8 * kWave) { return cut_list_of<MOST / kWave>(list, n, k, rows); } }
+    return cut_list_of<8>(list, n, k, rows);
 }
 
 // k entries in LDS into their order, by counting for each those before it.  A whole wavefront calls this.
-__device__ __forceinline__ void order_entries(uint32_t *key, int *index, int k)
+template <int PER>
+__device__ __forceinline__ void order_list_of(uint64_t *list, int k)
 {
-    constexpr int PER = kTopMost / kWave;
     int const lane = threadIdx.x % kWave;
-    uint32_t mine[PER];
-    int at[PER], rank[PER];
+    uint64_t mine[PER];
+    int rank[PER];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        int const e = i * kWave + lane;
-        mine[i] = e < k ? key[e] : 0u;
-        at[i]   = e < k ? index[e] : 0;
-        rank[i] = 0;
-    }
+    for (int i = 0; i < PER; ++i) { mine[i] = i * kWave + lane < k ? list[i * kWave + lane] : 0u; rank[i] = 0; }
+#pragma unroll 4
     for (int e = 0; e < k; ++e) {
-        uint32_t const other = key[e];
-        int const where = index[e];
+        uint64_t const other = list[e];
 #pragma unroll
-        for (int i = 0; i < PER; ++i) { rank[i] += (other > mine[i] || (other == mine[i] && where < at[i])) ? 1 : 0; }
+        for (int i = 0; i < PER; ++i) { rank[i] += other > mine[i] ? 1 : 0; }
     }
     wave_fence();
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        if (i * kWave + lane < k) { key[rank[i]] = mine[i]; index[rank[i]] = at[i]; }
-    }
+    for (int i = 0; i < PER; ++i) { if (i * kWave + lane < k) { list[rank[i]] = mine[i]; } }
     wave_fence();
+}
+__device__ __forceinline__ void order_list(uint64_t *list, int k)
+{
+    if (k <= kWave)          { order_list_of<1>(list, k); }
+    else if (k <= 2 * kWave) { order_list_of<2>(list, k); }
+    else                     { order_list_of<kTopMost / kWave>(list, k); }
 }
 
 // One category of k ordered entries: weights exp((z - z_0) / T); kept is the shortest prefix that holds top_p of their sum, of it those of at least min_p times the
 // largest; drawn is the first whose sum with those before it exceeds u times the sum of the kept.  All of it in 64 bits: the drawn index is a whole number that the
 // rounding of a sum must not move.  z_0 minus infinity or not a number: category -1, share 0.  A whole wavefront calls this.
-__device__ __forceinline__ void draw_category(uint32_t const *key, int const *index, int k, float u, float temperature, float top_p, float min_p, int &category, float &share)
+template <int PER>
+__device__ __forceinline__ void draw_of(uint64_t const *list, int k, float u, float temperature, float top_p, float min_p, int &category, float &share)
 {
-    constexpr int PER = kTopMost / kWave;
     int const lane = threadIdx.x % kWave;
-    float const z0 = value_of_key(key[0]);
+    float const z0 = value_of_key(key_of(list[0]));
     if (!(z0 > -__builtin_inff())) { category = -1; share = 0.0f; return; }     // wave-uniform
     double weight[PER], up_to[PER], before = 0.0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
         int const e = i * kWave + lane;
-        float const z = e < k ? value_of_key(key[e]) : -__builtin_inff();
+        float const z = e < k ? value_of_key(key_of(list[e])) : -__builtin_inff();
         weight[i] = z == z0 ? 1.0 : exp(((double)z - (double)z0) / (double)temperature);
         double sum = weight[i];
-        if (i * kWave < k) {                                                    // wave-uniform
-            for (int o = 1; o < kWave; o <<= 1) {
-                double const left = __shfl_up(sum, o);
-                if (lane >= o) { sum += left; }
-            }
+        for (int o = 1; o < kWave; o <<= 1) {
+            double const left = __shfl_up(sum, o);
+            if (lane >= o) { sum += left; }
         }
         up_to[i] = before + sum;
         before += __shfl(sum, kWave - 1);
@@ -160,135 +193,198 @@ __device__ __forceinline__ void draw_category(uint32_t const *key, int const *in
 #pragma unroll
     for (int i = 0; i < PER; ++i) { drawn += __popcll(__ballot(i * kWave + lane < kept && up_to[i] <= (double)u * total)); }
     drawn = drawn < kept ? drawn : kept - 1;
-    category = index[drawn];
+    category = channel_of(list[drawn]);
     double w = 0.0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) { if (drawn / kWave == i) { w = __shfl(weight[i], drawn % kWave); } }
     share = (float)(w / total);
 }
+// of the column at `at` of the buffers of one row per pixel
+__device__ __forceinline__ void draw_category(TopArgs const &a, uint64_t const *list, size_t at)
+{
+    int category;
+    float share;
+    if (a.top_size <= kWave) { draw_of<1>(list, a.top_size, a.u[at], a.temperature, a.top_p, a.min_p, category, share); }
+    else                     { draw_of<kTopMost / kWave>(list, a.top_size, a.u[at], a.temperature, a.top_p, a.min_p, category, share); }
+    if (threadIdx.x % kWave == 0) {
+        a.category[at] = category;
+        if (a.share != nullptr) { a.share[at] = share; }
+    }
+}
 
 // W = 4: a thread reads four frames of a channel, W = 1: one; TX threads side by side.  DRAW: a category instead of the list
 template <int W, int TX, bool DRAW>
-__global__ __launch_bounds__(kTopChunk * TX) void top_logits_scan_kernel(TopArgs a)
+__global__ __launch_bounds__(kTopRows<TX> * TX, 4) void top_logits_scan_kernel(TopArgs a)
 {
-    constexpr int COLS = W * TX, AHEAD = 4;
-    static_assert(COLS <= kTopChunk * TX / kWave, "a wavefront per column");
-    __shared__ uint32_t key[COLS][kTopList];
-    __shared__ int index[COLS][kTopList];
-    __shared__ int count[COLS];
+    constexpr int COLS = W * TX, ROWS = kTopRows<TX>, BLOCK = ROWS * TX, WAVES = BLOCK / kWave, HELD = kTopHeld, LIST = kTopList<TX>;
+    constexpr int PARTS = kTopMost / ROWS;                                      // groups of a thread's held channels: kTopMost groups per column
+    __shared__ uint64_t list[COLS][LIST];
+    __shared__ int count[COLS], before[COLS];
     __shared__ float bound[COLS];
-    __shared__ int full[3];
+    __shared__ int full[3], over;
     int const lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     int slab, tile;
     split_tile(xcd_remap(blockIdx.x, gridDim.x), a.tiles, slab, tile);
     int const tx = threadIdx.x % TX, ty = threadIdx.x / TX;
     ColumnUnit<W> const u(a.c, tile * TX + tx);
     int const begin = slab * a.c.slab_rows, end = begin + a.c.slab_rows < a.c.rows ? begin + a.c.slab_rows : a.c.rows;
-    int const chunks = (end - begin + kTopChunk - 1) / kTopChunk, k = a.top_size;
+    int const k = a.top_size;
     size_t const channel = (size_t)a.pix_size * a.frame_stride;
     float const *const y = a.y + (size_t)u.pix * a.frame_stride + u.f0;
 
-    if (threadIdx.x < COLS) { count[threadIdx.x] = 0; bound[threadIdx.x] = __builtin_nanf(""); }
-    if (threadIdx.x < 3) { full[threadIdx.x] = 0; }
-    float v[AHEAD][W], drop[W];
-    auto request = [&](int n, float (&to)[W]) {
-        int const row = begin + n * kTopChunk + ty;
-        column_load<W>(y + (size_t)(row < end ? row : begin) * channel, row < end ? u.live : 0, to);
+    float v[HELD][W], drop[W];
+    float const *const mine = y + (size_t)ty * channel;                         // (what is common to a load is added to it in scalar registers)
+    auto request = [&](int from) {
+        if (from + HELD * ROWS <= end) {                                        // workgroup-uniform
+#pragma unroll
+            for (int i = 0; i < HELD; ++i) { column_load<W>(mine + (size_t)(from + i * ROWS) * channel, u.span, v[i]); }
+        }
+        else {
+#pragma unroll
+            for (int i = 0; i < HELD; ++i) { column_load<W>(mine + (size_t)(from + i * ROWS) * channel, from + i * ROWS + ty < end ? u.span : 0, v[i]); }
+        }
     };
+    // (not a number drops nothing)
 #pragma unroll
-    for (int p = 0; p < AHEAD; ++p) { if (p < chunks) { request(p, v[p]); } }
+    for (int j = 0; j < W; ++j) { drop[j] = __builtin_nanf(""); }
+    if (threadIdx.x < COLS) { count[threadIdx.x] = 0; }
+    if (threadIdx.x == 0) { over = 0; }
+    if (threadIdx.x < 3) { full[threadIdx.x] = 0; }
+
+    for (int from = begin; from < end; from += HELD * ROWS) {
+        request(from);
+        if (from == begin && end - begin >= 2 * kTopMost) {
+            // the k-th largest of the maxima of kTopMost groups of channels: as many entries are no smaller, so it bounds the k-th largest entry from below, and hardly more than
+            // k entries reach it where the groups are many against k
+            uint32_t *const maxima = reinterpret_cast<uint32_t *>(&list[0][0]);                          // [COLS][kTopMost]
 #pragma unroll
-    for (int j = 0; j < W; ++j) { drop[j] = __builtin_nanf(""); }               // (nothing is dropped)
-    __syncthreads();
-    for (int n0 = 0; n0 < chunks; n0 += AHEAD) {
+            for (int g = 0; g < PARTS; ++g) {
 #pragma unroll
-        for (int p = 0; p < AHEAD; ++p) {
-            int const n = n0 + p;
-            if (n >= chunks) { break; }                                         // workgroup-uniform
-            int const row = begin + n * kTopChunk + ty;
+                for (int j = 0; j < W; ++j) {
+                    float top = -__builtin_inff();
 #pragma unroll
-            for (int j = 0; j < W; ++j) {
-                if (row < end && j < u.live && !(v[p][j] <= drop[j])) {
-                    int const col = tx * W + j, at = atomicAdd(&count[col], 1);
-                    key[col][at] = order_key(v[p][j]);
-                    index[col][at] = row;
-                    if (at >= kTopMost) { full[n % 3] = 1; }                    // the next chunk might not fit
+                    for (int i = g * HELD / PARTS; i < (g + 1) * HELD / PARTS; ++i) { top = fmaxf(top, from + i * ROWS + ty < end ? v[i][j] : top); }
+                    maxima[(tx * W + j) * kTopMost + g * ROWS + ty] = from + g * HELD / PARTS * ROWS + ty < end ? order_key(top) : 0u;        // (0: a group without channels)
                 }
             }
-            if (n + AHEAD < chunks) { request(n + AHEAD, v[p]); }
             __syncthreads();
-            // (three flags in turn: the one read now is written again three chunks on, and cleared behind the next barrier, which no one passes before all have read it)
-            bool const cut = full[n % 3] != 0;
-            if (threadIdx.x == 0) { full[(n + 2) % 3] = 0; }
-            if (cut) {                                                          // workgroup-uniform
-                if (wave < COLS && count[wave] > kTopMost) {
-                    constexpr int PER = kTopList / kWave;
-                    int const entries = count[wave];
-                    uint32_t ks[PER];
-                    int is[PER];
+            for (int col = wave; col < COLS; col += WAVES) {
+                constexpr int PER = kTopMost / kWave;
+                uint32_t key[PER];
+                int reach;
 #pragma unroll
-                    for (int i = 0; i < PER; ++i) {
-                        int const e = i * kWave + lane;
-                        ks[i] = e < entries ? key[wave][e] : 0u;
-                        is[i] = e < entries ? index[wave][e] : 0;
+                for (int i = 0; i < PER; ++i) { key[i] = maxima[col * kTopMost + i * kWave + lane]; }
+                uint32_t low = kth_key<PER>(key, kTopMost, k, reach);
+                // entries equal to the bound count: dropped is what is not above the key before it (that of -0 is no value's: the one before that)
+                low = low == 0u ? 0u : low == 0x80000000u ? low - 2u : low - 1u;
+                if (lane == 0) { bound[col] = value_of_key(low); }
+            }
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < W; ++j) { drop[j] = bound[tx * W + j]; }
+        }
+        // What is left goes to the lists, in any order.  All held channels at once; where a list would overflow they are taken back and appended with one load of channels
+        // at a time, each time cutting the lists that might not hold the next.
+        if (threadIdx.x < COLS) { before[threadIdx.x] = count[threadIdx.x]; }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) {
+            int const row = from + i * ROWS + ty;
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                if (row < end && j < u.live && !(v[i][j] <= drop[j])) {
+                    int const col = tx * W + j, at = atomicAdd(&count[col], 1);
+                    if (at < LIST) { list[col][at] = entry_of(order_key(v[i][j]), row); } else { over = 1; }
+                }
+            }
+        }
+        __syncthreads();
+        bool cut = from + HELD * ROWS < end;                                    // more to come: raise the bounds
+        if (over != 0) {                                                        // workgroup-uniform
+            __syncthreads();
+            if (threadIdx.x < COLS) { count[threadIdx.x] = before[threadIdx.x]; }
+            if (threadIdx.x == 0) { over = 0; }
+            // (the lists hold at most kTopMost entries here: those of the channels before were cut)
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < HELD; ++i) {
+                int const row = from + i * ROWS + ty;
+#pragma unroll
+                for (int j = 0; j < W; ++j) {
+                    if (row < end && j < u.live && !(v[i][j] <= drop[j])) {
+                        int const col = tx * W + j, at = atomicAdd(&count[col], 1);
+                        list[col][at] = entry_of(order_key(v[i][j]), row);
+                        if (at >= kTopMost) { full[i % 3] = 1; }                // the next channels might not fit
                     }
-                    wave_fence();
-                    uint32_t const low = select_largest<PER>(ks, is, entries, k, a.c.rows, key[wave], index[wave]);
-                    if (lane == 0) { count[wave] = k; bound[wave] = value_of_key(low); }
                 }
                 __syncthreads();
+                // (three flags in turn: the one read now is written again three loads on, and cleared behind the next barrier, which no one passes before all have read it)
+                bool const some = full[i % 3] != 0;
+                if (threadIdx.x == 0) { full[(i + 2) % 3] = 0; }
+                if (some) {                                                     // workgroup-uniform
+                    for (int col = wave; col < COLS; col += WAVES) {
+                        int const entries = count[col];
+                        if (entries > kTopMost) {
+                            uint32_t const low = cut_list<LIST>(list[col], entries, k, a.c.rows);
+                            if (lane == 0) { count[col] = k; bound[col] = value_of_key(low); }
+                        }
+                        else if (lane == 0) { bound[col] = __builtin_nanf(""); }
+                    }
+                    __syncthreads();
 #pragma unroll
-                for (int j = 0; j < W; ++j) { drop[j] = bound[tx * W + j]; }
+                    for (int j = 0; j < W; ++j) {
+                        float const b = bound[tx * W + j];
+                        if (b == b) { drop[j] = b; }
+                    }
+                }
+            }
+            __syncthreads();
+            if (threadIdx.x < 3) { full[threadIdx.x] = 0; }
+        }
+        if (cut) {                                                              // workgroup-uniform
+            for (int col = wave; col < COLS; col += WAVES) {
+                int const entries = count[col];
+                float low = __builtin_nanf("");
+                if (entries > k) {
+                    low = value_of_key(cut_list<LIST>(list[col], entries, k, a.c.rows));
+                    if (lane == 0) { count[col] = k; }
+                }
+                if (lane == 0) { bound[col] = low; }
+            }
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                float const b = bound[tx * W + j];
+                if (b == b) { drop[j] = b; }                                    // (a bound that is not a number, or none: the one before stays)
             }
         }
     }
-    if (wave < COLS) {
-        constexpr int PER = kTopList / kWave;
-        int entries = count[wave];
+    for (int col = wave; col < COLS; col += WAVES) {
+        int entries = count[col];
+        ColumnUnit<W> const of(a.c, tile * TX + col / W);
+        if (col % W >= of.live) { continue; }                                 // wave-uniform
         if (entries > k) {
-            uint32_t ks[PER];
-            int is[PER];
-#pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                int const e = i * kWave + lane;
-                ks[i] = e < entries ? key[wave][e] : 0u;
-                is[i] = e < entries ? index[wave][e] : 0;
-            }
-            wave_fence();
-            (void)select_largest<PER>(ks, is, entries, k, a.c.rows, key[wave], index[wave]);
-            wave_fence();
+            (void)cut_list<LIST>(list[col], entries, k, a.c.rows);
             entries = k;
         }
-        ColumnUnit<W> const mine(a.c, tile * TX + wave / W);
-        if (wave % W < mine.live) {
-            if (a.c.slabs > 1) {
-                uint2 *const to = a.candidates + ((size_t)slab * (a.c.units * W) + mine.column + wave % W) * k;
-                for (int e = lane; e < k; e += kWave) { to[e] = e < entries ? make_uint2(key[wave][e], (uint32_t)index[wave][e]) : make_uint2(0u, 0u); }    // (key 0: below every value)
-            }
-            else {
-                order_entries(key[wave], index[wave], k);
-                if (DRAW) {
-                    size_t const at = (size_t)mine.pix * a.frame_stride + mine.f0 + wave % W;
-                    int category;
-                    float share;
-                    draw_category(key[wave], index[wave], k, a.u[at], a.temperature, a.top_p, a.min_p, category, share);
-                    if (lane == 0) {
-                        a.category[at] = category;
-                        if (a.share != nullptr) { a.share[at] = share; }
-                    }
-                }
-            }
+        if (a.c.slabs > 1) {
+            uint64_t *const to = a.candidates + ((size_t)slab * (a.c.units * W) + of.column + col % W) * k;
+            for (int e = lane; e < k; e += kWave) { to[e] = e < entries ? list[col][e] : 0u; }          // (0: below every entry)
+        }
+        else {
+            order_list(list[col], k);
+            if (DRAW) { draw_category(a, list[col], (size_t)of.pix * a.frame_stride + of.f0 + col % W); }
         }
     }
     if (!DRAW && a.c.slabs == 1) {
         __syncthreads();
-        for (int e = threadIdx.x; e < k * COLS; e += kTopChunk * TX) {          // neighbouring columns side by side
+        for (int e = threadIdx.x; e < k * COLS; e += BLOCK) {                   // neighbouring columns side by side
             int const col = e % COLS, j = e / COLS;
             ColumnUnit<W> const of(a.c, tile * TX + col / W);
             if (col % W < of.live) {
                 size_t const at = ((size_t)j * a.pix_size + of.pix) * a.list_stride + of.f0 + col % W;
-                a.index[at] = index[col][j];
-                a.logit[at] = value_of_key(key[col][j]);
+                a.index[at] = channel_of(list[col][j]);
+                a.logit[at] = value_of_key(key_of(list[col][j]));
             }
         }
     }
@@ -298,43 +394,83 @@ __global__ __launch_bounds__(kTopChunk * TX) void top_logits_scan_kernel(TopArgs
 template <int W, bool DRAW>
 __global__ __launch_bounds__(kColBlock) void top_logits_join_kernel(TopArgs a)
 {
-    constexpr int PER = kTopJoin / kWave;
-    __shared__ uint32_t key[kColWaves][kTopMost];
-    __shared__ int index[kColWaves][kTopMost];
+    __shared__ uint64_t list[kColWaves][kTopJoin];
     int const lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, k = a.top_size, n = a.c.slabs * k;
     int const column = blockIdx.x * kColWaves + wave;
     ColumnUnit<W> const u(a.c, column / W);
     if (column % W >= u.live) { return; }                                       // (wavefronts of this kernel do not meet)
-    uint32_t ks[PER];
-    int is[PER];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        int const e = i * kWave + lane;
-        uint2 v = make_uint2(0u, 0u);
-        if (e < n) {
-            int const slab = e / k;
-            v = a.candidates[((size_t)slab * (a.c.units * W) + column) * k + (e - slab * k)];
-        }
-        ks[i] = v.x; is[i] = (int)v.y;
+    for (int e = lane; e < n; e += kWave) {
+        int const slab = e / k;
+        list[wave][e] = a.candidates[((size_t)slab * (a.c.units * W) + column) * k + (e - slab * k)];
     }
-    (void)select_largest<PER>(ks, is, n, k, a.c.rows, key[wave], index[wave]);
     wave_fence();
-    order_entries(key[wave], index[wave], k);
-    if (DRAW) {
-        size_t const at = (size_t)u.pix * a.frame_stride + u.f0 + column % W;
-        int category;
-        float share;
-        draw_category(key[wave], index[wave], k, a.u[at], a.temperature, a.top_p, a.min_p, category, share);
-        if (lane == 0) {
-            a.category[at] = category;
-            if (a.share != nullptr) { a.share[at] = share; }
-        }
-    }
+    (void)cut_list<kTopJoin>(list[wave], n, k, a.c.rows);
+    order_list(list[wave], k);
+    if (DRAW) { draw_category(a, list[wave], (size_t)u.pix * a.frame_stride + u.f0 + column % W); }
     else {
         for (int j = lane; j < k; j += kWave) {
             size_t const at = ((size_t)j * a.pix_size + u.pix) * a.list_stride + u.f0 + column % W;
-            a.index[at] = index[wave][j];
-            a.logit[at] = value_of_key(key[wave][j]);
+            a.index[at] = channel_of(list[wave][j]);
+            a.logit[at] = value_of_key(key_of(list[wave][j]));
+        }
+    }
+}
+
+// Few channels (at most MOST): a lane takes a column, its keys in registers, and finds one entry after the other.
+template <int MOST, bool DRAW>
+__global__ __launch_bounds__(kWave) void top_logits_few_kernel(TopArgs a)
+{
+    __shared__ float value[DRAW ? MOST : 1][kWave];
+    __shared__ int which[DRAW ? MOST : 1][kWave];
+    int const lane = threadIdx.x, column = blockIdx.x * kWave + lane, k = a.top_size;
+    ColumnUnit<1> const u(a.c, column);
+    size_t const channel = (size_t)a.pix_size * a.frame_stride, at = (size_t)u.pix * a.frame_stride + u.f0;
+    uint32_t key[MOST];
+#pragma unroll
+    for (int i = 0; i < MOST; ++i) { key[i] = i < a.c.rows ? order_key(a.y[at + i * channel]) : 0u; }           // (a lane without a column: the first one's)
+    for (int j = 0; j < k; ++j) {
+        uint32_t top = 0u;
+        int found = 0;
+#pragma unroll
+        for (int i = 0; i < MOST; ++i) {
+            if (key[i] > top) { top = key[i]; found = i; }
+        }
+#pragma unroll
+        for (int i = 0; i < MOST; ++i) { key[i] = i == found ? 0u : key[i]; }
+        if (DRAW) { value[j][lane] = value_of_key(top); which[j][lane] = found; }
+        else if (u.live > 0) {
+            size_t const to = ((size_t)j * a.pix_size + u.pix) * a.list_stride + u.f0;
+            a.index[to] = found;
+            a.logit[to] = value_of_key(top);
+        }
+    }
+    if (DRAW) {
+        float const z0 = value[0][lane];
+        auto weight = [&](int j) { float const z = value[j][lane]; return z == z0 ? 1.0 : exp(((double)z - (double)z0) / (double)a.temperature); };
+        int category = -1;
+        float share = 0.0f;
+        if (z0 > -__builtin_inff()) {
+            double all = 0.0, total = 0.0, sum = 0.0, w = 1.0;
+            if (a.top_p < 1.0f) { for (int j = 0; j < k; ++j) { all += weight(j); } }
+            int kept = 0;
+            for (; kept < k; ++kept) {
+                w = weight(kept);
+                if (kept > 0 && !(w > 0.0 && w >= (double)a.min_p && (a.top_p >= 1.0f || total < (double)a.top_p * all))) { break; }
+                total += w;
+            }
+            double const reach = (double)a.u[at] * total;
+            int drawn = 0;
+            for (; ; ++drawn) {
+                w = weight(drawn);
+                sum += w;
+                if (drawn == kept - 1 || !(sum <= reach)) { break; }
+            }
+            category = which[drawn][lane];
+            share = (float)(w / total);
+        }
+        if (u.live > 0) {
+            a.category[at] = category;
+            if (a.share != nullptr) { a.share[at] = share; }
         }
     }
 }

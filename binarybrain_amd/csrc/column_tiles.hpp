@@ -63,7 +63,8 @@ __device__ __forceinline__ void column_store(float *__restrict__ p, int live, fl
 {
     if constexpr (W == 4) {
         if (live == 4) {
-            *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
+            using V = float __attribute__((ext_vector_type(4)));
+            __builtin_nontemporal_store(V{v[0], v[1], v[2], v[3]}, reinterpret_cast<V *>(p));
             return;
         }
     }
@@ -71,18 +72,9 @@ __device__ __forceinline__ void column_store(float *__restrict__ p, int live, fl
     for (int j = 0; j < W; ++j) { if (j < live) { p[j] = v[j]; } }
 }
 
-// v of the lane `o` lanes away (o a power of two, wave-uniform)
-__device__ __forceinline__ float lane_xor_any(float v, int o)
-{
-    switch (o) {
-    case 1:  return lane_xor(v, 1);
-    case 2:  return lane_xor(v, 2);
-    case 4:  return lane_xor(v, 4);
-    case 8:  return lane_xor(v, 8);
-    case 16: return lane_xor(v, 16);
-    default: return lane_xor(v, 32);
-    }
-}
+// A second launch over the same data goes through it backwards (`block` of ColumnThread counted from the end): what the first launch read last is still in
+// the 256 MiB memory-side cache.
+__device__ __forceinline__ int backwards(int block, int blocks) { return blocks - 1 - block; }
 
 // where a thread of a workgroup stands: one unit, rows begin + lead, + step, ... below end of its slab
 template <int W>

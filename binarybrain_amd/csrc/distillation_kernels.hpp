@@ -60,11 +60,14 @@ template <int W>
 __device__ __forceinline__ void join_workgroup(float (&m)[W], float (&s)[W], int log_tx, float scale, float *share)
 {
     int const lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, tx = lane & ((1 << log_tx) - 1);
-    for (int o = 1 << log_tx; o < kWave; o <<= 1) {
-        float om[W], os[W];
 #pragma unroll
-        for (int j = 0; j < W; ++j) { om[j] = lane_xor_any(m[j], o); os[j] = lane_xor_any(s[j], o); }
-        join_sums<W>(m, s, om, os, scale);
+    for (int o = 1; o < kWave; o <<= 1) {
+        if (o >= 1 << log_tx) {                                                 // workgroup-uniform
+            float om[W], os[W];
+#pragma unroll
+            for (int j = 0; j < W; ++j) { om[j] = lane_xor(m[j], o); os[j] = lane_xor(s[j], o); }
+            join_sums<W>(m, s, om, os, scale);
+        }
     }
     float *const s_m = share, *const s_s = share + kColShareMax;
     if (lane < (1 << log_tx)) {
@@ -220,7 +223,7 @@ __global__ __launch_bounds__(kColBlock) void distillation_gradient_kernel(Distil
 {
     __shared__ float share[2 * kColShareMax];
     __shared__ float of_m[kWave * W], of_s[kWave * W], of_k[kWave * W];         // per column: reference, 1 / sum, w T / weight_sum (0: nothing to learn)
-    ColumnThread<W> const t(a.c, a.tiles, blockIdx.x, gridDim.x);
+    ColumnThread<W> const t(a.c, a.tiles, backwards(blockIdx.x, gridDim.x), gridDim.x);
     ColumnUnit<W> const u(a.c, (t.tile << a.c.log_tx) + t.tx);
     int const part = (int)threadIdx.x >> a.c.log_tx, parts = kColBlock >> a.c.log_tx;
     size_t const channel = (size_t)a.pix_size * a.frame_stride, place = (size_t)u.pix * a.frame_stride + u.f0;

@@ -70,12 +70,15 @@ template <int W>
 __device__ __forceinline__ void merge_workgroup(Moments<W> &m, int log_tx, float *share)
 {
     int const lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, tx = lane & ((1 << log_tx) - 1);
-    for (int o = 1 << log_tx; o < kWave; o <<= 1) {
-        float om[W], o2[W];
-        float const on = lane_xor_any(m.n, o);
 #pragma unroll
-        for (int j = 0; j < W; ++j) { om[j] = lane_xor_any(m.mean[j], o); o2[j] = lane_xor_any(m.m2[j], o); }
-        m.merge(on, om, o2);
+    for (int o = 1; o < kWave; o <<= 1) {
+        if (o >= 1 << log_tx) {                                                 // workgroup-uniform
+            float om[W], o2[W];
+            float const on = lane_xor(m.n, o);
+#pragma unroll
+            for (int j = 0; j < W; ++j) { om[j] = lane_xor(m.mean[j], o); o2[j] = lane_xor(m.m2[j], o); }
+            m.merge(on, om, o2);
+        }
     }
     float *const s_mean = share, *const s_m2 = share + kColShareMax, *const s_n = share + 2 * kColShareMax;
     if (lane < (1 << log_tx)) {
@@ -99,9 +102,12 @@ template <int W>
 __device__ __forceinline__ void add_workgroup(float (&a)[W], float (&b)[W], int log_tx, float *share)
 {
     int const lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, tx = lane & ((1 << log_tx) - 1);
-    for (int o = 1 << log_tx; o < kWave; o <<= 1) {
 #pragma unroll
-        for (int j = 0; j < W; ++j) { a[j] += lane_xor_any(a[j], o); b[j] += lane_xor_any(b[j], o); }
+    for (int o = 1; o < kWave; o <<= 1) {
+        if (o >= 1 << log_tx) {                                                 // workgroup-uniform
+#pragma unroll
+            for (int j = 0; j < W; ++j) { a[j] += lane_xor(a[j], o); b[j] += lane_xor(b[j], o); }
+        }
     }
     float *const s_a = share, *const s_b = share + kColShareMax;
     if (lane < (1 << log_tx)) {
@@ -193,7 +199,7 @@ template <int W, bool BIT>
 __global__ __launch_bounds__(kColBlock) void layer_norm_apply_kernel(LayerNormArgs a)
 {
     __shared__ float share[2 * kColShareMax + kColWaves * kWave];
-    ColumnThread<W> const t(a.c, a.tiles, blockIdx.x, gridDim.x);
+    ColumnThread<W> const t(a.c, a.tiles, backwards(blockIdx.x, gridDim.x), gridDim.x);
     ColumnUnit<W> const u(a.c, (t.tile << a.c.log_tx) + t.tx);
     int const part = (int)threadIdx.x >> a.c.log_tx, parts = kColBlock >> a.c.log_tx;
     Moments<W> m;
@@ -291,9 +297,12 @@ __global__ __launch_bounds__(kColBlock) void layer_norm_backward_sums_kernel(Lay
             }
         }
         if (a.row_partial != nullptr) {
-            for (int o = 1; o < (1 << a.c.log_tx); o <<= 1) {
 #pragma unroll
-                for (int i = 0; i < B; ++i) { s1[i] += lane_xor_any(s1[i], o); s2[i] += lane_xor_any(s2[i], o); }
+            for (int o = 1; o < kWave; o <<= 1) {
+                if (o < 1 << a.c.log_tx) {                                      // workgroup-uniform
+#pragma unroll
+                    for (int i = 0; i < B; ++i) { s1[i] += lane_xor(s1[i], o); s2[i] += lane_xor(s2[i], o); }
+                }
             }
             if (t.tx == 0) {
 #pragma unroll
@@ -336,7 +345,7 @@ __global__ __launch_bounds__(kColBlock) void layer_norm_backward_apply_kernel(La
         }
         return;
     }
-    ColumnThread<W> const t(a.c, a.tiles, blockIdx.x, a.main_blocks);
+    ColumnThread<W> const t(a.c, a.tiles, backwards(blockIdx.x, a.main_blocks), a.main_blocks);
     ColumnUnit<W> const u(a.c, (t.tile << a.c.log_tx) + t.tx);
     int const part = (int)threadIdx.x >> a.c.log_tx, parts = kColBlock >> a.c.log_tx;
     float mean[W], rstd[W], c1[W] = {}, c2[W] = {};

@@ -2630,6 +2630,7 @@ static int top_space(TopArgs &a, bool wide, int top_size, int pix_size, int ch_s
     top_split(a.c.units, ch_size, top_size, a.c.log_tx, a.c.tiles, a.c.slab_rows, a.c.slabs);
     if ((long long)a.c.tiles * a.c.slabs > 0x3fffffffLL) { return fail("%s: grid too large", name); }
     a.tiles = make_tile_divisor(a.c.tiles);
+    a.entries = make_tile_divisor(top_size);
     return 0;
 }
 

@@ -30,7 +30,7 @@ template <int TX> constexpr int kTopList = kTopMost + kTopRows<TX>;
 
 struct TopArgs {
     ColumnSpace c;                  // rows = channels
-    TileDivisor tiles;
+    TileDivisor tiles, entries;     // entries: top_size
     float const *y;
     int         *index;             // top logits: [top * pix][list_stride]
     float       *logit;
@@ -60,19 +60,27 @@ __device__ __forceinline__ uint64_t entry_of(uint32_t key, int channel) { return
 __device__ __forceinline__ uint32_t key_of(uint64_t entry)              { return (uint32_t)(entry >> 32); }
 __device__ __forceinline__ int      channel_of(uint64_t entry)          { return (int)~(uint32_t)entry; }
 
-// The k-th largest of n >= k keys, key i * 64 + lane in register i: bit by bit from the top, the keys that reach a candidate counted by ballots.  `reach`: how many keys
-// reach the returned bound; k where the search could stop early, and then the bound itself need not be a key.  A whole wavefront calls this.
+// The k-th largest of n >= k keys, key i * 64 + lane in register i (0 behind them): bit by bit from the top, the keys that reach a candidate counted by ballots; bits
+// that all keys agree in are passed over.  `reach`: how many keys reach the returned bound; k where the search could stop early, and then the bound itself need not be a
+// key.  A whole wavefront calls this.
 template <int PER>
 __device__ __forceinline__ uint32_t kth_key(uint32_t const (&key)[PER], int n, int k, int &reach)
 {
     int const lane = threadIdx.x % kWave;
-    uint32_t bound = 0u;
+    uint32_t const one = (uint32_t)__builtin_amdgcn_readfirstlane((int)key[0]);
+    uint32_t differ = 0u;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) { differ |= i * kWave + lane < n ? key[i] ^ one : 0u; }
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) { differ |= lane_xor(differ, o); }
+    uint32_t open = (uint32_t)__builtin_amdgcn_readfirstlane((int)differ), bound = one & ~open;
     reach = n;
-    for (int bit = 31; bit >= 0 && reach != k; --bit) {
-        uint32_t const candidate = bound | (1u << bit);
+    while (open != 0u && reach != k) {
+        uint32_t const bit = 0x80000000u >> __clz((int)open), candidate = bound | bit;
+        open &= ~bit;
         int count = 0;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) { count += __popcll(__ballot(i * kWave + lane < n && key[i] >= candidate)); }
+        for (int i = 0; i < PER; ++i) { count += __popcll(__ballot(key[i] >= candidate)); }
         if (count >= k) { bound = candidate; reach = count; }
     }
     return bound;
@@ -92,26 +100,26 @@ __device__ __forceinline__ uint32_t cut_list_of(uint64_t *list, int n, int k, in
         key[i] = key_of(v); channel[i] = channel_of(v);
     }
     wave_fence();
-    uint32_t const bound = kth_key<PER>(key, n, k, reach);
+    uint32_t const bound = kth_key<PER>(key, n, k, reach);                      // (above 0: so is every key, and what is behind the list is not taken)
     int last = rows;                                                            // of the entries that equal the bound, those up to here
     if (reach != k) {                                                           // (bound is the k-th largest key, and more than k entries reach it)
         int above = 0;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) { above += __popcll(__ballot(i * kWave + lane < n && key[i] > bound)); }
+        for (int i = 0; i < PER; ++i) { above += __popcll(__ballot(key[i] > bound)); }
         int const wanted = k - above;                                           // >= 1
         last = 0;
         for (int bit = 31 - __clz(rows); bit >= 0; --bit) {                     // the wanted-th smallest channel
             int const candidate = last | (1 << bit);
             int count = 0;
 #pragma unroll
-            for (int i = 0; i < PER; ++i) { count += __popcll(__ballot(i * kWave + lane < n && key[i] == bound && channel[i] < candidate)); }
+            for (int i = 0; i < PER; ++i) { count += __popcll(__ballot(key[i] == bound && channel[i] < candidate)); }
             if (count < wanted) { last = candidate; }
         }
     }
     int base = 0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-        bool const taken = i * kWave + lane < n && (key[i] > bound || (key[i] == bound && channel[i] <= last));
+        bool const taken = key[i] > bound || (key[i] == bound && channel[i] <= last);
         uint64_t const mask = __ballot(taken);
         if (taken) { list[base + bits_below_lane(mask)] = entry_of(key[i], channel[i]); }
         base += __popcll(mask);
@@ -251,8 +259,8 @@ __global__ __launch_bounds__(kTopRows<TX> * TX, 4) void top_logits_scan_kernel(T
     if (threadIdx.x == 0) { over = 0; }
     if (threadIdx.x < 3) { full[threadIdx.x] = 0; }
 
+    request(begin);
     for (int from = begin; from < end; from += HELD * ROWS) {
-        request(from);
         if (from == begin && end - begin >= 2 * kTopMost) {
             // the k-th largest of the maxima of kTopMost groups of channels: as many entries are no smaller, so it bounds the k-th largest entry from below, and hardly more than
             // k entries reach it where the groups are many against k
@@ -287,19 +295,36 @@ __global__ __launch_bounds__(kTopRows<TX> * TX, 4) void top_logits_scan_kernel(T
         // at a time, each time cutting the lists that might not hold the next.
         if (threadIdx.x < COLS) { before[threadIdx.x] = count[threadIdx.x]; }
         __syncthreads();
+        // (one request for a place per thread and column, for all that it has)
+        int at[W];
+        bool any = false;
 #pragma unroll
-        for (int i = 0; i < HELD; ++i) {
-            int const row = from + i * ROWS + ty;
+        for (int j = 0; j < W; ++j) {
+            int mine_of = 0;
 #pragma unroll
-            for (int j = 0; j < W; ++j) {
-                if (row < end && j < u.live && !(v[i][j] <= drop[j])) {
-                    int const col = tx * W + j, at = atomicAdd(&count[col], 1);
-                    if (at < LIST) { list[col][at] = entry_of(order_key(v[i][j]), row); } else { over = 1; }
+            for (int i = 0; i < HELD; ++i) { mine_of += from + i * ROWS + ty < end && !(v[i][j] <= drop[j]) ? 1 : 0; }
+            mine_of = j < u.live ? mine_of : 0;
+            at[j] = LIST;
+            if (mine_of > 0) {
+                any = true;
+                at[j] = atomicAdd(&count[tx * W + j], mine_of);
+                if (at[j] + mine_of > LIST) { over = 1; }
+            }
+        }
+        if (any) {
+#pragma unroll
+            for (int i = 0; i < HELD; ++i) {
+                int const row = from + i * ROWS + ty;
+#pragma unroll
+                for (int j = 0; j < W; ++j) {
+                    if (row < end && !(v[i][j] <= drop[j])) {
+                        if (at[j] < LIST) { list[tx * W + j][at[j]] = entry_of(order_key(v[i][j]), row); }
+                        at[j] += 1;
+                    }
                 }
             }
         }
         __syncthreads();
-        bool cut = from + HELD * ROWS < end;                                    // more to come: raise the bounds
         if (over != 0) {                                                        // workgroup-uniform
             __syncthreads();
             if (threadIdx.x < COLS) { count[threadIdx.x] = before[threadIdx.x]; }
@@ -341,11 +366,13 @@ __global__ __launch_bounds__(kTopRows<TX> * TX, 4) void top_logits_scan_kernel(T
             __syncthreads();
             if (threadIdx.x < 3) { full[threadIdx.x] = 0; }
         }
-        if (cut) {                                                              // workgroup-uniform
+        if (from + HELD * ROWS < end) {
+            // (more to come: lists that hold more than kTopMost entries are cut, which also raises their bounds.  The next channels are on their way meanwhile)
+            request(from + HELD * ROWS);
             for (int col = wave; col < COLS; col += WAVES) {
                 int const entries = count[col];
                 float low = __builtin_nanf("");
-                if (entries > k) {
+                if (entries > kTopMost) {
                     low = value_of_key(cut_list<LIST>(list[col], entries, k, a.c.rows));
                     if (lane == 0) { count[col] = k; }
                 }
@@ -399,9 +426,17 @@ __global__ __launch_bounds__(kColBlock) void top_logits_join_kernel(TopArgs a)
     int const column = blockIdx.x * kColWaves + wave;
     ColumnUnit<W> const u(a.c, column / W);
     if (column % W >= u.live) { return; }                                       // (wavefronts of this kernel do not meet)
-    for (int e = lane; e < n; e += kWave) {
-        int const slab = e / k;
-        list[wave][e] = a.candidates[((size_t)slab * (a.c.units * W) + column) * k + (e - slab * k)];
+    uint64_t v[kTopJoin / kWave];
+#pragma unroll
+    for (int i = 0; i < kTopJoin / kWave; ++i) {                                // (all requested before the first is waited for)
+        int const e = i * kWave + lane < n ? i * kWave + lane : 0;
+        int slab, j;
+        split_tile(e, a.entries, slab, j);
+        v[i] = a.candidates[((size_t)slab * (a.c.units * W) + column) * k + j];
+    }
+#pragma unroll
+    for (int i = 0; i < kTopJoin / kWave; ++i) {
+        if (i * kWave + lane < n) { list[wave][i * kWave + lane] = v[i]; }
     }
     wave_fence();
     (void)cut_list<kTopJoin>(list[wave], n, k, a.c.rows);
@@ -425,9 +460,12 @@ __global__ __launch_bounds__(kWave) void top_logits_few_kernel(TopArgs a)
     int const lane = threadIdx.x, column = blockIdx.x * kWave + lane, k = a.top_size;
     ColumnUnit<1> const u(a.c, column);
     size_t const channel = (size_t)a.pix_size * a.frame_stride, at = (size_t)u.pix * a.frame_stride + u.f0;
+    float v[MOST];
     uint32_t key[MOST];
 #pragma unroll
-    for (int i = 0; i < MOST; ++i) { key[i] = i < a.c.rows ? order_key(a.y[at + i * channel]) : 0u; }           // (a lane without a column: the first one's)
+    for (int i = 0; i < MOST; ++i) { v[i] = a.y[at + (i < a.c.rows ? i : 0) * channel]; }                       // (a lane without a column: the first one's)
+#pragma unroll
+    for (int i = 0; i < MOST; ++i) { key[i] = i < a.c.rows ? order_key(v[i]) : 0u; }
     for (int j = 0; j < k; ++j) {
         uint32_t top = 0u;
         int found = 0;

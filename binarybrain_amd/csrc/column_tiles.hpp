@@ -25,10 +25,10 @@ struct ColumnSpace {
     int rows, slab_rows, slabs;     // rows = nodes or channels
 };
 
-// the unit of a lane: where it lies in its row block and how many of its W frames exist (live 0: no such unit; it may load the first one, whose `span` frames exist)
+// the unit of a lane: where it lies in its row block and how many of its W frames exist (live 0: no such unit; it loads the first one)
 template <int W>
 struct ColumnUnit {
-    int pix, f0, live, span, column;        // column: of its first frame, in the compact order of units
+    int pix, f0, live, column;      // column: of its first frame, in the compact order of units
     __device__ __forceinline__ ColumnUnit(ColumnSpace const &c, int unit)
     {
         bool const in = unit < c.units;
@@ -36,26 +36,28 @@ struct ColumnUnit {
         int q;
         split_tile(u, c.units_per_row, pix, q);
         f0     = q * W;
-        span   = c.frame_size - f0 < W ? c.frame_size - f0 : W;
-        live   = in ? span : 0;
+        live   = in ? (c.frame_size - f0 < W ? c.frame_size - f0 : W) : 0;
         column = u * W;
     }
 };
 
-// W frames at p, the absent ones 0 (nothing behind the last frame is read)
-template <int W, class E>
-__device__ __forceinline__ void column_load(E const *__restrict__ p, int live, E (&v)[W])
+// W frames at p.  Whole: where the last unit of a row is not, what lies behind the frames is read too (a row's pitch is a multiple of W) and counts for nothing.
+template <int W>
+__device__ __forceinline__ void column_load(float const *__restrict__ p, float (&v)[W])
 {
     if constexpr (W == 4) {
-        if (live == 4) {
-            using V = std::conditional_t<std::is_same_v<E, float>, float4, int4>;
-            V const t = *reinterpret_cast<V const *>(p);
-            v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
-            return;
-        }
+        float4 const t = *reinterpret_cast<float4 const *>(p);
+        v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
     }
+    else { v[0] = p[0]; }
+}
+
+// the same of an array that ends with its last frame: the absent ones 0
+template <int W>
+__device__ __forceinline__ void line_load(float const *__restrict__ p, int live, float (&v)[W])
+{
 #pragma unroll
-    for (int j = 0; j < W; ++j) { v[j] = j < live ? p[j] : E(0); }
+    for (int j = 0; j < W; ++j) { v[j] = j < live ? p[j] : 0.0f; }
 }
 
 template <int W>

@@ -192,9 +192,8 @@ __global__ __launch_bounds__(kColBlock) void distillation_sums_kernel(DistillArg
         float v[B][W];
 #pragma unroll
         for (int i = 0; i < B; ++i) {
-            bool const in = whole || base + t.lead + i * t.step < t.end;
-            column_load<W>(y + (size_t)(base + i * t.step) * channel, in ? u.span : 0, v[i]);
-            if (!in) {
+            if (whole || base + t.lead + i * t.step < t.end) { column_load<W>(y + (size_t)(base + i * t.step) * channel, v[i]); }
+            else {
 #pragma unroll
                 for (int j = 0; j < W; ++j) { v[i][j] = -__builtin_inff(); }
             }
@@ -269,8 +268,7 @@ __global__ __launch_bounds__(kColBlock) void distillation_gradient_kernel(Distil
         float v[B][W];
 #pragma unroll
         for (int i = 0; i < B; ++i) {
-            bool const in = whole || base + t.lead + i * t.step < t.end;
-            column_load<W>(y + (size_t)(base + i * t.step) * channel, in ? u.span : 0, v[i]);
+            if (whole || base + t.lead + i * t.step < t.end) { column_load<W>(y + (size_t)(base + i * t.step) * channel, v[i]); }
         }
 #pragma unroll
         for (int i = 0; i < B; ++i) {

@@ -271,7 +271,7 @@ inline void column_split(int units, int rows, bool wide, int batch, int &log_tx,
     slabs = ceil_div(rows, slab_rows);
 }
 
-// The same for the selection of the largest logits: tiles of four units or of one, slabs of whole loads (what the threads hold at a time: 12 channels of each column), of which the second launch can
+// The same for the selection of the largest logits: tiles of four units or of one, slabs of multiples of 1024 channels, of which the second launch can
 // select from 1024 / top_size at most.
 inline void top_split(int units, int channels, int top_size, int &log_tx, int &tiles, int &slab_rows, int &slabs)
 {
@@ -279,7 +279,7 @@ inline void top_split(int units, int channels, int top_size, int &log_tx, int &t
     tiles = ceil_div(units, 1 << log_tx);
     int want = ceil_div(512, tiles);
     if (want > 1024 / top_size) { want = 1024 / top_size; }
-    int const load = log_tx ? 1536 : 3072, loads = ceil_div(channels, load);
+    int const load = 1024, loads = ceil_div(channels, load);
     slab_rows = ceil_div(loads, want < loads ? want : loads) * load;
     slabs = ceil_div(channels, slab_rows);
 }

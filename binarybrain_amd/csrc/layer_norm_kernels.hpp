@@ -35,14 +35,14 @@ struct LayerNormArgs {
 
 // W values of row `r` of a unit
 template <int W, bool BIT>
-__device__ __forceinline__ void layer_norm_load(void const *__restrict__ x, int stride, int r, int f0, int span, float (&v)[W])
+__device__ __forceinline__ void layer_norm_load(void const *__restrict__ x, int stride, int r, int f0, float (&v)[W])
 {
     if constexpr (BIT) {
         uint32_t const word = static_cast<uint32_t const *>(x)[(size_t)r * stride + (f0 >> 5)] >> (f0 & 31);
 #pragma unroll
         for (int j = 0; j < W; ++j) { v[j] = (float)((word >> j) & 1u); }
     }
-    else { column_load<W, float>(static_cast<float const *>(x) + (size_t)r * stride + f0, span, v); }
+    else { column_load<W>(static_cast<float const *>(x) + (size_t)r * stride + f0, v); }
 }
 
 // count, mean and squared deviation of W columns
@@ -143,7 +143,7 @@ __global__ __launch_bounds__(kColBlock) void layer_norm_stats_kernel(LayerNormAr
 #pragma unroll
             for (int i = 0; i < B; ++i) {
                 int const row = base + t.lead + i * t.step;
-                layer_norm_load<W, true>(a.x, a.x_stride, whole || row < t.end ? row : t.begin, u.f0, u.span, v[i]);
+                layer_norm_load<W, true>(a.x, a.x_stride, whole || row < t.end ? row : t.begin, u.f0, v[i]);
             }
 #pragma unroll
             for (int i = 0; i < B; ++i) {
@@ -166,7 +166,7 @@ __global__ __launch_bounds__(kColBlock) void layer_norm_stats_kernel(LayerNormAr
             for (int i = 0; i < B; ++i) {
                 int const row = base + t.lead + i * t.step;
                 bool const in = whole || row < t.end;
-                layer_norm_load<W, false>(a.x, a.x_stride, in ? row : t.begin, u.f0, u.span, v[i]);      // (an absent row: another, which counts for nothing)
+                layer_norm_load<W, false>(a.x, a.x_stride, in ? row : t.begin, u.f0, v[i]);      // (an absent row: another, which counts for nothing)
                 n += in ? 1.0f : 0.0f;
             }
             float const rn = whole ? 1.0f / B : n > 0.0f ? 1.0f / n : 0.0f;
@@ -247,7 +247,7 @@ __global__ __launch_bounds__(kColBlock) void layer_norm_apply_kernel(LayerNormAr
 #pragma unroll
         for (int i = 0; i < B; ++i) {
             int const there = base + t.lead + i * t.step, row = whole || there < t.end ? there : t.begin;
-            layer_norm_load<W, BIT>(a.x, a.x_stride, row, u.f0, u.span, v[i]);
+            layer_norm_load<W, BIT>(a.x, a.x_stride, row, u.f0, v[i]);
             g[i] = a.gamma != nullptr ? a.gamma[row] : 1.0f;
             b[i] = a.beta != nullptr ? a.beta[row] : 0.0f;
         }
@@ -272,24 +272,24 @@ __global__ __launch_bounds__(kColBlock) void layer_norm_backward_sums_kernel(Lay
     ColumnUnit<W> const u(a.c, (t.tile << a.c.log_tx) + t.tx);
     constexpr int B = 4;
     float mean[W], rstd[W], c1[W] = {}, c2[W] = {};
-    column_load<W>(a.mean + u.f0, u.span, mean);
-    column_load<W>(a.rstd + u.f0, u.span, rstd);
+    line_load<W>(a.mean + u.f0, u.live, mean);
+    line_load<W>(a.rstd + u.f0, u.live, rstd);
     t.template each<B>([&](int base, auto whole) {
         float x[B][W], d[B][W], g[B], s1[B], s2[B];
 #pragma unroll
         for (int i = 0; i < B; ++i) {
             int const there = base + t.lead + i * t.step, row = whole || there < t.end ? there : t.begin;
-            layer_norm_load<W, BIT>(a.x, a.x_stride, row, u.f0, u.span, x[i]);
-            column_load<W>(a.dy + (size_t)row * a.out_stride + u.f0, u.span, d[i]);
+            layer_norm_load<W, BIT>(a.x, a.x_stride, row, u.f0, x[i]);
+            column_load<W>(a.dy + (size_t)row * a.out_stride + u.f0, d[i]);
             g[i] = a.gamma != nullptr ? a.gamma[row] : 1.0f;
         }
 #pragma unroll
         for (int i = 0; i < B; ++i) {
-            bool const in = u.live > 0 && (whole || base + t.lead + i * t.step < t.end);     // (what is not there adds nothing)
+            bool const in = whole || base + t.lead + i * t.step < t.end;                // (what is not there adds nothing)
             s1[i] = 0.0f; s2[i] = 0.0f;
 #pragma unroll
             for (int j = 0; j < W; ++j) {
-                float const dj = in ? d[i][j] : 0.0f, xh = in ? (x[i][j] - mean[j]) * rstd[j] : 0.0f, gd = dj * g[i];
+                float const dj = in && j < u.live ? d[i][j] : 0.0f, xh = in && j < u.live ? (x[i][j] - mean[j]) * rstd[j] : 0.0f, gd = dj * g[i];
                 c1[j] += gd;
                 c2[j] = __builtin_fmaf(gd, xh, c2[j]);
                 s1[i] = __builtin_fmaf(dj, xh, s1[i]);
@@ -349,8 +349,8 @@ __global__ __launch_bounds__(kColBlock) void layer_norm_backward_apply_kernel(La
     ColumnUnit<W> const u(a.c, (t.tile << a.c.log_tx) + t.tx);
     int const part = (int)threadIdx.x >> a.c.log_tx, parts = kColBlock >> a.c.log_tx;
     float mean[W], rstd[W], c1[W] = {}, c2[W] = {};
-    column_load<W>(a.mean + u.f0, u.span, mean);
-    column_load<W>(a.rstd + u.f0, u.span, rstd);
+    line_load<W>(a.mean + u.f0, u.live, mean);
+    line_load<W>(a.rstd + u.f0, u.live, rstd);
     for (int s = part; s < a.c.slabs; s += parts) {
         float2 const *const p = a.partial + (size_t)s * (a.c.units * W) + u.column;
 #pragma unroll
@@ -371,8 +371,8 @@ __global__ __launch_bounds__(kColBlock) void layer_norm_backward_apply_kernel(La
 #pragma unroll
         for (int i = 0; i < B; ++i) {
             int const there = base + t.lead + i * t.step, row = whole || there < t.end ? there : t.begin;
-            layer_norm_load<W, BIT>(a.x, a.x_stride, row, u.f0, u.span, x[i]);
-            column_load<W>(a.dy + (size_t)row * a.out_stride + u.f0, u.span, d[i]);
+            layer_norm_load<W, BIT>(a.x, a.x_stride, row, u.f0, x[i]);
+            column_load<W>(a.dy + (size_t)row * a.out_stride + u.f0, d[i]);
             g[i] = a.gamma != nullptr ? a.gamma[row] : 1.0f;
         }
 #pragma unroll

@@ -131,10 +131,9 @@ __device__ __forceinline__ uint32_t cut_list_of(uint64_t *list, int n, int k, in
 template <int MOST>
 __device__ __forceinline__ uint32_t cut_list(uint64_t *list, int n, int k, int rows)
 {
-    if (n <= 2 * kWave) { return cut_list_of<2>(list, n, k, rows); }
     if (n <= 4 * kWave) { return cut_list_of<4>(list, n, k, rows); }
-    if constexpr (MOST > 8 * kWave) { if (n > 8 * kWave) { return cut_list_of<MOST / kWave>(list, n, k, rows); } }
-    return cut_list_of<8>(list, n, k, rows);
+    if constexpr (MOST > 8 * kWave) { if (n <= 8 * kWave) { return cut_list_of<8>(list, n, k, rows); } }
+    return cut_list_of<MOST / kWave>(list, n, k, rows);
 }
 
 // k entries in LDS into their order, by counting for each those before it.  A whole wavefront calls this.
@@ -245,11 +244,11 @@ __global__ __launch_bounds__(kTopRows<TX> * TX, 4) void top_logits_scan_kernel(T
     auto request = [&](int from) {
         if (from + HELD * ROWS <= end) {                                        // workgroup-uniform
 #pragma unroll
-            for (int i = 0; i < HELD; ++i) { column_load<W>(mine + (size_t)(from + i * ROWS) * channel, u.span, v[i]); }
+            for (int i = 0; i < HELD; ++i) { column_load<W>(mine + (size_t)(from + i * ROWS) * channel, v[i]); }
         }
         else {
 #pragma unroll
-            for (int i = 0; i < HELD; ++i) { column_load<W>(mine + (size_t)(from + i * ROWS) * channel, from + i * ROWS + ty < end ? u.span : 0, v[i]); }
+            for (int i = 0; i < HELD; ++i) { if (from + i * ROWS + ty < end) { column_load<W>(mine + (size_t)(from + i * ROWS) * channel, v[i]); } }
         }
     };
     // (not a number drops nothing)
@@ -331,14 +330,15 @@ __global__ __launch_bounds__(kTopRows<TX> * TX, 4) void top_logits_scan_kernel(T
             if (threadIdx.x == 0) { over = 0; }
             // (the lists hold at most kTopMost entries here: those of the channels before were cut)
             __syncthreads();
-#pragma unroll
-            for (int i = 0; i < HELD; ++i) {
+            for (int i = 0; i < HELD; ++i) {                                    // (read again: a loop cannot index registers, and unrolled it would not fit the instruction cache)
                 int const row = from + i * ROWS + ty;
+                float r[W];
+                if (row < end) { column_load<W>(mine + (size_t)(from + i * ROWS) * channel, r); }
 #pragma unroll
                 for (int j = 0; j < W; ++j) {
-                    if (row < end && j < u.live && !(v[i][j] <= drop[j])) {
+                    if (row < end && j < u.live && !(r[j] <= drop[j])) {
                         int const col = tx * W + j, at = atomicAdd(&count[col], 1);
-                        list[col][at] = entry_of(order_key(v[i][j]), row);
+                        list[col][at] = entry_of(order_key(r[j]), row);
                         if (at >= kTopMost) { full[i % 3] = 1; }                // the next channels might not fit
                     }
                 }

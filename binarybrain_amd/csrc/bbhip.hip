@@ -2446,6 +2446,8 @@ size_t bbhip_LayerNormalization_WorkspaceBytes(int node_size, int frame_size)
         ColumnSpace c;
         TileDivisor tiles;
         if (column_space(c, tiles, wide, 1, frame_size, node_size, backward ? kLayerNormBatch / 2 : kLayerNormBatch, __func__)) { return 0; }
+        int log_tx;
+        if (!backward && layer_norm_whole(c.units, node_size, wide, log_tx)) { continue; }
         size_t const bytes = layer_norm_partial_bytes(c, wide) + (backward ? (size_t)c.tiles * node_size * sizeof(float2) : 0);
         most = bytes > most ? bytes : most;
     }
@@ -2463,11 +2465,23 @@ static int layer_norm_forward(void const *x, bool bit, float *y, float const *ga
                       starts_on_16_bytes(mean) && starts_on_16_bytes(rstd);
     LayerNormArgs a{};
     if (column_space(a.c, a.tiles, wide, 1, frame_size, node_size, kLayerNormBatch, name)) { return 1; }
-    if (check_workspace(workspace, workspace_size, layer_norm_partial_bytes(a.c, wide), name)) { return 1; }
     a.x = x; a.out = y; a.gamma = gamma; a.beta = beta; a.mean = mean; a.rstd = rstd; a.eps = eps;
-    a.partial = static_cast<float2 *>(workspace);
     a.x_stride = x_stride; a.out_stride = y_stride;
     hipStream_t const st = static_cast<hipStream_t>(stream);
+    int log_tx;
+    if (layer_norm_whole(a.c.units, node_size, wide, log_tx)) {
+        a.c.log_tx = log_tx;
+        ScopedTimer tm(kTimeOther, st);
+        dim3 const grid((unsigned)ceil_div(a.c.units, 1 << log_tx)), block(kWholeBlock);
+#define BBHIP_LAYER_NORM(W, BIT) launch((layer_norm_whole_kernel<W, 4, BIT>), grid, block, 0, st, a)
+        if (wide) { if (bit) { BBHIP_LAYER_NORM(4, true); } else { BBHIP_LAYER_NORM(4, false); } }
+        else      { if (bit) { BBHIP_LAYER_NORM(1, true); } else { BBHIP_LAYER_NORM(1, false); } }
+#undef BBHIP_LAYER_NORM
+        BBHIP_LAUNCH_CHECK();
+        return 0;
+    }
+    if (check_workspace(workspace, workspace_size, layer_norm_partial_bytes(a.c, wide), name)) { return 1; }
+    a.partial = static_cast<float2 *>(workspace);
     ScopedTimer tm(kTimeOther, st);
     dim3 const grid((unsigned)(a.c.tiles * a.c.slabs)), block(kColBlock);
 #define BBHIP_LAYER_NORM(W, BIT)                                                                        \
@@ -2568,7 +2582,7 @@ static size_t distillation_partial_bytes(ColumnSpace const &c, bool wide) { retu
 
 size_t bbhip_LossDistillation_WorkspaceBytes(int pix_size, int ch_size, int frame_size)
 {
-    if (pix_size <= 0 || ch_size <= 0 || frame_size <= 0) { return 0; }
+    if (pix_size <= 0 || ch_size <= kDistillFew || frame_size <= 0) { return 0; }
     size_t most = 0;
     for (int wide = 0; wide < 2; ++wide) {
         ColumnSpace c;
@@ -2588,11 +2602,12 @@ int bbhip_fp32_LossDistillation(float const *dev_y_buf, int const *dev_index_buf
     if (!(dev_y_buf && dev_index_buf && dev_logit_buf && dev_dy_buf && dev_loss_buf)) { return fail("%s: null buffer", __func__); }
     if (check_logits(top_size, pix_size, ch_size, frame_size, frame_stride, list_frame_stride, __func__)) { return 1; }
     if (!(temperature > 0.0f && temperature < __builtin_inff())) { return fail("%s: the temperature must be positive", __func__); }
-    bool const wide = frame_size >= 4 && frame_stride % 4 == 0 && starts_on_16_bytes(dev_y_buf) && starts_on_16_bytes(dev_dy_buf) && starts_on_16_bytes(dev_loss_buf);
+    bool const few = ch_size <= kDistillFew;
+    bool const wide = !few && frame_size >= 4 && frame_stride % 4 == 0 && starts_on_16_bytes(dev_y_buf) && starts_on_16_bytes(dev_dy_buf) && starts_on_16_bytes(dev_loss_buf);
     DistillArgs a{};
     if (column_space(a.c, a.tiles, wide, pix_size, frame_size, ch_size, 8, __func__)) { return 1; }
-    size_t const partial = distillation_partial_bytes(a.c, wide);
-    if (check_workspace(dev_workspace, workspace_size, partial + (size_t)a.c.units * (wide ? 4 : 1) * sizeof(float4), __func__)) { return 1; }
+    size_t const partial = few ? 0 : distillation_partial_bytes(a.c, wide);
+    if (check_workspace(dev_workspace, workspace_size, few ? 0 : partial + (size_t)a.c.units * (wide ? 4 : 1) * sizeof(float4), __func__)) { return 1; }
     a.frames = make_tile_divisor(frame_size);
     a.y = dev_y_buf; a.index = dev_index_buf; a.logit = dev_logit_buf; a.weight = dev_weight_buf; a.dy = dev_dy_buf; a.loss = dev_loss_buf;
     a.partial = static_cast<float2 *>(dev_workspace);
@@ -2606,7 +2621,13 @@ int bbhip_fp32_LossDistillation(float const *dev_y_buf, int const *dev_index_buf
     hipStream_t const st = static_cast<hipStream_t>(stream);
     ScopedTimer tm(kTimeOther, st);
     dim3 const grid((unsigned)a.main_blocks), sums((unsigned)(a.main_blocks + ceil_div(pix_size * frame_size, kListColumns))), block(kColBlock);
-    if (wide) {
+    if (few) {
+        dim3 const columns((unsigned)ceil_div(a.c.units, kWave)), lane(kWave);
+        if (ch_size <= 8)       { launch((distillation_few_kernel<8>), columns, lane, 0, st, a); }
+        else if (ch_size <= 16) { launch((distillation_few_kernel<16>), columns, lane, 0, st, a); }
+        else                    { launch((distillation_few_kernel<32>), columns, lane, 0, st, a); }
+    }
+    else if (wide) {
         launch((distillation_sums_kernel<4>), sums, block, 0, st, a);
         launch((distillation_gradient_kernel<4>), grid, block, 0, st, a);
     }
@@ -2641,7 +2662,7 @@ static size_t top_candidate_bytes(TopArgs const &a, bool wide, int top_size)
 
 size_t bbhip_TopLogits_WorkspaceBytes(int top_size, int pix_size, int ch_size, int frame_size)
 {
-    if (check_logits(top_size, pix_size, ch_size, frame_size, frame_size, frame_size, __func__)) { return 0; }
+    if (check_logits(top_size, pix_size, ch_size, frame_size, frame_size, frame_size, __func__) || ch_size <= kTopFew) { return 0; }
     size_t most = 0;
     for (int wide = 0; wide < 2; ++wide) {
         TopArgs a{};

@@ -101,6 +101,18 @@ struct ColumnThread {
         for (; base + B * step <= end; base += B * step) { body(base, std::true_type()); }      // workgroup-uniform
         if (base < end) { body(base, std::false_type()); }
     }
+    // The same with the loads of the next B rows issued before the present ones are used: start(base, held) before what the use waits for anyway, then
+    // follow(held, start, use).  start loads only rows below end, use(base, held) uses only those.
+    template <int B, class Held, class S, class U>
+    __device__ __forceinline__ void follow(Held &held, S start, U use) const
+    {
+        for (int base = begin; base < end; base += B * step) {                  // workgroup-uniform
+            Held next = held;
+            if (base + B * step < end) { start(base + B * step, next); }
+            use(base, held);
+            held = next;
+        }
+    }
 };
 
 }  // namespace bbhip

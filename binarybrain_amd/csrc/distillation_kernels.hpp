@@ -228,6 +228,16 @@ __global__ __launch_bounds__(kColBlock) void distillation_gradient_kernel(Distil
     ColumnUnit<W> const u(a.c, (t.tile << a.c.log_tx) + t.tx);
     int const part = (int)threadIdx.x >> a.c.log_tx, parts = kColBlock >> a.c.log_tx;
     size_t const channel = (size_t)a.pix_size * a.frame_stride, place = (size_t)u.pix * a.frame_stride + u.f0;
+    float const *const y = a.y + place + (size_t)t.lead * channel;
+    constexpr int B = 4;
+    struct Held { float v[B][W]; } held;
+    auto const start = [&](int base, Held &h) {
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+            if (base + t.lead + i * t.step < t.end) { column_load<W>(y + (size_t)(base + i * t.step) * channel, h.v[i]); }
+        }
+    };
+    start(t.begin, held);
     float m[W], s[W] = {};
 #pragma unroll
     for (int j = 0; j < W; ++j) { m[j] = -__builtin_inff(); }
@@ -254,7 +264,6 @@ __global__ __launch_bounds__(kColBlock) void distillation_gradient_kernel(Distil
         if (t.slab == 0) { column_store<W>(a.loss + place, u.live, loss); }
     }
     __syncthreads();
-    float const *const y = a.y + place + (size_t)t.lead * channel;
     float *const dy = a.dy + place + (size_t)t.lead * channel;
     float ref[W], gain[W];
     bool learns[W];
@@ -263,19 +272,13 @@ __global__ __launch_bounds__(kColBlock) void distillation_gradient_kernel(Distil
         float const k = of_k[t.tx * W + j];
         ref[j] = of_m[t.tx * W + j]; gain[j] = k * of_s[t.tx * W + j]; learns[j] = !(k == 0.0f);
     }
-    constexpr int B = 4;
-    t.template each<B>([&](int base, auto whole) {
-        float v[B][W];
+    t.template follow<B>(held, start, [&](int base, Held &h) {
 #pragma unroll
         for (int i = 0; i < B; ++i) {
-            if (whole || base + t.lead + i * t.step < t.end) { column_load<W>(y + (size_t)(base + i * t.step) * channel, v[i]); }
-        }
+            if (base + t.lead + i * t.step < t.end) {
 #pragma unroll
-        for (int i = 0; i < B; ++i) {
-            if (whole || base + t.lead + i * t.step < t.end) {
-#pragma unroll
-                for (int j = 0; j < W; ++j) { v[i][j] = learns[j] ? exp_scaled(v[i][j] - ref[j], a.scale) * gain[j] : 0.0f; }
-                column_store<W>(dy + (size_t)(base + i * t.step) * channel, u.live, v[i]);
+                for (int j = 0; j < W; ++j) { h.v[i][j] = learns[j] ? exp_scaled(h.v[i][j] - ref[j], a.scale) * gain[j] : 0.0f; }
+                column_store<W>(dy + (size_t)(base + i * t.step) * channel, u.live, h.v[i]);
             }
         }
     });
@@ -327,6 +330,62 @@ __global__ __launch_bounds__(kColBlock) void distillation_gradient_kernel(Distil
             a.dy[here] = k * (exp_scaled(yc - of_m[col], a.scale) * of_s[col] - q * fabsf(l.y));
         }
         __syncthreads();
+    }
+}
+
+// Few channels (at most MOST): a lane takes a column, its logits and the shares of the list in registers.
+constexpr int kDistillFew = 32;
+template <int MOST>
+__global__ __launch_bounds__(kWave) void distillation_few_kernel(DistillArgs a)
+{
+    ColumnUnit<1> const u(a.c, blockIdx.x * kWave + threadIdx.x);               // (a lane without a column: the first one's, and nothing is stored)
+    size_t const channel = (size_t)a.pix_size * a.frame_stride, place = (size_t)u.pix * a.frame_stride + u.f0;
+    size_t const entry = (size_t)a.pix_size * a.list_stride, at = (size_t)u.pix * a.list_stride + u.f0;
+    float y[MOST], q[MOST];
+#pragma unroll
+    for (int i = 0; i < MOST; ++i) { y[i] = a.y[place + (i < a.c.rows ? i : 0) * channel]; q[i] = 0.0f; }
+    float const w = a.weight != nullptr ? a.weight[place] : 1.0f;
+    float top = -__builtin_inff();
+    bool any = false;
+#pragma unroll 4
+    for (int j = 0; j < a.top_size; ++j) {
+        bool const valid = (unsigned)a.index[at + j * entry] < (unsigned)a.c.rows;
+        float const z = a.logit[at + j * entry];
+        any = any || (valid && !(z == -__builtin_inff()));
+        top = valid ? fmaxf(top, z) : top;
+    }
+    float const r = reference_of(top);
+    float sum = 0.0f, entropy = 0.0f;
+#pragma unroll 4
+    for (int j = 0; j < a.top_size; ++j) {
+        int const c = a.index[at + j * entry];
+        float const z = a.logit[at + j * entry], d = z == top ? 0.0f : z - r;
+        float const e = (unsigned)c < (unsigned)a.c.rows ? exp_scaled(d, a.scale) : 0.0f;
+        sum += e;
+        entropy = e == 0.0f ? entropy : __builtin_fmaf(e, d, entropy);
+#pragma unroll
+        for (int i = 0; i < MOST; ++i) { q[i] += c == i ? e : 0.0f; }
+    }
+    float m = -__builtin_inff(), s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < MOST; ++i) { m = i < a.c.rows ? fmaxf(m, y[i]) : m; }
+    float const ref = reference_of(m);
+    float loss = entropy;
+#pragma unroll
+    for (int i = 0; i < MOST; ++i) {
+        float const d = y[i] - ref;
+        loss = q[i] == 0.0f ? loss : __builtin_fmaf(q[i], -d, loss);
+        y[i] = exp_scaled(d, a.scale);
+        s += i < a.c.rows ? y[i] : 0.0f;
+    }
+    bool const none = !any || w == 0.0f;
+    float const gain = w * a.coefficient, to_p = 1.0f / s, to_q = 1.0f / sum;
+    if (u.live > 0) {
+        a.loss[place] = none ? 0.0f : w * a.t_square * (loss * a.reciprocal_t * to_q - logf(sum) + logf(s));
+#pragma unroll
+        for (int i = 0; i < MOST; ++i) {
+            if (i < a.c.rows) { a.dy[place + i * channel] = none ? 0.0f : gain * (y[i] * to_p - q[i] * to_q); }
+        }
     }
 }
 

@@ -201,6 +201,20 @@ __global__ __launch_bounds__(kColBlock) void layer_norm_apply_kernel(LayerNormAr
     __shared__ float share[2 * kColShareMax + kColWaves * kWave];
     ColumnThread<W> const t(a.c, a.tiles, backwards(blockIdx.x, gridDim.x), gridDim.x);
     ColumnUnit<W> const u(a.c, (t.tile << a.c.log_tx) + t.tx);
+    constexpr int B = 4;
+    struct Held { float v[B][W], g[B], b[B]; } held;
+    auto const start = [&](int base, Held &h) {
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+            int const row = base + t.lead + i * t.step;
+            if (row < t.end) {
+                layer_norm_load<W, BIT>(a.x, a.x_stride, row, u.f0, h.v[i]);
+                h.g[i] = a.gamma != nullptr ? a.gamma[row] : 1.0f;
+                h.b[i] = a.beta != nullptr ? a.beta[row] : 0.0f;
+            }
+        }
+    };
+    start(t.begin, held);
     int const part = (int)threadIdx.x >> a.c.log_tx, parts = kColBlock >> a.c.log_tx;
     Moments<W> m;
     float ones[W] = {}, none[W] = {};
@@ -241,26 +255,121 @@ __global__ __launch_bounds__(kColBlock) void layer_norm_apply_kernel(LayerNormAr
         if (a.mean != nullptr) { column_store<W>(a.mean + u.f0, u.live, mean); }
         if (a.rstd != nullptr) { column_store<W>(a.rstd + u.f0, u.live, rstd); }
     }
-    constexpr int B = 4;
-    t.template each<B>([&](int base, auto whole) {
-        float v[B][W], g[B], b[B];
-#pragma unroll
-        for (int i = 0; i < B; ++i) {
-            int const there = base + t.lead + i * t.step, row = whole || there < t.end ? there : t.begin;
-            layer_norm_load<W, BIT>(a.x, a.x_stride, row, u.f0, v[i]);
-            g[i] = a.gamma != nullptr ? a.gamma[row] : 1.0f;
-            b[i] = a.beta != nullptr ? a.beta[row] : 0.0f;
-        }
+    t.template follow<B>(held, start, [&](int base, Held &h) {
 #pragma unroll
         for (int i = 0; i < B; ++i) {
             int const row = base + t.lead + i * t.step;
-            if (whole || row < t.end) {
+            if (row < t.end) {
 #pragma unroll
-                for (int j = 0; j < W; ++j) { v[i][j] = __builtin_fmaf((v[i][j] - mean[j]) * rstd[j], g[i], b[i]); }
-                column_store<W>(a.out + (size_t)row * a.out_stride + u.f0, u.live, v[i]);
+                for (int j = 0; j < W; ++j) { h.v[i][j] = __builtin_fmaf((h.v[i][j] - mean[j]) * rstd[j], h.g[i], h.b[i]); }
+                column_store<W>(a.out + (size_t)row * a.out_stride + u.f0, u.live, h.v[i]);
             }
         }
     });
+}
+
+// Forward pass in one launch, for columns that a workgroup of 1024 threads can hold with R = 4 rows of a unit per thread: x is read once and the mean is known before
+// the deviations are squared.  Packed bits are held as their words.
+constexpr int kWholeBlock = 1024, kWholeWaves = kWholeBlock / kWave;
+
+// the sum over the threads that hold the same unit, in every thread.  share: kWholeWaves * kWave * W floats
+template <int W>
+__device__ __forceinline__ void whole_sum(float (&v)[W], int log_tx, float *share)
+{
+    int const lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, tx = lane & ((1 << log_tx) - 1);
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) {
+        if (o >= 1 << log_tx) {                                                 // workgroup-uniform
+#pragma unroll
+            for (int j = 0; j < W; ++j) { v[j] += lane_xor(v[j], o); }
+        }
+    }
+    if (lane < (1 << log_tx)) {
+#pragma unroll
+        for (int j = 0; j < W; ++j) { share[((wave << log_tx) + tx) * W + j] = v[j]; }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < W; ++j) { v[j] = 0.0f; }
+#pragma unroll
+    for (int w = 0; w < kWholeWaves; ++w) {
+        float o[W];
+        column_load<W>(share + ((w << log_tx) + tx) * W, o);
+#pragma unroll
+        for (int j = 0; j < W; ++j) { v[j] += o[j]; }
+    }
+}
+
+template <int W, int R, bool BIT>
+__global__ __launch_bounds__(kWholeBlock) void layer_norm_whole_kernel(LayerNormArgs a)
+{
+    __shared__ __align__(16) float share[2][kWholeBlock * W];
+    int const tx = threadIdx.x & ((1 << a.c.log_tx) - 1), ty = (int)threadIdx.x >> a.c.log_tx, step = kWholeBlock >> a.c.log_tx;
+    ColumnUnit<W> const u(a.c, (xcd_remap(blockIdx.x, gridDim.x) << a.c.log_tx) + tx);
+    float const rows = (float)a.c.rows;
+    float v[BIT ? 1 : R][W], mean[W] = {}, q[W] = {};
+    uint32_t bits[BIT ? R : 1];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        int const row = ty + i * step;
+        if constexpr (BIT) { bits[i] = row < a.c.rows ? static_cast<uint32_t const *>(a.x)[(size_t)row * a.x_stride + (u.f0 >> 5)] : 0u; }
+        else {
+            if (row < a.c.rows) { column_load<W>(static_cast<float const *>(a.x) + (size_t)row * a.x_stride + u.f0, v[i]); }
+            else {
+#pragma unroll
+                for (int j = 0; j < W; ++j) { v[i][j] = 0.0f; }
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+            if constexpr (BIT) { mean[j] += (float)((bits[i] >> ((u.f0 & 31) + j)) & 1u); }
+            else               { mean[j] += v[i][j]; }
+        }
+    }
+    whole_sum<W>(mean, a.c.log_tx, share[0]);
+#pragma unroll
+    for (int j = 0; j < W; ++j) { mean[j] /= rows; }
+    if constexpr (BIT) {
+#pragma unroll
+        for (int j = 0; j < W; ++j) { q[j] = mean[j] * (1.0f - mean[j]); }
+    }
+    else {
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                float const d = ty + i * step < a.c.rows ? v[i][j] - mean[j] : 0.0f;
+                q[j] = __builtin_fmaf(d, d, q[j]);
+            }
+        }
+        whole_sum<W>(q, a.c.log_tx, share[1]);
+#pragma unroll
+        for (int j = 0; j < W; ++j) { q[j] /= rows; }
+    }
+    float rstd[W];
+#pragma unroll
+    for (int j = 0; j < W; ++j) { rstd[j] = 1.0f / sqrtf(q[j] + a.eps); }
+    if (ty == 0) {
+        if (a.mean != nullptr) { column_store<W>(a.mean + u.f0, u.live, mean); }
+        if (a.rstd != nullptr) { column_store<W>(a.rstd + u.f0, u.live, rstd); }
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        int const row = ty + i * step;
+        if (row < a.c.rows) {
+            float const g = a.gamma != nullptr ? a.gamma[row] : 1.0f, b = a.beta != nullptr ? a.beta[row] : 0.0f;
+            float y[W];
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                float const x = BIT ? (float)((bits[BIT ? i : 0] >> ((u.f0 & 31) + j)) & 1u) : v[BIT ? 0 : i][j];
+                y[j] = __builtin_fmaf((x - mean[j]) * rstd[j], g, b);
+            }
+            column_store<W>(a.out + (size_t)row * a.out_stride + u.f0, u.live, y);
+        }
+    }
 }
 
 // backward, first launch: per column of the slab sum g and sum g xh, per row of the tile sum dy xh and sum dy
@@ -347,6 +456,20 @@ __global__ __launch_bounds__(kColBlock) void layer_norm_backward_apply_kernel(La
     }
     ColumnThread<W> const t(a.c, a.tiles, backwards(blockIdx.x, a.main_blocks), a.main_blocks);
     ColumnUnit<W> const u(a.c, (t.tile << a.c.log_tx) + t.tx);
+    constexpr int B = 4;
+    struct Held { float x[B][W], d[B][W], g[B]; } held;
+    auto const start = [&](int base, Held &h) {
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+            int const row = base + t.lead + i * t.step;
+            if (row < t.end) {
+                layer_norm_load<W, BIT>(a.x, a.x_stride, row, u.f0, h.x[i]);
+                column_load<W>(a.dy + (size_t)row * a.out_stride + u.f0, h.d[i]);
+                h.g[i] = a.gamma != nullptr ? a.gamma[row] : 1.0f;
+            }
+        }
+    };
+    start(t.begin, held);
     int const part = (int)threadIdx.x >> a.c.log_tx, parts = kColBlock >> a.c.log_tx;
     float mean[W], rstd[W], c1[W] = {}, c2[W] = {};
     line_load<W>(a.mean + u.f0, u.live, mean);
@@ -365,26 +488,17 @@ __global__ __launch_bounds__(kColBlock) void layer_norm_backward_apply_kernel(La
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < W; ++j) { c1[j] = share[t.tx * W + j]; c2[j] = share[kColShareMax + t.tx * W + j]; }
-    constexpr int B = 4;
-    t.template each<B>([&](int base, auto whole) {
-        float x[B][W], d[B][W], g[B];
-#pragma unroll
-        for (int i = 0; i < B; ++i) {
-            int const there = base + t.lead + i * t.step, row = whole || there < t.end ? there : t.begin;
-            layer_norm_load<W, BIT>(a.x, a.x_stride, row, u.f0, x[i]);
-            column_load<W>(a.dy + (size_t)row * a.out_stride + u.f0, d[i]);
-            g[i] = a.gamma != nullptr ? a.gamma[row] : 1.0f;
-        }
+    t.template follow<B>(held, start, [&](int base, Held &h) {
 #pragma unroll
         for (int i = 0; i < B; ++i) {
             int const row = base + t.lead + i * t.step;
-            if (whole || row < t.end) {
+            if (row < t.end) {
 #pragma unroll
                 for (int j = 0; j < W; ++j) {
-                    float const xh = (x[i][j] - mean[j]) * rstd[j];
-                    d[i][j] = rstd[j] * (__builtin_fmaf(d[i][j], g[i], -c1[j]) - xh * c2[j]);
+                    float const xh = (h.x[i][j] - mean[j]) * rstd[j];
+                    h.d[i][j] = rstd[j] * (__builtin_fmaf(h.d[i][j], h.g[i], -c1[j]) - xh * c2[j]);
                 }
-                column_store<W>(a.out + (size_t)row * a.out_stride + u.f0, u.live, d[i]);
+                column_store<W>(a.out + (size_t)row * a.out_stride + u.f0, u.live, h.d[i]);
             }
         }
     });

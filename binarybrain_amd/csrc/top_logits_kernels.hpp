@@ -224,7 +224,6 @@ template <int W, int TX, bool DRAW>
 __global__ __launch_bounds__(kTopRows<TX> * TX, 4) void top_logits_scan_kernel(TopArgs a)
 {
     constexpr int COLS = W * TX, ROWS = kTopRows<TX>, BLOCK = ROWS * TX, WAVES = BLOCK / kWave, HELD = kTopHeld, LIST = kTopList<TX>;
-    constexpr int PARTS = kTopMost / ROWS;                                      // groups of a thread's held channels: kTopMost groups per column
     __shared__ uint64_t list[COLS][LIST];
     __shared__ int count[COLS], before[COLS];
     __shared__ float bound[COLS];
@@ -261,9 +260,11 @@ __global__ __launch_bounds__(kTopRows<TX> * TX, 4) void top_logits_scan_kernel(T
     request(begin);
     for (int from = begin; from < end; from += HELD * ROWS) {
         if (from == begin && end - begin >= 2 * kTopMost) {
-            // the k-th largest of the maxima of kTopMost groups of channels: as many entries are no smaller, so it bounds the k-th largest entry from below, and hardly more than
-            // k entries reach it where the groups are many against k
-            uint32_t *const maxima = reinterpret_cast<uint32_t *>(&list[0][0]);                          // [COLS][kTopMost]
+            // The k-th largest of the maxima of 512 groups of channels: as many entries are no smaller, so it bounds the k-th largest entry from below, and hardly more than
+            // k entries reach it where the groups are many against k (68 and 316 of 1536 random logits reach the bound of k = 64 and 256).
+            constexpr int GROUPS = 2 * kTopMost, PARTS = GROUPS / ROWS, PER = GROUPS / kWave;
+            uint32_t *const maxima = reinterpret_cast<uint32_t *>(&list[0][0]);                          // [COLS][GROUPS]
+            static_assert(GROUPS * sizeof(uint32_t) <= LIST * sizeof(uint64_t) && HELD % PARTS == 0, "they fit where the lists will be");
 #pragma unroll
             for (int g = 0; g < PARTS; ++g) {
 #pragma unroll
@@ -271,17 +272,16 @@ __global__ __launch_bounds__(kTopRows<TX> * TX, 4) void top_logits_scan_kernel(T
                     float top = -__builtin_inff();
 #pragma unroll
                     for (int i = g * HELD / PARTS; i < (g + 1) * HELD / PARTS; ++i) { top = fmaxf(top, from + i * ROWS + ty < end ? v[i][j] : top); }
-                    maxima[(tx * W + j) * kTopMost + g * ROWS + ty] = from + g * HELD / PARTS * ROWS + ty < end ? order_key(top) : 0u;        // (0: a group without channels)
+                    maxima[(tx * W + j) * GROUPS + g * ROWS + ty] = from + g * HELD / PARTS * ROWS + ty < end ? order_key(top) : 0u;      // (0: a group without channels)
                 }
             }
             __syncthreads();
             for (int col = wave; col < COLS; col += WAVES) {
-                constexpr int PER = kTopMost / kWave;
                 uint32_t key[PER];
                 int reach;
 #pragma unroll
-                for (int i = 0; i < PER; ++i) { key[i] = maxima[col * kTopMost + i * kWave + lane]; }
-                uint32_t low = kth_key<PER>(key, kTopMost, k, reach);
+                for (int i = 0; i < PER; ++i) { key[i] = maxima[col * GROUPS + i * kWave + lane]; }
+                uint32_t low = kth_key<PER>(key, GROUPS, k, reach);
                 // entries equal to the bound count: dropped is what is not above the key before it (that of -0 is no value's: the one before that)
                 low = low == 0u ? 0u : low == 0x80000000u ? low - 2u : low - 1u;
                 if (lane == 0) { bound[col] = value_of_key(low); }

@@ -16,7 +16,8 @@ def refused(name, *args):
     return lib.bbhip_GetLastErrorString().decode()
 
 
-def norm(x=P, y=P, gamma=P, beta=P, mean=P, rstd=P, eps=1e-5, nodes=8, frames=16, xs=16, ys=16, work=P, size=MIB):
+# (sizes that need a workspace: short columns and few channels go without one)
+def norm(x=P, y=P, gamma=P, beta=P, mean=P, rstd=P, eps=1e-5, nodes=20000, frames=16, xs=16, ys=16, work=P, size=MIB):
     return (x, y, gamma, beta, mean, rstd, eps, nodes, frames, xs, ys, work, size, None)
 
 
@@ -49,12 +50,12 @@ def top(y=P, index=P, logit=P, k=4, pix=1, ch=10, frames=16, s=16, ls=16, work=P
 
 
 @pytest.mark.parametrize("what", [dict(y=None), dict(index=None), dict(logit=None), dict(k=0), dict(k=11), dict(k=257, ch=1000), dict(pix=0), dict(ch=-1), dict(frames=0), dict(s=15),
-                                  dict(ls=15), dict(pix=1 << 16, ch=1 << 16), dict(work=C.c_void_p((1 << 20) + 64)), dict(ch=100000, frames=1, work=None), dict(ch=100000, frames=1, size=8)])
+                                  dict(ls=15), dict(pix=1 << 16, ch=1 << 16), dict(ch=100000, frames=1, work=C.c_void_p((1 << 20) + 64)), dict(ch=100000, frames=1, work=None), dict(ch=100000, frames=1, size=8)])
 def test_top_logits_refuses(what):
     assert "TopLogits" in refused("fp32_TopLogits", *top(**what))
 
 
-def distill(y=P, index=P, logit=P, weight=P, dy=P, loss=P, t=1.0, ws=1.0, k=4, pix=1, ch=10, frames=16, s=16, ls=16, work=P, size=MIB):
+def distill(y=P, index=P, logit=P, weight=P, dy=P, loss=P, t=1.0, ws=1.0, k=4, pix=1, ch=100, frames=16, s=16, ls=16, work=P, size=MIB):
     return (y, index, logit, weight, dy, loss, t, ws, k, pix, ch, frames, s, ls, work, size, None)
 
 
@@ -97,3 +98,16 @@ def test_calls_refuse_what_is_not_on_the_device():
             call()
     with pytest.raises(TypeError):
         ops.top_logits([1, 2], 2, 4, 1, 8)
+
+
+def test_rules_and_objects():
+    """tests/cpp/test_head.cpp --rules: how the column operators divide their work over many sizes, and the host classes' objects"""
+    import os
+    import subprocess
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    exe = os.path.join(root, "tests", "cpp", "test_head")
+    if not os.path.exists(exe):
+        from binarybrain_amd.build import build_cpp_tests
+        build_cpp_tests()
+    res = subprocess.run([exe, "--rules"], stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=120)
+    assert res.returncode == 0, res.stdout

@@ -2447,7 +2447,8 @@ size_t bbhip_LayerNormalization_WorkspaceBytes(int node_size, int frame_size)
         TileDivisor tiles;
         if (column_space(c, tiles, wide, 1, frame_size, node_size, backward ? kLayerNormBatch / 2 : kLayerNormBatch, __func__)) { return 0; }
         int log_tx;
-        if (!backward && layer_norm_whole(c.units, node_size, wide, log_tx)) { continue; }
+        bool longer;
+        if (!backward && layer_norm_whole(c.units, node_size, wide, true, log_tx, longer)) { continue; }          // (of packed bits and of fp32: the former need no less)
         size_t const bytes = layer_norm_partial_bytes(c, wide) + (backward ? (size_t)c.tiles * node_size * sizeof(float2) : 0);
         most = bytes > most ? bytes : most;
     }
@@ -2469,13 +2470,15 @@ static int layer_norm_forward(void const *x, bool bit, float *y, float const *ga
     a.x_stride = x_stride; a.out_stride = y_stride;
     hipStream_t const st = static_cast<hipStream_t>(stream);
     int log_tx;
-    if (layer_norm_whole(a.c.units, node_size, wide, log_tx)) {
+    bool longer;
+    if (layer_norm_whole(a.c.units, node_size, wide, bit, log_tx, longer)) {
         a.c.log_tx = log_tx;
         ScopedTimer tm(kTimeOther, st);
         dim3 const grid((unsigned)ceil_div(a.c.units, 1 << log_tx)), block(kWholeBlock);
-#define BBHIP_LAYER_NORM(W, BIT) launch((layer_norm_whole_kernel<W, 4, BIT>), grid, block, 0, st, a)
-        if (wide) { if (bit) { BBHIP_LAYER_NORM(4, true); } else { BBHIP_LAYER_NORM(4, false); } }
-        else      { if (bit) { BBHIP_LAYER_NORM(1, true); } else { BBHIP_LAYER_NORM(1, false); } }
+#define BBHIP_LAYER_NORM(W, R, BIT) launch((layer_norm_whole_kernel<W, R, BIT>), grid, block, 0, st, a)
+        if (bit)         { if (wide) { BBHIP_LAYER_NORM(4, 4, true); }   else { BBHIP_LAYER_NORM(1, 4, true); } }
+        else if (longer) { if (wide) { BBHIP_LAYER_NORM(4, 16, false); } else { BBHIP_LAYER_NORM(1, 16, false); } }
+        else             { if (wide) { BBHIP_LAYER_NORM(4, 4, false); }  else { BBHIP_LAYER_NORM(1, 4, false); } }
 #undef BBHIP_LAYER_NORM
         BBHIP_LAUNCH_CHECK();
         return 0;

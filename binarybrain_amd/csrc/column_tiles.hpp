@@ -60,13 +60,16 @@ __device__ __forceinline__ void line_load(float const *__restrict__ p, int live,
     for (int j = 0; j < W; ++j) { v[j] = j < live ? p[j] : 0.0f; }
 }
 
-template <int W>
+// STREAM: past the caches (what a second launch reads again would lose its place in them to the output).  Large outputs in segments of less than a cache line go through
+// them, which joins the neighbours' halves: 4096 x 8192 frames in tiles of 64 bytes 75 us past the caches, 61 through them (1024 x 8192 14.4 and 16.3).
+template <int W, bool STREAM = true>
 __device__ __forceinline__ void column_store(float *__restrict__ p, int live, float const (&v)[W])
 {
     if constexpr (W == 4) {
         if (live == 4) {
             using V = float __attribute__((ext_vector_type(4)));
-            __builtin_nontemporal_store(V{v[0], v[1], v[2], v[3]}, reinterpret_cast<V *>(p));
+            if constexpr (STREAM) { __builtin_nontemporal_store(V{v[0], v[1], v[2], v[3]}, reinterpret_cast<V *>(p)); }
+            else                  { *reinterpret_cast<V *>(p) = V{v[0], v[1], v[2], v[3]}; }
             return;
         }
     }

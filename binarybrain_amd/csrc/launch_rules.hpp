@@ -271,19 +271,22 @@ inline void column_split(int units, int rows, bool wide, int batch, int &log_tx,
     slabs = ceil_div(rows, slab_rows);
 }
 
-// Layer norm's forward pass in one launch: the tile (2^log_tx units, of which a workgroup of 1024 threads holds 1024 >> log_tx rows per load), or false where a thread would have to
-// hold more than four rows with tiles of 64 bytes of a row.  Tiles as wide as four rows allow, narrower ones where compute units would be left without work.  In one launch and in two: 1024 nodes x 1000 frames
-// 7.6 and 8.7 us, x 4096 9.6 and 13.0, x 8192 15.7 and 19.9, 256 x 8192 6.9 and 8.2, 4096 x 1 6.9 and 7.7; with sixteen rows held 2048 x 1000 11.3 and 8.8,
-// 4096 x 1000 19.7 and 14.0, 4096 x 4096 32 and 34, 4096 x 8192 62 and 61.  Segments of 64 bytes serve as long as input and output stay in the memory-side cache: 1000 x 20000 33 and 39,
-// 1024 x 32768 81 and 62; with wider ones 64 x 524288 44 and 66, 4 x 1000000 42 and 68.
-inline bool layer_norm_whole(int units, int rows, bool wide, int &log_tx)
+// Layer norm's forward pass in one launch: the tile (2^log_tx units, of which a workgroup of 1024 threads holds 1024 >> log_tx rows per load), or false where two launches are taken.
+// Tiles as wide as four rows per thread allow, down to 64 bytes of a row, narrower ones also where compute units would be left without work.  In one launch and in two: 1024 nodes x 1000
+// frames 7.6 and 8.7 us, x 8192 14.4 and 19.9, 256 x 8192 6.9 and 8.2, 64 x 65536 7.6 and 12.3, 64 x 524288 44 and 66, 4096 x 1 6.9 and 7.7; with tiles of 64 bytes input and output have to
+// stay in the memory-side cache: 1000 x 20000 33 and 39, 1024 x 32768 81 and 62.
+// Longer columns (16 rows per thread, which leaves one workgroup per compute unit) where the launch has one or two rounds of workgroups: 4096 x 4096 27 and 35, 4096 x 8192 55 and 62, 2048 x 4096
+// 17.8 and 19.6; with fewer 3000 x 3000 21.0 and 21.6, 2048 x 2048 14.1 and 12.6, 4096 x 1000 22.4 and 13.5; with more 1500 x 20000 67 and 57, 2048 x 16384 74 and 63, 4096 x 16384 180 and 127.
+inline bool layer_norm_whole(int units, int rows, bool wide, bool bit, int &log_tx, bool &longer)
 {
     int const narrowest = wide ? 2 : 4;
     log_tx = 0;
     while ((1 << log_tx) < units && log_tx < 6) { ++log_tx; }
     while (log_tx > narrowest && (rows > 4 * (1024 >> log_tx) || ceil_div(units, 1 << log_tx) < 256)) { --log_tx; }
-    bool const cached = (long long)units * rows <= (wide ? 6 << 20 : 24 << 20);              // 96 MiB
-    return rows <= 4 * (1024 >> log_tx) && (cached || log_tx > narrowest);
+    longer = rows > 4 * (1024 >> log_tx);
+    int const tiles = ceil_div(units, 1 << log_tx);
+    if (longer) { return !bit && rows <= 16 * (1024 >> log_tx) && tiles >= 256 && tiles <= 512; }
+    return log_tx > narrowest || (long long)units * rows <= (wide ? 6 << 20 : 24 << 20);        // 96 MiB
 }
 
 // The same for the selection of the largest logits: tiles of four units, or of one where those would leave half of the compute units without work, slabs of multiples of 1024 channels, of which the second launch can

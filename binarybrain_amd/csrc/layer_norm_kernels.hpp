@@ -268,7 +268,7 @@ __global__ __launch_bounds__(kColBlock) void layer_norm_apply_kernel(LayerNormAr
     });
 }
 
-// Forward pass in one launch, for columns that a workgroup of 1024 threads can hold with R = 4 rows of a unit per thread: x is read once and the mean is known before
+// Forward pass in one launch, for columns that a workgroup of 1024 threads can hold, R = 4 or 16 rows of a unit per thread: x is read once and the mean is known before
 // the deviations are squared.  Packed bits are held as their words.
 constexpr int kWholeBlock = 1024, kWholeWaves = kWholeBlock / kWave;
 
@@ -367,7 +367,7 @@ __global__ __launch_bounds__(kWholeBlock) void layer_norm_whole_kernel(LayerNorm
                 float const x = BIT ? (float)((bits[BIT ? i : 0] >> ((u.f0 & 31) + j)) & 1u) : v[BIT ? 0 : i][j];
                 y[j] = __builtin_fmaf((x - mean[j]) * rstd[j], g, b);
             }
-            column_store<W>(a.out + (size_t)row * a.out_stride + u.f0, u.live, y);
+            column_store<W, R <= 4>(a.out + (size_t)row * a.out_stride + u.f0, u.live, y);
         }
     }
 }

@@ -36,7 +36,12 @@ static void test_rules(void)
             bool ok = log_tx >= 0 && log_tx <= 6 && ((long long)tiles << log_tx) >= units && ((long long)(tiles - 1) << log_tx) < units;
             ok = ok && slabs >= 1 && slabs <= 64 && (long long)slabs * slab_rows >= rows && (long long)(slabs - 1) * slab_rows < rows;
             check(ok, "column_split", units, rows);
-            if (bbhip::layer_norm_whole(units, rows, wide != 0, log_tx)) { check(log_tx >= 0 && log_tx <= 6 && rows <= 4 * (1024 >> log_tx), "layer_norm_whole", units, rows); }
+            for (int bit = 0; bit < 2; ++bit) {
+                bool longer = false;
+                if (bbhip::layer_norm_whole(units, rows, wide != 0, bit != 0, log_tx, longer)) {
+                    check(log_tx >= 0 && log_tx <= 6 && rows <= (longer ? 16 : 4) * (1024 >> log_tx) && !(bit && longer), "layer_norm_whole", units, rows);
+                }
+            }
         }
         int const channels = rows < top ? top : rows;
         bbhip::top_split(units, channels, top, log_tx, tiles, slab_rows, slabs);

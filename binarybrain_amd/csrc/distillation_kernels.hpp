@@ -36,7 +36,7 @@ constexpr int kListColumns = 4;                                 // columns of a 
 constexpr int kListParts   = kColBlock / kListColumns;
 constexpr int kListHeld    = 256 / kListParts;                  // entries of a thread (lists of up to 256)
 constexpr int kListSlots   = 512;                               // hash table of a column: twice the longest list
-constexpr int kFoundMost   = 4 * kColBlock;                      // entries that a workgroup looks at at a time
+constexpr int kFoundMost   = 16 * kColBlock;                     // entries that a workgroup looks at at a time
 constexpr int kDistillShare = 4 * kColBlock + kListSlots * kListColumns;        // floats: the sums of a tile, or the lists' values and tables
 static_assert(kDistillShare >= 2 * kColShareMax, "both uses fit");
 
@@ -222,7 +222,8 @@ template <int W>
 __global__ __launch_bounds__(kColBlock) void distillation_gradient_kernel(DistillArgs a)
 {
     __shared__ float share[2 * kColShareMax];
-    __shared__ int found, found_entry[kFoundMost], found_channel[kFoundMost];   // listed channels of the slab
+    __shared__ int found;
+    __shared__ uint16_t found_entry[kFoundMost];                                // listed channels of the slab (a tile has at most 2^16 entries)
     __shared__ float of_m[kWave * W], of_s[kWave * W], of_k[kWave * W];         // per column: reference, 1 / sum, w T / weight_sum (0: nothing to learn)
     ColumnThread<W> const t(a.c, a.tiles, backwards(blockIdx.x, gridDim.x), gridDim.x);
     ColumnUnit<W> const u(a.c, (t.tile << a.c.log_tx) + t.tx);
@@ -289,26 +290,27 @@ __global__ __launch_bounds__(kColBlock) void distillation_gradient_kernel(Distil
     for (int e0 = 0; e0 < columns * a.top_size; e0 += kFoundMost) {             // workgroup-uniform
         if (threadIdx.x == 0) { found = 0; }
         __syncthreads();
+        int c[kFoundMost / kColBlock];
 #pragma unroll
         for (int i = 0; i < kFoundMost / kColBlock; ++i) {
             int const e = e0 + i * kColBlock + threadIdx.x, col = e & (columns - 1), j = e >> log_columns;
             ColumnUnit<W> const at(a.c, (t.tile << a.c.log_tx) + col / W);
-            if (e < columns * a.top_size && col % W < at.live) {
-                int const c = a.index[(size_t)at.pix * a.list_stride + at.f0 + col % W + j * entry];
-                if (c >= begin && c < t.end) {
-                    int const to = atomicAdd(&found, 1);
-                    found_entry[to] = e; found_channel[to] = c;
-                }
-            }
+            c[i] = -1;
+            if (e < columns * a.top_size && col % W < at.live) { c[i] = a.index[(size_t)at.pix * a.list_stride + at.f0 + col % W + j * entry]; }
+        }
+#pragma unroll
+        for (int i = 0; i < kFoundMost / kColBlock; ++i) {
+            if (c[i] >= begin && c[i] < t.end) { found_entry[atomicAdd(&found, 1)] = (uint16_t)(e0 + i * kColBlock + threadIdx.x); }
         }
         // (the store below comes after the one of p above, of another wavefront perhaps: behind a wait for it and a barrier)
         __builtin_amdgcn_s_waitcnt(0x0f70);                                     // vmcnt(0)
         __syncthreads();
         for (int h = threadIdx.x; h < found; h += kColBlock) {
-            int const e = found_entry[h], c = found_channel[h], col = e & (columns - 1), j = e >> log_columns;
+            int const e = found_entry[h], col = e & (columns - 1), j = e >> log_columns;
             float const k = of_k[col];
             if (k == 0.0f) { continue; }
             ColumnUnit<W> const at(a.c, (t.tile << a.c.log_tx) + col / W);
+            int const c = a.index[(size_t)at.pix * a.list_stride + at.f0 + col % W + j * entry];
             float const *const logit = a.logit + (size_t)at.pix * a.list_stride + at.f0 + col % W;
             size_t const here = (size_t)at.pix * a.frame_stride + at.f0 + col % W + (size_t)c * channel;
             float4 const l = a.lists[at.column + col % W];

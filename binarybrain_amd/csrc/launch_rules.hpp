@@ -256,12 +256,14 @@ inline int pool_shared_rows(int lanes, long long nodes)
 }
 
 // How the operators down the columns divide `units` (of four frames, or of one) and `rows` among workgroups of 256 threads: tiles of 2^log_tx units, slabs of rows.
-// Sixteen units of four frames are a segment of 256 bytes of a row, 64 of one frame likewise; fewer where there are fewer.  Slabs until the launch has
+// Sixteen units of four frames are a segment of 256 bytes of a row, 64 of one frame likewise; fewer where there are fewer, up to 64 where few rows leave a workgroup little to do (backward pass
+// of 64 nodes x 65536 frames 28.1 us with 16 units, 19.9 with 64; x 524288 249 and 136; 1024 x 8192 31.9 and 39.9).  Slabs until the launch has
 // 2048 workgroups, of at least `batch` rows per thread, at most 64 (every workgroup of the second launch adds its columns' slabs up).
 inline void column_split(int units, int rows, bool wide, int batch, int &log_tx, int &tiles, int &slab_rows, int &slabs)
 {
     log_tx = 0;
     while ((1 << log_tx) < units && log_tx < (wide ? 4 : 6)) { ++log_tx; }
+    while (log_tx < 6 && rows <= 128 && ceil_div(units, 2 << log_tx) >= 256) { ++log_tx; }
     tiles = ceil_div(units, 1 << log_tx);
     int const step = (4 * 64 >> log_tx) * batch;                        // rows that a workgroup reads at a time
     int want = ceil_div(2048, tiles);

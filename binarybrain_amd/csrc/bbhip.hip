@@ -2710,10 +2710,13 @@ static int run_top(TopArgs &a, bool draw, int ch_size, int frame_size, void *wor
     ScopedTimer tm(kTimeOther, st);
     dim3 const grid((unsigned)(a.c.tiles * a.c.slabs)), block((unsigned)(a.c.log_tx ? kTopRows<4> * 4 : kTopRows<1>));
     dim3 const join((unsigned)ceil_div(a.c.units * (wide ? 4 : 1), kColWaves)), join_block(kColBlock);
-#define BBHIP_TOP(W, TX)                                                                                \
-    do {                                                                                                \
-        if (draw) { launch((top_logits_scan_kernel<W, TX, true>), grid, block, 0, st, a); }             \
-        else      { launch((top_logits_scan_kernel<W, TX, false>), grid, block, 0, st, a); }            \
+    bool const few = a.top_size <= kTopFewGroups;
+#define BBHIP_TOP(W, TX)                                                                                                                    \
+    do {                                                                                                                                    \
+        if (draw) { if (few) { launch((top_logits_scan_kernel<W, TX, true, 256>), grid, block, 0, st, a); }                                 \
+                    else     { launch((top_logits_scan_kernel<W, TX, true, 512>), grid, block, 0, st, a); } }                               \
+        else      { if (few) { launch((top_logits_scan_kernel<W, TX, false, 256>), grid, block, 0, st, a); }                                \
+                    else     { launch((top_logits_scan_kernel<W, TX, false, 512>), grid, block, 0, st, a); } }                              \
     } while (0)
     if (wide) { if (a.c.log_tx) { BBHIP_TOP(4, 4); } else { BBHIP_TOP(4, 1); } }
     else      { if (a.c.log_tx) { BBHIP_TOP(1, 4); } else { BBHIP_TOP(1, 1); } }

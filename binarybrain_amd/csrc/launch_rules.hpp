@@ -291,12 +291,14 @@ inline bool layer_norm_whole(int units, int rows, bool wide, bool bit, int &log_
     return log_tx > narrowest || (long long)units * rows <= (wide ? 6 << 20 : 24 << 20);        // 96 MiB
 }
 
-// The same for the selection of the largest logits: tiles of four units, or of one where those would leave half of the compute units without work, slabs of multiples of 1024 channels, of which the second launch can
+// The same for the selection of the largest logits: tiles of four units, or of one where those would leave compute units without
+// work (1001 channels x 777 frames, k = 17 15.8 and 11.4 us, 10007 x 256, k = 40 24.0 and 21.0; of fewer than 512 channels a wavefront per column serves either way: 100 x 256 10.7 and 15.9), slabs of multiples of 1024 channels, of which the second launch can
 // select from 1024 / top_size at most.
 inline void top_split(int units, int channels, int top_size, int &log_tx, int &tiles, int &slab_rows, int &slabs)
 {
     int const most = 1024 / top_size;
-    log_tx = units > 1 && ceil_div(units, 4) * most >= 128 ? 2 : 0;
+    int const share = most < ceil_div(channels, 1024) ? most : ceil_div(channels, 1024);
+    log_tx = units > 1 && (channels < 512 || (long long)ceil_div(units, 4) * share >= 256) ? 2 : 0;
     tiles = ceil_div(units, 1 << log_tx);
     int want = ceil_div(512, tiles);
     if (want > most) { want = most; }

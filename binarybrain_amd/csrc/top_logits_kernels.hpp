@@ -28,6 +28,9 @@ constexpr int kTopHeld = 12;
 // ... and a column's list holds these besides the kTopMost that it is cut to
 template <int TX> constexpr int kTopList = kTopMost + kTopRows<TX>;
 
+// up to this k the bounds come from 256 groups of channels, above from 512 (72 of 1536 random logits reach the bound of k = 64, 316 that of k = 256)
+constexpr int kTopFewGroups = 96;
+
 struct TopArgs {
     ColumnSpace c;                  // rows = channels
     TileDivisor tiles, entries;     // entries: top_size
@@ -131,8 +134,8 @@ __device__ __forceinline__ uint32_t cut_list_of(uint64_t *list, int n, int k, in
 template <int MOST>
 __device__ __forceinline__ uint32_t cut_list(uint64_t *list, int n, int k, int rows)
 {
-    if (n <= 4 * kWave) { return cut_list_of<4>(list, n, k, rows); }
-    if constexpr (MOST > 8 * kWave) { if (n <= 8 * kWave) { return cut_list_of<8>(list, n, k, rows); } }
+    constexpr int SHORT = MOST > 8 * kWave ? 8 : 4;
+    if (n <= SHORT * kWave) { return cut_list_of<SHORT>(list, n, k, rows); }
     return cut_list_of<MOST / kWave>(list, n, k, rows);
 }
 
@@ -158,9 +161,8 @@ __device__ __forceinline__ void order_list_of(uint64_t *list, int k)
 }
 __device__ __forceinline__ void order_list(uint64_t *list, int k)
 {
-    if (k <= kWave)          { order_list_of<1>(list, k); }
-    else if (k <= 2 * kWave) { order_list_of<2>(list, k); }
-    else                     { order_list_of<kTopMost / kWave>(list, k); }
+    if (k <= kWave) { order_list_of<1>(list, k); }
+    else            { order_list_of<kTopMost / kWave>(list, k); }
 }
 
 // One category of k ordered entries: weights exp((z - z_0) / T); kept is the shortest prefix that holds top_p of their sum, of it those of at least min_p times the
@@ -219,8 +221,8 @@ __device__ __forceinline__ void draw_category(TopArgs const &a, uint64_t const *
     }
 }
 
-// W = 4: a thread reads four frames of a channel, W = 1: one; TX threads side by side.  DRAW: a category instead of the list
-template <int W, int TX, bool DRAW>
+// W = 4: a thread reads four frames of a channel, W = 1: one; TX threads side by side.  DRAW: a category instead of the list.  GROUPS: of channels, whose maxima give the bounds
+template <int W, int TX, bool DRAW, int GROUPS>
 __global__ __launch_bounds__(kTopRows<TX> * TX, 4) void top_logits_scan_kernel(TopArgs a)
 {
     constexpr int COLS = W * TX, ROWS = kTopRows<TX>, BLOCK = ROWS * TX, WAVES = BLOCK / kWave, HELD = kTopHeld, LIST = kTopList<TX>;
@@ -260,9 +262,9 @@ __global__ __launch_bounds__(kTopRows<TX> * TX, 4) void top_logits_scan_kernel(T
     request(begin);
     for (int from = begin; from < end; from += HELD * ROWS) {
         if (from == begin && end - begin >= 2 * kTopMost) {
-            // The k-th largest of the maxima of 512 groups of channels: as many entries are no smaller, so it bounds the k-th largest entry from below, and hardly more than
-            // k entries reach it where the groups are many against k (68 and 316 of 1536 random logits reach the bound of k = 64 and 256).
-            constexpr int GROUPS = 2 * kTopMost, PARTS = GROUPS / ROWS, PER = GROUPS / kWave;
+            // The k-th largest of the maxima of the groups: as many entries are no smaller, so it bounds the k-th largest entry from below, and hardly more than k entries
+            // reach it where the groups are many against k.
+            constexpr int PARTS = GROUPS / ROWS, PER = GROUPS / kWave;
             uint32_t *const maxima = reinterpret_cast<uint32_t *>(&list[0][0]);                          // [COLS][GROUPS]
             static_assert(GROUPS * sizeof(uint32_t) <= LIST * sizeof(uint64_t) && HELD % PARTS == 0, "they fit where the lists will be");
 #pragma unroll

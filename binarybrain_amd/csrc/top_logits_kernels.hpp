@@ -457,7 +457,7 @@ __global__ __launch_bounds__(kColBlock) void top_logits_join_kernel(TopArgs a)
 template <int MOST, bool DRAW>
 __global__ __launch_bounds__(kWave) void top_logits_few_kernel(TopArgs a)
 {
-    __shared__ float value[DRAW ? MOST : 1][kWave];
+    __shared__ double weight[DRAW ? MOST : 1][kWave];
     __shared__ int which[DRAW ? MOST : 1][kWave];
     int const lane = threadIdx.x, column = blockIdx.x * kWave + lane, k = a.top_size;
     ColumnUnit<1> const u(a.c, column);
@@ -468,6 +468,8 @@ __global__ __launch_bounds__(kWave) void top_logits_few_kernel(TopArgs a)
     for (int i = 0; i < MOST; ++i) { v[i] = a.y[at + (i < a.c.rows ? i : 0) * channel]; }                       // (a lane without a column: the first one's)
 #pragma unroll
     for (int i = 0; i < MOST; ++i) { key[i] = i < a.c.rows ? order_key(v[i]) : 0u; }
+    float z0 = 0.0f;
+    double all = 0.0;
     for (int j = 0; j < k; ++j) {
         uint32_t top = 0u;
         int found = 0;
@@ -477,7 +479,13 @@ __global__ __launch_bounds__(kWave) void top_logits_few_kernel(TopArgs a)
         }
 #pragma unroll
         for (int i = 0; i < MOST; ++i) { key[i] = i == found ? 0u : key[i]; }
-        if (DRAW) { value[j][lane] = value_of_key(top); which[j][lane] = found; }
+        if (DRAW) {
+            float const z = value_of_key(top);
+            if (j == 0) { z0 = z; }
+            double const w = z == z0 ? 1.0 : exp(((double)z - (double)z0) / (double)a.temperature);
+            weight[j][lane] = w; which[j][lane] = found;
+            all += w;
+        }
         else if (u.live > 0) {
             size_t const to = ((size_t)j * a.pix_size + u.pix) * a.list_stride + u.f0;
             a.index[to] = found;
@@ -485,23 +493,20 @@ __global__ __launch_bounds__(kWave) void top_logits_few_kernel(TopArgs a)
         }
     }
     if (DRAW) {
-        float const z0 = value[0][lane];
-        auto weight = [&](int j) { float const z = value[j][lane]; return z == z0 ? 1.0 : exp(((double)z - (double)z0) / (double)a.temperature); };
         int category = -1;
         float share = 0.0f;
         if (z0 > -__builtin_inff()) {
-            double all = 0.0, total = 0.0, sum = 0.0, w = 1.0;
-            if (a.top_p < 1.0f) { for (int j = 0; j < k; ++j) { all += weight(j); } }
+            double total = 0.0, sum = 0.0, w = 1.0;
             int kept = 0;
             for (; kept < k; ++kept) {
-                w = weight(kept);
+                w = weight[kept][lane];
                 if (kept > 0 && !(w > 0.0 && w >= (double)a.min_p && (a.top_p >= 1.0f || total < (double)a.top_p * all))) { break; }
                 total += w;
             }
             double const reach = (double)a.u[at] * total;
             int drawn = 0;
             for (; ; ++drawn) {
-                w = weight(drawn);
+                w = weight[drawn][lane];
                 sum += w;
                 if (drawn == kept - 1 || !(sum <= reach)) { break; }
             }

@@ -2723,14 +2723,16 @@ static int run_top(TopArgs &a, bool draw, int ch_size, int frame_size, void *wor
 #undef BBHIP_TOP
     BBHIP_LAUNCH_CHECK();
     if (a.c.slabs > 1) {
-        if (wide) {
-            if (draw) { launch((top_logits_join_kernel<4, true>), join, join_block, 0, st, a); }
-            else      { launch((top_logits_join_kernel<4, false>), join, join_block, 0, st, a); }
-        }
-        else {
-            if (draw) { launch((top_logits_join_kernel<1, true>), join, join_block, 0, st, a); }
-            else      { launch((top_logits_join_kernel<1, false>), join, join_block, 0, st, a); }
-        }
+        int const entries = a.c.slabs * a.top_size;
+#define BBHIP_TOP(W, DRAW)                                                                                                      \
+    do {                                                                                                                        \
+        if (entries <= 4 * kWave)      { launch((top_logits_join_kernel<W, DRAW, 4>), join, join_block, 0, st, a); }            \
+        else if (entries <= 8 * kWave) { launch((top_logits_join_kernel<W, DRAW, 8>), join, join_block, 0, st, a); }            \
+        else                           { launch((top_logits_join_kernel<W, DRAW, kTopJoin / kWave>), join, join_block, 0, st, a); } \
+    } while (0)
+        if (wide) { if (draw) { BBHIP_TOP(4, true); } else { BBHIP_TOP(4, false); } }
+        else      { if (draw) { BBHIP_TOP(1, true); } else { BBHIP_TOP(1, false); } }
+#undef BBHIP_TOP
         BBHIP_LAUNCH_CHECK();
     }
     return 0;

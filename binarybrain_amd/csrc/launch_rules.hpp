@@ -292,18 +292,19 @@ inline bool layer_norm_whole(int units, int rows, bool wide, bool bit, int &log_
 }
 
 // The same for the selection of the largest logits: tiles of four units, or of one where those would leave compute units without
-// work (1001 channels x 777 frames, k = 17 15.8 and 11.4 us, 10007 x 256, k = 40 24.0 and 21.0; of fewer than 512 channels a wavefront per column serves either way: 100 x 256 10.7 and 15.9), slabs of multiples of 1024 channels, of which the second launch can
-// select from 1024 / top_size at most.
+// work (1001 channels x 777 frames, k = 17 15.8 and 11.4 us, 10007 x 256, k = 40 24.0 and 21.0; of fewer than 512 channels a wavefront per column serves either way: 100 x 256 10.7 and 15.9), slabs of multiples
+// of 1024 channels, not shorter than what a workgroup holds at a time (1360 channels x 238 frames, k = 9, 9.8 us in one slab, 22.9 in two), of which the second launch can select from 1024 / top_size.
 inline void top_split(int units, int channels, int top_size, int &log_tx, int &tiles, int &slab_rows, int &slabs)
 {
     int const most = 1024 / top_size;
-    int const share = most < ceil_div(channels, 1024) ? most : ceil_div(channels, 1024);
+    int const share = most < ceil_div(channels, 3072) ? most : ceil_div(channels, 3072);
     log_tx = units > 1 && (channels < 512 || (long long)ceil_div(units, 4) * share >= 256) ? 2 : 0;
     tiles = ceil_div(units, 1 << log_tx);
     int want = ceil_div(512, tiles);
     if (want > most) { want = most; }
-    int const load = 1024, loads = ceil_div(channels, load);
-    slab_rows = ceil_div(loads, want < loads ? want : loads) * load;
+    int const held = log_tx ? 1536 : 3072, loads = ceil_div(channels, 1024);
+    slab_rows = ceil_div(loads, want < loads ? want : loads) * 1024;
+    if (slab_rows < held) { slab_rows = held; }                         // (what the threads of a workgroup hold: less would take as long)
     slabs = ceil_div(channels, slab_rows);
 }
 

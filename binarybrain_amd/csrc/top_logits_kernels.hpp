@@ -89,21 +89,13 @@ __device__ __forceinline__ uint32_t kth_key(uint32_t const (&key)[PER], int n, i
     return bound;
 }
 
-// The k largest of n > k entries of `list`, to its front in any order; returns a lower bound of their keys.  rows: above every channel.  A whole wavefront calls this.
+// The k largest of n > k entries, entry i * 64 + lane in register i (key 0 behind them), to the front of `list` in any order; returns a lower bound of their keys.  rows:
+// above every channel.  A whole wavefront calls this.
 template <int PER>
-__device__ __forceinline__ uint32_t cut_list_of(uint64_t *list, int n, int k, int rows)
+__device__ __forceinline__ uint32_t select_entries(uint32_t const (&key)[PER], int const (&channel)[PER], int n, int k, int rows, uint64_t *list)
 {
-    int const lane = threadIdx.x % kWave;
-    uint32_t key[PER];
-    int channel[PER], reach;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        int const e = i * kWave + lane;
-        uint64_t const v = e < n ? list[e] : 0u;
-        key[i] = key_of(v); channel[i] = channel_of(v);
-    }
-    wave_fence();
-    uint32_t const bound = kth_key<PER>(key, n, k, reach);                      // (above 0: so is every key, and what is behind the list is not taken)
+    int reach;
+    uint32_t const bound = kth_key<PER>(key, n, k, reach);                      // (above 0: so is every key, and what is behind the entries is not taken)
     int last = rows;                                                            // of the entries that equal the bound, those up to here
     if (reach != k) {                                                           // (bound is the k-th largest key, and more than k entries reach it)
         int above = 0;
@@ -130,12 +122,27 @@ __device__ __forceinline__ uint32_t cut_list_of(uint64_t *list, int n, int k, in
     wave_fence();
     return bound;
 }
+// the same within a list in LDS
+template <int PER>
+__device__ __forceinline__ uint32_t cut_list_of(uint64_t *list, int n, int k, int rows)
+{
+    int const lane = threadIdx.x % kWave;
+    uint32_t key[PER];
+    int channel[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        int const e = i * kWave + lane;
+        uint64_t const v = e < n ? list[e] : 0u;
+        key[i] = key_of(v); channel[i] = channel_of(v);
+    }
+    wave_fence();
+    return select_entries<PER>(key, channel, n, k, rows, list);
+}
 // with as many registers as the list needs
 template <int MOST>
 __device__ __forceinline__ uint32_t cut_list(uint64_t *list, int n, int k, int rows)
 {
-    constexpr int SHORT = MOST > 8 * kWave ? 8 : 4;
-    if (n <= SHORT * kWave) { return cut_list_of<SHORT>(list, n, k, rows); }
+    if (n <= 4 * kWave) { return cut_list_of<4>(list, n, k, rows); }
     return cut_list_of<MOST / kWave>(list, n, k, rows);
 }
 
@@ -419,36 +426,35 @@ __global__ __launch_bounds__(kTopRows<TX> * TX, 4) void top_logits_scan_kernel(T
     }
 }
 
-// the largest of the slabs' lists: a wavefront per column
-template <int W, bool DRAW>
+// the largest of the slabs' lists: a wavefront per column, PER entries per lane
+template <int W, bool DRAW, int PER>
 __global__ __launch_bounds__(kColBlock) void top_logits_join_kernel(TopArgs a)
 {
-    __shared__ uint64_t list[kColWaves][kTopJoin];
+    __shared__ uint64_t lists[kColWaves][kTopMost];
     int const lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, k = a.top_size, n = a.c.slabs * k;
     int const column = blockIdx.x * kColWaves + wave;
     ColumnUnit<W> const u(a.c, column / W);
     if (column % W >= u.live) { return; }                                       // (wavefronts of this kernel do not meet)
-    uint64_t v[kTopJoin / kWave];
+    uint64_t *const list = lists[wave];
+    uint64_t v[PER];
 #pragma unroll
-    for (int i = 0; i < kTopJoin / kWave; ++i) {                                // (all requested before the first is waited for)
-        int const e = i * kWave + lane < n ? i * kWave + lane : 0;
+    for (int i = 0; i < PER; ++i) {                                             // (all requested before the first is waited for)
         int slab, j;
-        split_tile(e, a.entries, slab, j);
+        split_tile(i * kWave + lane < n ? i * kWave + lane : 0, a.entries, slab, j);
         v[i] = a.candidates[((size_t)slab * (a.c.units * W) + column) * k + j];
     }
+    uint32_t key[PER];
+    int channel[PER];
 #pragma unroll
-    for (int i = 0; i < kTopJoin / kWave; ++i) {
-        if (i * kWave + lane < n) { list[wave][i * kWave + lane] = v[i]; }
-    }
-    wave_fence();
-    (void)cut_list<kTopJoin>(list[wave], n, k, a.c.rows);
-    order_list(list[wave], k);
-    if (DRAW) { draw_category(a, list[wave], (size_t)u.pix * a.frame_stride + u.f0 + column % W); }
+    for (int i = 0; i < PER; ++i) { key[i] = i * kWave + lane < n ? key_of(v[i]) : 0u; channel[i] = channel_of(v[i]); }
+    (void)select_entries<PER>(key, channel, n, k, a.c.rows, list);
+    order_list(list, k);
+    if (DRAW) { draw_category(a, list, (size_t)u.pix * a.frame_stride + u.f0 + column % W); }
     else {
         for (int j = lane; j < k; j += kWave) {
             size_t const at = ((size_t)j * a.pix_size + u.pix) * a.list_stride + u.f0 + column % W;
-            a.index[at] = channel_of(list[wave][j]);
-            a.logit[at] = value_of_key(key_of(list[wave][j]));
+            a.index[at] = channel_of(list[j]);
+            a.logit[at] = value_of_key(key_of(list[j]));
         }
     }
 }

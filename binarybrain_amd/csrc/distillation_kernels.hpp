@@ -11,6 +11,8 @@
 // whether a list names a channel twice.  The second launch joins the slabs and writes dy: first p for every channel of its slab, then, behind a
 // barrier, the few channels of the lists.  Exponents are taken of differences to the maximum, (y - m) * (log2 e / T): the rounding of the product
 // grows with the distance from the maximum and weighs as little as the term itself.
+// 32768 channels x 2048 frames, lists of 64: sums 44 us = 6.1 TB/s, gradient 112 us = 4.8 TB/s (a copy 5.1): the logits pass the fabric twice.  Up to 32 channels a lane
+// holds a whole column and one launch does all (21 channels x 66560 places 41.6 -> 9.3 us).
 #pragma once
 
 #include "layer_norm_kernels.hpp"

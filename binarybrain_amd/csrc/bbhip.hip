@@ -2604,7 +2604,7 @@ int bbhip_fp32_LossDistillation(float const *dev_y_buf, int const *dev_index_buf
     clear_hints();
     if (!(dev_y_buf && dev_index_buf && dev_logit_buf && dev_dy_buf && dev_loss_buf)) { return fail("%s: null buffer", __func__); }
     if (check_logits(top_size, pix_size, ch_size, frame_size, frame_stride, list_frame_stride, __func__)) { return 1; }
-    if (!(temperature > 0.0f && temperature < __builtin_inff())) { return fail("%s: the temperature must be positive", __func__); }
+    if (!(temperature >= 1.0e-18f && temperature <= 1.0e18f)) { return fail("%s: the temperature must lie in [1e-18, 1e18] (its square and its reciprocal are taken)", __func__); }
     bool const few = ch_size <= kDistillFew;
     bool const wide = !few && frame_size >= 4 && frame_stride % 4 == 0 && starts_on_16_bytes(dev_y_buf) && starts_on_16_bytes(dev_dy_buf) && starts_on_16_bytes(dev_loss_buf);
     DistillArgs a{};

@@ -500,7 +500,7 @@ int bbhip_fp32_TopLogits(float const *dev_y_buf, int *dev_index_buf, float *dev_
  *     q = softmax(z / T) over the entries, p = softmax(y / T) over the channels, w the place's weight (dev_weight_buf [pix] rows of frame_stride, NULL: 1)
  *     dev_loss_buf[pix][frame] = w * T^2 * sum_j q_j * (log q_j - log p_{i_j}),   dy[c] = w * T * (p_c - q_c) / weight_sum.
  * The caller passes weight_sum = the sum of the weights and reports sum(dev_loss_buf) / weight_sum, whose gradient dy is.  A place without entries, or whose entries are all
- * minus infinity, or with weight 0 has loss 0 and gradient 0 whatever its logits are.  dev_loss_buf has rows of frame_stride too. */
+ * minus infinity, or with weight 0 has loss 0 and gradient 0 whatever its logits are.  dev_loss_buf has rows of frame_stride too.  temperature: 1e-18 .. 1e18. */
 size_t bbhip_LossDistillation_WorkspaceBytes(int pix_size, int ch_size, int frame_size);
 int bbhip_fp32_LossDistillation(float const *dev_y_buf, int const *dev_index_buf, float const *dev_logit_buf, float const *dev_weight_buf, float *dev_dy_buf,
                                 float *dev_loss_buf, float temperature, float weight_sum, int top_size, int pix_size, int ch_size, int frame_size,

@@ -414,3 +414,83 @@ def test_one_logit_is_the_largest(ops):
     y = logits_of("equal", rng, (90, 33))
     category, share = ops.categorical_sampling(dev(y), dev(rng.random((1, 33)).astype(F32)), 90, 1, 33, top_size=1)
     assert np.array_equal(host(category)[0], y.argmax(0)) and np.all(host(share) == 1.0)
+
+
+# ---- edges -------------------------------------------------------------------------------------------------------------------------
+def test_buffers_beyond_4_gib(ops):
+    """offsets that do not fit 32 bits: 70000 rows of 16384 frames; the first and last columns against 64 bits, the last rows written"""
+    import torch
+    nodes, F, k = 70000, 16384, 3
+    gen = torch.Generator(device="cuda"); gen.manual_seed(1)
+    x = torch.randn((nodes, F), generator=gen, device="cuda")
+    some = [0, 1, 4095, 8190, F - 2, F - 1]
+    v = host(x[:, some])
+    one, zero = np.ones(nodes, F32), np.zeros(nodes, F32)
+    y, mean, rstd = ops.layer_normalization_forward(x, dev(one), dev(zero), F)
+    check_norm(v, one, zero, host(y[:, some]), host(mean)[some], host(rstd)[some], *ref.layer_norm(v, one, zero, float(F32(1e-5))))
+    dx, dgamma, dbeta = ops.layer_normalization_backward(x, y, dev(one), mean, rstd, F)
+    wdx, _, _ = ref.layer_norm_backward(v, host(y[:, some]), one, host(mean)[some], host(rstd)[some])
+    g, at_mean, at_rstd = (host(a).astype(np.float64) for a in (y[:, some], mean[some], rstd[some]))
+    xh = (v - at_mean) * at_rstd
+    a, b = np.abs(g).mean(0), np.abs(g * xh).mean(0)
+    near(host(dx[:, some]), wdx, at_rstd * (8 * U * (np.abs(g) + a + np.abs(xh) * b) + 204 * U * (a + np.abs(xh) * b)), "dx")
+    last = (x[-4:].double() - mean.double()) * rstd.double()
+    near(host(dgamma)[-4:], host((y[-4:].double() * last).sum(1)), 204 * U * host((y[-4:].double() * last).abs().sum(1)), "dgamma")
+    del y, dx
+    index, logit = ops.top_logits(x, k, nodes, 1, F)
+    wi, wv = ref.top_logits(v, k)
+    assert np.array_equal(host(index[:, some]), wi) and np.array_equal(host(logit[:, some]), wv)
+    dy, loss = ops.loss_distillation(x, index, logit, nodes, 1, F, weight_sum=1.0)
+    check_distill(v, wi, wv, np.ones(len(some), F32), 1.0, 1.0, host(dy[:, some]), host(loss[:, some])[0])
+
+
+def test_a_batch_of_padding_only(ops):
+    """weights that are all 0, and so is their sum: no loss, no gradient, nothing that is not a number"""
+    rng = np.random.default_rng(40)
+    for C in (20, 500):
+        y, index, z, _ = distill_case(rng, C, 16, 5)
+        w = np.zeros((1, 16), F32)
+        dy, loss = ops.loss_distillation(dev(y), dev(index), dev(z), C, 1, 16, weight=dev(w))
+        assert not host(dy).any() and not host(loss).any()
+
+
+def test_lists_longer_than_the_channels(ops):
+    """a teacher's record may hold more entries than there are channels: most of them name one again"""
+    rng = np.random.default_rng(41)
+    for C in (4, 60):
+        k = 200
+        y = rng.standard_normal((C, 24)).astype(F32)
+        index, z = rng.integers(-2, C + 2, (k, 24)).astype(np.int32), rng.standard_normal((k, 24)).astype(F32)
+        dy, loss = ops.loss_distillation(dev(y), dev(index), dev(z), C, 1, 24, temperature=1.5, weight_sum=2.0)
+        check_distill(y, index, z, np.ones(24, F32), 1.5, 2.0, host(dy), host(loss)[0])
+
+
+def test_numbers_outside_the_unit_interval(ops):
+    """u below 0 draws the first of the kept, u of 1 and above the last"""
+    y = np.repeat(np.log(np.array([0.1, 0.6, 0.3], F32))[:, None], 4, 1)
+    u = np.array([[-1.0, 1.0, 7.0, 0.0]], F32)
+    for pad in (0, 50):
+        z = np.concatenate([y, np.full((pad, 4), -30.0, F32)])
+        category, _ = ops.categorical_sampling(dev(z), dev(u), 3 + pad, 1, 4, top_size=3)
+        assert host(category)[0].tolist() == [1, 0, 0, 1]
+
+
+def test_refusals_on_the_device(ops):
+    import torch
+    from binarybrain_amd.capi import BbhipError
+    x, i, line = torch.zeros(40, 8, device="cuda"), torch.zeros((4, 8), dtype=torch.int32, device="cuda"), torch.zeros(40, device="cuda")
+    z, one = torch.zeros(4, 8, device="cuda"), torch.zeros(1, 8, device="cuda")
+    for call in (lambda: ops.layer_normalization_forward(x, line[:3], line, 8), lambda: ops.layer_normalization_forward(x, line, line.double(), 8),
+                 lambda: ops.layer_normalization_forward(x.double(), line, line, 8), lambda: ops.layer_normalization_forward(x, line, line, 9),
+                 lambda: ops.layer_normalization_forward(x, line, line, 0), lambda: ops.layer_normalization_forward(x, line, line, 8, eps=-1.0),
+                 lambda: ops.layer_normalization_forward(x.t(), line, line, 8), lambda: ops.bit_layer_normalization_forward(x, line, line, 8, 8),
+                 lambda: ops.layer_normalization_backward(x, x[:20], line, line[:8], line[:8], 8), lambda: ops.layer_normalization_backward(x, x, line, line[:7], line[:8], 8),
+                 lambda: ops.layer_normalization_backward(x, x, line, line[:8], line[:8], 8, dgamma=line), lambda: ops.top_logits(x, 41, 40, 1, 8),
+                 lambda: ops.top_logits(x, 3, 39, 1, 8), lambda: ops.top_logits(x, 0, 40, 1, 8), lambda: ops.loss_distillation(x, i.float(), z, 40, 1, 8),
+                 lambda: ops.loss_distillation(x, i, z[:3], 40, 1, 8), lambda: ops.loss_distillation(x, i, z, 40, 1, 8, weight=x), lambda: ops.loss_distillation(x, i, z, 40, 1, 8, temperature=0.0),
+                 lambda: ops.loss_distillation(x, i[:3].contiguous(), z[:3].contiguous(), 20, 2, 8), lambda: ops.categorical_sampling(x, one, 40, 1, 8, top_size=0),
+                 lambda: ops.categorical_sampling(x, one, 40, 1, 8, top_size=41), lambda: ops.categorical_sampling(x, one, 40, 1, 8, top_size=3, top_p=0.0),
+                 lambda: ops.categorical_sampling(x, one, 40, 1, 8, top_size=3, min_p=2.0), lambda: ops.categorical_sampling(x, one, 40, 1, 8, top_size=3, temperature=-1.0),
+                 lambda: ops.categorical_sampling(x, torch.zeros(1, 16, device="cuda"), 40, 1, 8, top_size=3)):
+        with pytest.raises(BbhipError):
+            call()

@@ -59,7 +59,7 @@ def distill(y=P, index=P, logit=P, weight=P, dy=P, loss=P, t=1.0, ws=1.0, k=4, p
     return (y, index, logit, weight, dy, loss, t, ws, k, pix, ch, frames, s, ls, work, size, None)
 
 
-@pytest.mark.parametrize("what", [dict(y=None), dict(index=None), dict(logit=None), dict(dy=None), dict(loss=None), dict(t=0.0), dict(t=-1.0), dict(t=float("inf")), dict(t=float("nan")),
+@pytest.mark.parametrize("what", [dict(y=None), dict(index=None), dict(logit=None), dict(dy=None), dict(loss=None), dict(t=0.0), dict(t=-1.0), dict(t=float("inf")), dict(t=float("nan")), dict(t=1e-30), dict(t=1e30),
                                   dict(k=0), dict(k=257), dict(pix=-1), dict(ch=0), dict(frames=0), dict(s=8), dict(ls=8), dict(work=None), dict(size=1)])
 def test_distillation_refuses(what):
     assert "LossDistillation" in refused("fp32_LossDistillation", *distill(**what))

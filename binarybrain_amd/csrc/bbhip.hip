@@ -2414,7 +2414,7 @@ int bbhip_fp32_StochasticBatchNormalization_Backward(float const *dev_x_buf, flo
 static int column_space(ColumnSpace &c, TileDivisor &tiles, bool wide, int pix_size, int frame_size, int rows, int batch, char const *name)
 {
     int const per_row = ceil_div(frame_size, wide ? 4 : 1);
-    if ((long long)pix_size * per_row > (1 << 28)) { return fail("%s: too many frames", name); }
+    if ((long long)pix_size * per_row > (1 << 28) || rows > (1 << 30)) { return fail("%s: more than 2^28 units of frames or 2^30 rows", name); }
     c.units_per_row = make_tile_divisor(per_row);
     c.units = pix_size * per_row;
     c.frame_size = frame_size;
@@ -2576,7 +2576,7 @@ static int check_logits(int top_size, int pix_size, int ch_size, int frame_size,
     if (!(top_size > 0 && pix_size > 0 && ch_size > 0 && frame_size > 0)) { return fail("%s: sizes must be positive", name); }
     if (frame_stride < frame_size || list_stride < frame_size) { return fail("%s: frame stride shorter than the frames", name); }
     if (top_size > kTopMost) { return fail("%s: top_size=%d: at most %d", name, top_size, kTopMost); }
-    if ((long long)pix_size * ch_size > 0x7fffffffLL || (long long)pix_size * frame_size > 0x3fffffffLL) { return fail("%s: node count too large", name); }
+    if ((long long)pix_size * ch_size > (1 << 30) || (long long)pix_size * frame_size > (1 << 30) - 4) { return fail("%s: more than 2^30 nodes or places", name); }
     return 0;
 }
 

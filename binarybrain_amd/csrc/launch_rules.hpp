@@ -297,14 +297,15 @@ inline bool layer_norm_whole(int units, int rows, bool wide, bool bit, int &log_
 inline void top_split(int units, int channels, int top_size, int &log_tx, int &tiles, int &slab_rows, int &slabs)
 {
     int const most = 1024 / top_size;
-    int const share = most < ceil_div(channels, 3072) ? most : ceil_div(channels, 3072);
+    int const narrow = 12 * 256, wide = 12 * 128;                       // channels of a column that a workgroup's threads hold, with tiles of one unit and of four
+    int const share = most < ceil_div(channels, narrow) ? most : ceil_div(channels, narrow);
     log_tx = units > 1 && (channels < 512 || (long long)ceil_div(units, 4) * share >= 256) ? 2 : 0;
     tiles = ceil_div(units, 1 << log_tx);
     int want = ceil_div(512, tiles);
     if (want > most) { want = most; }
-    int const held = log_tx ? 1536 : 3072, loads = ceil_div(channels, 1024);
+    int const held = log_tx ? wide : narrow, loads = ceil_div(channels, 1024);
     slab_rows = ceil_div(loads, want < loads ? want : loads) * 1024;
-    if (slab_rows < held) { slab_rows = held; }                         // (what the threads of a workgroup hold: less would take as long)
+    if (slab_rows < held) { slab_rows = held; }                         // (less would take as long)
     slabs = ceil_div(channels, slab_rows);
 }
 

@@ -494,3 +494,27 @@ def test_refusals_on_the_device(ops):
                  lambda: ops.categorical_sampling(x, torch.zeros(1, 16, device="cuda"), 40, 1, 8, top_size=3)):
         with pytest.raises(BbhipError):
             call()
+
+
+def test_buffers_that_do_not_start_on_16_bytes(ops):
+    """the same bits of whole numbers and selections, results as near as elsewhere, from buffers shifted by one float"""
+    import torch
+    rng = np.random.default_rng(42)
+    shifted = lambda a: torch.cat([torch.zeros(1, dtype=dev(a).dtype, device="cuda"), dev(a).reshape(-1)])[1:].view(a.shape)
+    C, F, k = 700, 24, 9
+    y, index, z, w = distill_case(rng, C, F, k)
+    one, zero = np.ones(C, F32), np.zeros(C, F32)
+    t = shifted(y)
+    assert t.data_ptr() % 16 == 4 and t.is_contiguous()
+    got = ops.layer_normalization_forward(t, shifted(one), shifted(zero), F)
+    check_norm(y, one, zero, *(host(a) for a in got), *ref.layer_norm(y, one, zero, float(F32(1e-5))))
+    dx, dg, db = ops.layer_normalization_backward(t, shifted(z[:1] + y), shifted(one), got[1], got[2], F)
+    check_norm_backward(y, z[:1] + y, one, host(got[1]), host(got[2]), host(dx), host(dg), host(db), *ref.layer_norm_backward(y, z[:1] + y, one, host(got[1]), host(got[2])))
+    gi, gv = ops.top_logits(t, k, C, 1, F)
+    wi, wv = ref.top_logits(y, k)
+    assert np.array_equal(host(gi), wi) and np.array_equal(host(gv), wv)
+    dy, loss = ops.loss_distillation(t, shifted(index), shifted(z), C, 1, F, weight=shifted(w[None]), weight_sum=3.0)
+    check_distill(y, index, z, w, 1.0, 3.0, host(dy), host(loss)[0])
+    u = rng.random((1, F)).astype(F32)
+    category, _ = ops.categorical_sampling(t, shifted(u), C, 1, F, top_size=k, top_p=0.8)
+    assert np.array_equal(host(category)[0], ref.sampling(y, u[0], 1.0, k, 0.8, 0.0)[0])

@@ -22,7 +22,7 @@ def norm(x=P, y=P, gamma=P, beta=P, mean=P, rstd=P, eps=1e-5, nodes=20000, frame
 
 
 @pytest.mark.parametrize("what", [dict(x=None), dict(y=None), dict(nodes=0), dict(nodes=-3), dict(frames=0), dict(xs=15), dict(ys=15), dict(eps=-1.0), dict(eps=float("nan")),
-                                  dict(work=None), dict(size=16), dict(work=C.c_void_p((1 << 20) + 16)), dict(nodes=1 << 20, frames=1 << 30, xs=1 << 30, ys=1 << 30)])
+                                  dict(work=None), dict(size=16), dict(work=C.c_void_p((1 << 20) + 16)), dict(nodes=1 << 20, frames=(1 << 30) + 3, xs=(1 << 30) + 3, ys=(1 << 30) + 3), dict(nodes=(1 << 30) + 1)])
 def test_layer_norm_forward_refuses(what):
     assert "LayerNormalization_Forward" in refused("fp32_LayerNormalization_Forward", *norm(**what))
     if what not in (dict(xs=15),):
@@ -50,7 +50,7 @@ def top(y=P, index=P, logit=P, k=4, pix=1, ch=10, frames=16, s=16, ls=16, work=P
 
 
 @pytest.mark.parametrize("what", [dict(y=None), dict(index=None), dict(logit=None), dict(k=0), dict(k=11), dict(k=257, ch=1000), dict(pix=0), dict(ch=-1), dict(frames=0), dict(s=15),
-                                  dict(ls=15), dict(pix=1 << 16, ch=1 << 16), dict(ch=100000, frames=1, work=C.c_void_p((1 << 20) + 64)), dict(ch=100000, frames=1, work=None), dict(ch=100000, frames=1, size=8)])
+                                  dict(ls=15), dict(pix=1 << 16, ch=1 << 16), dict(ch=(1 << 30) + 1), dict(pix=1 << 27), dict(ch=100000, frames=1, work=C.c_void_p((1 << 20) + 64)), dict(ch=100000, frames=1, work=None), dict(ch=100000, frames=1, size=8)])
 def test_top_logits_refuses(what):
     assert "TopLogits" in refused("fp32_TopLogits", *top(**what))
 

@@ -2,7 +2,8 @@
 // not one of the layer's are no entries), the student's logits y, the temperature T and the weight w of the place:
 //   q_j = exp(z_j / T) / sum_j exp(z_j / T),   p_c = exp(y_c / T) / sum_c exp(y_c / T),
 //   loss = w T^2 sum_j q_j (log q_j - log p_{i_j}),   dy_c = w T (p_c - sum_{j : i_j = c} q_j) / weight_sum.
-// A place without entries (or whose kept logits are all minus infinity) and one with w = 0 has loss 0 and gradient 0 whatever its logits are.
+// An entry of minus infinity has no share and is passed over wherever entries are counted: by the table of channels named twice, and by the launch that
+// takes the shares off dy, where it would be a second writer of a channel that an entry with a share names.  A place without entries (or whose kept logits are all minus infinity) and one with w = 0 has loss 0 and gradient 0 whatever its logits are.
 //
 // Two launches.  The first takes, per column and slab of channels, the running maximum m and the sum of exp((y - m) / T) in one pass; workgroups behind
 // those read the lists and leave per column the largest z, the reciprocal of their sum E, the largest listed logit y_r of the student, and
@@ -27,7 +28,7 @@ struct DistillArgs {
     int const   *index;
     float       *dy, *loss;
     float2      *partial;           // [slabs][units * W]: (m, sum)
-    float4      *lists;             // [units * W]: (z_max, 1 / E (0: no entries, negative: a channel is named twice), the lists' part of the loss, y_r)
+    float4      *lists;             // [units * W]: (z_max, 1 / E (0: no entries, sign bit set: a channel is named twice), the lists' part of the loss, y_r)
     float scale;                    // log2(e) / T
     float reciprocal_t, t_square, coefficient;      // 1 / T, T^2, T / weight_sum
     int   top_size, pix_size, frame_stride, list_stride;
@@ -170,7 +171,7 @@ __device__ __forceinline__ void distillation_lists(DistillArgs const &a, int blo
         sum = 0.0f; loss = 0.0f;
         for (int w = 0; w < kColWaves; ++w) { sum += of_wave[w * kListColumns + col].x; loss += of_wave[w * kListColumns + col].y; }
         float const q = any > 0.0f ? 1.0f / sum : 0.0f;
-        a.lists[(size_t)pix * a.c.units_per_row.count * a.unit_width + f] = make_float4(top, twice > 0.0f ? -q : q, loss * a.reciprocal_t / sum - logf(sum), yr);
+        a.lists[(size_t)pix * a.c.units_per_row.count * a.unit_width + f] = make_float4(top, __builtin_copysignf(q, twice > 0.0f ? -1.0f : 1.0f), loss * a.reciprocal_t / sum - logf(sum), yr);
     }
 }
 
@@ -317,16 +318,18 @@ __global__ __launch_bounds__(kColBlock) void distillation_gradient_kernel(Distil
             size_t const here = (size_t)at.pix * a.frame_stride + at.f0 + col % W + (size_t)c * channel;
             float4 const l = a.lists[at.column + col % W];
             float const z = logit[j * entry], yc = a.y[here];
+            if (z == -__builtin_inff()) { continue; }                           // (no share: what stands there is right, or another entry's thread writes it)
             auto weight = [&](float v) { return exp_scaled(v == l.x ? 0.0f : v - reference_of(l.x), a.scale); };
             float q = weight(z);
-            if (l.y < 0.0f) {                                                   // a channel may be named twice: its shares are added in the list's order, by its first entry's thread
+            if (__builtin_signbitf(l.y)) {                                      // a channel may be named twice: its shares are added in the list's order, by its first entry's thread
                 int const *const index = a.index + (size_t)at.pix * a.list_stride + at.f0 + col % W;
                 int first = a.top_size;
                 q = 0.0f;
                 for (int o = 0; o < a.top_size; ++o) {
-                    if (index[o * entry] == c) {
+                    float const zo = logit[o * entry];
+                    if (index[o * entry] == c && !(zo == -__builtin_inff())) {
                         first = first < o ? first : o;
-                        q += weight(logit[o * entry]);
+                        q += weight(zo);
                     }
                 }
                 if (first != j) { continue; }

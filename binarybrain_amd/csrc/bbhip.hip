@@ -2466,7 +2466,7 @@ static int layer_norm_forward(void const *x, bool bit, float *y, float const *ga
                       starts_on_16_bytes(mean) && starts_on_16_bytes(rstd);
     LayerNormArgs a{};
     if (column_space(a.c, a.tiles, wide, 1, frame_size, node_size, kLayerNormBatch, name)) { return 1; }
-    a.x = x; a.out = y; a.gamma = gamma; a.beta = beta; a.mean = mean; a.rstd = rstd; a.eps = eps;
+    a.x = x; a.out = y; a.gamma = gamma; a.beta = beta; a.mean = mean; a.rstd = rstd; a.eps = eps; a.inverse_rows = 1.0 / (double)node_size;
     a.x_stride = x_stride; a.out_stride = y_stride;
     hipStream_t const st = static_cast<hipStream_t>(stream);
     int log_tx;

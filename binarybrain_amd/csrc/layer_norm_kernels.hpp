@@ -6,7 +6,8 @@
 //
 // Means and squared deviations are formed over eight rows at a time and merged pairwise with their counts (the update of Chan, Golub and
 // LeVeque), so a mean that is large against the deviation costs no digits; packed bits are counted, and their squared deviation is
-// ones * zeros / N.  All sums are taken in a fixed order: the same input gives the same bits on every run.
+// ones * zeros / N.  Squares are summed in 32 bits; the square of what float32 holds need not be one itself (values around 1e20 or, with eps 0, deviations of
+// 1e-25), and where a frame's sum leaves the range its deviations are read and squared again in 64 bits.  All sums are taken in a fixed order: the same input gives the same bits on every run.
 //
 // Columns that a workgroup can hold go in one launch (forward; layer_norm_whole in launch_rules.hpp has both sides).  Any other size goes in two: the sums of a slab of rows per workgroup (forward: mean and squared deviation; backward: the two sums per
 // frame and, of the same reading, the two sums per node over the tile's frames), then every workgroup adds up the slabs of its frames and writes.
@@ -26,9 +27,10 @@ struct LayerNormArgs {
     float       *out;               // y or dx
     float const *gamma, *beta;      // NULL: 1 and 0
     float       *mean, *rstd;       // forward: written unless NULL; backward: read
-    float2      *partial;           // [slabs][units * W]: forward (mean, squared deviation) or (ones, -), backward (sum g, sum g xh)
+    float2      *partial;           // [slabs][units * W]: forward (mean, squared deviation; negative: less the root of its mean) or (ones, -), backward (sum g, sum g xh)
     float2      *row_partial;       // [tiles][rows]: (sum dy xh, sum dy)
     float       *dgamma, *dbeta;    // backward
+    double inverse_rows;            // forward
     float eps, reciprocal_rows;
     int   x_stride, out_stride;     // (dy has the pitch of dx)
     int   accumulate;               // dgamma, dbeta: added to
@@ -47,6 +49,22 @@ __device__ __forceinline__ void layer_norm_load(void const *__restrict__ x, int 
     else { column_load<W>(static_cast<float const *>(x) + (size_t)r * stride + f0, v); }
 }
 
+// t = m 4^half with m in [0.5, 2), so that a root is taken in 32 bits whatever the size of t (0, infinities and what is not a number: half 0)
+__device__ __forceinline__ float mantissa_of(double t, int &half)
+{
+    int const e = __builtin_amdgcn_frexp_exp(t) & ~1;
+    half = e / 2;
+    return (float)__builtin_amdgcn_ldexp(t, -e);
+}
+__device__ __forceinline__ float root_of(double t)         { int half; float const m = mantissa_of(t, half); return __builtin_amdgcn_ldexpf(sqrtf(m), half); }
+__device__ __forceinline__ float inverse_root_of(double t) { int half; float const m = mantissa_of(t, half); return __builtin_amdgcn_ldexpf(1.0f / sqrtf(m), -half); }
+
+// A variance (with eps) of this range comes from 32 bits: what underflows in its sum (2^-149 a square) is nothing to it, and nothing has overflowed.
+constexpr float kVarianceLeast = 0x1p-90f, kVarianceMost = 0x1p120f;
+__device__ __forceinline__ bool variance_in_range(float t) { return !(t < kVarianceLeast || t > kVarianceMost); }      // (what is not a number stays it)
+// A slab's sum of squares beyond this is formed again.  It does not get there while no thread's own sum and mean, of 256 or 1024 threads and at most 2^24 rows, are beyond these.
+constexpr float kSquaresMost = 0x1p110f, kThreadSquares = 0x1p98f, kThreadMean = 0x1p40f;
+
 // count, mean and squared deviation of W columns
 template <int W>
 struct Moments {
@@ -59,7 +77,7 @@ struct Moments {
         for (int j = 0; j < W; ++j) {
             float const d = omean[j] - mean[j];
             mean[j] = __builtin_fmaf(d, share, mean[j]);
-            m2[j]   = __builtin_fmaf(d * d, weight, m2[j] + om2[j]);
+            m2[j]   = __builtin_fmaf(d * weight, d, m2[j] + om2[j]);         // (weight 0: nothing, whatever d * d would be)
         }
         n = total;
     }
@@ -127,11 +145,54 @@ __device__ __forceinline__ void add_workgroup(float (&a)[W], float (&b)[W], int 
 
 constexpr int kLayerNormBatch = 8;      // rows that a thread has in flight
 
+// The end of a slab that may have columns whose squares leave the range of 32 bits: theirs are summed in 64 about the slab's mean (wavefront 0's m), the rows are read again.
+// A column's result goes by its own values alone: those in range keep the bits that they have elsewhere.
+template <int W>
+__device__ __forceinline__ void layer_norm_stats_far(LayerNormArgs const &a, ColumnThread<W> const &t, ColumnUnit<W> const &u, Moments<W> const &m, float *share)
+{
+    int const lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, columns = W << a.c.log_tx;       // (no more than threads)
+    __syncthreads();                                                            // (the sums in `share` have been read)
+    if (threadIdx.x < (1u << a.c.log_tx)) {
+#pragma unroll
+        for (int j = 0; j < W; ++j) { share[t.tx * W + j] = m.mean[j]; share[kColShareMax + t.tx * W + j] = m.m2[j]; }
+    }
+    __syncthreads();
+    float mean[W];
+    double s[W] = {};
+#pragma unroll
+    for (int j = 0; j < W; ++j) { mean[j] = share[t.tx * W + j]; }
+    float const of_column = share[threadIdx.x], m2 = share[kColShareMax + threadIdx.x];                // (of column threadIdx.x, if there is one)
+    float const *const x = static_cast<float const *>(a.x) + u.f0;
+#pragma unroll 1
+    for (int row = t.begin + t.lead; row < t.end; row += t.step) {
+        float v[W];
+        column_load<W>(x + (size_t)row * a.x_stride, v);
+#pragma unroll
+        for (int j = 0; j < W; ++j) { double const d = (double)(v[j] - mean[j]); s[j] = __builtin_fma(d, d, s[j]); }
+    }
+    __syncthreads();                                                            // (all have their means)
+    double *const sums = reinterpret_cast<double *>(share);                     // [kColWaves][columns]
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+        for (int o = 1 << a.c.log_tx; o < kWave; o <<= 1) { s[j] += __shfl_xor(s[j], o); }
+        if (lane < (1 << a.c.log_tx)) { sums[wave * columns + t.tx * W + j] = s[j]; }
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < columns && (t.tile << a.c.log_tx) + (int)threadIdx.x / W < a.c.units) {
+        double all = 0.0;
+        for (int w = 0; w < kColWaves; ++w) { all += sums[w * columns + threadIdx.x]; }
+        float const n = (float)(t.end - t.begin);
+        bool const out = m2 > kSquaresMost || (a.eps < kVarianceLeast && m2 < kVarianceLeast * n);
+        a.partial[(size_t)t.slab * (a.c.units * W) + ((size_t)t.tile << a.c.log_tx) * W + threadIdx.x] = make_float2(of_column, out ? -root_of(all / (double)n) : m2);
+    }
+}
+
 // mean and squared deviation (packed bits: the ones) of every column over a slab
 template <int W, bool BIT>
 __global__ __launch_bounds__(kColBlock) void layer_norm_stats_kernel(LayerNormArgs a)
 {
-    __shared__ float share[2 * kColShareMax + kColWaves * kWave];
+    __shared__ __align__(16) float share[2 * kColShareMax + kColWaves * kWave];
+    __shared__ int far[kColWaves];
     ColumnThread<W> const t(a.c, a.tiles, blockIdx.x, gridDim.x);
     ColumnUnit<W> const u(a.c, (t.tile << a.c.log_tx) + t.tx);
     constexpr int B = kLayerNormBatch;
@@ -188,12 +249,40 @@ __global__ __launch_bounds__(kColBlock) void layer_norm_stats_kernel(LayerNormAr
             }
             m.merge(n, mean, m2);
         });
+        bool beyond = false;
+#pragma unroll
+        for (int j = 0; j < W; ++j) { beyond = beyond || (j < u.live && (m.m2[j] > kThreadSquares || fabsf(m.mean[j]) > kThreadMean)); }
+        beyond = __any(beyond);
+        if (threadIdx.x % kWave == 0) { far[threadIdx.x / kWave] = beyond ? 1 : 0; }
         merge_workgroup<W>(m, a.c.log_tx, share);
+        int some = 0;
+#pragma unroll
+        for (int w = 0; w < kColWaves; ++w) { some |= far[w]; }
+        if (some != 0 || a.eps < kVarianceLeast) {                              // workgroup-uniform
+            layer_norm_stats_far<W>(a, t, u, m, share);
+            return;
+        }
         if (writes) {
 #pragma unroll
             for (int j = 0; j < W; ++j) { partial[j] = make_float2(m.mean[j], m.m2[j]); }
         }
     }
+}
+
+// rstd of a column whose variance is beyond the range of 32 bits: its slabs joined in 64.  partial: its entry of the first slab
+__device__ __forceinline__ float layer_norm_join_far(LayerNormArgs const &a, float2 const *partial, size_t pitch)
+{
+    double n = 0.0, mean = 0.0, m2 = 0.0;
+#pragma unroll 1
+    for (int s = 0; s < a.c.slabs; ++s) {
+        float2 const p = partial[s * pitch];
+        int const left = a.c.rows - s * a.c.slab_rows;
+        double const on = (double)(left < a.c.slab_rows ? left : a.c.slab_rows), d = (double)p.x - mean, share = on / (n + on);
+        m2 += (p.y < 0.0f ? (double)p.y * (double)p.y * on : (double)p.y) + d * d * (n * share);
+        mean += d * share;
+        n += on;
+    }
+    return inverse_root_of(__builtin_fma(m2, a.inverse_rows, (double)a.eps));
 }
 
 // y, from the slabs' sums; the workgroups of the first slab write mean and rstd
@@ -230,24 +319,38 @@ __global__ __launch_bounds__(kColBlock) void layer_norm_apply_kernel(LayerNormAr
 #pragma unroll
             for (int j = 0; j < W; ++j) { ones[j] += mean[j]; }
         }
-        else { m.merge((float)(left < a.c.slab_rows ? left : a.c.slab_rows), mean, m2); }
+        else {
+#pragma unroll
+            for (int j = 0; j < W; ++j) { m2[j] = m2[j] < 0.0f ? __builtin_inff() : m2[j]; }            // (formed in 64 bits: below)
+            m.merge((float)(left < a.c.slab_rows ? left : a.c.slab_rows), mean, m2);
+        }
     }
     if constexpr (BIT) { add_workgroup<W>(ones, none, a.c.log_tx, share); }
     else               { merge_workgroup<W>(m, a.c.log_tx, share); }
     __syncthreads();                                                            // (the partial sums in `share` have been read)
     if (threadIdx.x < (1u << a.c.log_tx)) {
+        float var[W], of[W];
+        bool beyond = false;
 #pragma unroll
         for (int j = 0; j < W; ++j) {
-            float mean, var;
+            float mean;
             if constexpr (BIT) {
                 float const rows = (float)a.c.rows;
                 mean = ones[j] / rows;
-                var  = mean * ((rows - ones[j]) / rows);
+                var[j] = mean * ((rows - ones[j]) / rows);
             }
-            else { mean = m.mean[j]; var = fmaxf(0.0f, m.m2[j] / (float)a.c.rows); }
+            else { mean = m.mean[j]; var[j] = m.m2[j] / (float)a.c.rows; beyond = beyond || !variance_in_range(var[j] + a.eps); }
             share[t.tx * W + j] = mean;
-            share[kColShareMax + t.tx * W + j] = 1.0f / sqrtf(var + a.eps);
+            of[j] = 1.0f / sqrtf(var[j] + a.eps);
         }
+        if (beyond) {
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                if (!variance_in_range(var[j] + a.eps)) { of[j] = layer_norm_join_far(a, a.partial + u.column + j, (size_t)a.c.units * W); }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < W; ++j) { share[kColShareMax + t.tx * W + j] = of[j]; }
     }
     __syncthreads();
     float mean[W], rstd[W];
@@ -271,7 +374,8 @@ __global__ __launch_bounds__(kColBlock) void layer_norm_apply_kernel(LayerNormAr
 }
 
 // Forward pass in one launch, for columns that a workgroup of 1024 threads can hold, R = 4 or 16 rows of a unit per thread: x is read once and the mean is known before
-// the deviations are squared.  Packed bits are held as their words.
+// the deviations are squared.  Packed bits are held as their words.  The squares are summed in 32 bits; where a thread's sum shows that a total might leave
+// their range, or eps is so small that squares below it count, the workgroup sums them again in 64.
 constexpr int kWholeBlock = 1024, kWholeWaves = kWholeBlock / kWave;
 
 // the sum over the threads that hold the same unit, in every thread.  share: kWholeWaves * kWave * W floats
@@ -302,21 +406,72 @@ __device__ __forceinline__ void whole_sum(float (&v)[W], int log_tx, float *shar
     }
 }
 
+// The same of one frame of a unit in 64 bits, for the rare call: few registers, so that the common one keeps its own.  share: kWholeWaves * kWave doubles, in use before
+__device__ __forceinline__ double whole_sum_double(double v, int log_tx, double *share)
+{
+    int const lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, tx = lane & ((1 << log_tx) - 1);
+    for (int o = 1 << log_tx; o < kWave; o <<= 1) { v += __shfl_xor(v, o); }
+    __syncthreads();
+    if (lane < (1 << log_tx)) { share[(wave << log_tx) + tx] = v; }
+    __syncthreads();
+    v = 0.0;
+#pragma unroll 1
+    for (int w = 0; w < kWholeWaves; ++w) { v += share[(w << log_tx) + tx]; }
+    return v;
+}
+
+// The rest of the pass for a workgroup with frames whose squares leave the range of 32 bits: theirs are summed in 64, x is read again.  A frame's result goes by its own
+// values alone: those in range have the bits that they have elsewhere.  (Behind a return, so that the common call keeps its registers.)
+template <int W>
+__device__ __forceinline__ void layer_norm_whole_far(LayerNormArgs const &a, ColumnUnit<W> const &u, int ty, int step, float (&mean)[W], float (&var)[W], float (&rstd)[W],
+                                                     double *share)
+{
+    float const *const x = static_cast<float const *>(a.x) + u.f0;
+    double s[W] = {};
+#pragma unroll 1
+    for (int row = ty; row < a.c.rows; row += step) {
+        float v[W];
+        column_load<W>(x + (size_t)row * a.x_stride, v);
+#pragma unroll
+        for (int j = 0; j < W; ++j) { double const d = (double)(v[j] - mean[j]); s[j] = __builtin_fma(d, d, s[j]); }
+    }
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+        double const all = whole_sum_double(s[j], a.c.log_tx, share);
+        if (!variance_in_range(var[j] + a.eps)) { rstd[j] = inverse_root_of(__builtin_fma(all, a.inverse_rows, (double)a.eps)); }
+    }
+    if (ty == 0) {
+        if (a.mean != nullptr) { column_store<W>(a.mean + u.f0, u.live, mean); }
+        if (a.rstd != nullptr) { column_store<W>(a.rstd + u.f0, u.live, rstd); }
+    }
+#pragma unroll 1
+    for (int row = ty; row < a.c.rows; row += step) {
+        float const g = a.gamma != nullptr ? a.gamma[row] : 1.0f, b = a.beta != nullptr ? a.beta[row] : 0.0f;
+        float v[W];
+        column_load<W>(x + (size_t)row * a.x_stride, v);
+#pragma unroll
+        for (int j = 0; j < W; ++j) { v[j] = __builtin_fmaf((v[j] - mean[j]) * rstd[j], g, b); }
+        column_store<W>(a.out + (size_t)row * a.out_stride + u.f0, u.live, v);
+    }
+}
+
 template <int W, int R, bool BIT>
 __global__ __launch_bounds__(kWholeBlock) void layer_norm_whole_kernel(LayerNormArgs a)
 {
     __shared__ __align__(16) float share[2][kWholeBlock * W];
+    __shared__ int far;
     int const tx = threadIdx.x & ((1 << a.c.log_tx) - 1), ty = (int)threadIdx.x >> a.c.log_tx, step = kWholeBlock >> a.c.log_tx;
     ColumnUnit<W> const u(a.c, (xcd_remap(blockIdx.x, gridDim.x) << a.c.log_tx) + tx);
     float const rows = (float)a.c.rows;
     float v[BIT ? 1 : R][W], mean[W] = {}, q[W] = {};
     uint32_t bits[BIT ? R : 1];
+    float const *const mine = static_cast<float const *>(a.x) + (size_t)ty * a.x_stride + u.f0;        // (what is common to a load is added to it in scalar registers)
 #pragma unroll
     for (int i = 0; i < R; ++i) {
         int const row = ty + i * step;
         if constexpr (BIT) { bits[i] = row < a.c.rows ? static_cast<uint32_t const *>(a.x)[(size_t)row * a.x_stride + (u.f0 >> 5)] : 0u; }
         else {
-            if (row < a.c.rows) { column_load<W>(static_cast<float const *>(a.x) + (size_t)row * a.x_stride + u.f0, v[i]); }
+            if (row < a.c.rows) { column_load<W>(mine + (size_t)(i * step) * a.x_stride, v[i]); }
             else {
 #pragma unroll
                 for (int j = 0; j < W; ++j) { v[i][j] = 0.0f; }
@@ -331,6 +486,7 @@ __global__ __launch_bounds__(kWholeBlock) void layer_norm_whole_kernel(LayerNorm
             else               { mean[j] += v[i][j]; }
         }
     }
+    if (threadIdx.x == 0) { far = 0; }                                          // (set behind the barrier in the first sum)
     whole_sum<W>(mean, a.c.log_tx, share[0]);
 #pragma unroll
     for (int j = 0; j < W; ++j) { mean[j] /= rows; }
@@ -347,6 +503,10 @@ __global__ __launch_bounds__(kWholeBlock) void layer_norm_whole_kernel(LayerNorm
                 q[j] = __builtin_fmaf(d, d, q[j]);
             }
         }
+        bool beyond = false;
+#pragma unroll
+        for (int j = 0; j < W; ++j) { beyond = beyond || (j < u.live && q[j] > kThreadSquares); }
+        if (beyond) { far = 1; }
         whole_sum<W>(q, a.c.log_tx, share[1]);
 #pragma unroll
         for (int j = 0; j < W; ++j) { q[j] /= rows; }
@@ -354,13 +514,22 @@ __global__ __launch_bounds__(kWholeBlock) void layer_norm_whole_kernel(LayerNorm
     float rstd[W];
 #pragma unroll
     for (int j = 0; j < W; ++j) { rstd[j] = 1.0f / sqrtf(q[j] + a.eps); }
+    if constexpr (!BIT) {
+        if (far != 0 || a.eps < kVarianceLeast) {                               // workgroup-uniform
+            layer_norm_whole_far<W>(a, u, ty, step, mean, q, rstd, reinterpret_cast<double *>(&share[0][0]));
+            return;
+        }
+    }
     if (ty == 0) {
         if (a.mean != nullptr) { column_store<W>(a.mean + u.f0, u.live, mean); }
         if (a.rstd != nullptr) { column_store<W>(a.rstd + u.f0, u.live, rstd); }
     }
+    int ry = ty;
+    asm volatile("" : "+v"(ry));                                                // (the rows' numbers are formed again: kept over the sums they would cost as many registers)
+    float *const out = a.out + (size_t)ry * a.out_stride + u.f0;
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-        int const row = ty + i * step;
+        int const row = ry + i * step;
         if (row < a.c.rows) {
             float const g = a.gamma != nullptr ? a.gamma[row] : 1.0f, b = a.beta != nullptr ? a.beta[row] : 0.0f;
             float y[W];
@@ -369,7 +538,7 @@ __global__ __launch_bounds__(kWholeBlock) void layer_norm_whole_kernel(LayerNorm
                 float const x = BIT ? (float)((bits[BIT ? i : 0] >> ((u.f0 & 31) + j)) & 1u) : v[BIT ? 0 : i][j];
                 y[j] = __builtin_fmaf((x - mean[j]) * rstd[j], g, b);
             }
-            column_store<W, R <= 4>(a.out + (size_t)row * a.out_stride + u.f0, u.live, y);
+            column_store<W, R <= 4>(out + (size_t)(i * step) * a.out_stride, u.live, y);
         }
     }
 }

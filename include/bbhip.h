@@ -470,7 +470,8 @@ int bbhip_fp32_StochasticBatchNormalization_Backward(float const *dev_x_buf, flo
 /* LayerNormalization: every frame is normalised over all nodes, then each node is mapped by its own gamma and beta (NULL: 1 and 0):
  *     mean = sum x / N, var = sum (x - mean)^2 / N, rstd = 1 / sqrt(var + eps), y = ((x - mean) * rstd) * gamma[node] + beta[node].
  * dev_mean_buf and dev_rstd_buf ([frame_size], what the backward pass needs) may be NULL.  The bit entry reads packed bits as 0 and 1; x_frame_stride counts
- * words there.  y may be x (fp32). */
+ * words there.  y may be x (fp32).  Frames of finite values up to 1e30 have the statistics of the definition, whatever becomes of the squares in 32 bits; a frame that
+ * holds an infinity or what is not a number has no number for rstd and y.  Either is the frame's own: the others keep their bits. */
 size_t bbhip_LayerNormalization_WorkspaceBytes(int node_size, int frame_size);
 int bbhip_fp32_LayerNormalization_Forward(float const *dev_x_buf, float *dev_y_buf, float const *dev_gamma, float const *dev_beta, float *dev_mean_buf,
                                           float *dev_rstd_buf, float eps, int node_size, int frame_size, int x_frame_stride, int y_frame_stride,

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import head_reference as ref
-from test_gpu_head_operators import F32, as_rows, check_distill, columns, distill_case, ops  # noqa: F401 (ops: the fixture)
+from test_gpu_head_operators import F32, check_distill, check_norm, check_norm_backward, distill_case, ops  # noqa: F401 (ops: the fixture)
 from util import dev, host
 
 pytestmark = pytest.mark.gpu
@@ -39,3 +39,58 @@ def test_distillation_of_lists_padded_with_minus_infinity(ops, shape):
     for _ in range(3):
         again = call()
         assert np.array_equal(again[0], dy) and np.array_equal(again[1], loss)
+
+
+# ---- layer normalisation of far values -------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("nodes", [100, 1000, 20000])                         # one launch, one launch, two
+@pytest.mark.parametrize("frames", [9, 12])                                  # rows that start on 4 bytes, on 16
+@pytest.mark.parametrize("kind", [(1e20, 0.01, 1e-5), (1e30, 0.01, 1e-5), (-1e30, 1.0, 1e-5), (1e18, 1.0, 1e-5), (1e-20, 0.01, 0.0), (1e-25, 1.0, 0.0), (1e-3, 1.0, 1e-5)])
+def test_layer_norm_of_far_values(ops, nodes, frames, kind):
+    """values whose squares leave the range of float32, upwards and (with eps 0) downwards: statistics and y are those of the definition all the same.
+    A rounding of the mean is at most U of the largest value, 100 of them 6e-6 of it: with deviations of 1 % of the values 6e-4 of the deviation, which check_norm counts."""
+    scale, spread, eps = kind
+    rng = np.random.default_rng(nodes + frames)
+    x = (scale * (1.0 + spread * rng.standard_normal((nodes, frames)))).astype(F32)
+    gamma, beta = (1 + 0.3 * rng.standard_normal(nodes)).astype(F32), rng.standard_normal(nodes).astype(F32)
+    y, mean, rstd = ops.layer_normalization_forward(dev(x), dev(gamma), dev(beta), frames, eps=eps)
+    check_norm(x, gamma, beta, host(y), host(mean), host(rstd), *ref.layer_norm(x, gamma, beta, float(F32(eps))))
+    assert np.all(np.abs(host(rstd) / ref.layer_norm(x, gamma, beta, float(F32(eps)))[2] - 1) < 1e-4)
+    # what the forward pass leaves serves the backward pass
+    dy = rng.standard_normal((nodes, frames)).astype(F32)
+    dx, dgamma, dbeta = ops.layer_normalization_backward(dev(x), dev(dy), dev(gamma), mean, rstd, frames)
+    check_norm_backward(x, dy, gamma, host(mean), host(rstd), host(dx), host(dgamma), host(dbeta), *ref.layer_norm_backward(x, dy, gamma, host(mean), host(rstd)))
+
+
+@pytest.mark.parametrize("nodes", [300, 20000])
+@pytest.mark.parametrize("frames", [40, 41])
+def test_layer_norm_of_frames_that_are_not_finite(ops, nodes, frames):
+    """rstd of a frame that holds an infinity or what is not a number is not a number, in one launch and in two, and so is all of its y; the others keep their bits"""
+    rng = np.random.default_rng(nodes)
+    x = rng.standard_normal((nodes, frames)).astype(F32)
+    clean = [host(a) for a in ops.layer_normalization_forward(dev(x), None, None, frames)]
+    x[17, 3], x[250, 21], x[0, 22], x[nodes - 1, 30] = np.nan, np.inf, -np.inf, np.nan
+    y, mean, rstd = (host(a) for a in ops.layer_normalization_forward(dev(x), None, None, frames))
+    touched = np.isin(np.arange(frames), (3, 21, 22, 30))
+    assert np.all(np.isnan(rstd[touched])) and not np.any(np.isfinite(mean[touched])) and np.all(np.isnan(y[:, touched]))
+    assert np.array_equal(y[:, ~touched], clean[0][:, ~touched]) and np.array_equal(mean[~touched], clean[1][~touched]) and np.array_equal(rstd[~touched], clean[2][~touched])
+
+
+@pytest.mark.parametrize("nodes", [100, 300, 3000, 20000])
+@pytest.mark.parametrize("frames", [40, 41])
+@pytest.mark.parametrize("eps", [1e-5, 0.0])
+def test_layer_norm_of_far_frames_among_others(ops, nodes, frames, eps):
+    """far values in all rows of a frame, in half of them and in one: that frame's statistics follow the definition, every other frame keeps its bits"""
+    rng = np.random.default_rng(nodes)
+    x = rng.standard_normal((nodes, frames)).astype(F32)
+    gamma, beta = (1 + 0.3 * rng.standard_normal(nodes)).astype(F32), rng.standard_normal(nodes).astype(F32)
+    clean = [host(a) for a in ops.layer_normalization_forward(dev(x), dev(gamma), dev(beta), frames, eps=eps)]
+    x[:, 5] = 1e25 * (np.arange(nodes) - nodes / 3)
+    x[nodes // 2:, 6] = 1e28
+    x[nodes - 2, 7] = -1e29
+    x[:, 18] *= F32(1e-25)
+    y, mean, rstd = (host(a) for a in ops.layer_normalization_forward(dev(x), dev(gamma), dev(beta), frames, eps=eps))
+    wy, wmean, wrstd = ref.layer_norm(x, gamma, beta, float(F32(eps)))
+    check_norm(x, gamma, beta, y, mean, rstd, wy, wmean, wrstd)
+    assert np.all(np.abs(rstd / wrstd - 1) < 1e-4)
+    same = ~np.isin(np.arange(frames), (5, 6, 7, 18))
+    assert np.array_equal(y[:, same], clean[0][:, same]) and np.array_equal(mean[same], clean[1][same]) and np.array_equal(rstd[same], clean[2][same])

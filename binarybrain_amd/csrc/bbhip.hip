@@ -2410,17 +2410,23 @@ int bbhip_fp32_StochasticBatchNormalization_Backward(float const *dev_x_buf, flo
 }
 
 // ---- operators down the columns: LayerNormalization, LossDistillation, TopLogits, CategoricalSampling ----
+static int check_launch(long long workgroups, int threads, char const *name)
+{
+    if (!launch_holds(workgroups, threads)) { return fail("%s: a launch of %lld workgroups of %d threads: 2^32 threads or more", name, workgroups, threads); }
+    return 0;
+}
+
 // How a call divides `pix_size * frame_size` columns of `rows` rows among workgroups.  `wide`: units of four frames.  `batch`: rows that a thread reads at a time.
 static int column_space(ColumnSpace &c, TileDivisor &tiles, bool wide, int pix_size, int frame_size, int rows, int batch, char const *name)
 {
     int const per_row = ceil_div(frame_size, wide ? 4 : 1);
-    if ((long long)pix_size * per_row > (1 << 28) || rows > (1 << 30)) { return fail("%s: more than 2^28 units of frames or 2^30 rows", name); }
+    if ((long long)pix_size * per_row > (1 << 28) || rows > (1 << 30)) { return fail("%s: more than 2^28 places (in fours where rows start on 16 bytes) or 2^30 nodes", name); }
     c.units_per_row = make_tile_divisor(per_row);
     c.units = pix_size * per_row;
     c.frame_size = frame_size;
     c.rows = rows;
     column_split(c.units, rows, wide, batch, c.log_tx, c.tiles, c.slab_rows, c.slabs);
-    if ((long long)c.tiles * c.slabs > 0x3fffffffLL) { return fail("%s: grid too large", name); }
+    if (check_launch((long long)c.tiles * c.slabs, kColBlock, name)) { return 1; }
     tiles = make_tile_divisor(c.tiles);
     return 0;
 }
@@ -2445,7 +2451,7 @@ size_t bbhip_LayerNormalization_WorkspaceBytes(int node_size, int frame_size)
         bool const wide = (form & 1) != 0, backward = (form & 2) != 0;
         ColumnSpace c;
         TileDivisor tiles;
-        if (column_space(c, tiles, wide, 1, frame_size, node_size, backward ? kLayerNormBatch / 2 : kLayerNormBatch, __func__)) { return 0; }
+        if (column_space(c, tiles, wide, 1, frame_size, node_size, backward ? kLayerNormBatch / 2 : kLayerNormBatch, __func__)) { continue; }        // (a form that is refused)
         int log_tx;
         bool longer;
         if (!backward && layer_norm_whole(c.units, node_size, wide, true, log_tx, longer)) { continue; }          // (of packed bits and of fp32: the former need no less)
@@ -2529,6 +2535,7 @@ static int layer_norm_backward(void const *x, bool bit, float const *dy, float *
     LayerNormArgs a{};
     if (column_space(a.c, a.tiles, wide, 1, frame_size, node_size, kLayerNormBatch / 2, name)) { return 1; }
     bool const weights = dgamma != nullptr || dbeta != nullptr;
+    if (check_launch((long long)a.c.tiles * a.c.slabs + (weights ? ceil_div(node_size, kWave) : 0), kColBlock, name)) { return 1; }
     size_t const partial = layer_norm_partial_bytes(a.c, wide);
     if (check_workspace(workspace, workspace_size, partial + (weights ? (size_t)a.c.tiles * node_size * sizeof(float2) : 0), name)) { return 1; }
     a.x = x; a.dy = dy; a.out = dx; a.gamma = gamma; a.mean = const_cast<float *>(mean); a.rstd = const_cast<float *>(rstd);
@@ -2571,26 +2578,30 @@ int bbhip_bit_fp32_LayerNormalization_Backward(int const *dev_x_buf, float const
 }
 
 // what the operators on logits ask of their sizes
+constexpr int kPlacesMost = (1 << 30) - 4;          // (in fours they are counted by an int)
 static int check_logits(int top_size, int pix_size, int ch_size, int frame_size, int frame_stride, int list_stride, char const *name)
 {
     if (!(top_size > 0 && pix_size > 0 && ch_size > 0 && frame_size > 0)) { return fail("%s: sizes must be positive", name); }
     if (frame_stride < frame_size || list_stride < frame_size) { return fail("%s: frame stride shorter than the frames", name); }
     if (top_size > kTopMost) { return fail("%s: top_size=%d: at most %d", name, top_size, kTopMost); }
-    if ((long long)pix_size * ch_size > (1 << 30) || (long long)pix_size * frame_size > (1 << 30) - 4) { return fail("%s: more than 2^30 nodes or places", name); }
+    if ((long long)pix_size * ch_size > (1 << 30) || (long long)pix_size * frame_size > kPlacesMost) { return fail("%s: more than 2^30 nodes or places", name); }
     return 0;
 }
 
 // ---- LossDistillation ----
+// of the first launch: the sums' and behind them the lists'
+static long long distillation_workgroups(ColumnSpace const &c, int places) { return (long long)c.tiles * c.slabs + ceil_div(places, kListColumns); }
 static size_t distillation_partial_bytes(ColumnSpace const &c, bool wide) { return align256((size_t)c.slabs * c.units * (wide ? 4 : 1) * sizeof(float2)); }
 
 size_t bbhip_LossDistillation_WorkspaceBytes(int pix_size, int ch_size, int frame_size)
 {
-    if (pix_size <= 0 || ch_size <= kDistillFew || frame_size <= 0) { return 0; }
+    if (pix_size <= 0 || ch_size <= kDistillFew || frame_size <= 0 || (long long)pix_size * frame_size > kPlacesMost) { return 0; }
     size_t most = 0;
     for (int wide = 0; wide < 2; ++wide) {
         ColumnSpace c;
         TileDivisor tiles;
-        if (column_space(c, tiles, wide != 0, pix_size, frame_size, ch_size, 8, __func__)) { return 0; }
+        if (column_space(c, tiles, wide != 0, pix_size, frame_size, ch_size, 8, __func__) ||
+            check_launch(distillation_workgroups(c, pix_size * frame_size), kColBlock, __func__)) { continue; }         // (a form that is refused)
         size_t const bytes = distillation_partial_bytes(c, wide != 0) + (size_t)c.units * (wide ? 4 : 1) * sizeof(float4);
         most = bytes > most ? bytes : most;
     }
@@ -2609,6 +2620,7 @@ int bbhip_fp32_LossDistillation(float const *dev_y_buf, int const *dev_index_buf
     bool const wide = !few && frame_size >= 4 && frame_stride % 4 == 0 && starts_on_16_bytes(dev_y_buf) && starts_on_16_bytes(dev_dy_buf) && starts_on_16_bytes(dev_loss_buf);
     DistillArgs a{};
     if (column_space(a.c, a.tiles, wide, pix_size, frame_size, ch_size, 8, __func__)) { return 1; }
+    if (!few && check_launch(distillation_workgroups(a.c, pix_size * frame_size), kColBlock, __func__)) { return 1; }
     size_t const partial = few ? 0 : distillation_partial_bytes(a.c, wide);
     if (check_workspace(dev_workspace, workspace_size, few ? 0 : partial + (size_t)a.c.units * (wide ? 4 : 1) * sizeof(float4), __func__)) { return 1; }
     a.frames = make_tile_divisor(frame_size);
@@ -2623,7 +2635,7 @@ int bbhip_fp32_LossDistillation(float const *dev_y_buf, int const *dev_index_buf
     a.main_blocks = a.c.tiles * a.c.slabs; a.unit_width = wide ? 4 : 1;
     hipStream_t const st = static_cast<hipStream_t>(stream);
     ScopedTimer tm(kTimeOther, st);
-    dim3 const grid((unsigned)a.main_blocks), sums((unsigned)(a.main_blocks + ceil_div(pix_size * frame_size, kListColumns))), block(kColBlock);
+    dim3 const grid((unsigned)a.main_blocks), sums((unsigned)distillation_workgroups(a.c, pix_size * frame_size)), block(kColBlock);
     if (few) {
         dim3 const columns((unsigned)ceil_div(a.c.units, kWave)), lane(kWave);
         if (ch_size <= 8)       { launch((distillation_few_kernel<8>), columns, lane, 0, st, a); }
@@ -2652,7 +2664,7 @@ static int top_space(TopArgs &a, bool wide, int top_size, int pix_size, int ch_s
     a.c.frame_size = frame_size;
     a.c.rows = ch_size;
     top_split(a.c.units, ch_size, top_size, a.c.log_tx, a.c.tiles, a.c.slab_rows, a.c.slabs);
-    if ((long long)a.c.tiles * a.c.slabs > 0x3fffffffLL) { return fail("%s: grid too large", name); }
+    if (check_launch((long long)a.c.tiles * a.c.slabs, a.c.log_tx ? kTopRows<4> * 4 : kTopRows<1>, name)) { return 1; }
     a.tiles = make_tile_divisor(a.c.tiles);
     a.entries = make_tile_divisor(top_size);
     return 0;
@@ -2669,7 +2681,7 @@ size_t bbhip_TopLogits_WorkspaceBytes(int top_size, int pix_size, int ch_size, i
     size_t most = 0;
     for (int wide = 0; wide < 2; ++wide) {
         TopArgs a{};
-        if (top_space(a, wide != 0, top_size, pix_size, ch_size, frame_size, __func__)) { return 0; }
+        if (top_space(a, wide != 0, top_size, pix_size, ch_size, frame_size, __func__)) { continue; }        // (a form that is refused)
         size_t const bytes = top_candidate_bytes(a, wide != 0, top_size);
         most = bytes > most ? bytes : most;
     }

@@ -255,6 +255,9 @@ inline int pool_shared_rows(int lanes, long long nodes)
     return (lanes > 32 && (nodes <= 256 || (nodes > 16384 && full))) ? 1 : 256 / lanes;
 }
 
+// What a launch can hold: fewer than 2^32 threads.
+inline bool launch_holds(long long workgroups, int threads) { return workgroups > 0 && workgroups <= 0xffffffffLL / threads; }
+
 // How the operators down the columns divide `units` (of four frames, or of one) and `rows` among workgroups of 256 threads: tiles of 2^log_tx units, slabs of rows.
 // Sixteen units of four frames are a segment of 256 bytes of a row, 64 of one frame likewise; fewer where there are fewer, up to 64 where few rows leave a workgroup little to do (backward pass
 // of 64 nodes x 65536 frames 28.1 us with 16 units, 19.9 with 64; x 524288 249 and 136; 1024 x 8192 31.9 and 39.9).  Slabs until the launch has
@@ -287,6 +290,7 @@ inline bool layer_norm_whole(int units, int rows, bool wide, bool bit, int &log_
     while (log_tx > narrowest && (rows > 4 * (1024 >> log_tx) || ceil_div(units, 1 << log_tx) < 256)) { --log_tx; }
     longer = rows > 4 * (1024 >> log_tx);
     int const tiles = ceil_div(units, 1 << log_tx);
+    if (!launch_holds(tiles, 1024)) { return false; }
     if (longer) { return !bit && rows <= 16 * (1024 >> log_tx) && tiles >= 256 && tiles <= 512; }
     return log_tx > narrowest || (long long)units * rows <= (wide ? 6 << 20 : 24 << 20);        // 96 MiB
 }

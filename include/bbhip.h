@@ -465,7 +465,10 @@ int bbhip_fp32_StochasticBatchNormalization_Backward(float const *dev_x_buf, flo
  * (NULL where that is 0).  It needs no clearing, holds nothing between calls and may be shared by calls that follow one another on a stream; calls that may
  * overlap (two streams, two graphs) take one each.  Every sum is taken in a fixed order: the same input gives the same bits on every run.  Padding behind the
  * last frame of a row is not written and counts for nothing; where rows start on 16 bytes (buffers and strides) they are read four frames at a time, up to three floats
- * of padding among them.  Buffers must not overlap unless an entry says so.  At most 2^30 nodes, and 2^28 places (pixels times frames; in fours where rows start on 16 bytes). */
+ * of padding among them.  Buffers must not overlap unless an entry says so.  A launch has fewer than 2^32 threads, which bounds what a call can serve; more is refused before
+ * anything is launched, and its ..._WorkspaceBytes is 0.  With `places` for pixels times frames, counted in fours where rows start on 16 bytes: 2^28 - 16 places and 2^30 nodes,
+ * except for the gradients of LayerNormalization's weights (2^29 nodes) and, of more than 32 channels, for TopLogits and CategoricalSampling (2^25 - 4 places) and
+ * LossDistillation (2^25 places whether in fours or not). */
 
 /* LayerNormalization: every frame is normalised over all nodes, then each node is mapped by its own gamma and beta (NULL: 1 and 0):
  *     mean = sum x / N, var = sum (x - mean)^2 / N, rstd = 1 / sqrt(var + eps), y = ((x - mean) * rstd) * gamma[node] + beta[node].

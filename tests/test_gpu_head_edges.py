@@ -4,7 +4,8 @@ import numpy as np
 import pytest
 
 import head_reference as ref
-from test_gpu_head_operators import F32, check_distill, check_norm, check_norm_backward, distill_case, ops  # noqa: F401 (ops: the fixture)
+from head_reference import U
+from test_gpu_head_operators import F32, check_distill, check_norm, check_norm_backward, distill_case, near, ops  # noqa: F401 (ops: the fixture)
 from util import dev, host
 
 pytestmark = pytest.mark.gpu
@@ -94,3 +95,48 @@ def test_layer_norm_of_far_frames_among_others(ops, nodes, frames, eps):
     assert np.all(np.abs(rstd / wrstd - 1) < 1e-4)
     same = ~np.isin(np.arange(frames), (5, 6, 7, 18))
     assert np.array_equal(y[:, same], clean[0][:, same]) and np.array_equal(mean[same], clean[1][same]) and np.array_equal(rstd[same], clean[2][same])
+
+
+# ---- near the ends of the ranges -------------------------------------------------------------------------------------------------------
+def test_layer_norm_of_more_than_2_28_frames(ops):
+    """what only the form with rows on 16 bytes serves; dgamma against sums in 64 bits, 2^18 tiles of 256 frames in a chain"""
+    import torch
+    nodes, F = 2, (1 << 28) + 8
+    gen = torch.Generator(device="cuda"); gen.manual_seed(2)
+    x, dy = torch.randn((nodes, F), generator=gen, device="cuda"), torch.randn((nodes, F), generator=gen, device="cuda")
+    gamma, beta = np.array([1.5, 0.5], F32), np.array([-1.0, 2.0], F32)
+    y, mean, rstd = ops.layer_normalization_forward(x, dev(gamma), dev(beta), F)
+    dx, dgamma, dbeta = ops.layer_normalization_backward(x, dy, dev(gamma), mean, rstd, F)
+    for part in (slice(0, 2000), slice((1 << 28) - 1000, F)):
+        v, d, m, r = host(x[:, part]), host(dy[:, part]), host(mean[part]), host(rstd[part])
+        check_norm(v, gamma, beta, host(y[:, part]), m, r, *ref.layer_norm(v, gamma, beta, float(F32(1e-5))))
+        wdx, wdg, wdb = ref.layer_norm_backward(v, d, gamma, m, r)
+        check_norm_backward(v, d, gamma, m, r, host(dx[:, part]), wdg, wdb, wdx, wdg, wdb)
+    for n in range(nodes):
+        each = dy[n].double() * ((x[n].double() - mean.double()) * rstd.double())
+        near(float(dgamma[n]), float(each.sum()), (2 ** 18 + 200) * U * float(each.abs().sum()), "dgamma")
+        near(float(dbeta[n]), float(dy[n].double().sum()), (2 ** 18 + 200) * U * float(dy[n].abs().double().sum()), "dbeta")
+
+
+def test_logits_of_many_places(ops):
+    """33 channels: 2^25 places of distillation, 2^27 - 16 of selection in fours"""
+    import torch
+    C, k = 33, 2
+    gen = torch.Generator(device="cuda"); gen.manual_seed(3)
+    F = 1 << 25
+    y = torch.randn((C, F), generator=gen, device="cuda")
+    index, logit = ops.top_logits(y, k, C, 1, F)
+    dy, loss = ops.loss_distillation(y, index, logit, C, 1, F, temperature=2.0, weight_sum=3.0)
+    for part in (slice(0, 500), slice(F // 2 - 250, F // 2 + 250), slice(F - 500, F)):
+        v = host(y[:, part])
+        wi, wv = ref.top_logits(v, k)
+        assert np.array_equal(host(index[:, part]), wi) and np.array_equal(host(logit[:, part]), wv)
+        check_distill(v, wi, wv, np.ones(500, F32), 2.0, 3.0, host(dy[:, part]), host(loss[:, part])[0])
+    del y, dy, loss, index, logit
+    F = (1 << 27) - 16
+    y, u = torch.randn((C, F), generator=gen, device="cuda"), torch.rand((1, F), generator=gen, device="cuda")
+    category, share = ops.categorical_sampling(y, u, C, 1, F, top_size=k)
+    for part in (slice(0, 500), slice(F // 2 - 250, F // 2 + 250), slice(F - 500, F)):
+        wc, ws = ref.sampling(host(y[:, part]), host(u[0, part]), 1.0, k, 1.0, 0.0)
+        assert np.array_equal(host(category[0, part]), wc)
+        near(host(share[0, part]), ws, 2 * U * ws, "share")

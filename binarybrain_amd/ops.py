@@ -485,10 +485,12 @@ def loss_distillation(y, index, logit, ch_size, pix_size, frame_size, temperatur
     return native.loss_distillation(y, index, logit, ch_size, pix_size, frame_size, temperature, weight, weight_sum)
 
 
-def categorical_sampling(y, u, ch_size, pix_size, frame_size, temperature=1.0, top_size=50, top_p=1.0, min_p=0.0, want_share=True):
-    """A channel of every pixel and frame drawn from softmax(y / temperature) by the given u in [0, 1) ([pix, stride]), among the top_size (at most 256) largest
-    logits, of them the shortest prefix that holds top_p of their probability, of it those of at least min_p times the largest probability:
+def categorical_sampling(y, u, ch_size, pix_size, frame_size, temperature=1.0, top_size=None, top_p=1.0, min_p=0.0, want_share=True):
+    """A channel of every pixel and frame drawn from softmax(y / temperature) by the given u in [0, 1) ([pix, stride]), among the top_size (at most 256; None: 50, of fewer channels
+    all) largest logits, of them the shortest prefix that holds top_p of their probability, of it those of at least min_p times the largest probability:
     (category int32 [pix, stride], -1 where nothing can be drawn, share float32 or None)."""
+    if top_size is None:
+        top_size = min(50, ch_size)
     return native.categorical_sampling(y, u, ch_size, pix_size, frame_size, temperature, top_size, top_p, min_p, want_share)
 
 

@@ -140,3 +140,15 @@ def test_logits_of_many_places(ops):
         wc, ws = ref.sampling(host(y[:, part]), host(u[0, part]), 1.0, k, 1.0, 0.0)
         assert np.array_equal(host(category[0, part]), wc)
         near(host(share[0, part]), ws, 2 * U * ws, "share")
+
+
+# ---- defaults --------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("C", [1, 10, 49, 50, 51, 300])
+def test_sampling_with_the_defaults(ops, C):
+    """50 of the largest logits, or all of fewer channels"""
+    rng = np.random.default_rng(C)
+    y, u = (3 * rng.standard_normal((C, 40))).astype(F32), rng.random(40).astype(F32)
+    category, share = ops.categorical_sampling(dev(y), dev(u[None]), C, 1, 40)
+    wc, ws = ref.sampling(y, u, 1.0, min(C, 50), 1.0, 0.0)
+    assert np.array_equal(host(category)[0], wc)
+    near(host(share)[0], ws, 2 * U * ws, "share")

@@ -52,6 +52,46 @@ static void test_rules(void)
     }
 }
 
+// the variants that the tests of large calls are there for (test_gpu_head_edges.py): a rule that is tuned again must not leave a kernel without them
+static void test_variants(void)
+{
+    // nodes, frames, rows on 16 bytes, one launch with 16 rows per thread
+    struct { int nodes, frames; bool wide, longer; } const norms[] = {
+        {1025, 4097, true, true}, {1100, 4099, true, true}, {4096, 8190, true, true}, {257, 4097, false, true}, {1024, 8191, false, true},
+        {4097, 8190, true, false}, {3000, 8193, true, false}, {1025, 8191, false, false}};
+    for (auto const &n : norms) {
+        int log_tx = 0;
+        bool longer = false;
+        bool const whole = bbhip::layer_norm_whole(n.wide ? (n.frames + 3) / 4 : n.frames, n.nodes, n.wide, false, log_tx, longer);
+        check(n.longer ? whole && longer : !whole, "layer norm of long columns", n.nodes, n.frames);
+    }
+    // channels, frames, rows on 16 bytes, k, slabs: all with four units side by side
+    struct { int channels, frames; bool wide; int top, slabs; } const tops[] = {
+        {3100, 2050, true, 64, 3}, {3100, 2050, true, 200, 3}, {10000, 1030, true, 100, 5}, {2000, 1025, false, 40, 2}, {3200, 2050, false, 120, 1}, {2500, 2050, false, 7, 1}};
+    for (auto const &t : tops) {
+        int log_tx = 0, tiles = 0, slab_rows = 0, slabs = 0;
+        bbhip::top_split(t.wide ? (t.frames + 3) / 4 : t.frames, t.channels, t.top, log_tx, tiles, slab_rows, slabs);
+        check(log_tx == 2 && slabs == t.slabs, "selection of large calls", t.channels, slabs);
+    }
+}
+
+// what a launch cannot hold, no rule asks of it
+static void test_launches(void)
+{
+    check(bbhip::launch_holds((1LL << 24) - 1, 256) && !bbhip::launch_holds(1LL << 24, 256) && !bbhip::launch_holds(0, 64) && !bbhip::launch_holds(1LL << 40, 1024), "launch_holds");
+    for (int rows = 1; rows <= 4096; rows = rows < 64 ? rows + 1 : rows * 2) {
+        for (int units = 1 << 20; units <= 1 << 28; units *= 2) {
+            int log_tx = 0;
+            bool longer = false;
+            for (int form = 0; form < 4; ++form) {
+                if (bbhip::layer_norm_whole(units, rows, (form & 1) != 0, (form & 2) != 0, log_tx, longer)) {
+                    check(bbhip::launch_holds((units + (1LL << log_tx) - 1) >> log_tx, 1024), "one launch of layer norm", units, rows);
+                }
+            }
+        }
+    }
+}
+
 static void test_objects(void)
 {
     auto layer = bb::LayerNormalization<float, float>::Create(0.125f);
@@ -229,7 +269,7 @@ static void test_chain(int ch, int pix, int frames)
 int main(int argc, char **argv)
 {
     try {
-        if (argc > 1 && std::strcmp(argv[1], "--rules") == 0) { test_rules(); test_objects(); }
+        if (argc > 1 && std::strcmp(argv[1], "--rules") == 0) { test_rules(); test_variants(); test_launches(); test_objects(); }
         else {
             if (!bb::Manager::IsDeviceAvailable()) { std::printf("no device available\n"); return 2; }
             test_objects();

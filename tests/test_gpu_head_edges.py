@@ -5,7 +5,7 @@ import pytest
 
 import head_reference as ref
 from head_reference import U
-from test_gpu_head_operators import F32, check_distill, check_norm, check_norm_backward, distill_case, near, ops  # noqa: F401 (ops: the fixture)
+from test_gpu_head_operators import F32, check_distill, check_norm, check_norm_backward, distill_case, logits_of, near, ops, padded, same_values  # noqa: F401 (ops: the fixture)
 from util import dev, host
 
 pytestmark = pytest.mark.gpu
@@ -152,3 +152,69 @@ def test_sampling_with_the_defaults(ops, C):
     wc, ws = ref.sampling(y, u, 1.0, min(C, 50), 1.0, 0.0)
     assert np.array_equal(host(category)[0], wc)
     near(host(share)[0], ws, 2 * U * ws, "share")
+
+
+# ---- variants that only large calls take (tests/cpp/test_head.cpp --rules holds that these shapes take them) ----------------------------
+@pytest.mark.parametrize("shape", [(1025, 4097, 4100), (1100, 4099, 4100), (4096, 8190, 8192), (257, 4097, 4097), (1024, 8191, 8191),      # 16 rows per thread, of four frames and of one
+                                   (4097, 8190, 8192), (3000, 8193, 8196), (1025, 8191, 8191)])                                            # just beyond: two launches
+def test_layer_norm_of_long_columns(ops, shape):
+    nodes, F, stride = shape
+    rng = np.random.default_rng(nodes)
+    x = (rng.standard_normal((nodes, F), dtype=F32) * rng.uniform(0.5, 3, F).astype(F32) + rng.uniform(-4, 4, F).astype(F32))
+    gamma, beta = (1 + 0.3 * rng.standard_normal(nodes)).astype(F32), rng.standard_normal(nodes).astype(F32)
+    given = dev(padded(x, stride))
+    y, mean, rstd = ops.layer_normalization_forward(given, dev(gamma), dev(beta), F)
+    got, mean, rstd = host(y)[:, :F], host(mean), host(rstd)
+    for at in range(0, F, 1024):                                             # (in parts: 64-bit copies of the whole are large)
+        part = slice(at, at + 1024)
+        check_norm(x[:, part], gamma, beta, got[:, part], mean[part], rstd[part], *ref.layer_norm(x[:, part], gamma, beta, float(F32(1e-5))))
+    # in place, without statistics: the same bits, and the padding stays
+    from binarybrain_amd import capi
+    import torch
+    work = torch.empty(max(int(capi.lib().bbhip_LayerNormalization_WorkspaceBytes(nodes, F)), 1), dtype=torch.uint8, device="cuda")
+    p, g, b = capi.ptr, dev(gamma), dev(beta)
+    capi.check(capi.lib().bbhip_fp32_LayerNormalization_Forward(p(given), p(given), p(g), p(b), None, None, 1e-5, nodes, F, stride, stride, p(work), work.numel(), capi.stream_ptr()))
+    torch.cuda.synchronize()
+    again = host(given)
+    assert np.array_equal(again[:, :F], got) and np.all(np.isnan(again[:, F:]))
+
+
+SCAN_SHAPES = [
+    # channels, frames, stride, k: four units of a row side by side, of four frames where the pitch allows
+    (3100, 2050, 2052, 64), (3100, 2050, 2052, 200), (10000, 1030, 1032, 100),       # several slabs and the join, bounds from 256 and from 512 groups
+    (2000, 1025, 1025, 40), (3200, 2050, 2051, 120), (2500, 2050, 2051, 7),          # one frame per thread; one slab in several rounds
+]
+
+
+def sorted_logits(y, k):
+    """the operator's order by a stable sort of 64-bit numbers: infinity for what is not a number, the next below for infinity"""
+    v = y.astype(np.float64) + 0.0
+    v = np.where(np.isnan(v), np.inf, np.where(v == np.inf, 1e308, v))
+    order = np.argsort(-np.ascontiguousarray(v.T), axis=1, kind="stable")[:, :k].T.astype(np.int32)
+    return order, np.take_along_axis(y, order, 0)
+
+
+@pytest.mark.parametrize("shape", SCAN_SHAPES)
+@pytest.mark.parametrize("kind", ["random", "equal", "constant", "ascending", "descending", "special"])
+def test_top_logits_of_large_calls(ops, shape, kind):
+    C, F, stride, k = shape
+    y = logits_of(kind, np.random.default_rng(C + F), (C, F))
+    index, logit = ops.top_logits(dev(padded(y, stride, np.inf)), k, C, 1, F)
+    wi, wv = sorted_logits(y, k)
+    assert np.array_equal(host(index)[:, :F], wi) and same_values(host(logit)[:, :F], wv)
+
+
+@pytest.mark.parametrize("shape", [SCAN_SHAPES[1], SCAN_SHAPES[2], SCAN_SHAPES[3], SCAN_SHAPES[4]])
+@pytest.mark.parametrize("rule", [(0.7, 0.9, 0.0), (2.0, 1.0, 0.02)])
+def test_sampling_of_large_calls(ops, shape, rule):
+    C, F, stride, k = shape
+    t, top_p, min_p = rule
+    for kind in ("equal", "ascending", "special"):
+        rng = np.random.default_rng(C + 5 * F)
+        y, u = logits_of(kind, rng, (C, F)), rng.random(F).astype(F32)
+        category, share = ops.categorical_sampling(dev(padded(y, stride, np.inf)), dev(padded(u[None], stride)), C, 1, F, temperature=t, top_size=k, top_p=top_p, min_p=min_p)
+        wi, wv = sorted_logits(y, k)
+        wc, ws = ref.sampling(wv, u, t, k, top_p, min_p)                     # (of the k largest in their order: positions, then channels)
+        wc = np.where(wc >= 0, np.take_along_axis(wi, np.maximum(wc, 0)[None], 0)[0], -1)
+        assert np.array_equal(host(category)[0, :F], wc), kind
+        near(host(share)[0, :F], ws, 2 * U * ws, kind)

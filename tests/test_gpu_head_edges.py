@@ -5,7 +5,7 @@ import pytest
 
 import head_reference as ref
 from head_reference import U
-from test_gpu_head_operators import F32, check_distill, check_norm, check_norm_backward, distill_case, logits_of, near, ops, padded, same_values  # noqa: F401 (ops: the fixture)
+from test_gpu_head_operators import F32, check_distill, check_norm, check_norm_backward, columns, distill_case, logits_of, near, ops, padded, same_values  # noqa: F401 (ops: the fixture)
 from util import dev, host
 
 pytestmark = pytest.mark.gpu
@@ -218,3 +218,98 @@ def test_sampling_of_large_calls(ops, shape, rule):
         wc = np.where(wc >= 0, np.take_along_axis(wi, np.maximum(wc, 0)[None], 0)[0], -1)
         assert np.array_equal(host(category)[0, :F], wc), kind
         near(host(share)[0, :F], ws, 2 * U * ws, kind)
+
+
+# ---- a mean that is large against the deviation ----------------------------------------------------------------------------------------
+@pytest.mark.parametrize("nodes", [1000, 3000])                              # one launch, two
+@pytest.mark.parametrize("stride", [72, 70])                                 # four frames at a time, one
+@pytest.mark.parametrize("offset", [1e3, 1e4, 1e5])
+def test_layer_norm_of_a_large_mean_by_its_roundings(ops, nodes, stride, offset):
+    """The longest way of a value into the mean has 25 roundings of at most U * offset: eight rows summed and scaled (5.4: their partial sums are k * offset, over 8), then a
+    merge each for a second batch, 3 wavefronts, 12 slabs of a thread and 3 wavefronts again; in one launch 3 rows, up to 4 lane steps, 16 wavefronts and a quotient.
+    A group of n rows whose mean is off by e <= 25 U offset adds e^2 to the variance, and to the sum of squares between groups at most 2 e / sqrt(n) of unit deviation: over the
+    levels (8 rows 3.8, 16 rows 3.2, 64 rows 1.6 + 5.3, the rest 2) no more than 16 U offset, half of that in rstd."""
+    rng = np.random.default_rng(nodes)
+    F, c = 70, offset * U
+    x = (offset + rng.standard_normal((nodes, F))).astype(F32)
+    y, mean, rstd = ops.layer_normalization_forward(dev(padded(x, stride)), None, None, F)
+    one, zero = np.ones(nodes, F32), np.zeros(nodes, F32)
+    wy, wmean, wrstd = ref.layer_norm(x, one, zero, float(F32(1e-5)))
+    near(host(mean), wmean, 25 * c * 1.01, "mean")                           # (the largest value is a little above the offset)
+    rel = 8 * c + 0.5 * (25 * c) ** 2 + 128 * U
+    near(host(rstd), wrstd, wrstd * rel, "rstd")
+    near(host(y)[:, :F], wy, wrstd * 26 * c * (1 + rel) + np.abs(wy) * (rel + 4 * U), "y")
+
+
+# ---- workspaces ------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("shape", [(40, 1, 8, 3), (700, 1, 24, 9), (1000, 1, 1, 50), (2000, 3, 13, 40), (5000, 1, 300, 20), (9000, 1, 68, 100), (20000, 1, 5, 50), (3000, 1, 1000, 4)])
+def test_workspaces_of_the_size_asked_for(ops, shape):
+    """each entry does with the bytes that its ..._WorkspaceBytes names, from rows on 16 bytes and from rows that are not, and leaves what lies behind them"""
+    import torch
+    from binarybrain_amd import capi
+    C, P, F, k = shape
+    lib, p, nodes = capi.lib(), capi.ptr, C * P
+    rng = np.random.default_rng(C + F)
+    S = (F + 3) // 4 * 4 + 4
+
+    def rows(a, off):                                                        # [rows, S], `off` floats behind a start on 256 bytes
+        t = torch.zeros(a.shape[0] * S + off, dtype=torch.float32 if a.dtype == F32 else torch.int32, device="cuda")[off:].view(a.shape[0], S)
+        t[:, :F] = dev(a)
+        return t
+
+    def run(name, size, *args):
+        work = torch.full((size + 512,), 0xa5, dtype=torch.uint8, device="cuda")
+        capi.check(getattr(lib, "bbhip_" + name)(*args, p(work) if size else None, size, capi.stream_ptr()))
+        torch.cuda.synchronize()
+        assert bool((work[size:] == 0xa5).all()), name
+
+    x, dy = rng.standard_normal((nodes, F)).astype(F32), rng.standard_normal((nodes, F)).astype(F32)
+    line = lambda n: torch.ones(n, device="cuda")
+    got = []
+    for off in (0, 1):
+        a, d, out = rows(x, off), rows(dy, off), rows(np.zeros_like(x), off)
+        bits = torch.zeros((nodes, (F + 31) // 32), dtype=torch.int32, device="cuda")
+        mean, rstd, g, b = line(F + 4)[off:], line(F + 4)[off:], line(nodes), line(nodes)
+        norm = lib.bbhip_LayerNormalization_WorkspaceBytes(nodes, F)
+        run("fp32_LayerNormalization_Forward", norm, p(a), p(out), p(g), p(b), p(mean), p(rstd), 1e-5, nodes, F, S, S)
+        y = host(out)[:, :F].copy()
+        run("bit_fp32_LayerNormalization_Forward", norm, p(bits), p(out), p(g), p(b), p(line(F + 4)[off:]), p(line(F + 4)[off:]), 1e-5, nodes, F, bits.shape[1], S)
+        dg, db = line(nodes), line(nodes)
+        run("fp32_LayerNormalization_Backward", norm, p(a), p(d), p(out), p(g), p(mean), p(rstd), p(dg), p(db), 0, nodes, F, S, S)
+        dx = host(out)[:, :F].copy()
+        run("bit_fp32_LayerNormalization_Backward", norm, p(bits), p(d), p(out), p(g), p(mean), p(rstd), p(dg), p(db), 0, nodes, F, bits.shape[1], S)
+        top = lib.bbhip_TopLogits_WorkspaceBytes(k, P, C, F)
+        index, logit = rows(np.zeros((k * P, F), np.int32), off), rows(np.zeros((k * P, F), F32), off)
+        run("fp32_TopLogits", top, p(a), p(index), p(logit), k, P, C, F, S, S)
+        loss, category, u = rows(np.zeros((P, F), F32), off), rows(np.zeros((P, F), np.int32), off), rows(rng.random((P, F)).astype(F32) if not off else got[0][5], off)
+        run("fp32_LossDistillation", lib.bbhip_LossDistillation_WorkspaceBytes(P, C, F), p(a), p(index), p(logit), None, p(out), p(loss), 2.0, 1.0, k, P, C, F, S, S)
+        run("fp32_CategoricalSampling", top, p(a), p(u), p(category), None, 1.0, k, 0.9, 0.0, P, C, F, S)
+        got.append((y, dx, host(index)[:, :F], host(logit)[:, :F], host(category)[:, :F], host(u)[:, :F].copy(), host(out)[:, :F], host(loss)[:, :F]))
+    one = np.ones(nodes, F32)
+    wy, _, wrstd = ref.layer_norm(x, one, one, float(F32(1e-5)))
+    for y, dx, index, logit, category, _, dy_of, loss in got:
+        near(y, wy, 5e-5, "y")                                               # (132 U of values up to 5, and the mean's 100 U times 5)
+        wi, wv = ref.top_logits(columns(x, C, P, F), k)
+        assert np.array_equal(columns(index, k, P, F), wi) and np.array_equal(columns(logit, k, P, F), wv)
+        check_distill(columns(x, C, P, F), wi, wv, np.ones(P * F, F32), 2.0, 1.0, columns(dy_of, C, P, F), columns(loss, 1, P, F)[0])
+    assert np.array_equal(got[0][4], got[1][4])
+    near(got[0][1], got[1][1], 5e-5 * wrstd.max() * (1 + np.abs(dy).max()), "dx")
+
+
+@pytest.mark.parametrize("shape", [(300, 41, 44), (1024, 1000, 1000), (5000, 130, 131), (64, 5000, 5000)])
+def test_layer_norm_backward_in_place(ops, shape):
+    """dx may be dy: the same bits, and the padding stays"""
+    import torch
+    from binarybrain_amd import capi
+    nodes, F, S = shape
+    rng = np.random.default_rng(nodes)
+    x, dy = dev(rng.standard_normal((nodes, S)).astype(F32)), dev(padded(rng.standard_normal((nodes, F)).astype(F32), S))
+    gamma, line = dev(rng.standard_normal(nodes).astype(F32)), lambda: torch.zeros(nodes, device="cuda")
+    _, mean, rstd = ops.layer_normalization_forward(x, gamma, None, F)
+    dx, dgamma, dbeta = ops.layer_normalization_backward(x, dy, gamma, mean, rstd, F)
+    size, p, dg, db = capi.lib().bbhip_LayerNormalization_WorkspaceBytes(nodes, F), capi.ptr, line(), line()
+    work = torch.empty(size, dtype=torch.uint8, device="cuda")
+    capi.check(capi.lib().bbhip_fp32_LayerNormalization_Backward(p(x), p(dy), p(dy), p(gamma), p(mean), p(rstd), p(dg), p(db), 0, nodes, F, S, S, p(work), size, capi.stream_ptr()))
+    torch.cuda.synchronize()
+    assert np.array_equal(host(dy)[:, :F], host(dx)[:, :F]) and np.all(np.isnan(host(dy)[:, F:]))
+    assert np.array_equal(host(dg), host(dgamma)) and np.array_equal(host(db), host(dbeta))

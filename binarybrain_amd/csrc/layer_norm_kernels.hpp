@@ -255,10 +255,17 @@ __global__ __launch_bounds__(kColBlock) void layer_norm_stats_kernel(LayerNormAr
         beyond = __any(beyond);
         if (threadIdx.x % kWave == 0) { far[threadIdx.x / kWave] = beyond ? 1 : 0; }
         merge_workgroup<W>(m, a.c.log_tx, share);
+        if (a.eps < kVarianceLeast) {                                           // (small sums count, too: those of the whole slab are wavefront 0's)
+            bool low = false;
+#pragma unroll
+            for (int j = 0; j < W; ++j) { low = low || (writes && j < u.live && m.m2[j] < kVarianceLeast * (float)(t.end - t.begin)); }
+            if (low) { far[0] = 1; }
+            __syncthreads();
+        }
         int some = 0;
 #pragma unroll
         for (int w = 0; w < kColWaves; ++w) { some |= far[w]; }
-        if (some != 0 || a.eps < kVarianceLeast) {                              // workgroup-uniform
+        if (some != 0) {                                                        // workgroup-uniform
             layer_norm_stats_far<W>(a, t, u, m, share);
             return;
         }
@@ -375,7 +382,7 @@ __global__ __launch_bounds__(kColBlock) void layer_norm_apply_kernel(LayerNormAr
 
 // Forward pass in one launch, for columns that a workgroup of 1024 threads can hold, R = 4 or 16 rows of a unit per thread: x is read once and the mean is known before
 // the deviations are squared.  Packed bits are held as their words.  The squares are summed in 32 bits; where a thread's sum shows that a total might leave
-// their range, or eps is so small that squares below it count, the workgroup sums them again in 64.
+// their range, or a variance is so small that squares below it count, the workgroup sums them again in 64.
 constexpr int kWholeBlock = 1024, kWholeWaves = kWholeBlock / kWave;
 
 // the sum over the threads that hold the same unit, in every thread.  share: kWholeWaves * kWave * W floats
@@ -515,7 +522,14 @@ __global__ __launch_bounds__(kWholeBlock) void layer_norm_whole_kernel(LayerNorm
 #pragma unroll
     for (int j = 0; j < W; ++j) { rstd[j] = 1.0f / sqrtf(q[j] + a.eps); }
     if constexpr (!BIT) {
-        if (far != 0 || a.eps < kVarianceLeast) {                               // workgroup-uniform
+        if (a.eps < kVarianceLeast) {                                           // (small variances count, too)
+            bool low = false;
+#pragma unroll
+            for (int j = 0; j < W; ++j) { low = low || (j < u.live && q[j] + a.eps < kVarianceLeast); }
+            if (low) { far = 1; }
+            __syncthreads();
+        }
+        if (far != 0) {                                                         // workgroup-uniform
             layer_norm_whole_far<W>(a, u, ty, step, mean, q, rstd, reinterpret_cast<double *>(&share[0][0]));
             return;
         }

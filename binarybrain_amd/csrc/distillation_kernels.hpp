@@ -318,10 +318,10 @@ __global__ __launch_bounds__(kColBlock) void distillation_gradient_kernel(Distil
             size_t const here = (size_t)at.pix * a.frame_stride + at.f0 + col % W + (size_t)c * channel;
             float4 const l = a.lists[at.column + col % W];
             float const z = logit[j * entry], yc = a.y[here];
-            if (z == -__builtin_inff()) { continue; }                           // (no share: what stands there is right, or another entry's thread writes it)
+            bool const shares = !(z == -__builtin_inff());                      // (else: what stands there is right, or another entry's thread writes it)
             auto weight = [&](float v) { return exp_scaled(v == l.x ? 0.0f : v - reference_of(l.x), a.scale); };
             float q = weight(z);
-            if (__builtin_signbitf(l.y)) {                                      // a channel may be named twice: its shares are added in the list's order, by its first entry's thread
+            if (shares && __builtin_signbitf(l.y)) {                            // a channel may be named twice: its shares are added in the list's order, by its first entry's thread
                 int const *const index = a.index + (size_t)at.pix * a.list_stride + at.f0 + col % W;
                 int first = a.top_size;
                 q = 0.0f;
@@ -334,7 +334,7 @@ __global__ __launch_bounds__(kColBlock) void distillation_gradient_kernel(Distil
                 }
                 if (first != j) { continue; }
             }
-            a.dy[here] = k * (exp_scaled(yc - of_m[col], a.scale) * of_s[col] - q * fabsf(l.y));
+            if (shares) { a.dy[here] = k * (exp_scaled(yc - of_m[col], a.scale) * of_s[col] - q * fabsf(l.y)); }
         }
         __syncthreads();
     }

@@ -61,7 +61,7 @@ __device__ __forceinline__ void line_load(float const *__restrict__ p, int live,
 }
 
 // STREAM: past the caches (what a second launch reads again would lose its place in them to the output).  Large outputs in segments of less than a cache line go through
-// them, which joins the neighbours' halves: 4096 x 8192 frames in tiles of 64 bytes 75 us past the caches, 61 through them (1024 x 8192 14.4 and 16.3).
+// them, which joins the neighbours' halves: 4096 x 8192 frames in tiles of 64 bytes 68 us past the caches, 58 through them (1024 x 8192 14.4 and 16.3).
 template <int W, bool STREAM = true>
 __device__ __forceinline__ void column_store(float *__restrict__ p, int live, float const (&v)[W])
 {

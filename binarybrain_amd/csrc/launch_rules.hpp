@@ -278,10 +278,10 @@ inline void column_split(int units, int rows, bool wide, int batch, int &log_tx,
 
 // Layer norm's forward pass in one launch: the tile (2^log_tx units, of which a workgroup of 1024 threads holds 1024 >> log_tx rows per load), or false where two launches are taken.
 // Tiles as wide as four rows per thread allow, down to 64 bytes of a row, narrower ones also where compute units would be left without work.  In one launch and in two: 1024 nodes x 1000
-// frames 7.6 and 8.7 us, x 8192 14.4 and 19.9, 256 x 8192 6.9 and 8.2, 64 x 65536 7.6 and 12.3, 64 x 524288 44 and 66, 4096 x 1 6.9 and 7.7; with tiles of 64 bytes input and output have to
-// stay in the memory-side cache: 1000 x 20000 33 and 39, 1024 x 32768 81 and 62.
-// Longer columns (16 rows per thread, which leaves one workgroup per compute unit) where the launch has one or two rounds of workgroups: 4096 x 4096 27 and 35, 4096 x 8192 55 and 62, 2048 x 4096
-// 17.8 and 19.6; with fewer 3000 x 3000 21.0 and 21.6, 2048 x 2048 14.1 and 12.6, 4096 x 1000 22.4 and 13.5; with more 1500 x 20000 67 and 57, 2048 x 16384 74 and 63, 4096 x 16384 180 and 127.
+// frames 7.8 and 9.2 us, x 8192 14.7 and 20.2, 256 x 8192 7.0 and 8.7, 64 x 65536 7.7 and 12.2, 64 x 524288 45 and 62, 4096 x 1 7.0 and 8.1; with tiles of 64 bytes input and output have to
+// stay in the memory-side cache: 1000 x 20000 33 and 40, 1024 x 32768 83 and 63.
+// Longer columns (16 rows per thread, which leaves one workgroup per compute unit) where the launch has one or two rounds of workgroups: 4096 x 4096 26 and 35, 4096 x 8192 50 and 63, 2048 x 4096
+// 16.8 and 20.1; with fewer 3000 x 3000 19.8 and 22.1, but 2048 x 2048 13.1 and 12.8, 4096 x 1000 20.3 and 13.8; with more 1500 x 20000 64 and 57, 2048 x 16384 67 and 64, 4096 x 16384 170 and 126.
 inline bool layer_norm_whole(int units, int rows, bool wide, bool bit, int &log_tx, bool &longer)
 {
     int const narrowest = wide ? 2 : 4;

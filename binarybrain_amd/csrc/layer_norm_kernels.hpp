@@ -7,11 +7,12 @@
 // Means and squared deviations are formed over eight rows at a time and merged pairwise with their counts (the update of Chan, Golub and
 // LeVeque), so a mean that is large against the deviation costs no digits; packed bits are counted, and their squared deviation is
 // ones * zeros / N.  Squares are summed in 32 bits; the square of what float32 holds need not be one itself (values around 1e20 or, with eps 0, deviations of
-// 1e-25), and where a frame's sum leaves the range its deviations are read and squared again in 64 bits.  All sums are taken in a fixed order: the same input gives the same bits on every run.
+// 1e-25), and where a frame's sum leaves the range its deviations are read and squared again in 64 bits.  (Squares of 64 bits throughout cost 4 to 9 % of small calls.)
+// All sums are taken in a fixed order: the same input gives the same bits on every run.
 //
 // Columns that a workgroup can hold go in one launch (forward; layer_norm_whole in launch_rules.hpp has both sides).  Any other size goes in two: the sums of a slab of rows per workgroup (forward: mean and squared deviation; backward: the two sums per
 // frame and, of the same reading, the two sums per node over the tile's frames), then every workgroup adds up the slabs of its frames and writes.
-// 4096 nodes x 8192 frames, inputs not in the caches: forward 61 us = 4.4 TB/s (147 MB read, 148 written; one workgroup per compute unit reads, waits and writes in turn), backward 118 us
+// 4096 nodes x 8192 frames, inputs not in the caches: forward 57 us = 4.7 TB/s (135 MB read, 135 written; one workgroup per compute unit reads, waits and writes in turn), backward 118 us
 // (42 + 64 with what fits in the memory-side cache): 640 MB through the fabric at 6 TB/s, of which 403 would do if x and dy were read once.
 #pragma once
 
@@ -539,7 +540,7 @@ __global__ __launch_bounds__(kWholeBlock) void layer_norm_whole_kernel(LayerNorm
         if (a.rstd != nullptr) { column_store<W>(a.rstd + u.f0, u.live, rstd); }
     }
     int ry = ty;
-    asm volatile("" : "+v"(ry));                                                // (the rows' numbers are formed again: kept over the sums they would cost as many registers)
+    asm volatile("" : "+v"(ry));                                                // (the rows' numbers are formed again: kept over the sums they cost registers that do not suffice: 4096 x 8192 54.5 us and 50.5)
     float *const out = a.out + (size_t)ry * a.out_stride + u.f0;
 #pragma unroll
     for (int i = 0; i < R; ++i) {

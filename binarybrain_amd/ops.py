@@ -479,7 +479,7 @@ def top_logits(y, top_size, ch_size, pix_size, frame_size):
 def loss_distillation(y, index, logit, ch_size, pix_size, frame_size, temperature=1.0, weight=None, weight_sum=None):
     """Distillation from a teacher's kept logits ([top*pix, stride] channels and values, channel -1: no entry): (dy, loss [pix, stride]).  The loss of the
     batch is loss[:, :frame_size].sum() / weight_sum, whose gradient dy is.  weight [pix, stride]: of each pixel and frame (None: 1);
-    weight_sum defaults to the sum of the weights of the frames in use, taken in float64."""
+    weight_sum defaults to the sum of the weights of the frames in use, taken in float64 and read by the host (a captured step gives its own)."""
     if weight_sum is None:
         weight_sum = float(pix_size * frame_size) if weight is None else float(weight[:, :frame_size].sum(dtype=torch.float64).item())
     return native.loss_distillation(y, index, logit, ch_size, pix_size, frame_size, temperature, weight, weight_sum)

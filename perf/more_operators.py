@@ -227,7 +227,8 @@ def _loss(s):
         else:
             loss, dx, dW, db = ops.loss_dense_softmax_cross_entropy(s["x"], s["W"], s["b"], s["label"], f, weight=s["weight"], weight_sum=s["weight_sum"],
                                                                     want_gradients=s["gradients"])
-        return (loss[:, :f], dx[:, :f], dW, db) if s["gradients"] else loss[:, :f]
+        loss = loss[None, :, :f]
+        return (loss, dx[:, :f], dW, db) if s["gradients"] else loss
     x, label = _values(s), s["label"][0, :f].long()
     counts = (label >= 0) & (label < s["channels"])
     w = torch.where(counts, s["weight"][0, :f], 0.0)

@@ -12,7 +12,7 @@ NATIVE_PATH = os.path.join(LIB_DIR, "_bbops.so")
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # packed fp32 VALU instructions are disabled on purpose: scalar fp32 code must not be auto-vectorised into v_pk_* forms
-FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared", "-munsafe-fp-atomics",
+FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-munsafe-fp-atomics",
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
@@ -28,9 +28,18 @@ def _run(cmd, verbose):
         print(out)
 
 
-def build_library(verbose=False):
+# translation units of the library: the LUT layers and what surrounds them; dense layers, their loss and the clipping of gradients
+UNITS = ("bbhip", "dense")
+
+
+def build_library(verbose=False, units=UNITS):
+    """`units`: those to compile (side by side); the others' object files are taken as they are"""
+    from concurrent.futures import ThreadPoolExecutor
     os.makedirs(LIB_DIR, exist_ok=True)
-    _run([HIPCC] + FLAGS + [os.path.join(CSRC, "bbhip.hip"), "-o", LIB_PATH], verbose)
+    obj = lambda name: os.path.join(LIB_DIR, name + ".o")
+    with ThreadPoolExecutor(len(UNITS)) as pool:
+        list(pool.map(lambda name: _run([HIPCC] + FLAGS + ["-c", os.path.join(CSRC, name + ".hip"), "-o", obj(name)], verbose), units))
+    _run([HIPCC] + FLAGS + ["-shared"] + [obj(name) for name in UNITS] + ["-o", LIB_PATH], verbose)
     return LIB_PATH
 
 
@@ -50,7 +59,7 @@ def build_native(verbose=False):
 def build_bench_probe(verbose=False):
     """bench_gather_probe.so beside bench.py: the instrumentation kernel of `bench.py --workload gather_ceiling` (not part of the library)."""
     out = os.path.join(ROOT, "bench_gather_probe.so")
-    _run([HIPCC] + FLAGS + ["-I" + ROOT, os.path.join(ROOT, "bench_gather_probe.hip"), "-o", out], verbose)
+    _run([HIPCC] + FLAGS + ["-shared", "-I" + ROOT, os.path.join(ROOT, "bench_gather_probe.hip"), "-o", out], verbose)
     return out
 
 

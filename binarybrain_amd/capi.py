@@ -115,6 +115,20 @@ _SIGNATURES = {
     "bbhip_fp32_TopLogits": (C.c_int, [_vp, _vp, _vp] + [_i] * 6 + [_vp, C.c_size_t, _vp]),
     "bbhip_LossDistillation_WorkspaceBytes": (C.c_size_t, [_i] * 3),
     "bbhip_fp32_LossDistillation": (C.c_int, [_vp] * 6 + [_f, _f] + [_i] * 6 + [_vp, C.c_size_t, _vp]),
+    "bbhip_DenseAffine_WorkspaceBytes": (C.c_size_t, [_i] * 3),
+    "bbhip_fp32_DenseAffine_Forward": (C.c_int, [_vp] * 5 + [_i] * 7 + [_vp, C.c_size_t, _vp]),
+    "bbhip_bit_fp32_DenseAffine_Forward": (C.c_int, [_vp] * 5 + [_i] * 7 + [_vp, C.c_size_t, _vp]),
+    "bbhip_fp32_bit_DenseAffine_Forward": (C.c_int, [_vp] * 5 + [_i] * 6 + [_vp, C.c_size_t, _vp]),
+    "bbhip_bit_bit_DenseAffine_Forward": (C.c_int, [_vp] * 5 + [_i] * 6 + [_vp, C.c_size_t, _vp]),
+    "bbhip_fp32_DenseAffine_Backward": (C.c_int, [_vp] * 8 + [_i] * 8 + [_vp, C.c_size_t, _vp]),
+    "bbhip_bit_fp32_DenseAffine_Backward": (C.c_int, [_vp] * 8 + [_i] * 8 + [_vp, C.c_size_t, _vp]),
+    "bbhip_LossDenseSoftmaxCrossEntropy_WorkspaceBytes": (C.c_size_t, [_i] * 4),
+    "bbhip_fp32_LossDenseSoftmaxCrossEntropy": (C.c_int, [_vp] * 9 + [_f] + [_i] * 6 + [_vp, C.c_size_t, _vp]),
+    "bbhip_bit_fp32_LossDenseSoftmaxCrossEntropy": (C.c_int, [_vp] * 9 + [_f] + [_i] * 6 + [_vp, C.c_size_t, _vp]),
+    "bbhip_GradientNorm_WorkspaceBytes": (C.c_size_t, []),
+    "bbhip_fp32_GradientNorm": (C.c_int, [_i, _vp, _vp, _f, _vp, _vp, C.c_size_t, _vp]),
+    "bbhip_fp32_GradientClip": (C.c_int, [_i, _vp, _vp, _f, _vp, _vp, C.c_size_t, _vp]),
+    "bbhip_fp32_OptimizerAdam_Clipped": (C.c_int, [_i] + [_vp] * 5 + [_f, C.c_double, C.c_double, _f] + [_vp, _i, _vp, C.c_size_t, _vp]),
     "bbhip_fp32_CategoricalSampling": (C.c_int, [_vp] * 4 + [_f, _i, _f, _f] + [_i] * 4 + [_vp, C.c_size_t, _vp]),
     "bbhip_fp32_StochasticLut_Forward": (C.c_int, [_i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _f, _vp]),
     "bbhip_fp32_StochasticLut_Forward_NoAlloc": (C.c_int, [_i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _f, _vp]),

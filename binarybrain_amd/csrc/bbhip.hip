@@ -16,6 +16,7 @@
 #include <vector>
 
 #include "../../include/bbhip.h"
+#include "host_calls.hpp"
 #include "launch_rules.hpp"
 #include "lut_kernels.hpp"
 #include "corner_forward_kernels.hpp"
@@ -46,8 +47,9 @@ namespace {
 //  errors
 // ------------------------------------------------------------------------------------------------
 thread_local std::string g_last_error;
+}  // namespace
 
-int fail(char const *fmt, ...)
+int bbhip::fail(char const *fmt, ...)
 {
     char buf[512];
     va_list ap;
@@ -58,18 +60,12 @@ int fail(char const *fmt, ...)
     return 1;
 }
 
-#define BBHIP_TRY(expr)                                                                              \
-    do {                                                                                             \
-        hipError_t e_ = (expr);                                                                      \
-        if (e_ != hipSuccess) { return fail("%s: %s (%s:%d)", #expr, hipGetErrorString(e_), __FILE__, __LINE__); } \
-    } while (0)
+namespace {
 
 #define BBHIP_REQUIRE(cond)                                                                          \
     do {                                                                                             \
         if (!(cond)) { return fail("%s: rejected argument: %s", __func__, #cond); }                  \
     } while (0)
-
-#define BBHIP_LAUNCH_CHECK() BBHIP_TRY(hipGetLastError())
 
 // ------------------------------------------------------------------------------------------------
 //  global switches
@@ -91,12 +87,17 @@ thread_local PackedOutputHint g_packed_out_hint = {nullptr, 0, 0};
 thread_local int g_dw_overwrite_hint = 0;
 // bbhip_HintZeroOutputPadding: the next call with packed output writes its rows up to the row pitch
 thread_local int g_zero_padding_hint = 0;
-static inline void clear_hints(void)
+}  // namespace
+
+void bbhip::clear_hints(void)
 {
     g_dw_overwrite_hint = 0; g_zero_padding_hint = 0;
     g_input_node_hint = 0; g_packed_hint = PackedInputHint{nullptr, 0, 0, 0}; g_tables_hint = PreparedTablesHint{nullptr, 0, 0};
     g_packed_out_hint = PackedOutputHint{nullptr, 0, 0};
 }
+
+namespace {
+
 static inline bool tables_fit(PreparedTablesHint const &t, size_t bytes)
 {
     return t.buf != nullptr && t.bytes >= bytes && (reinterpret_cast<uintptr_t>(t.buf) & 255u) == 0;
@@ -105,29 +106,28 @@ static inline bool tables_fit(PreparedTablesHint const &t, size_t bytes)
 // ------------------------------------------------------------------------------------------------
 //  optional kernel timer: HIP events around the dominant kernel of each entry point, on the launch stream
 // ------------------------------------------------------------------------------------------------
-enum TimedKernel : int { kTimeForward = 0, kTimeBackward = 1, kTimeBinary = 2, kTimeDx = 3, kTimeOther = 4, kTimedKinds = 5 };
-struct TimedLaunch { hipEvent_t start, stop; int which; };
 bool g_timer_on = false;
 std::mutex g_timed_mtx;                      // guards g_timed: calls may come from several host threads
 std::vector<TimedLaunch> g_timed;
+}  // namespace
 
-struct ScopedTimer {
-    hipStream_t st; bool on; TimedLaunch t;
-    ScopedTimer(int which, hipStream_t s, bool allowed = true) : st(s), on(g_timer_on && allowed)
-    {
-        if (!on) { return; }
-        t.which = which;
-        if (hipEventCreate(&t.start) != hipSuccess || hipEventCreate(&t.stop) != hipSuccess) { on = false; return; }
-        (void)hipEventRecord(t.start, st);
-    }
-    ~ScopedTimer()
-    {
-        if (!on) { return; }
-        (void)hipEventRecord(t.stop, st);
-        std::lock_guard<std::mutex> lk(g_timed_mtx);
-        g_timed.push_back(t);
-    }
-};
+bbhip::ScopedTimer::ScopedTimer(int which, hipStream_t s, bool allowed) : st(s), on(g_timer_on && allowed)
+{
+    if (!on) { return; }
+    t.which = which;
+    if (hipEventCreate(&t.start) != hipSuccess || hipEventCreate(&t.stop) != hipSuccess) { on = false; return; }
+    (void)hipEventRecord(t.start, st);
+}
+
+bbhip::ScopedTimer::~ScopedTimer()
+{
+    if (!on) { return; }
+    (void)hipEventRecord(t.stop, st);
+    std::lock_guard<std::mutex> lk(g_timed_mtx);
+    g_timed.push_back(t);
+}
+
+namespace {
 
 // integer tunable from the environment: unset, empty or negative = the default
 int env_int(char const *name, int def)
@@ -243,21 +243,6 @@ int arena_get(size_t bytes, char **out, hipStream_t st, Scratch const *fixed = n
     }
     *out = static_cast<char *>(a.ptr);
     return 0;
-}
-
-inline size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
-
-// A launch without the call-configuration stack and the copies that the <<<>>> form's host stub goes through: 2.7 us of host time for a kernel
-// with 400 bytes of arguments instead of 3.2, and the host is what a program of small layers waits for.  Errors are read by BBHIP_LAUNCH_CHECK.
-template <class... P, class... A>
-void launch(void (*kernel)(P...), dim3 grid, dim3 block, unsigned lds_bytes, hipStream_t st, A const &... args)
-{
-    // an argument of the parameter's own type is passed where it lies
-    std::tuple<std::conditional_t<std::is_same_v<P, A>, A const &, P>...> const held{args...};
-    std::apply([&](auto const &... v) {
-        void *where[] = {const_cast<void *>(static_cast<void const *>(&v))...};
-        (void)hipLaunchKernel(reinterpret_cast<void const *>(kernel), grid, block, where, lds_bytes, st);
-    }, held);
 }
 
 // words [first, stride) of packed rows = 0 (first: packed_padding_end)
@@ -2430,16 +2415,6 @@ static int column_space(ColumnSpace &c, TileDivisor &tiles, bool wide, int pix_s
     tiles = make_tile_divisor(c.tiles);
     return 0;
 }
-
-// an entry's workspace, as its ...WorkspaceBytes counts it
-static int check_workspace(void const *workspace, size_t size, size_t needed, char const *name)
-{
-    if (size < needed || (needed > 0 && workspace == nullptr)) { return fail("%s: a workspace of %zu bytes is needed, %zu given", name, needed, workspace ? size : (size_t)0); }
-    if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0)  { return fail("%s: the workspace must be aligned to 256 bytes", name); }
-    return 0;
-}
-
-static bool starts_on_16_bytes(void const *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 static size_t layer_norm_partial_bytes(ColumnSpace const &c, bool wide) { return align256((size_t)c.slabs * c.units * (wide ? 4 : 1) * sizeof(float2)); }
 

@@ -602,6 +602,206 @@ categorical_sampling(T y, T u, int ch, int pix, int frames, float temperature, i
     return {std::move(category), std::move(share)};
 }
 
+// ---- dense layers, the loss on top of one, clipped gradients --------------------------------------------------------------------------
+struct DenseCall : HeadCall {
+    using HeadCall::HeadCall;
+    // [a, b] float32 without a pitch
+    void table(char const *what, T t, int64_t a, int64_t b) const
+    {
+        rows(what, t, at::kFloat, a, b);
+        if (t.size(1) != b) { refuse(std::string(what) + " must be [" + std::to_string(a) + ", " + std::to_string(b) + "]"); }
+    }
+    // x and W of a call -> inputs, outputs
+    std::pair<int, int> layer(bool bit, T x, T W, int frames) const
+    {
+        if (x.dim() != 2 || W.dim() != 2 || x.size(0) > 2147483647LL || W.size(0) > 2147483647LL) { refuse("x and W must have rows"); }
+        sizes(frames, 1); sizes((int)x.size(0), 1); sizes((int)W.size(0), 1);
+        rows("x", x, bit ? at::kInt : at::kFloat, x.size(0), bit ? (frames - 1) / 32 + 1 : frames);
+        table("W", W, W.size(0), x.size(0));
+        return {rows_of(x), rows_of(W)};
+    }
+    // a buffer of one row or a line
+    void frames_line(char const *what, T t, at::ScalarType type, int frames) const
+    {
+        if (t.device() != device)    { refuse(std::string(what) + " is on another device"); }
+        if (t.scalar_type() != type) { refuse(std::string(what) + (type == at::kFloat ? " must be float32" : " must be int32")); }
+        if (!(t.dim() == 1 || (t.dim() == 2 && t.size(0) == 1)) || t.numel() < frames) { refuse(std::string(what) + " must be [1, at least " + std::to_string(frames) + "]"); }
+    }
+};
+
+at::Tensor dense_affine_forward_as(bool bit, bool bit_out, char const *name, T x, T W, OptTensor b, int frames, int y_stride, int activation, OptTensor residual)
+{
+    DenseCall const c(x, name);
+    auto const [inputs, outputs] = c.layer(bit, x, W, frames);
+    c.line("b", b, outputs);
+    if ((bit_out ? (int64_t)y_stride * 32 : y_stride) < frames) { c.refuse("the output's rows are shorter than the frames"); }
+    if (residual) { c.rows("residual", *residual, at::kFloat, outputs, frames); }
+    at::Tensor y = bit_out ? zeros_i32(x, outputs, y_stride) : rows_f32(x, outputs, y_stride);
+    at::Tensor const work = c.workspace(x, bbhip_DenseAffine_WorkspaceBytes(inputs, outputs, frames));
+    int const r_stride = residual ? stride_of(*residual) : 0;
+    if (bit_out) {
+        if (bit) {
+            call(bbhip_bit_bit_DenseAffine_Forward, data<int const>(x), data<int>(y), data<float const>(W), data<float const>(b), data<float const>(residual), inputs, outputs,
+                 frames, stride_of(x), y_stride, r_stride, address(work), bytes_of(work), c.stream());
+        }
+        else {
+            call(bbhip_fp32_bit_DenseAffine_Forward, data<float const>(x), data<int>(y), data<float const>(W), data<float const>(b), data<float const>(residual), inputs, outputs,
+                 frames, stride_of(x), y_stride, r_stride, address(work), bytes_of(work), c.stream());
+        }
+    }
+    else if (bit) {
+        call(bbhip_bit_fp32_DenseAffine_Forward, data<int const>(x), data<float>(y), data<float const>(W), data<float const>(b), data<float const>(residual), activation, inputs,
+             outputs, frames, stride_of(x), y_stride, r_stride, address(work), bytes_of(work), c.stream());
+    }
+    else {
+        call(bbhip_fp32_DenseAffine_Forward, data<float const>(x), data<float>(y), data<float const>(W), data<float const>(b), data<float const>(residual), activation, inputs,
+             outputs, frames, stride_of(x), y_stride, r_stride, address(work), bytes_of(work), c.stream());
+    }
+    return y;
+}
+at::Tensor dense_affine_forward(T x, T W, OptTensor b, int frames, int y_stride, int activation, OptTensor residual)
+{
+    return dense_affine_forward_as(false, false, "dense_affine_forward", x, W, b, frames, y_stride, activation, residual);
+}
+at::Tensor bit_dense_affine_forward(T x, T W, OptTensor b, int frames, int y_stride, int activation, OptTensor residual)
+{
+    return dense_affine_forward_as(true, false, "bit_dense_affine_forward", x, W, b, frames, y_stride, activation, residual);
+}
+at::Tensor dense_affine_forward_bits(T x, T W, OptTensor b, int frames, int y_words, OptTensor residual)
+{
+    return dense_affine_forward_as(false, true, "dense_affine_forward_bits", x, W, b, frames, y_words, 0, residual);
+}
+at::Tensor bit_dense_affine_forward_bits(T x, T W, OptTensor b, int frames, int y_words, OptTensor residual)
+{
+    return dense_affine_forward_as(true, true, "bit_dense_affine_forward_bits", x, W, b, frames, y_words, 0, residual);
+}
+
+// dW and db of a call: the caller's, to be added to, or new ones
+struct WeightGradients {
+    at::Tensor dW, db;
+    bool accumulate;
+    WeightGradients(DenseCall const &c, T like, OptTensor dW_in, OptTensor db_in, bool want, int outputs, int inputs) : accumulate((bool)dW_in)
+    {
+        if ((bool)dW_in != (bool)db_in) { c.refuse("dW and db come together"); }
+        if (accumulate) {
+            c.table("dW", *dW_in, outputs, inputs); c.line("db", *db_in, outputs);
+            dW = *dW_in; db = *db_in;
+        }
+        else if (want) { dW = rows_f32(like, outputs, inputs); db = line_f32(like, outputs); }
+    }
+};
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor>
+dense_affine_backward_as(bool bit, char const *name, T x, T dy, T W, int frames, int activation, OptTensor y, OptTensor dW_in, OptTensor db_in, bool want_dx,
+                         bool want_weights, bool want_dr)
+{
+    DenseCall const c(x, name);
+    auto const [inputs, outputs] = c.layer(bit, x, W, frames);
+    c.rows("dy", dy, at::kFloat, outputs, frames);
+    int const S = stride_of(dy);
+    if (y) {
+        c.rows("y", *y, at::kFloat, outputs, frames);
+        if (stride_of(*y) != S) { c.refuse("y must have the row pitch of dy"); }
+    }
+    else if (activation != 0) { c.refuse("an activation's gradient needs the forward pass's output y"); }
+    WeightGradients g(c, x, dW_in, db_in, want_weights, outputs, inputs);
+    at::Tensor dx, dr;
+    if (want_dx) { dx = rows_f32(x, inputs, S); }
+    if (want_dr) { dr = rows_f32(x, outputs, S); }
+    if (!want_dx && !want_dr && !g.dW.defined()) { c.refuse("no gradient is asked for"); }
+    at::Tensor const work = c.workspace(x, bbhip_DenseAffine_WorkspaceBytes(inputs, outputs, frames));
+    if (bit) {
+        call(bbhip_bit_fp32_DenseAffine_Backward, data<int const>(x), data<float const>(dy), data<float const>(y), data<float const>(W), (float *)address(dx),
+             (float *)address(g.dW), (float *)address(g.db), (float *)address(dr), activation, (int)g.accumulate, inputs, outputs, frames, stride_of(x), S, S, address(work),
+             bytes_of(work), c.stream());
+    }
+    else {
+        call(bbhip_fp32_DenseAffine_Backward, data<float const>(x), data<float const>(dy), data<float const>(y), data<float const>(W), (float *)address(dx),
+             (float *)address(g.dW), (float *)address(g.db), (float *)address(dr), activation, (int)g.accumulate, inputs, outputs, frames, stride_of(x), S, S, address(work),
+             bytes_of(work), c.stream());
+    }
+    return {std::move(dx), std::move(g.dW), std::move(g.db), std::move(dr)};
+}
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor>
+dense_affine_backward(T x, T dy, T W, int frames, int activation, OptTensor y, OptTensor dW, OptTensor db, bool want_dx, bool want_weights, bool want_dr)
+{
+    return dense_affine_backward_as(false, "dense_affine_backward", x, dy, W, frames, activation, y, dW, db, want_dx, want_weights, want_dr);
+}
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor>
+bit_dense_affine_backward(T x, T dy, T W, int frames, int activation, OptTensor y, OptTensor dW, OptTensor db, bool want_dx, bool want_weights, bool want_dr)
+{
+    return dense_affine_backward_as(true, "bit_dense_affine_backward", x, dy, W, frames, activation, y, dW, db, want_dx, want_weights, want_dr);
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor>
+loss_dense_as(bool bit, char const *name, T x, T W, OptTensor b, T label, int frames, int stride, OptTensor weight, float weight_sum, OptTensor dW_in, OptTensor db_in,
+              bool want_dx, bool want_weights)
+{
+    DenseCall const c(x, name);
+    auto const [inputs, channels] = c.layer(bit, x, W, frames);
+    c.line("b", b, channels);
+    if (stride < frames) { c.refuse("the outputs' rows are shorter than the frames"); }
+    c.frames_line("label", label, at::kInt, frames);
+    if (weight) { c.frames_line("weight", *weight, at::kFloat, frames); }
+    WeightGradients g(c, x, dW_in, db_in, want_weights, channels, inputs);
+    at::Tensor dx, loss = rows_f32(x, 1, stride);
+    if (want_dx) { dx = rows_f32(x, inputs, stride); }
+    at::Tensor const work = c.workspace(x, bbhip_LossDenseSoftmaxCrossEntropy_WorkspaceBytes(inputs, channels, frames, want_dx || g.dW.defined()));
+    if (bit) {
+        call(bbhip_bit_fp32_LossDenseSoftmaxCrossEntropy, data<int const>(x), data<float const>(W), data<float const>(b), data<int const>(label), data<float const>(weight),
+             (float *)address(dx), (float *)address(g.dW), (float *)address(g.db), data<float>(loss), weight_sum, (int)g.accumulate, inputs, channels, frames, stride_of(x),
+             stride, address(work), bytes_of(work), c.stream());
+    }
+    else {
+        call(bbhip_fp32_LossDenseSoftmaxCrossEntropy, data<float const>(x), data<float const>(W), data<float const>(b), data<int const>(label), data<float const>(weight),
+             (float *)address(dx), (float *)address(g.dW), (float *)address(g.db), data<float>(loss), weight_sum, (int)g.accumulate, inputs, channels, frames, stride_of(x),
+             stride, address(work), bytes_of(work), c.stream());
+    }
+    return {std::move(loss), std::move(dx), std::move(g.dW), std::move(g.db)};
+}
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor>
+loss_dense_softmax_cross_entropy(T x, T W, OptTensor b, T label, int frames, int stride, OptTensor weight, float weight_sum, OptTensor dW, OptTensor db, bool want_dx, bool want_weights)
+{
+    return loss_dense_as(false, "loss_dense_softmax_cross_entropy", x, W, b, label, frames, stride, weight, weight_sum, dW, db, want_dx, want_weights);
+}
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor>
+bit_loss_dense_softmax_cross_entropy(T x, T W, OptTensor b, T label, int frames, int stride, OptTensor weight, float weight_sum, OptTensor dW, OptTensor db, bool want_dx,
+                                     bool want_weights)
+{
+    return loss_dense_as(true, "bit_loss_dense_softmax_cross_entropy", x, W, b, label, frames, stride, weight, weight_sum, dW, db, want_dx, want_weights);
+}
+
+// tables: int32 element counts and int64 addresses, as many entries each
+template <class... A> void same_lists(HeadCall const &c, T sizes, A const &... addresses)
+{
+    auto const list = [&](T t, at::ScalarType type) {
+        if (t.device() != c.device || t.scalar_type() != type || t.dim() != 1 || t.size(0) != sizes.size(0)) { c.refuse("tables of int32 counts and int64 addresses on one device"); }
+    };
+    list(sizes, at::kInt);
+    (list(addresses, at::kLong), ...);
+    if (sizes.size(0) > 2147483647LL) { c.refuse("too many tensors"); }
+}
+at::Tensor gradient_norm(T sizes, T grads, float max_norm, bool clip)
+{
+    HeadCall const c(sizes, clip ? "gradient_clip" : "gradient_norm");
+    same_lists(c, sizes, grads);
+    at::Tensor norm = line_f32(sizes, 2);
+    at::Tensor const work = c.workspace(sizes, bbhip_GradientNorm_WorkspaceBytes());
+    call(clip ? bbhip_fp32_GradientClip : bbhip_fp32_GradientNorm, (int)sizes.size(0), data<int const>(sizes), (float *const *)grads.data_ptr(), max_norm, data<float>(norm),
+         address(work), bytes_of(work), c.stream());
+    return norm;
+}
+at::Tensor adam_clipped(T sizes, T params, T grads, T m, T v, float lr_t, double beta1, double beta2, float max_norm, bool zero_grads)
+{
+    HeadCall const c(sizes, "adam_clipped");
+    same_lists(c, sizes, params, grads, m, v);
+    at::Tensor norm = line_f32(sizes, 2);
+    at::Tensor const work = c.workspace(sizes, bbhip_GradientNorm_WorkspaceBytes());
+    call(bbhip_fp32_OptimizerAdam_Clipped, (int)sizes.size(0), data<int const>(sizes), (float *const *)params.data_ptr(), (float *const *)grads.data_ptr(),
+         (float *const *)m.data_ptr(), (float *const *)v.data_ptr(), lr_t, beta1, beta2, max_norm, data<float>(norm), (int)zero_grads, address(work), bytes_of(work), c.stream());
+    return norm;
+}
+
 // ---- Adam ------------------------------------------------------------------------------------------------------------------------
 // the bias-corrected rate (AdamState.lr_t), every operation rounded to float: 0.1 us where numpy's scalars take 1.0
 double adam_rate(float lr, float b1, float b2)
@@ -631,6 +831,9 @@ PyMethodDef methods[] = {
     BBHIP_FUNCTION(binary_lut_forward), BBHIP_FUNCTION(classifier_tail), BBHIP_FUNCTION(adam_rate),
     BBHIP_FUNCTION(layer_normalization_forward), BBHIP_FUNCTION(bit_layer_normalization_forward), BBHIP_FUNCTION(layer_normalization_backward),
     BBHIP_FUNCTION(bit_layer_normalization_backward), BBHIP_FUNCTION(top_logits), BBHIP_FUNCTION(loss_distillation), BBHIP_FUNCTION(categorical_sampling),
+    BBHIP_FUNCTION(dense_affine_forward), BBHIP_FUNCTION(bit_dense_affine_forward), BBHIP_FUNCTION(dense_affine_forward_bits), BBHIP_FUNCTION(bit_dense_affine_forward_bits),
+    BBHIP_FUNCTION(dense_affine_backward), BBHIP_FUNCTION(bit_dense_affine_backward), BBHIP_FUNCTION(loss_dense_softmax_cross_entropy),
+    BBHIP_FUNCTION(bit_loss_dense_softmax_cross_entropy), BBHIP_FUNCTION(gradient_norm), BBHIP_FUNCTION(adam_clipped),
     BBHIP_FUNCTION(new_rows), BBHIP_FUNCTION(new_bits), BBHIP_FUNCTION(new_padded_bits), BBHIP_FUNCTION(new_zero_bits), BBHIP_FUNCTION(new_line),
     BBHIP_ENTRY(fp32_Vector_set), BBHIP_ENTRY(fp32_Vector_clamp), BBHIP_ENTRY(fp32_Vector_add_ex), BBHIP_ENTRY(fp32_Vector_mul_ex),
     BBHIP_ENTRY(fp32_Vector_div_ex), BBHIP_ENTRY(fp32_Vector_sqrt), BBHIP_ENTRY(fp32_Vector_exp), BBHIP_ENTRY(fp32_Vector_min),

@@ -76,13 +76,17 @@ class AdamState:
     """Device-side tables of one parameter list for bbhip_fp32_OptimizerAdam, with the bias-correction products kept
     on the host as the reference does (include/bb/OptimizerAdam.h:104-110, 166-180)."""
 
-    def __init__(self, params, grads, learning_rate=0.001, beta1=0.9, beta2=0.999):
+    def __init__(self, params, grads, learning_rate=0.001, beta1=0.9, beta2=0.999, m=None, v=None):
         for tensor in (*params, *grads):
             if not tensor.is_cuda or not tensor.is_contiguous():
                 raise capi.BbhipError("bbhip ops need contiguous device tensors")
         self.params, self.grads = list(params), list(grads)
-        self.m = [torch.zeros_like(p) for p in params]
-        self.v = [torch.zeros_like(p) for p in params]
+        self.m = [torch.zeros_like(p) for p in params] if m is None else list(m)
+        self.v = [torch.zeros_like(p) for p in params] if v is None else list(v)
+        for p, *others in zip(self.params, self.grads, self.m, self.v, strict=True):
+            for tensor in (p, *others):
+                if not tensor.is_cuda or not tensor.is_contiguous() or tensor.dtype != torch.float32 or tensor.numel() != p.numel():
+                    raise capi.BbhipError("AdamState: contiguous float32 device tensors, those of a parameter of one size")
         dev = params[0].device
         table = lambda ts: torch.tensor([t.data_ptr() for t in ts], dtype=torch.int64, device=dev)
         self.t_params, self.t_grads, self.t_m, self.t_v = table(self.params), table(self.grads), table(self.m), table(self.v)
@@ -90,19 +94,31 @@ class AdamState:
         f32 = np.float32
         self.lr, self.beta1, self.beta2 = f32(learning_rate), f32(beta1), f32(beta2)
         self.b1, self.b2 = f32(beta1), f32(beta2)
+        self.betas = float(beta1), float(beta2)         # of the clipped step, which takes 1 - beta in 64 bits
 
     def lr_t(self):
         """the bias-corrected rate of the next step: lr * sqrt(1 - b2) / (1 - b1), every operation rounded to float"""
         return np.float32(native.adam_rate(self.lr, self.b1, self.b2))
 
-    def step(self):
+    def _clipped(self, max_norm, zero_grads):
+        norm = native.adam_clipped(self.t_size, self.t_params, self.t_grads, self.t_m, self.t_v, self.lr_t(), *self.betas, float(max_norm), zero_grads)
+        self.b1 = self.b1 * self.beta1
+        self.b2 = self.b2 * self.beta2
+        return norm
+
+    def step(self, max_norm=None):
+        """One step.  With max_norm the gradients count scaled to that norm where theirs, as one vector, is larger (they stay as they are): returns (norm, scale) [2]."""
+        if max_norm is not None:
+            return self._clipped(max_norm, False)
         native.fp32_OptimizerAdam(len(self.params), self.t_size, self.t_params, self.t_grads, self.t_m, self.t_v,
                                   self.lr_t(), self.beta1, self.beta2)
         self.b1 = self.b1 * self.beta1
         self.b2 = self.b2 * self.beta2
 
-    def update(self):
-        """Optimizer::Update of the reference = step, then the gradients set to zero (include/bb/Optimizer.h:31-35), in one launch."""
+    def update(self, max_norm=None):
+        """Optimizer::Update of the reference = step, then the gradients set to zero (include/bb/Optimizer.h:31-35), in one launch (with max_norm two)."""
+        if max_norm is not None:
+            return self._clipped(max_norm, True)
         native.fp32_OptimizerAdam_Update(len(self.params), self.t_size, self.t_params, self.t_grads, self.t_m, self.t_v,
                                          self.lr_t(), self.beta1, self.beta2)
         self.b1 = self.b1 * self.beta1
@@ -110,6 +126,31 @@ class AdamState:
 
 
 BORDER_MODES = {"constant": 0, "reflect": 1, "reflect_101": 2, "replicate": 3, "wrap": 4}
+
+
+class GradientTable:
+    """A list of gradients (contiguous float32 device tensors that keep their storage, none twice) as one vector: its norm, and the list scaled to a norm."""
+
+    def __init__(self, grads):
+        self.grads = list(grads)
+        for g in self.grads:
+            if not g.is_cuda or not g.is_contiguous() or g.dtype != torch.float32 or g.device != self.grads[0].device or g.numel() > 0x7fffffff:
+                raise capi.BbhipError("GradientTable: contiguous float32 tensors on one device, of fewer than 2^31 elements")
+        if not self.grads:
+            raise capi.BbhipError("GradientTable: no gradients")
+        if len({g.data_ptr() for g in self.grads if g.numel()}) != sum(1 for g in self.grads if g.numel()):
+            raise capi.BbhipError("GradientTable: a gradient is listed twice")
+        dev = self.grads[0].device
+        self.t_size = torch.tensor([g.numel() for g in self.grads], dtype=torch.int32, device=dev)
+        self.t_grads = torch.tensor([g.data_ptr() for g in self.grads], dtype=torch.int64, device=dev)
+
+    def norm(self, max_norm=float("inf")):
+        """(norm, scale) [2]: the square root of the sum of all squares, and what brings the gradients to max_norm (1 where they are not above it)"""
+        return native.gradient_norm(self.t_size, self.t_grads, float(max_norm), False)
+
+    def clip_(self, max_norm):
+        """the same, and the gradients multiplied by the scale"""
+        return native.gradient_norm(self.t_size, self.t_grads, float(max_norm), True)
 
 
 def im2col_geometry(h, w, fh, fw, ys=1, xs=1, padding="valid"):
@@ -492,6 +533,69 @@ def categorical_sampling(y, u, ch_size, pix_size, frame_size, temperature=1.0, t
     if top_size is None:
         top_size = min(50, ch_size)
     return native.categorical_sampling(y, u, ch_size, pix_size, frame_size, temperature, top_size, top_p, min_p, want_share)
+
+
+_ACTIVATIONS = {"none": 0, "relu": 1, "sigmoid": 2, "hard_tanh": 3}
+
+
+def _activation(name):
+    if name not in _ACTIVATIONS:
+        raise capi.BbhipError("activation %r is none of %s" % (name, ", ".join(_ACTIVATIONS)))
+    return _ACTIVATIONS[name]
+
+
+def dense_affine_forward(x, W, b, frame_size, activation="none", residual=None, y_stride=None):
+    """y = activation(W x + b + residual): fp32 x [inputs, stride], W [outputs, inputs], b [outputs] or None, residual [outputs, any stride] or None -> y [outputs, y_stride]
+    (by default x's stride).  activation: none, relu, sigmoid or hard_tanh (limits -1 and 1)."""
+    return native.dense_affine_forward(x, W, b, frame_size, x.shape[-1] if y_stride is None else y_stride, _activation(activation), residual)
+
+
+def bit_dense_affine_forward(xbits, W, b, frame_size, y_stride, activation="none", residual=None):
+    """The same over packed bits [inputs, words], read as 0 and 1."""
+    return native.bit_dense_affine_forward(xbits, W, b, frame_size, y_stride, _activation(activation), residual)
+
+
+def dense_affine_forward_bits(x, W, b, frame_size, y_words=None, residual=None):
+    """Packed bits [outputs, y_words], set where W x + b + residual > 0; words behind the frames are 0."""
+    return native.dense_affine_forward_bits(x, W, b, frame_size, synth.frame_stride_bit(frame_size) if y_words is None else y_words, residual)
+
+
+def bit_dense_affine_forward_bits(xbits, W, b, frame_size, y_words=None, residual=None):
+    """The same over packed bits."""
+    return native.bit_dense_affine_forward_bits(xbits, W, b, frame_size, xbits.shape[-1] if y_words is None else y_words, residual)
+
+
+def dense_affine_backward(x, dy, W, frame_size, activation="none", y=None, dW=None, db=None, want_dx=True, want_weights=True, want_dr=False):
+    """-> (dx, dW, db, dr), dr the residual's gradient; None for what is not wanted.  y: the forward pass's output, with the row pitch of dy (needed with an activation).  dW and db
+    given: added to in place."""
+    return native.dense_affine_backward(x, dy, W, frame_size, _activation(activation), y, dW, db, want_dx, want_weights, want_dr)
+
+
+def bit_dense_affine_backward(xbits, dy, W, frame_size, activation="none", y=None, dW=None, db=None, want_dx=True, want_weights=True, want_dr=False):
+    """The same for a forward pass over packed bits; dx is the gradient of the bits' values."""
+    return native.bit_dense_affine_backward(xbits, dy, W, frame_size, _activation(activation), y, dW, db, want_dx, want_weights, want_dr)
+
+
+def _loss_weight_sum(label, weight, weight_sum, channels, frame_size):
+    if weight_sum is not None:
+        return weight_sum
+    label = label.reshape(-1)[:frame_size]
+    counts = (label >= 0) & (label < channels)
+    return float((counts if weight is None else torch.where(counts, weight.reshape(-1)[:frame_size], 0.0)).sum(dtype=torch.float64).item())
+
+
+def loss_dense_softmax_cross_entropy(x, W, b, label, frame_size, weight=None, weight_sum=None, dW=None, db=None, want_gradients=True, want_dx=True, want_weights=True):
+    """The cross entropy of softmax(W x + b) against label (int32 [1, at least frame_size]; negative, or no channel: the frame does not count), and its gradients, without ever holding the
+    logits of all channels: (loss [1, stride of x], dx, dW, db), None for what is not wanted.  The loss of the batch is loss[:, :frame_size].sum() / weight_sum, whose gradient they are.
+    weight [1, ...]: of each frame (None: 1); weight_sum defaults to the sum of the weights that count, read by the host (a captured step gives its own).  dW and db given: added to in place."""
+    return native.loss_dense_softmax_cross_entropy(x, W, b, label, frame_size, x.shape[-1], weight, _loss_weight_sum(label, weight, weight_sum, W.shape[0], frame_size), dW, db,
+                                                   want_gradients and want_dx, want_gradients and want_weights)
+
+
+def bit_loss_dense_softmax_cross_entropy(xbits, W, b, label, frame_size, stride, weight=None, weight_sum=None, dW=None, db=None, want_gradients=True, want_dx=True, want_weights=True):
+    """The same over packed bits; loss and dx have rows of `stride`."""
+    return native.bit_loss_dense_softmax_cross_entropy(xbits, W, b, label, frame_size, stride, weight, _loss_weight_sum(label, weight, weight_sum, W.shape[0], frame_size), dW, db,
+                                                       want_gradients and want_dx, want_gradients and want_weights)
 
 
 def conv_bit_to_real(xbits, frame_size, y_stride, value0=0.0, value1=1.0):

@@ -520,6 +520,69 @@ int bbhip_fp32_CategoricalSampling(float const *dev_y_buf, float const *dev_u_bu
                                    float top_p, float min_p, int pix_size, int ch_size, int frame_size, int frame_stride, void *dev_workspace,
                                    size_t workspace_size, void *stream);
 
+/* ---- dense layers, the loss on top of one, clipped gradients (no counterpart in the reference's device library; its DenseAffine is a host loop over a BLAS) ----
+ * As at the head of a network, scratch comes from the caller: dev_workspace, 256-byte aligned, of at least the bytes that the ...WorkspaceBytes of the same sizes says (it
+ * may be 0); nothing in it need be cleared or kept.  Calls that overlap in time need workspaces of their own.  Results have the same bits on every run.
+ *
+ * DenseAffine: every output node sees every input node.  W is [output_node_size][input_node_size], b [output_node_size] (NULL: none), residual frames (NULL: none) have rows
+ * of residual_frame_stride and may be the output buffer itself:
+ *     y[o][f] = activation(sum over i of W[o][i] * x[i][f] + b[o] + residual[o][f])
+ * activation: 0 none, 1 relu, 2 sigmoid, 3 hard tanh (limits -1 and 1).  bit_...: x is packed bits, read as 0 and 1; ..._bit: y is packed bits, set where the sum is above 0 (the bits
+ * behind the last frame of its word are 0; further words of a row are left alone). 
+ * At most 2^24 nodes and 2^26 frames. */
+size_t bbhip_DenseAffine_WorkspaceBytes(int input_node_size, int output_node_size, int frame_size);
+int bbhip_fp32_DenseAffine_Forward(float const *dev_x_buf, float *dev_y_buf, float const *dev_W, float const *dev_b, float const *dev_residual_buf, int activation,
+                                   int input_node_size, int output_node_size, int frame_size, int x_frame_stride, int y_frame_stride, int residual_frame_stride,
+                                   void *dev_workspace, size_t workspace_size, void *stream);
+int bbhip_bit_fp32_DenseAffine_Forward(int const *dev_x_buf, float *dev_y_buf, float const *dev_W, float const *dev_b, float const *dev_residual_buf, int activation,
+                                       int input_node_size, int output_node_size, int frame_size, int x_frame_stride, int y_frame_stride, int residual_frame_stride,
+                                       void *dev_workspace, size_t workspace_size, void *stream);
+int bbhip_fp32_bit_DenseAffine_Forward(float const *dev_x_buf, int *dev_y_buf, float const *dev_W, float const *dev_b, float const *dev_residual_buf, int input_node_size,
+                                       int output_node_size, int frame_size, int x_frame_stride, int y_frame_stride, int residual_frame_stride, void *dev_workspace,
+                                       size_t workspace_size, void *stream);
+int bbhip_bit_bit_DenseAffine_Forward(int const *dev_x_buf, int *dev_y_buf, float const *dev_W, float const *dev_b, float const *dev_residual_buf, int input_node_size,
+                                      int output_node_size, int frame_size, int x_frame_stride, int y_frame_stride, int residual_frame_stride, void *dev_workspace,
+                                      size_t workspace_size, void *stream);
+/* With dz = dy * activation'(y), the derivative taken from the forward pass's output dev_y_buf (NULL without an activation; a closed activation passes 0 whatever dy is):
+ *     dx[i][f] = sum over o of W[o][i] * dz[o][f],   dW[o][i] = sum over f of dz[o][f] * x[i][f],   db[o] = sum over f of dz[o][f],   dr = dz (the residual's gradient).
+ * Each of dx, dW, dr may be NULL, db too (it is formed with dW); dW and db are added to what they hold with accumulate, as dW of the LUT layers, else written.  dy, y and dr have
+ * rows of frame_stride.  No output may overlap an input. */
+int bbhip_fp32_DenseAffine_Backward(float const *dev_x_buf, float const *dev_dy_buf, float const *dev_y_buf, float const *dev_W, float *dev_dx_buf, float *dev_dW,
+                                    float *dev_db, float *dev_dr_buf, int activation, int accumulate, int input_node_size, int output_node_size, int frame_size,
+                                    int x_frame_stride, int dx_frame_stride, int frame_stride, void *dev_workspace, size_t workspace_size, void *stream);
+int bbhip_bit_fp32_DenseAffine_Backward(int const *dev_x_buf, float const *dev_dy_buf, float const *dev_y_buf, float const *dev_W, float *dev_dx_buf, float *dev_dW,
+                                        float *dev_db, float *dev_dr_buf, int activation, int accumulate, int input_node_size, int output_node_size, int frame_size,
+                                        int x_frame_stride, int dx_frame_stride, int frame_stride, void *dev_workspace, size_t workspace_size, void *stream);
+
+/* LossDenseSoftmaxCrossEntropy: the cross entropy of p = softmax(W x + b) over ch_size channels (W [ch][input]) against one label per frame, and its gradients, in pieces of the
+ * channels: the logits are never held whole, the workspace does not grow with the channels beyond a piece's.  With w the frame's weight (dev_weight_buf, NULL: 1)
+ *     dev_loss_buf[f] = -w * log p_label,   dz[c] = w / weight_sum * (p_c - [c is the label]),   dx = W^T dz,   dW = dz x^T,   db = sum over frames of dz.
+ * The caller passes weight_sum = the sum of the weights that count and reports sum(dev_loss_buf) / weight_sum, whose gradients these are.  A frame whose label is negative or not below ch_size, or
+ * whose weight is 0, does not count: loss 0, dx 0 and no part of dW and db, whatever it holds.  dx, dW and db (which is formed with dW) may be NULL: without any of them the loss alone is
+ * computed, in half the time or less.  dW and db are added to what they hold with accumulate.  gradients: whether there will be any. */
+size_t bbhip_LossDenseSoftmaxCrossEntropy_WorkspaceBytes(int input_node_size, int ch_size, int frame_size, int gradients);
+int bbhip_fp32_LossDenseSoftmaxCrossEntropy(float const *dev_x_buf, float const *dev_W, float const *dev_b, int const *dev_label_buf, float const *dev_weight_buf,
+                                            float *dev_dx_buf, float *dev_dW, float *dev_db, float *dev_loss_buf, float weight_sum, int accumulate, int input_node_size,
+                                            int ch_size, int frame_size, int x_frame_stride, int dx_frame_stride, void *dev_workspace, size_t workspace_size, void *stream);
+int bbhip_bit_fp32_LossDenseSoftmaxCrossEntropy(int const *dev_x_buf, float const *dev_W, float const *dev_b, int const *dev_label_buf, float const *dev_weight_buf,
+                                                float *dev_dx_buf, float *dev_dW, float *dev_db, float *dev_loss_buf, float weight_sum, int accumulate,
+                                                int input_node_size, int ch_size, int frame_size, int x_frame_stride, int dx_frame_stride, void *dev_workspace,
+                                                size_t workspace_size, void *stream);
+
+/* The norm of `size` gradients as if they were one vector (device tables of element counts and addresses, as the Adam entries take them), and the scale that brings it to max_norm:
+ *     dev_norm[0] = sqrt(sum of all g^2),   dev_norm[1] = norm > max_norm ? max_norm / norm : 1
+ * with sums in 64 bits.  max_norm: 0 up to infinity (measure only).  GradientClip also multiplies every gradient by the scale; OptimizerAdam_Clipped makes the Adam step with the scaled gradients
+ * and leaves them as they are, or with zero_grads sets them to zero (its betas are in 64 bits: 1 - beta2 of 0.999 as a float is off by 1.3e-5; of betas that are floats it is the bits of the plain step).  Where an element is infinite the scale is 0 (and that element's product not a number); where one is not a
+ * number the norm is none either, and the scale is 1.  No tensor may be in a list twice. */
+size_t bbhip_GradientNorm_WorkspaceBytes(void);
+int bbhip_fp32_GradientNorm(int size, int const *dev_size_table, float *const *dev_grads_buf_table, float max_norm, float *dev_norm, void *dev_workspace,
+                            size_t workspace_size, void *stream);
+int bbhip_fp32_GradientClip(int size, int const *dev_size_table, float *const *dev_grads_buf_table, float max_norm, float *dev_norm, void *dev_workspace,
+                            size_t workspace_size, void *stream);
+int bbhip_fp32_OptimizerAdam_Clipped(int size, int const *dev_size_table, float *const *dev_params_buf_table, float *const *dev_grads_buf_table,
+                                     float *const *dev_m_buf_table, float *const *dev_v_buf_table, float lr_t, double beta1, double beta2, float max_norm, float *dev_norm,
+                                     int zero_grads, void *dev_workspace, size_t workspace_size, void *stream);
+
 /* ---- StochasticLut ---- */
 /* bbcu_fp32_StochasticLut_Forward<N>, include/bbcu/bbcu.h:667-681 */
 int bbhip_fp32_StochasticLut_Forward(int n, float const *dev_x_buf, float *dev_y_buf, int const *dev_input_index,

@@ -3,12 +3,15 @@
 
 #include <hip/hip_runtime.h>
 
+#include <new>
+
 #include "../../include/bbhip.h"
 #include "host_calls.hpp"
 #include "launch_rules.hpp"
 #include "dense_rules.hpp"
 #include "dense_direct_kernels.hpp"
 #include "dense_loss_kernels.hpp"
+#include "dense_packed_kernels.hpp"
 #include "gradient_norm_kernels.hpp"
 
 using namespace bbhip;
@@ -18,8 +21,9 @@ namespace {
 // a product as the entries describe it, before it is known how it is computed
 struct Product {
     Operand     a, b;
+    int         kind_a, kind_b;
     DenseOutput out;
-    bool wanted = true;
+    bool wanted = true, again = false;          // again: elements that come out as no number are formed again
 };
 
 Operand rows_of(float const *p, long long stride, int rows, int depth)
@@ -87,6 +91,150 @@ int direct_backward(Product const &dw, Product const &dx, bool bit, hipStream_t 
     return 0;
 }
 
+// ---- products by way of packed halves ----
+// Takes pieces of a workspace, or counts them (base null)
+struct Carver {
+    char *base;
+    size_t at = 0;
+    template <class E> E *take(size_t count)
+    {
+        E *const p = base ? reinterpret_cast<E *>(base + at) : nullptr;
+        at += align256(count * sizeof(E));
+        return p;
+    }
+};
+
+bool is_bits(int kind) { return kind == kBitRows || kind == kBitColumns; }
+
+// an operand's halves and scales in a workspace, and the job that writes them
+struct Packed {
+    uint4 *halves;
+    int   *exponent;
+    int    blocks, steps, pieces;
+    Packed() = default;
+    Packed(Carver &c, int rows, int depth, bool bits) : blocks(ceil_div(rows, 32)), steps(pack_steps(depth)), pieces(bits ? 1 : 2)
+    {
+        halves = c.take<uint4>((size_t)blocks * steps * pieces * 64);
+        exponent = bits ? nullptr : c.take<int>((size_t)blocks * 32);
+    }
+    PackJob job(Operand const &o, int kind) const
+    {
+        PackJob j{};
+        j.src = o; j.kind = kind; j.halves = halves; j.exponent = exponent; j.k_steps = steps;
+        bool const side_by_side = kind == kRows || kind == kBitRows || kind == kGradRows;
+        j.blocks = side_by_side ? blocks * 4 : blocks;
+        return j;
+    }
+};
+
+struct Jobs {
+    PackArgs a{};
+    int count = 0;
+    void add(PackJob const &j) { a.job[count++] = j; }
+    int run(hipStream_t st, char const *name) const
+    {
+        long long total = 0;
+        for (int i = 0; i < count; ++i) { total += a.job[i].blocks; }
+        if (check_tiles(total, kPackBlock, name)) { return 1; }
+        launch(dense_pack_kernel, dim3((unsigned)total), dim3(kPackBlock), 0, st, a);
+        BBHIP_LAUNCH_CHECK();
+        return 0;
+    }
+};
+
+float *sums_of(Carver &c, PackedShape const &s, int m, int n) { return s.slabs > 1 ? c.take<float>((size_t)s.slabs * m * (ceil_div(n, 64) * 64)) : nullptr; }
+
+int packed_product(PackedProduct &d, Product const &p, PackedShape const &s, Packed const &a, Packed const &b, float *sums, char const *name)
+{
+    d = PackedProduct{};
+    if (!p.wanted) { d.b_pieces = 2; return 0; }
+    d.a = a.halves; d.ea = a.exponent; d.a_blocks = a.blocks;
+    d.b = b.halves; d.eb = b.exponent; d.b_blocks = b.blocks; d.b_pieces = b.pieces;
+    d.k_steps = s.k_steps; d.m_tiles = s.m_tiles; d.n_tiles = s.n_tiles; d.slabs = s.slabs; d.slab_stages = s.slab_stages;
+    if (check_tiles(s.workgroups(), s.large ? 512 : 256, name)) { return 1; }
+    d.workgroups = (int)s.workgroups();
+    d.sums = sums; d.sums_pitch = ceil_div(p.out.columns, 64) * 64; d.sums_slab = d.sums_pitch * p.out.rows;
+    d.out = p.out;
+    d.src_a = p.a; d.src_b = p.b; d.kind_a = p.again ? p.kind_a : -1; d.kind_b = p.kind_b;
+    return 0;
+}
+
+// p and behind it q, whose operands are not packed bits
+int packed_run(PackedProduct const &p, PackedProduct const &q, bool large, hipStream_t st, char const *name)
+{
+    if (check_tiles((long long)p.workgroups + q.workgroups, large ? 512 : 256, name)) { return 1; }
+    if (p.workgroups + q.workgroups == 0) { return 0; }
+    dim3 const grid((unsigned)(p.workgroups + q.workgroups));
+    if (large) {
+        if (p.b_pieces == 1) { launch((dense_packed_kernel<4, 2, 4, 1>), grid, dim3(512), 0, st, p, q); }
+        else                 { launch((dense_packed_kernel<4, 2, 4, 2>), grid, dim3(512), 0, st, p, q); }
+    }
+    else {
+        if (p.b_pieces == 1) { launch((dense_packed_kernel<2, 2, 2, 1>), grid, dim3(256), 0, st, p, q); }
+        else                 { launch((dense_packed_kernel<2, 2, 2, 2>), grid, dim3(256), 0, st, p, q); }
+    }
+    BBHIP_LAUNCH_CHECK();
+    auto const join_blocks = [](PackedProduct const &d) { return d.slabs > 1 ? ((long long)d.out.rows * d.sums_pitch + 255) / 256 : 0; };
+    long long const first = join_blocks(p), second = join_blocks(q);
+    if (first + second > 0) {
+        if (check_tiles(first + second, 256, name)) { return 1; }
+        launch(dense_join_kernel, dim3((unsigned)(first + second)), dim3(256), 0, st, p, q, (unsigned)first);
+        BBHIP_LAUNCH_CHECK();
+    }
+    return 0;
+}
+
+// of a layer's forward pass
+struct ForwardSpace {
+    PackedShape shape;
+    Packed W, x;
+    float *sums;
+    ForwardSpace(Carver &c, int inputs, int outputs, int frames, bool bit)
+        : shape(best_shape(outputs, frames, inputs)), W(c, outputs, inputs, false), x(c, frames, inputs, bit), sums(sums_of(c, shape, outputs, frames)) {}
+};
+
+// of its backward pass
+struct BackwardSpace {
+    PackedShape dw, dx;
+    Packed dz_rows, x, W, dz_columns;
+    float *dw_sums, *dx_sums;
+    BackwardSpace(Carver &c, int inputs, int outputs, int frames, bool bit)
+    {
+        best_shapes(outputs, inputs, frames, inputs, frames, outputs, dw, dx);
+        dz_rows = Packed(c, outputs, frames, false);
+        x = Packed(c, inputs, frames, bit);
+        W = Packed(c, inputs, outputs, false);
+        dz_columns = Packed(c, frames, outputs, false);
+        dw_sums = sums_of(c, dw, outputs, inputs);
+        dx_sums = sums_of(c, dx, inputs, frames);
+    }
+    // the last piece of a loss, of fewer channels: the same places, the same divisions of the k axis or fewer
+    void cut(int inputs, int outputs, int frames)
+    {
+        dw = packed_shape(dw.large, dw.slabs, outputs, inputs, frames);
+        dx = packed_shape(dx.large, dx.slabs, inputs, frames, outputs);
+        dz_rows.blocks = ceil_div(outputs, 32);
+        W.steps = dz_columns.steps = pack_steps(outputs);
+    }
+    // jobs of both products (x apart: the pieces of a loss share it); the rows' job may leave db and dz on its way
+    void add_jobs(Jobs &jobs, Product const &w, Product const &i, bool with_x, float *db, int accumulate, float *dz, long long dz_stride) const
+    {
+        if (w.wanted || dz) {
+            PackJob j = dz_rows.job(w.a, kGradRows);
+            j.line = db; j.accumulate = accumulate; j.dz = dz; j.dz_stride = dz_stride;
+            jobs.add(j);
+        }
+        if (w.wanted && with_x) { jobs.add(x.job(w.b, w.kind_b)); }
+        if (i.wanted) { jobs.add(W.job(i.a, i.kind_a)); jobs.add(dz_columns.job(i.b, i.kind_b)); }
+    }
+    int run(Product const &w, Product const &i, hipStream_t st, char const *name) const
+    {
+        PackedProduct p, q;
+        if (packed_product(p, w, dw, dz_rows, x, dw_sums, name) || packed_product(q, i, dx, W, dz_columns, dx_sums, name)) { return 1; }
+        return packed_run(p, q, dw.large, st, name);
+    }
+};
+
 // ---- what an entry checks ----
 int check_sizes(int inputs, int outputs, int frames, char const *name)
 {
@@ -128,14 +276,25 @@ int dense_forward(void const *x, bool bit, void *y, bool bit_out, float const *W
     Product p;
     p.a = rows_of(W, inputs, outputs, inputs);
     p.b = frames_as_columns(x, x_stride, inputs, frames);
+    p.kind_a = kRows; p.kind_b = bit ? kBitColumns : kColumns; p.again = true;
     p.out = DenseOutput{};
     p.out.kind = bit_out ? kOutBits : kOutForward;
     p.out.rows = outputs; p.out.columns = frames; p.out.out = y; p.out.stride = y_stride;
     p.out.bias = b; p.out.residual = residual; p.out.residual_stride = residual_stride; p.out.activation = activation;
     hipStream_t const st = static_cast<hipStream_t>(stream);
-    if (check_workspace(workspace, workspace_size, 0, name)) { return 1; }
+    if (!product_packed(outputs, frames, inputs)) {
+        ScopedTimer tm(kTimeOther, st);
+        return direct_forward(p, bit, st, name);
+    }
+    Carver c{static_cast<char *>(workspace)};
+    ForwardSpace const s(c, inputs, outputs, frames, bit);
+    if (check_workspace(workspace, workspace_size, c.at, name)) { return 1; }
     ScopedTimer tm(kTimeOther, st);
-    return direct_forward(p, bit, st, name);
+    Jobs jobs;
+    jobs.add(s.W.job(p.a, p.kind_a));
+    jobs.add(s.x.job(p.b, p.kind_b));
+    PackedProduct d, none{};
+    return jobs.run(st, name) || packed_product(d, p, s.shape, s.W, s.x, s.sums, name) || packed_run(d, none, s.shape.large, st, name);
 }
 
 int dense_backward(void const *x, bool bit, float const *dy, float const *y, float const *W, float *dx, float *dW, float *db, float *dr, int activation,
@@ -156,15 +315,25 @@ int dense_backward(void const *x, bool bit, float const *dy, float const *y, flo
     w.wanted = dW != nullptr;
     w.a = g; w.a.rows = outputs; w.a.depth = frames;
     w.b = frames_as_depth(x, bit, x_stride, inputs, frames);
+    w.kind_a = kGradRows; w.kind_b = bit ? kBitRows : kRows;
     w.out = DenseOutput{};
     w.out.kind = kOutStore; w.out.rows = outputs; w.out.columns = inputs; w.out.out = dW; w.out.stride = inputs; w.out.accumulate = accumulate; w.out.line = db;
     i.wanted = dx != nullptr;
     i.a = rows_of(W, inputs, inputs, outputs);
     i.b = g; i.b.rows = frames; i.b.depth = outputs;
+    i.kind_a = kColumns; i.kind_b = kGradColumns; w.again = i.again = true;
     i.out = DenseOutput{};
     i.out.kind = kOutStore; i.out.rows = inputs; i.out.columns = frames; i.out.out = dx; i.out.stride = dx_stride;
     hipStream_t const st = static_cast<hipStream_t>(stream);
-    if (check_workspace(workspace, workspace_size, 0, name)) { return 1; }
+    if (product_packed(outputs, frames, inputs)) {
+        Carver c{static_cast<char *>(workspace)};
+        BackwardSpace const s(c, inputs, outputs, frames, bit);
+        if (check_workspace(workspace, workspace_size, c.at, name)) { return 1; }
+        ScopedTimer tm(kTimeOther, st);
+        Jobs jobs;
+        s.add_jobs(jobs, w, i, true, db, accumulate, dr, stride);
+        return jobs.run(st, name) || s.run(w, i, st, name);
+    }
     ScopedTimer tm(kTimeOther, st);
     if (direct_backward(w, i, bit, st, name)) { return 1; }
     if (dr) {
@@ -179,18 +348,29 @@ int dense_backward(void const *x, bool bit, float const *dy, float const *y, flo
 // ---- the loss on top of a dense layer ----
 struct LossSpace {
     LossPlan plan;
-    size_t partial, label_logit, top, share, coef, logits, total;          // offsets
-    LossSpace(int inputs, int channels, int frames, bool gradients) : plan(loss_plan(inputs, channels, frames))
+    float2 *partial;
+    float *label_logit, *top = nullptr, *share = nullptr, *coef = nullptr, *logits = nullptr;
+    Packed W, x;                        // packed: of a piece's logits
+    alignas(BackwardSpace) char backward_space[sizeof(BackwardSpace)];
+    size_t total;
+    BackwardSpace const &backward(void) const { return *reinterpret_cast<BackwardSpace const *>(backward_space); }
+    LossSpace(char *base, int inputs, int channels, int frames, bool bit, bool gradients) : plan(loss_plan(inputs, channels, frames))
     {
-        size_t at = 0;
-        auto const take = [&](size_t bytes) { size_t const was = at; at += align256(bytes); return was; };
-        partial     = take((size_t)plan.tiles * frames * sizeof(float2));
-        label_logit = take((size_t)frames * 4);
-        top         = take(gradients ? (size_t)frames * 4 : 0);
-        share       = take(gradients ? (size_t)frames * 4 : 0);
-        coef        = take(gradients ? (size_t)frames * 4 : 0);
-        logits      = take(gradients ? (size_t)plan.piece * plan.stride * 4 : 0);
-        total       = at;
+        Carver c{base};
+        partial     = c.take<float2>((size_t)plan.tiles * frames);
+        label_logit = c.take<float>((size_t)frames);
+        if (gradients) {
+            top    = c.take<float>((size_t)frames);
+            share  = c.take<float>((size_t)frames);
+            coef   = c.take<float>((size_t)frames);
+            logits = c.take<float>((size_t)plan.piece * plan.stride);
+        }
+        if (plan.packed) {
+            W = Packed(c, plan.piece, inputs, false);
+            x = Packed(c, frames, inputs, bit);
+            if (gradients) { new (backward_space) BackwardSpace(c, inputs, plan.piece, frames, bit); }
+        }
+        total = c.at;
     }
 };
 
@@ -204,13 +384,13 @@ int dense_loss(void const *x, bool bit, float const *W, float const *b, int cons
     if (check_sizes(inputs, channels, frames, name)) { return 1; }
     if (check_stride(bit, x_stride, frames, name) || (dx && check_stride(false, dx_stride, frames, name))) { return 1; }
     bool const gradients = dx || dW;
-    LossSpace const s(inputs, channels, frames, gradients);
+    LossSpace const s(static_cast<char *>(workspace), inputs, channels, frames, bit, gradients);
     if (check_workspace(workspace, workspace_size, s.total, name)) { return 1; }
-    char *const base = static_cast<char *>(workspace);
-    float *const logits = reinterpret_cast<float *>(base + s.logits), *const coef = reinterpret_cast<float *>(base + s.coef);
+    float *const logits = s.logits, *const coef = s.coef;
     hipStream_t const st = static_cast<hipStream_t>(stream);
     ScopedTimer tm(kTimeOther, st);
     int const pieces = ceil_div(channels, s.plan.piece);
+    bool x_packed = false, x_rows_packed = false;
     auto const logit_piece = [&](int piece, bool store) {
         int const first = piece * s.plan.piece, count = channels - first < s.plan.piece ? channels - first : s.plan.piece;
         Product p;
@@ -219,18 +399,24 @@ int dense_loss(void const *x, bool bit, float const *W, float const *b, int cons
         p.out = DenseOutput{};
         p.out.kind = kOutLogits; p.out.rows = count; p.out.columns = frames; p.out.out = store ? logits : nullptr; p.out.stride = s.plan.stride;
         p.out.bias = b ? b + first : nullptr;
-        p.out.partial = reinterpret_cast<float2 *>(base + s.partial) + (size_t)(first / kLossTile) * frames;
-        p.out.label = label; p.out.label_logit = reinterpret_cast<float *>(base + s.label_logit); p.out.first_channel = first;
-        return direct_forward(p, bit, st, name);
+        p.out.partial = s.partial + (size_t)(first / s.plan.tile) * frames;
+        p.out.label = label; p.out.label_logit = s.label_logit; p.out.first_channel = first;
+        if (!s.plan.packed) { return direct_forward(p, bit, st, name); }
+        Jobs jobs;
+        jobs.add(s.W.job(p.a, kRows));
+        if (!x_packed) { jobs.add(s.x.job(p.b, bit ? kBitColumns : kColumns)); x_packed = true; }
+        PackedShape const shape = packed_shape(s.plan.logits.large, 1, count, frames, inputs);
+        PackedProduct d, none{};
+        Packed W_piece = s.W;
+        W_piece.blocks = ceil_div(count, 32);
+        return (int)(jobs.run(st, name) || packed_product(d, p, shape, W_piece, s.x, nullptr, name) || packed_run(d, none, shape.large, st, name));
     };
     // the pieces' largest logits and sums; the last piece's logits stay for its gradient
     for (int piece = 0; piece < pieces; ++piece) { if (logit_piece(piece, gradients && piece == pieces - 1)) { return 1; } }
     LossFinishArgs f{};
-    f.partial = reinterpret_cast<float2 const *>(base + s.partial); f.label_logit = reinterpret_cast<float const *>(base + s.label_logit);
+    f.partial = s.partial; f.label_logit = s.label_logit;
     f.label = label; f.weight = weight; f.loss = loss;
-    f.top = gradients ? reinterpret_cast<float *>(base + s.top) : nullptr;
-    f.share = gradients ? reinterpret_cast<float *>(base + s.share) : nullptr;
-    f.coef = gradients ? coef : nullptr;
+    f.top = s.top; f.share = s.share; f.coef = coef;
     f.reciprocal_weight_sum = (float)(1.0 / (double)weight_sum);
     f.tiles = s.plan.tiles; f.frames = frames; f.channels = channels;
     launch(dense_loss_finish_kernel, dim3((unsigned)ceil_div(frames, kFinishFrames)), dim3(kFinishFrames * kFinishGroups), 0, st, f);
@@ -247,15 +433,26 @@ int dense_loss(void const *x, bool bit, float const *W, float const *b, int cons
         w.a = g; w.a.rows = count; w.a.depth = frames;
         w.b = frames_as_depth(x, bit, x_stride, inputs, frames);
         if (!bit) { w.b.coef = coef; }
+        w.kind_a = kGradRows; w.kind_b = bit ? kBitRows : kRows;
         w.out = DenseOutput{};
         w.out.kind = kOutStore; w.out.rows = count; w.out.columns = inputs; w.out.out = dW + (size_t)first * inputs; w.out.stride = inputs;
         w.out.accumulate = accumulate; w.out.line = db ? db + first : nullptr;
         i.wanted = dx != nullptr;
         i.a = rows_of(W + (size_t)first * inputs, inputs, inputs, count);
         i.b = g; i.b.rows = frames; i.b.depth = count;
+        i.kind_a = kColumns; i.kind_b = kGradColumns;
         i.out = DenseOutput{};
         i.out.kind = kOutStore; i.out.rows = inputs; i.out.columns = frames; i.out.out = dx; i.out.stride = dx_stride; i.out.accumulate = piece != pieces - 1;
-        if (direct_backward(w, i, bit, st, name)) { return 1; }
+        if (!s.plan.packed) {
+            if (direct_backward(w, i, bit, st, name)) { return 1; }
+            continue;
+        }
+        Jobs jobs;
+        BackwardSpace b = s.backward();
+        if (count != s.plan.piece) { b.cut(inputs, count, frames); }
+        b.add_jobs(jobs, w, i, !x_rows_packed, w.out.line, accumulate, nullptr, 0);
+        x_rows_packed = true;
+        if (jobs.run(st, name) || b.run(w, i, st, name)) { return 1; }
     }
     return 0;
 }
@@ -280,8 +477,11 @@ int squares(int size, int const *sizes, float *const *grads, void *workspace, si
 
 size_t bbhip_DenseAffine_WorkspaceBytes(int input_node_size, int output_node_size, int frame_size)
 {
-    (void)input_node_size; (void)output_node_size; (void)frame_size;
-    return 0;
+    if (check_sizes(input_node_size, output_node_size, frame_size, __func__) || !product_packed(output_node_size, frame_size, input_node_size)) { return 0; }
+    Carver forward{nullptr}, backward{nullptr};
+    ForwardSpace const f(forward, input_node_size, output_node_size, frame_size, false);
+    BackwardSpace const b(backward, input_node_size, output_node_size, frame_size, false);
+    return forward.at > backward.at ? forward.at : backward.at;
 }
 
 int bbhip_fp32_DenseAffine_Forward(float const *dev_x_buf, float *dev_y_buf, float const *dev_W, float const *dev_b, float const *dev_residual_buf, int activation,
@@ -335,7 +535,9 @@ int bbhip_bit_fp32_DenseAffine_Backward(int const *dev_x_buf, float const *dev_d
 size_t bbhip_LossDenseSoftmaxCrossEntropy_WorkspaceBytes(int input_node_size, int ch_size, int frame_size, int gradients)
 {
     if (check_sizes(input_node_size, ch_size, frame_size, __func__)) { return 0; }
-    return LossSpace(input_node_size, ch_size, frame_size, gradients != 0).total;
+    size_t const bits = LossSpace(nullptr, input_node_size, ch_size, frame_size, true, gradients != 0).total;
+    size_t const values = LossSpace(nullptr, input_node_size, ch_size, frame_size, false, gradients != 0).total;
+    return bits > values ? bits : values;
 }
 
 int bbhip_fp32_LossDenseSoftmaxCrossEntropy(float const *dev_x_buf, float const *dev_W, float const *dev_b, int const *dev_label_buf, float const *dev_weight_buf,

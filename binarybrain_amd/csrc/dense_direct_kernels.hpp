@@ -22,9 +22,6 @@ struct DirectProduct {
     int tiles;
 };
 
-// D of element `reg` of lane `lane`: row, column within the tile
-__device__ __forceinline__ int acc_row(int reg, int lane) { return (reg & 3) + 8 * (reg >> 2) + 4 * (lane >> 5); }
-
 template <int KA, int KB, int WAVES>
 __device__ __forceinline__ void direct_product(DirectProduct const &t, int tile, float *lds)
 {

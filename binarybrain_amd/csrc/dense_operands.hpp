@@ -188,6 +188,9 @@ __device__ __forceinline__ void load_values(Operand const &o, int row, int k, fl
     }
 }
 
+// Row of element `reg` of lane `lane` in the result of a 32 x 32 matrix instruction; the column is lane & 31.
+__device__ __forceinline__ int acc_row(int reg, int lane) { return (reg & 3) + 8 * (reg >> 2) + 4 * (lane >> 5); }
+
 // ---- what becomes of an element of the product -----------------------------------------------------------------------------------------
 enum DenseOutputKind : int {
     kOutForward = 0,        // y = activation(D + bias + residual)

@@ -1,0 +1,417 @@
+// Products of dense layers on the fp16 matrix instructions, to the accuracy of fp32: large problems.
+//
+// A value v of an operand's row is scaled by a power of two that brings the largest of its row into [2^14, 2^15), and split into two halves, v 2^e = h + l with
+// h = fp16(v 2^e), l = fp16(v 2^e - h): 22 bits, so that  a b = (ah bh + ah bl + al bh) 2^-(ea + eb)  up to 3 * 2^-22 of a product at most (the product of the two lower halves is left
+// out) and about 2^-24 on the average: what rounding the factors to fp32 would cost.  The matrix instruction multiplies halves exactly and sums in fp32.  Three fp16 products run
+// at 2.5 PFLOP/s / 3 where the fp32 matrix instructions have 0.157; a packed-bit operand is one half without any error, so its products are two.  What the scaling
+// costs: a value more than 2^15 times smaller than the largest of its row keeps fewer bits, and is off by at most 2^-40 of that one.
+//
+// Two launches.  The first reads each operand as it lies and leaves its halves in the order in which the matrix instructions want them: blocks of 32 rows x 16 k,
+// 1 KiB each, lane l's sixteen bytes (row l & 31, k 8 (l >> 5) .. + 8) at 16 l, so that the second launch moves them to LDS and from there to registers with 16-byte accesses
+// that meet no bank twice, without a transposition anywhere.  In the second, a workgroup of eight wavefronts owns 256 x 256 elements (128 x 128: four) and walks k in stages of 32,
+// the loads of the next stage to LDS in flight behind the products of the present one.
+// Where there are too few tiles for the device, several workgroups share a tile's k axis and a third launch adds their sums in a fixed order.
+#pragma once
+
+#include "dense_operands.hpp"
+
+namespace bbhip {
+
+typedef _Float16 DenseHalf8 __attribute__((ext_vector_type(8)));
+typedef float    DenseAcc16 __attribute__((ext_vector_type(16)));
+
+constexpr int kPackBlock = 512, kStageK = 32;
+constexpr int kPackHeld = 8;                    // groups of eight values that a thread keeps between finding the largest and splitting
+
+struct PackJob {
+    Operand src;
+    int    kind;
+    uint4 *halves;              // [row blocks][k steps][1 or 2][64 lanes]
+    int   *exponent;            // of each row (null: packed bits, which are not scaled)
+    int    k_steps;             // of 16, even
+    int    blocks;              // workgroups
+    float *line;                // gradients as rows: their sums (null: not wanted), added with accumulate
+    int    accumulate;
+    float *dz;                  // gradients as rows: themselves (null: not wanted), rows of dz_stride
+    long long dz_stride;
+};
+
+constexpr int kPackJobs = 4;
+struct PackArgs { PackJob job[kPackJobs]; };
+
+__device__ __forceinline__ uint32_t two_halves(float a, float b)
+{
+    typedef _Float16 Half2 __attribute__((ext_vector_type(2)));
+    Half2 const h = {(_Float16)a, (_Float16)b};
+    return __builtin_bit_cast(uint32_t, h);
+}
+
+// finite magnitude
+__device__ __forceinline__ float magnitude(float v) { float const a = fabsf(v); return a < INFINITY ? a : 0.0f; }
+
+// KIND's values of (row, octet of k) pairs, `ROWS` rows side by side.  Rows whose k are neighbours: eight (a thread's 32 bytes, 256 of a row per wavefront); others: 32 (128 bytes of a
+// row of the buffer per half wavefront).
+template <int KIND, int ROWS>
+__device__ __forceinline__ void pack_rows(PackJob const &j, int block, float *share)
+{
+    constexpr int kOctets = kPackBlock / ROWS;                      // side by side
+    constexpr bool kBits = KIND == kBitRows || KIND == kBitColumns;
+    constexpr int kPieces = kBits ? 1 : 2;
+    int const at = threadIdx.x % ROWS, octet0 = threadIdx.x / ROWS, row = block * ROWS + at;
+    int const octets = j.k_steps * 2;
+    bool const there = row < j.src.rows;
+    float held[kPackHeld][8];
+    float top = 0.0f, sum = 0.0f;
+    int e = 0;
+    if (!kBits) {
+        int i = 0;
+#pragma unroll
+        for (int u = 0; u < kPackHeld; ++u) {
+            int const o = octet0 + u * kOctets;
+#pragma unroll
+            for (int q = 0; q < 8; ++q) { held[u][q] = 0.0f; }
+            if (there && o * 8 < j.src.depth) { load_values<KIND, 8>(j.src, row, o * 8, held[u]); }
+#pragma unroll
+            for (int q = 0; q < 8; ++q) { top = fmaxf(top, magnitude(held[u][q])); sum += held[u][q]; }
+        }
+        for (i = kPackHeld; octet0 + i * kOctets < octets; ++i) {
+            float v[8];
+            int const o = octet0 + i * kOctets;
+            if (!there || o * 8 >= j.src.depth) { break; }
+            load_values<KIND, 8>(j.src, row, o * 8, v);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) { top = fmaxf(top, magnitude(v[q])); sum += v[q]; }
+        }
+        // over the threads of a row: within the wavefront, then through LDS in a fixed order
+#pragma unroll
+        for (int step = ROWS; step < 64; step *= 2) { top = fmaxf(top, __shfl_xor(top, step)); sum += __shfl_xor(sum, step); }
+        constexpr int kWaves = kPackBlock / 64;
+        int const wave = threadIdx.x / 64;
+        if ((threadIdx.x & 63) < ROWS) { share[wave * ROWS + at] = top; share[(kWaves + wave) * ROWS + at] = sum; }
+        __syncthreads();
+        top = 0.0f; sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) { top = fmaxf(top, share[w * ROWS + at]); sum += share[(kWaves + w) * ROWS + at]; }
+        e = top > 0.0f ? 14 - ilogbf(top) : 0;
+        if (threadIdx.x < ROWS) {
+            j.exponent[row] = e;
+            if constexpr (KIND == kGradRows) { if (j.line && there) { j.line[row] = j.accumulate ? j.line[row] + sum : sum; } }
+        }
+    }
+    auto const write = [&](int o, float const (&v)[8]) {
+        uint4 *to = j.halves + (((long long)(row >> 5) * j.k_steps + (o >> 1)) * kPieces) * 64 + (o & 1) * 32 + (row & 31);
+        if constexpr (kBits) {
+            to[0] = make_uint4(two_halves(v[0], v[1]), two_halves(v[2], v[3]), two_halves(v[4], v[5]), two_halves(v[6], v[7]));
+        }
+        else {
+            float h[8], l[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                h[q] = ldexpf(v[q], e);
+                float const upper = (float)(_Float16)h[q];
+                // (the difference of an infinity to itself is no number, its lower half 0)
+                l[q] = fabsf(upper) < INFINITY ? h[q] - upper : 0.0f;
+            }
+            to[0]  = make_uint4(two_halves(h[0], h[1]), two_halves(h[2], h[3]), two_halves(h[4], h[5]), two_halves(h[6], h[7]));
+            to[64] = make_uint4(two_halves(l[0], l[1]), two_halves(l[2], l[3]), two_halves(l[4], l[5]), two_halves(l[6], l[7]));
+        }
+        if constexpr (KIND == kGradRows) {
+            if (j.dz && there) {
+                float *d = j.dz + row * j.dz_stride + o * 8;
+                if (o * 8 + 8 <= j.src.depth && (reinterpret_cast<uintptr_t>(d) & 15) == 0) {
+                    reinterpret_cast<float4 *>(d)[0] = make_float4(v[0], v[1], v[2], v[3]);
+                    reinterpret_cast<float4 *>(d)[1] = make_float4(v[4], v[5], v[6], v[7]);
+                }
+                else {
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) { if (o * 8 + q < j.src.depth) { d[q] = v[q]; } }
+                }
+            }
+        }
+    };
+    int const from = kBits ? 0 : kPackHeld;
+    if (!kBits) {
+#pragma unroll
+        for (int u = 0; u < kPackHeld; ++u) { if (octet0 + u * kOctets < octets) { write(octet0 + u * kOctets, held[u]); } }
+    }
+    for (int i = from; octet0 + i * kOctets < octets; ++i) {
+        int const o = octet0 + i * kOctets;
+        float v[8] = {};
+        if (there && o * 8 < j.src.depth) { load_values<KIND, 8>(j.src, row, o * 8, v); }
+        write(o, v);
+    }
+}
+
+__global__ __launch_bounds__(kPackBlock) void dense_pack_kernel(PackArgs a)
+{
+    __shared__ float share[2 * kPackBlock / 64 * 32];
+    int block = blockIdx.x, which = 0;
+    while (block >= a.job[which].blocks) { block -= a.job[which].blocks; ++which; }
+    PackJob const &j = a.job[which];
+    switch (j.kind) {
+    case kRows:       pack_rows<kRows, 8>(j, block, share); break;
+    case kColumns:    pack_rows<kColumns, 32>(j, block, share); break;
+    case kBitRows:    pack_rows<kBitRows, 8>(j, block, share); break;
+    case kBitColumns: pack_rows<kBitColumns, 32>(j, block, share); break;
+    case kGradRows:   pack_rows<kGradRows, 8>(j, block, share); break;
+    default:          pack_rows<kGradColumns, 32>(j, block, share); break;
+    }
+}
+
+// ---- the product ------------------------------------------------------------------------------------------------------------------------
+struct PackedProduct {
+    uint4 const *a, *b;             // halves
+    int   const *ea, *eb;           // exponents of the rows (eb null: 0)
+    int   a_blocks, b_blocks;       // row blocks of 32
+    int   k_steps;
+    int   b_pieces;
+    int   m_tiles, n_tiles;
+    int   slabs, slab_stages;       // of the k axis
+    int   workgroups;
+    float *sums;                    // slabs > 1: [slab][m][n], n padded to pitch
+    long long sums_pitch, sums_slab;
+    DenseOutput out;
+    Operand src_a, src_b;           // where an element is formed again if it is no number
+    int   kind_a, kind_b;           // (kind_a negative: not asked for)
+};
+
+// An element straight from the operands.  The halves of an infinity times a lower half of 0 are no number where the value's product is infinite: elements that come out as no number are
+// formed again in fp32, value by value, so that infinities and NaN are what the formula says.  (Slow, and only for operands that hold some.)
+__device__ __forceinline__ float element_again(Operand const &a, int kind_a, Operand const &b, int kind_b, int m, int n)
+{
+    float d = 0.0f;
+    for (int k = 0; k < a.depth && d == d; ++k) {
+        float const u = kind_a == kRows ? operand_at<kRows>(a, m, k) : kind_a == kColumns ? operand_at<kColumns>(a, m, k) : operand_at<kGradRows>(a, m, k);
+        float const v = kind_b == kRows ? operand_at<kRows>(b, n, k) : kind_b == kColumns ? operand_at<kColumns>(b, n, k) :
+                        kind_b == kBitRows ? operand_at<kBitRows>(b, n, k) : kind_b == kBitColumns ? operand_at<kBitColumns>(b, n, k) : operand_at<kGradColumns>(b, n, k);
+        d = fmaf(u, v, d);
+    }
+    return d;
+}
+
+// workgroup -> place in the list of tiles: workgroups go round the eight XCDs, each of which gets a run of neighbours
+__device__ __forceinline__ int xcd_run(int id, int total)
+{
+    int const x = id & 7, q = total >> 3, r = total & 7;
+    return x * q + min(x, r) + (id >> 3);
+}
+
+// four elements of a row of D that lie side by side, n a multiple of 4; `all`: the four exist and may be moved with 16-byte accesses
+__device__ __forceinline__ void finish_four(DenseOutput const &o, float (&d)[4], int m, int n, bool all)
+{
+    if (o.kind == kOutForward || o.kind == kOutLogits) {
+        float r[4] = {};
+        float const b = o.bias ? o.bias[m] : 0.0f;
+        if (o.residual) {
+            float const *from = o.residual + m * o.residual_stride + n;
+            if (all) { load_floats(from, true, r); }
+            else {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) { if (n + q < o.columns) { r[q] = from[q]; } }
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) { d[q] = activated(d[q] + b + r[q], o.activation); }
+    }
+    float *to = static_cast<float *>(o.out) + m * o.stride + n;
+    if (all) {
+        float4 v = make_float4(d[0], d[1], d[2], d[3]);
+        if (o.accumulate) {
+            float4 const w = *reinterpret_cast<float4 const *>(to);
+            v = make_float4(w.x + v.x, w.y + v.y, w.z + v.z, w.w + v.w);
+        }
+        *reinterpret_cast<float4 *>(to) = v;
+        return;
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) { if (n + q < o.columns) { to[q] = o.accumulate ? to[q] + d[q] : d[q]; } }
+}
+
+// 32 x 64 elements of a wavefront, in LDS (rows of kTilePitch floats), become what they are for: 16 lanes across a row
+constexpr int kTilePitch = 68;
+__device__ __forceinline__ void finish_tile(DenseOutput const &o, float const *tile, int m0, int n0, int lane)
+{
+    int const n = n0 + (lane & 15) * 4;
+    bool const vec = n + 4 <= o.columns && o.stride % 4 == 0 && (reinterpret_cast<uintptr_t>(o.out) & 15) == 0 &&
+                     (!o.residual || (o.residual_stride % 4 == 0 && (reinterpret_cast<uintptr_t>(o.residual) & 15) == 0));
+    for (int step = 0; step < 8; ++step) {
+        int const row = step * 4 + (lane >> 4), m = m0 + row;
+        if (m >= o.rows || n >= o.columns) { continue; }
+        float d[4];
+        load_floats(tile + row * kTilePitch + (lane & 15) * 4, true, d);
+        finish_four(o, d, m, n, vec);
+    }
+}
+
+// the same to packed bits: a row of 64 columns is two words
+__device__ __forceinline__ void finish_tile_bits(DenseOutput const &o, float const *tile, int m0, int n0, int lane)
+{
+    int const n = n0 + lane;
+    for (int row = 0; row < 32 && m0 + row < o.rows; ++row) {
+        bool const inside = n < o.columns;
+        uint64_t const bits = __ballot(inside && before_activation(o, tile[row * kTilePitch + lane], m0 + row, inside ? n : 0) > 0.0f);
+        if ((lane & 31) == 0 && inside) { static_cast<uint32_t *>(o.out)[(m0 + row) * o.stride + (n >> 5)] = (uint32_t)(bits >> (lane & 32)); }
+    }
+}
+
+template <int TM, int WM, int WN, int PB>
+__device__ __forceinline__ void packed_tile(PackedProduct const &p, int id, char *lds)
+{
+    constexpr int TN = 2, kWaves = WM * WN, kBM = TM * WM, kBN = TN * WN;           // blocks of 32 rows
+    static_assert(kBM == kWaves && kBN == kWaves, "each wavefront loads one row block of either operand");
+    constexpr int kStageA = kBM * 4096, kStage = kStageA + kBN * 2048 * PB;
+    int const lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int const tiles = p.m_tiles * p.n_tiles;
+    int const slab = id / tiles;
+    int const t = xcd_run(id % tiles, tiles);
+    // runs of eight tiles down, then across: what a run's workgroups read at a time is a few row blocks of either operand
+    int const band = t / (8 * p.n_tiles), rest = t - band * 8 * p.n_tiles, high = min(8, p.m_tiles - band * 8);
+    int const m_tile = band * 8 + rest % high, n_tile = rest / high;
+    int const rb_a = m_tile * kBM, rb_b = n_tile * kBN;
+    int const first = slab * p.slab_stages, last = min(first + p.slab_stages, p.k_steps / 2);
+
+    // a stage is 32 k: of each row block four (packed bits: two) neighbouring blocks of 1 KiB, which a wavefront moves to LDS as they are
+    char const *from_a = reinterpret_cast<char const *>(p.a) + ((long long)min(rb_a + wave, p.a_blocks - 1) * p.k_steps + 2 * first) * 2048;
+    char const *from_b = reinterpret_cast<char const *>(p.b) + ((long long)min(rb_b + wave, p.b_blocks - 1) * p.k_steps + 2 * first) * (1024 * PB);
+    auto const fetch = [&](int buffer) {
+        typedef const __attribute__((address_space(1))) void *Global;
+        typedef __attribute__((address_space(3))) void *Shared;
+        Global const a = (Global)(from_a + lane * 16), b = (Global)(from_b + lane * 16);
+        Shared const to_a = (Shared)(lds + buffer * kStage + wave * 4096), to_b = (Shared)(lds + buffer * kStage + kStageA + wave * 2048 * PB);
+        __builtin_amdgcn_global_load_lds(a, to_a, 16, 0, 0);
+        __builtin_amdgcn_global_load_lds(a, to_a, 16, 1024, 0);
+        __builtin_amdgcn_global_load_lds(a, to_a, 16, 2048, 0);
+        __builtin_amdgcn_global_load_lds(a, to_a, 16, 3072, 0);
+        __builtin_amdgcn_global_load_lds(b, to_b, 16, 0, 0);
+        __builtin_amdgcn_global_load_lds(b, to_b, 16, 1024, 0);
+        if constexpr (PB == 2) {
+            __builtin_amdgcn_global_load_lds(b, to_b, 16, 2048, 0);
+            __builtin_amdgcn_global_load_lds(b, to_b, 16, 3072, 0);
+        }
+        from_a += 4096; from_b += 2048 * PB;
+    };
+
+    int const wm = wave / WN, wn = wave % WN;
+    DenseAcc16 acc[TM][TN] = {};
+    fetch(0);
+    for (int stage = first; stage < last; ++stage) {
+        int const buffer = (stage - first) & 1;
+        // this wavefront's loads of the stage have arrived; behind the barrier all wavefronts' have, and nobody reads the other buffer any more
+        __builtin_amdgcn_s_waitcnt(0x0f70);
+        __syncthreads();
+        if (stage + 1 < last) { fetch(buffer ^ 1); }
+        char const *from = lds + buffer * kStage + lane * 16;
+#pragma unroll
+        for (int step = 0; step < 2; ++step) {
+            DenseHalf8 a[TM][2], b[TN][PB];
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+#pragma unroll
+                for (int q = 0; q < 2; ++q) { a[i][q] = *reinterpret_cast<DenseHalf8 const *>(from + (((wm * TM + i) * 2 + step) * 2 + q) * 1024); }
+            }
+#pragma unroll
+            for (int j = 0; j < TN; ++j) {
+#pragma unroll
+                for (int q = 0; q < PB; ++q) { b[j][q] = *reinterpret_cast<DenseHalf8 const *>(from + kStageA + (((wn * TN + j) * 2 + step) * PB + q) * 1024); }
+            }
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+#pragma unroll
+                for (int j = 0; j < TN; ++j) {
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][1], b[j][0], acc[i][j], 0, 0, 0);
+                    if constexpr (PB == 2) { acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][0], b[j][1], acc[i][j], 0, 0, 0); }
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][0], b[j][0], acc[i][j], 0, 0, 0);
+                }
+            }
+        }
+    }
+
+    // 32 x 64 elements at a time go through LDS, so that a lane has neighbours of a row to store, or the rows of a column to sum
+    DenseOutput o = p.out;
+    if (p.slabs > 1) {
+        o.kind = kOutStore; o.out = p.sums + slab * p.sums_slab; o.stride = p.sums_pitch; o.accumulate = 0; o.line = nullptr;
+    }
+    float *const tile = reinterpret_cast<float *>(lds) + wave * 32 * kTilePitch;
+    int const n0 = (rb_b + wn * TN) * 32;
+    int eb[TN];
+#pragma unroll
+    for (int j = 0; j < TN; ++j) { eb[j] = p.eb ? p.eb[min(n0 + j * 32 + (lane & 31), p.b_blocks * 32 - 1)] : 0; }
+    float2 column = make_float2(-INFINITY, 0.0f);
+    __syncthreads();                            // (the stages are done with LDS)
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+        int const rb = rb_a + wm * TM + i, m0 = rb * 32;
+        if (rb >= p.a_blocks) { continue; }
+        bool odd = false;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            int const row = acc_row(r, lane), ea = p.ea[m0 + row];
+#pragma unroll
+            for (int j = 0; j < TN; ++j) {
+                float const d = ldexpf(acc[i][j][r], -(ea + eb[j]));           // the scales come off
+                odd = odd || d != d;
+                tile[row * kTilePitch + j * 32 + (lane & 31)] = d;
+            }
+        }
+        if (p.kind_a >= 0 && p.slabs == 1 && __any(odd)) {
+            for (int row = 0; row < 32; ++row) {
+                if (m0 + row < o.rows && n0 + lane < o.columns) { tile[row * kTilePitch + lane] = element_again(p.src_a, p.kind_a, p.src_b, p.kind_b, m0 + row, n0 + lane); }
+            }
+        }
+        if (o.kind == kOutBits) { finish_tile_bits(o, tile, m0, n0, lane); continue; }
+        if (o.kind == kOutLogits && n0 + lane < o.columns) {
+            // (largest, sum of exponents) of the 32 rows of this lane's column
+            int const n = n0 + lane, rows = min(32, o.rows - m0), label = o.label[n] - o.first_channel - m0;
+            float2 s = make_float2(-INFINITY, 0.0f);
+            for (int row = 0; row < rows; ++row) { s.x = fmaxf(s.x, tile[row * kTilePitch + lane] + (o.bias ? o.bias[m0 + row] : 0.0f)); }
+            for (int row = 0; row < rows; ++row) {
+                float const z = tile[row * kTilePitch + lane] + (o.bias ? o.bias[m0 + row] : 0.0f);
+                s.y += z == -INFINITY ? 0.0f : exp_of_nonpositive(z - s.x);
+                if (row == label) { o.label_logit[n] = z; }
+            }
+            column = joined(column, s);
+        }
+        if (o.out) { finish_tile(o, tile, m0, n0, lane); }
+    }
+    if (o.kind == kOutLogits && n0 + lane < o.columns && rb_a + wm * TM < p.a_blocks) {
+        o.partial[(long long)((rb_a + wm * TM) / TM) * o.columns + n0 + lane] = column;
+    }
+}
+
+// one product, and behind it another (workgroups 0: none)
+template <int TM, int WM, int WN, int PB>
+__global__ __launch_bounds__(WM * WN * 64) void dense_packed_kernel(PackedProduct p, PackedProduct q)
+{
+    __shared__ __attribute__((aligned(1024))) char lds[2 * (TM * WM + 2 * WN) * 4096];
+    if ((int)blockIdx.x < p.workgroups) { packed_tile<TM, WM, WN, PB>(p, blockIdx.x, lds); }
+    else                                { packed_tile<TM, WM, WN, 2>(q, blockIdx.x - p.workgroups, lds); }
+}
+
+// the slabs' sums of a product, in order, and what becomes of them: a thread per element, a wavefront within a row
+__device__ __forceinline__ void join_slabs(PackedProduct const &p, long long id)
+{
+    DenseOutput const &o = p.out;
+    int const pitch = (o.columns + 63) / 64 * 64, lane = threadIdx.x & 63;
+    int const m = (int)(id / pitch), n = (int)(id % pitch);
+    if (m >= o.rows) { return; }
+    bool const inside = n < o.columns;
+    float d = 0.0f;
+    if (inside) {
+        for (int s = 0; s < p.slabs; ++s) { d += p.sums[s * p.sums_slab + m * p.sums_pitch + n]; }
+        if (d != d && p.kind_a >= 0) { d = element_again(p.src_a, p.kind_a, p.src_b, p.kind_b, m, n); }
+    }
+    if (o.kind == kOutForward) { if (inside) { static_cast<float *>(o.out)[m * o.stride + n] = activated(before_activation(o, d, m, n), o.activation); } }
+    else if (o.kind == kOutBits) {
+        uint64_t const bits = __ballot(inside && before_activation(o, d, m, n) > 0.0f);
+        if ((lane & 31) == 0 && inside) { static_cast<uint32_t *>(o.out)[m * o.stride + (n >> 5)] = (uint32_t)(bits >> (lane & 32)); }
+    }
+    else if (inside) { store_element(o, d, m, n); }
+}
+
+__global__ __launch_bounds__(256) void dense_join_kernel(PackedProduct p, PackedProduct q, unsigned first_blocks)
+{
+    if (blockIdx.x < first_blocks) { join_slabs(p, (long long)blockIdx.x * 256 + threadIdx.x); }
+    else                           { join_slabs(q, (long long)(blockIdx.x - first_blocks) * 256 + threadIdx.x); }
+}
+
+}  // namespace bbhip

@@ -53,6 +53,23 @@ int direct(DirectProduct &d, Product const &p, int columns, char const *name, in
 
 int direct_forward(Product const &p, bool bit, hipStream_t st, char const *name)
 {
+    if (p.out.columns <= kFewFrames && p.out.kind != kOutLogits) {
+        DirectProduct d{};
+        d.a = p.a; d.b = p.b; d.out = p.out;
+        long long const blocks = ceil_div(p.out.rows, kFewWaves);
+        if (check_tiles(blocks, kFewWaves * 64, name)) { return 1; }
+        dim3 const grid((unsigned)blocks), block(kFewWaves * 64);
+        if (p.out.columns == 1) {
+            if (bit) { launch((dense_few_frames_kernel<kBitColumns, 1>), grid, block, 0, st, d); }
+            else     { launch((dense_few_frames_kernel<kColumns, 1>), grid, block, 0, st, d); }
+        }
+        else {
+            if (bit) { launch((dense_few_frames_kernel<kBitColumns, kFewFrames>), grid, block, 0, st, d); }
+            else     { launch((dense_few_frames_kernel<kColumns, kFewFrames>), grid, block, 0, st, d); }
+        }
+        BBHIP_LAUNCH_CHECK();
+        return 0;
+    }
     int const waves = direct_waves(p.a.depth);
     DirectProduct d;
     if (direct(d, p, p.out.columns, name, waves)) { return 1; }
@@ -69,13 +86,23 @@ int direct_forward(Product const &p, bool bit, hipStream_t st, char const *name)
     return 0;
 }
 
-int direct_backward(Product const &dw, Product const &dx, bool bit, hipStream_t st, char const *name)
+// dw.a and dx.b are gradients; where these are more than dy itself, or wanted, they are formed first and lie in `dz`
+int direct_backward(Product const &dw, Product const &dx, float *dz, long long dz_stride, bool bit, hipStream_t st, char const *name)
 {
     int const waves = direct_waves(dw.wanted && dw.a.depth > dx.a.depth ? dw.a.depth : dx.a.depth);
     DirectProduct w, x;
-    Product with_line = dw;
+    Product with_line = dw, from_dz = dx;
+    if (dz) {
+        DzArgs z{dw.a, dz, dz_stride, ceil_div(dw.a.depth, 1024)};
+        long long const blocks = (long long)z.per_row * dw.a.rows;
+        if (check_tiles(blocks, 256, name)) { return 1; }
+        launch(dense_dz_kernel, dim3((unsigned)blocks), dim3(256), 0, st, z);
+        BBHIP_LAUNCH_CHECK();
+        with_line.a = rows_of(dz, dz_stride, dw.a.rows, dw.a.depth);
+        from_dz.b = rows_of(dz, dz_stride, dx.b.rows, dx.b.depth);
+    }
     if (dw.out.line) { with_line.b.ones = dw.b.rows; }
-    if (direct(w, with_line, dw.out.columns + (dw.out.line ? 1 : 0), name, waves) || direct(x, dx, dx.out.columns, name, waves) ||
+    if (direct(w, with_line, dw.out.columns + (dw.out.line ? 1 : 0), name, waves) || direct(x, from_dz, dx.out.columns, name, waves) ||
         check_tiles((long long)w.tiles + x.tiles, waves * 64, name)) { return 1; }
     if (w.tiles + x.tiles == 0) { return 0; }
     dim3 const grid((unsigned)(w.tiles + x.tiles)), block((unsigned)waves * 64);
@@ -235,6 +262,9 @@ struct BackwardSpace {
     }
 };
 
+// dz of a small backward pass
+float *small_dz(Carver &c, int outputs, int frames) { return c.take<float>((size_t)outputs * (ceil_div(frames, 64) * 64)); }
+
 // ---- what an entry checks ----
 int check_sizes(int inputs, int outputs, int frames, char const *name)
 {
@@ -334,15 +364,12 @@ int dense_backward(void const *x, bool bit, float const *dy, float const *y, flo
         s.add_jobs(jobs, w, i, true, db, accumulate, dr, stride);
         return jobs.run(st, name) || s.run(w, i, st, name);
     }
+    Carver c{static_cast<char *>(workspace)};
+    float *dz = small_dz(c, outputs, frames);
+    if (dr || activation == kActNone) { dz = dr; }
+    else if (check_workspace(workspace, workspace_size, c.at, name)) { return 1; }
     ScopedTimer tm(kTimeOther, st);
-    if (direct_backward(w, i, bit, st, name)) { return 1; }
-    if (dr) {
-        Operand o = g;
-        o.rows = outputs; o.depth = frames;
-        launch(dense_dz_kernel, dim3((unsigned)ceil_div(frames, 256), (unsigned)(outputs < 65535 ? outputs : 65535), (unsigned)ceil_div(outputs, 65535)), dim3(256), 0, st, o, dr, (long long)stride);
-        BBHIP_LAUNCH_CHECK();
-    }
-    return 0;
+    return direct_backward(w, i, dz, dr ? stride : ceil_div(frames, 64) * 64, bit, st, name);
 }
 
 // ---- the loss on top of a dense layer ----
@@ -444,7 +471,8 @@ int dense_loss(void const *x, bool bit, float const *W, float const *b, int cons
         i.out = DenseOutput{};
         i.out.kind = kOutStore; i.out.rows = inputs; i.out.columns = frames; i.out.out = dx; i.out.stride = dx_stride; i.out.accumulate = piece != pieces - 1;
         if (!s.plan.packed) {
-            if (direct_backward(w, i, bit, st, name)) { return 1; }
+            // (in the place of the logits)
+            if (direct_backward(w, i, logits, s.plan.stride, bit, st, name)) { return 1; }
             continue;
         }
         Jobs jobs;
@@ -477,8 +505,12 @@ int squares(int size, int const *sizes, float *const *grads, void *workspace, si
 
 size_t bbhip_DenseAffine_WorkspaceBytes(int input_node_size, int output_node_size, int frame_size)
 {
-    if (check_sizes(input_node_size, output_node_size, frame_size, __func__) || !product_packed(output_node_size, frame_size, input_node_size)) { return 0; }
+    if (check_sizes(input_node_size, output_node_size, frame_size, __func__)) { return 0; }
     Carver forward{nullptr}, backward{nullptr};
+    if (!product_packed(output_node_size, frame_size, input_node_size)) {
+        small_dz(backward, output_node_size, frame_size);
+        return backward.at;
+    }
     ForwardSpace const f(forward, input_node_size, output_node_size, frame_size, false);
     BackwardSpace const b(backward, input_node_size, output_node_size, frame_size, false);
     return forward.at > backward.at ? forward.at : backward.at;

@@ -1,10 +1,13 @@
-// Products of dense layers straight from the operands as they lie, on the fp32 matrix instructions: small problems, and few frames.
+// Products of dense layers straight from the operands as they lie, in fp32: small problems, and few frames.
 //
-// A workgroup owns a tile of 32 x 32 elements; its wavefronts share the k axis (chunks of 32, taken in turn) and add their tiles up through LDS in a fixed order.
+// dense_direct_kernel: a workgroup owns a tile of 32 x 32 elements; its wavefronts share the k axis (chunks of 32, taken in turn) and add their tiles up through LDS in a fixed order.
 // v_mfma_f32_32x32x2_f32 takes one value per lane and operand: lane l holds row l & 31 at the k of its half, l >> 5, so a lane loads 16 consecutive k of one row
 // (64 bytes where these are neighbours in memory, 16 times 128 bytes of a half wavefront where rows are) and the 16 instructions of a chunk each take one of them:
 // which k meets which in an instruction does not matter as long as both operands agree.  Every product and sum is fp32; no operand is written anywhere.
 // One launch, and what it costs is the latency of a chunk's loads and 16 x 64 cycles of matrix instructions per chunk and wavefront.
+//
+// dense_few_frames_kernel: up to eight frames, where a tile of 32 would be mostly empty and the weights are all there is to read.  A wavefront owns an output node and
+// walks its row of W 1 KiB at a time, the frames lie in LDS.
 #pragma once
 
 #include "dense_operands.hpp"
@@ -13,7 +16,7 @@ namespace bbhip {
 
 typedef float DenseAcc __attribute__((ext_vector_type(16)));
 
-constexpr int kDirectTile = 32, kDirectChunk = 32;
+constexpr int kDirectTile = 32, kDirectChunk = 32, kDirectRun = 16;
 
 struct DirectProduct {
     Operand     a, b;
@@ -22,32 +25,98 @@ struct DirectProduct {
     int tiles;
 };
 
+// What a lane loads of an operand for a chunk, as it comes from memory: a loop holds the next chunk's while the present one's is multiplied, so nothing is computed of it before.
+template <int KIND>
+struct RawRun {
+    static constexpr int kWords = KIND == kBitRows ? 1 : kDirectRun;
+    uint32_t w[kWords];
+    float    coef[KIND == kRows ? kDirectRun : 1];
+
+    // k .. k + 16 of a row; `whole`: all of them exist (the same for the wavefront), else what is behind the last one is some other value of the row
+    __device__ __forceinline__ void load(Operand const &o, int row, int k, bool whole)
+    {
+        uint32_t const *p = static_cast<uint32_t const *>(o.p);
+        if constexpr (KIND == kRows) {
+            p += row * o.stride;
+            if (whole && o.vec) {
+#pragma unroll
+                for (int j = 0; j < kDirectRun; j += 4) {
+                    uint4 const q = *reinterpret_cast<uint4 const *>(p + k + j);
+                    w[j] = q.x; w[j + 1] = q.y; w[j + 2] = q.z; w[j + 3] = q.w;
+                }
+            }
+            else {
+#pragma unroll
+                for (int j = 0; j < kDirectRun; ++j) { w[j] = p[min(k + j, o.depth - 1)]; }
+            }
+            if (o.coef) {
+#pragma unroll
+                for (int j = 0; j < kDirectRun; ++j) { coef[j] = o.coef[min(k + j, o.depth - 1)]; }
+            }
+        }
+        if constexpr (KIND == kColumns || KIND == kBitColumns) {
+            p += KIND == kColumns ? row : row >> 5;
+            if (whole) {
+                p += k * o.stride;
+#pragma unroll
+                for (int j = 0; j < kDirectRun; ++j) { w[j] = p[j * o.stride]; }
+            }
+            else {
+#pragma unroll
+                for (int j = 0; j < kDirectRun; ++j) { w[j] = p[min(k + j, o.depth - 1) * o.stride]; }
+            }
+        }
+        if constexpr (KIND == kBitRows) { w[0] = p[row * o.stride + (min(k, o.depth - 1) >> 5)]; }
+    }
+
+    __device__ __forceinline__ float value(Operand const &o, int row, int k, int j, bool whole, bool ones) const
+    {
+        float v;
+        if constexpr (KIND == kRows)       { v = __builtin_bit_cast(float, w[j]); if (o.coef) { v = coef[j] == 0.0f ? 0.0f : v; } }
+        if constexpr (KIND == kColumns)    { v = __builtin_bit_cast(float, w[j]); }
+        if constexpr (KIND == kBitColumns) { v = (float)((w[j] >> (row & 31)) & 1u); }
+        if constexpr (KIND == kBitRows)    { v = (float)((w[0] >> ((k & 31) + j)) & 1u); }
+        if (KIND == kRows || KIND == kBitRows) { v = ones ? 1.0f : v; }
+        return whole || k + j < o.depth ? v : 0.0f;
+    }
+};
+
 template <int KA, int KB, int WAVES>
 __device__ __forceinline__ void direct_product(DirectProduct const &t, int tile, float *lds)
 {
     int const m0 = tile / t.n_tiles * kDirectTile, n0 = (tile % t.n_tiles) * kDirectTile;
-    int const lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int const lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int const r = lane & 31, half = lane >> 5;
-    // (rows behind the last one read the last one: their elements are not stored)
-    int const row_a = min(m0 + r, t.a.rows - 1);
-    int const row_b = (n0 + r < t.b.rows || n0 + r == t.b.ones) ? n0 + r : t.b.rows - 1;
+    // (rows behind the last one read the last one: their elements are not stored; so does the row of ones)
+    int const row_a = min(m0 + r, t.a.rows - 1), row_b = min(n0 + r, t.b.rows - 1);
+    bool const ones = n0 + r == t.b.ones;
     int const chunks = (t.a.depth + kDirectChunk - 1) / kDirectChunk;
     DenseAcc acc = {};
-    float a[16], b[16];
-    if (wave < chunks) {
-        load_values<KA, 16>(t.a, row_a, wave * kDirectChunk + half * 16, a);
-        load_values<KB, 16>(t.b, row_b, wave * kDirectChunk + half * 16, b);
-    }
+    RawRun<KA> a, an;
+    RawRun<KB> b, bn;
+    auto const fetch = [&](RawRun<KA> &u, RawRun<KB> &v, int c) {
+        bool const whole = (c + 1) * kDirectChunk <= t.a.depth;
+        u.load(t.a, row_a, c * kDirectChunk + half * kDirectRun, whole);
+        v.load(t.b, row_b, c * kDirectChunk + half * kDirectRun, whole);
+    };
+    if (wave < chunks) { fetch(a, b, wave); }
     for (int c = wave; c < chunks; c += WAVES) {
-        float an[16], bn[16];
-        if (c + WAVES < chunks) {
-            load_values<KA, 16>(t.a, row_a, (c + WAVES) * kDirectChunk + half * 16, an);
-            load_values<KB, 16>(t.b, row_b, (c + WAVES) * kDirectChunk + half * 16, bn);
+        bool const whole = (c + 1) * kDirectChunk <= t.a.depth;
+        int const k = c * kDirectChunk + half * kDirectRun;
+        if (c + WAVES < chunks) { fetch(an, bn, c + WAVES); }
+        if (whole) {
+#pragma unroll
+            for (int j = 0; j < kDirectRun; ++j) {
+                acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a.value(t.a, row_a, k, j, true, false), b.value(t.b, row_b, k, j, true, ones), acc, 0, 0, 0);
+            }
         }
+        else {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) { acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], acc, 0, 0, 0); }
-#pragma unroll
-        for (int j = 0; j < 16; ++j) { a[j] = an[j]; b[j] = bn[j]; }
+            for (int j = 0; j < kDirectRun; ++j) {
+                acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a.value(t.a, row_a, k, j, false, false), b.value(t.b, row_b, k, j, false, ones), acc, 0, 0, 0);
+            }
+        }
+        a = an; b = bn;
     }
 #pragma unroll
     for (int j = 0; j < 16; ++j) { lds[(wave * 16 + j) * 64 + lane] = acc[j]; }
@@ -68,7 +137,7 @@ __device__ __forceinline__ void direct_product(DirectProduct const &t, int tile,
             if (inside) { static_cast<float *>(o.out)[m * o.stride + n] = activated(before_activation(o, d, m, n), o.activation); }
         }
         else if (o.kind == kOutBits) {
-            uint64_t const bits = __ballot(inside && before_activation(o, d, m, n) > 0.0f);
+            uint64_t const bits = __ballot(inside && before_activation(o, d, inside ? m : 0, inside ? n : 0) > 0.0f);
             if (r == 0 && m < o.rows) { static_cast<uint32_t *>(o.out)[m * o.stride + (n0 >> 5)] = (uint32_t)(bits >> (half * 32)); }
         }
         else if (o.kind == kOutStore) {
@@ -108,20 +177,93 @@ __global__ __launch_bounds__(WAVES * 64) void dense_direct_kernel(DirectProduct 
     direct_product<KA, KB, WAVES>(t, blockIdx.x, lds);
 }
 
-// the weights' gradient (x as KX) and behind it the input's, in one launch
+// the weights' gradient (x as KX) and behind it the input's, in one launch; dz as it lies
 template <int KX, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void dense_direct_backward_kernel(DirectProduct dw, DirectProduct dx)
 {
     __shared__ float lds[WAVES * 16 * 64];
-    if ((int)blockIdx.x < dw.tiles) { direct_product<kGradRows, KX, WAVES>(dw, blockIdx.x, lds); }
-    else                            { direct_product<kColumns, kGradColumns, WAVES>(dx, blockIdx.x - dw.tiles, lds); }
+    if ((int)blockIdx.x < dw.tiles) { direct_product<kRows, KX, WAVES>(dw, blockIdx.x, lds); }
+    else                            { direct_product<kColumns, kColumns, WAVES>(dx, blockIdx.x - dw.tiles, lds); }
 }
 
-// dr = dz: one value per thread
-__global__ __launch_bounds__(256) void dense_dz_kernel(Operand o, float *out, long long stride)
+// dz of a call, written: 1024 elements of a row per workgroup, units of a row dealt out by a flat list
+struct DzArgs { Operand o; float *dz; long long stride; int per_row; };
+__global__ __launch_bounds__(256) void dense_dz_kernel(DzArgs a)
 {
-    int const frame = blockIdx.x * 256 + threadIdx.x, row = blockIdx.y + blockIdx.z * 65535;
-    if (frame < o.depth && row < o.rows) { out[row * stride + frame] = operand_at<kGradRows>(o, row, frame); }
+    int const row = (int)(blockIdx.x / (unsigned)a.per_row), first = (int)(blockIdx.x % (unsigned)a.per_row) * 1024;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        int const frame = first + i * 256 + threadIdx.x;
+        if (frame < a.o.depth) { a.dz[row * a.stride + frame] = operand_at<kGradRows>(a.o, row, frame); }
+    }
+}
+
+// ---- up to eight frames ---------------------------------------------------------------------------------------------------------------------
+constexpr int kFewFrames = 8, kFewWaves = 4, kFewPiece = 1024;             // values of k in LDS at a time
+
+// p.b: columns or packed bits.  A wavefront owns one row of p.a: lane l takes four values of every 256.
+template <int KB, int FRAMES>
+__global__ __launch_bounds__(kFewWaves * 64) void dense_few_frames_kernel(DirectProduct t)
+{
+    __shared__ __attribute__((aligned(16))) float x[FRAMES][kFewPiece];
+    int const lane = threadIdx.x & 63, m = blockIdx.x * kFewWaves + (threadIdx.x >> 6);
+    Operand const &a = t.a, &b = t.b;
+    float const *w = static_cast<float const *>(a.p) + min(m, a.rows - 1) * a.stride;
+    int const frames = min(FRAMES, b.rows);
+    float acc[FRAMES] = {};
+    for (int k0 = 0; k0 < a.depth; k0 += kFewPiece) {
+        int const here = min(kFewPiece, a.depth - k0);
+        if (k0) { __syncthreads(); }
+        float v[kFewPiece / 256][4];
+#pragma unroll
+        for (int i = 0; i < kFewPiece / 256; ++i) {
+            int const k = k0 + i * 256 + lane * 4;
+            if (a.vec && k + 4 <= a.depth) { load_floats(w + k, true, v[i]); }
+            else {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) { v[i][q] = k + q < a.depth ? w[k + q] : 0.0f; }
+            }
+        }
+        for (int i = threadIdx.x; i < kFewPiece; i += kFewWaves * 64) {
+            if constexpr (KB == kBitColumns) {
+                uint32_t const bits = i < here ? static_cast<uint32_t const *>(b.p)[(k0 + i) * b.stride] : 0u;
+#pragma unroll
+                for (int f = 0; f < FRAMES; ++f) { x[f][i] = (float)((bits >> f) & 1u); }
+            }
+            else {
+#pragma unroll
+                for (int f = 0; f < FRAMES; ++f) { x[f][i] = i < here && f < frames ? static_cast<float const *>(b.p)[(k0 + i) * b.stride + f] : 0.0f; }
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kFewPiece / 256; ++i) {
+            if (i * 256 >= here) { continue; }
+#pragma unroll
+            for (int f = 0; f < FRAMES; ++f) {
+                float u[4];
+                load_floats(&x[f][i * 256 + lane * 4], true, u);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) { acc[f] = fmaf(v[i][q], u[q], acc[f]); }
+            }
+        }
+    }
+#pragma unroll
+    for (int f = 0; f < FRAMES; ++f) {
+#pragma unroll
+        for (int step = 32; step > 0; step /= 2) { acc[f] += __shfl_xor(acc[f], step); }
+    }
+    // lane f finishes frame f
+    float d = acc[0];
+#pragma unroll
+    for (int f = 1; f < FRAMES; ++f) { d = lane == f ? acc[f] : d; }
+    DenseOutput const &o = t.out;
+    bool const inside = m < o.rows && lane < o.columns && lane < FRAMES;
+    if (o.kind == kOutBits) {
+        uint64_t const bits = __ballot(inside && before_activation(o, d, inside ? m : 0, inside ? lane : 0) > 0.0f);
+        if (lane == 0 && m < o.rows) { static_cast<uint32_t *>(o.out)[m * o.stride] = (uint32_t)bits; }
+    }
+    else if (inside) { static_cast<float *>(o.out)[m * o.stride + lane] = activated(before_activation(o, d, m, lane), o.activation); }
 }
 
 }  // namespace bbhip

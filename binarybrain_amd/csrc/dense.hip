@@ -74,9 +74,9 @@ int direct_forward(Product const &p, bool bit, hipStream_t st, char const *name)
     DirectProduct d;
     if (direct(d, p, p.out.columns, name, waves)) { return 1; }
     dim3 const grid((unsigned)d.tiles), block((unsigned)waves * 64);
-    if (waves == 16) {
-        if (bit) { launch((dense_direct_kernel<kRows, kBitColumns, 16>), grid, block, 0, st, d); }
-        else     { launch((dense_direct_kernel<kRows, kColumns, 16>), grid, block, 0, st, d); }
+    if (waves == 8) {
+        if (bit) { launch((dense_direct_kernel<kRows, kBitColumns, 8>), grid, block, 0, st, d); }
+        else     { launch((dense_direct_kernel<kRows, kColumns, 8>), grid, block, 0, st, d); }
     }
     else {
         if (bit) { launch((dense_direct_kernel<kRows, kBitColumns, 4>), grid, block, 0, st, d); }
@@ -106,9 +106,9 @@ int direct_backward(Product const &dw, Product const &dx, float *dz, long long d
         check_tiles((long long)w.tiles + x.tiles, waves * 64, name)) { return 1; }
     if (w.tiles + x.tiles == 0) { return 0; }
     dim3 const grid((unsigned)(w.tiles + x.tiles)), block((unsigned)waves * 64);
-    if (waves == 16) {
-        if (bit) { launch((dense_direct_backward_kernel<kBitRows, 16>), grid, block, 0, st, w, x); }
-        else     { launch((dense_direct_backward_kernel<kRows, 16>), grid, block, 0, st, w, x); }
+    if (waves == 8) {
+        if (bit) { launch((dense_direct_backward_kernel<kBitRows, 8>), grid, block, 0, st, w, x); }
+        else     { launch((dense_direct_backward_kernel<kRows, 8>), grid, block, 0, st, w, x); }
     }
     else {
         if (bit) { launch((dense_direct_backward_kernel<kBitRows, 4>), grid, block, 0, st, w, x); }
@@ -148,8 +148,7 @@ struct Packed {
     {
         PackJob j{};
         j.src = o; j.kind = kind; j.halves = halves; j.exponent = exponent; j.k_steps = steps;
-        bool const side_by_side = kind == kRows || kind == kBitRows || kind == kGradRows;
-        j.blocks = side_by_side ? blocks * 4 : blocks;
+        j.blocks = blocks * (32 / kPackRows);
         return j;
     }
 };

@@ -20,7 +20,7 @@ namespace bbhip {
 typedef _Float16 DenseHalf8 __attribute__((ext_vector_type(8)));
 typedef float    DenseAcc16 __attribute__((ext_vector_type(16)));
 
-constexpr int kPackBlock = 512, kStageK = 32;
+constexpr int kPackBlock = 512, kPackRows = 8;
 constexpr int kPackHeld = 8;                    // groups of eight values that a thread keeps between finding the largest and splitting
 
 struct PackJob {
@@ -46,15 +46,23 @@ __device__ __forceinline__ uint32_t two_halves(float a, float b)
     return __builtin_bit_cast(uint32_t, h);
 }
 
+// workgroup -> place in the list of tiles: workgroups go round the eight XCDs, each of which gets a run of neighbours
+__device__ __forceinline__ int xcd_run(int id, int total)
+{
+    int const x = id & 7, q = total >> 3, r = total & 7;
+    return x * q + min(x, r) + (id >> 3);
+}
+
 // finite magnitude
 __device__ __forceinline__ float magnitude(float v) { float const a = fabsf(v); return a < INFINITY ? a : 0.0f; }
 
-// KIND's values of (row, octet of k) pairs, `ROWS` rows side by side.  Rows whose k are neighbours: eight (a thread's 32 bytes, 256 of a row per wavefront); others: 32 (128 bytes of a
-// row of the buffer per half wavefront).
-template <int KIND, int ROWS>
+// Eight rows and all their k per workgroup: what it writes are whole lines of 128 bytes (eight rows' 16), and with 64 groups of eight k side by side a thread holds all values of a row of up to 4096
+// between finding the largest and splitting.  Where rows are columns of the buffer it reads 32 bytes at a time; workgroups that share a line run on one XCD (xcd_run).  With 32 rows per
+// workgroup a batch of 65 frames of 6144 bits and as many weights took 30 us.
+template <int KIND>
 __device__ __forceinline__ void pack_rows(PackJob const &j, int block, float *share)
 {
-    constexpr int kOctets = kPackBlock / ROWS;                      // side by side
+    constexpr int ROWS = kPackRows, kOctets = kPackBlock / ROWS;      // side by side
     constexpr bool kBits = KIND == kBitRows || KIND == kBitColumns;
     constexpr int kPieces = kBits ? 1 : 2;
     int const at = threadIdx.x % ROWS, octet0 = threadIdx.x / ROWS, row = block * ROWS + at;
@@ -144,17 +152,18 @@ __device__ __forceinline__ void pack_rows(PackJob const &j, int block, float *sh
 
 __global__ __launch_bounds__(kPackBlock) void dense_pack_kernel(PackArgs a)
 {
-    __shared__ float share[2 * kPackBlock / 64 * 32];
+    __shared__ float share[2 * kPackBlock / 64 * kPackRows];
     int block = blockIdx.x, which = 0;
     while (block >= a.job[which].blocks) { block -= a.job[which].blocks; ++which; }
     PackJob const &j = a.job[which];
+    block = xcd_run(block, j.blocks);
     switch (j.kind) {
-    case kRows:       pack_rows<kRows, 8>(j, block, share); break;
-    case kColumns:    pack_rows<kColumns, 32>(j, block, share); break;
-    case kBitRows:    pack_rows<kBitRows, 8>(j, block, share); break;
-    case kBitColumns: pack_rows<kBitColumns, 32>(j, block, share); break;
-    case kGradRows:   pack_rows<kGradRows, 8>(j, block, share); break;
-    default:          pack_rows<kGradColumns, 32>(j, block, share); break;
+    case kRows:       pack_rows<kRows>(j, block, share); break;
+    case kColumns:    pack_rows<kColumns>(j, block, share); break;
+    case kBitRows:    pack_rows<kBitRows>(j, block, share); break;
+    case kBitColumns: pack_rows<kBitColumns>(j, block, share); break;
+    case kGradRows:   pack_rows<kGradRows>(j, block, share); break;
+    default:          pack_rows<kGradColumns>(j, block, share); break;
     }
 }
 
@@ -189,12 +198,6 @@ __device__ __forceinline__ float element_again(Operand const &a, int kind_a, Ope
     return d;
 }
 
-// workgroup -> place in the list of tiles: workgroups go round the eight XCDs, each of which gets a run of neighbours
-__device__ __forceinline__ int xcd_run(int id, int total)
-{
-    int const x = id & 7, q = total >> 3, r = total & 7;
-    return x * q + min(x, r) + (id >> 3);
-}
 
 // four elements of a row of D that lie side by side, n a multiple of 4; `all`: the four exist and may be moved with 16-byte accesses
 __device__ __forceinline__ void finish_four(DenseOutput const &o, float (&d)[4], int m, int n, bool all)

@@ -8,7 +8,7 @@ namespace bbhip {
 constexpr int kDenseNodesMost = 1 << 24, kDenseFramesMost = 1 << 26;
 
 // Wavefronts that share the k axis of a tile in dense_direct_kernel.
-inline int direct_waves(int depth) { return depth >= 512 ? 16 : 4; }
+inline int direct_waves(int depth) { return depth >= 256 ? 8 : 4; }
 
 // Whether a product goes by way of packed halves (two launches at least, and both operands are written once more) instead of straight from its operands.
 inline bool product_packed(int m, int n, int k) { return (long long)m * n * k >= 1LL << 26 && m >= 32 && n >= 32 && k >= 32; }

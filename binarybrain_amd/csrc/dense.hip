@@ -185,29 +185,55 @@ int packed_product(PackedProduct &d, Product const &p, PackedShape const &s, Pac
     return 0;
 }
 
+// the sums of the products whose k axis workgroups share
+int packed_join(PackedProduct const &p, PackedProduct const &q, hipStream_t st, char const *name)
+{
+    auto const blocks = [](PackedProduct const &d) { return d.slabs > 1 ? ((long long)d.out.rows * d.sums_pitch + 255) / 256 : 0; };
+    long long const first = blocks(p), second = blocks(q);
+    if (first + second == 0) { return 0; }
+    if (check_tiles(first + second, 256, name)) { return 1; }
+    launch(dense_join_kernel, dim3((unsigned)(first + second)), dim3(256), 0, st, p, q, (unsigned)first);
+    BBHIP_LAUNCH_CHECK();
+    return 0;
+}
+
+int packed_run(PackedProduct const &p, bool large, hipStream_t st, char const *name)
+{
+    dim3 const grid((unsigned)p.workgroups), block(large ? 512 : 256);
+#define BBHIP_PACKED(USE)                                                                               \
+    do {                                                                                                \
+        if (large) {                                                                                    \
+            if (p.b_pieces == 1) { launch((dense_packed_kernel<USE, 4, 2, 4, 1, 4>), grid, block, 0, st, p); } \
+            else                 { launch((dense_packed_kernel<USE, 4, 2, 4, 2, 4>), grid, block, 0, st, p); } \
+        }                                                                                               \
+        else {                                                                                          \
+            if (p.b_pieces == 1) { launch((dense_packed_kernel<USE, 2, 2, 2, 1, 4>), grid, block, 0, st, p); } \
+            else                 { launch((dense_packed_kernel<USE, 2, 2, 2, 2, 4>), grid, block, 0, st, p); } \
+        }                                                                                               \
+    } while (0)
+    if (p.out.kind == kOutLogits) { BBHIP_PACKED(kUseLogits); }
+    else                          { BBHIP_PACKED(kUseForward); }
+#undef BBHIP_PACKED
+    BBHIP_LAUNCH_CHECK();
+    return packed_join(p, PackedProduct{}, st, name);
+}
+
 // p and behind it q, whose operands are not packed bits
 int packed_run(PackedProduct const &p, PackedProduct const &q, bool large, hipStream_t st, char const *name)
 {
     if (check_tiles((long long)p.workgroups + q.workgroups, large ? 512 : 256, name)) { return 1; }
     if (p.workgroups + q.workgroups == 0) { return 0; }
-    dim3 const grid((unsigned)(p.workgroups + q.workgroups));
+    dim3 const grid((unsigned)(p.workgroups + q.workgroups)), block(large ? 512 : 256);
     if (large) {
-        if (p.b_pieces == 1) { launch((dense_packed_kernel<4, 2, 4, 1>), grid, dim3(512), 0, st, p, q); }
-        else                 { launch((dense_packed_kernel<4, 2, 4, 2>), grid, dim3(512), 0, st, p, q); }
+        if (p.b_pieces == 1) { launch((dense_packed_pair_kernel<4, 2, 4, 1, 4>), grid, block, 0, st, p, q); }
+        else                 { launch((dense_packed_pair_kernel<4, 2, 4, 2, 4>), grid, block, 0, st, p, q); }
     }
     else {
-        if (p.b_pieces == 1) { launch((dense_packed_kernel<2, 2, 2, 1>), grid, dim3(256), 0, st, p, q); }
-        else                 { launch((dense_packed_kernel<2, 2, 2, 2>), grid, dim3(256), 0, st, p, q); }
+        if (p.b_pieces == 1) { launch((dense_packed_pair_kernel<2, 2, 2, 1, 4>), grid, block, 0, st, p, q); }
+        else                 { launch((dense_packed_pair_kernel<2, 2, 2, 2, 4>), grid, block, 0, st, p, q); }
     }
     BBHIP_LAUNCH_CHECK();
-    auto const join_blocks = [](PackedProduct const &d) { return d.slabs > 1 ? ((long long)d.out.rows * d.sums_pitch + 255) / 256 : 0; };
-    long long const first = join_blocks(p), second = join_blocks(q);
-    if (first + second > 0) {
-        if (check_tiles(first + second, 256, name)) { return 1; }
-        launch(dense_join_kernel, dim3((unsigned)(first + second)), dim3(256), 0, st, p, q, (unsigned)first);
-        BBHIP_LAUNCH_CHECK();
-    }
-    return 0;
+    return packed_join(p, q, st, name);
 }
 
 // of a layer's forward pass
@@ -322,8 +348,8 @@ int dense_forward(void const *x, bool bit, void *y, bool bit_out, float const *W
     Jobs jobs;
     jobs.add(s.W.job(p.a, p.kind_a));
     jobs.add(s.x.job(p.b, p.kind_b));
-    PackedProduct d, none{};
-    return jobs.run(st, name) || packed_product(d, p, s.shape, s.W, s.x, s.sums, name) || packed_run(d, none, s.shape.large, st, name);
+    PackedProduct d;
+    return jobs.run(st, name) || packed_product(d, p, s.shape, s.W, s.x, s.sums, name) || packed_run(d, s.shape.large, st, name);
 }
 
 int dense_backward(void const *x, bool bit, float const *dy, float const *y, float const *W, float *dx, float *dW, float *db, float *dr, int activation,
@@ -432,10 +458,10 @@ int dense_loss(void const *x, bool bit, float const *W, float const *b, int cons
         jobs.add(s.W.job(p.a, kRows));
         if (!x_packed) { jobs.add(s.x.job(p.b, bit ? kBitColumns : kColumns)); x_packed = true; }
         PackedShape const shape = packed_shape(s.plan.logits.large, 1, count, frames, inputs);
-        PackedProduct d, none{};
+        PackedProduct d;
         Packed W_piece = s.W;
         W_piece.blocks = ceil_div(count, 32);
-        return (int)(jobs.run(st, name) || packed_product(d, p, shape, W_piece, s.x, nullptr, name) || packed_run(d, none, shape.large, st, name));
+        return (int)(jobs.run(st, name) || packed_product(d, p, shape, W_piece, s.x, nullptr, name) || packed_run(d, shape.large, st, name));
     };
     // the pieces' largest logits and sums; the last piece's logits stay for its gradient
     for (int piece = 0; piece < pieces; ++piece) { if (logit_piece(piece, gradients && piece == pieces - 1)) { return 1; } }

@@ -8,8 +8,8 @@
 //
 // Two launches.  The first reads each operand as it lies and leaves its halves in the order in which the matrix instructions want them: blocks of 32 rows x 16 k,
 // 1 KiB each, lane l's sixteen bytes (row l & 31, k 8 (l >> 5) .. + 8) at 16 l, so that the second launch moves them to LDS and from there to registers with 16-byte accesses
-// that meet no bank twice, without a transposition anywhere.  In the second, a workgroup of eight wavefronts owns 256 x 256 elements (128 x 128: four) and walks k in stages of 32,
-// the loads of the next stage to LDS in flight behind the products of the present one.
+// that meet no bank twice, without a transposition anywhere.  In the second, a workgroup of eight wavefronts owns 256 x 256 elements (128 x 128: four) and walks k in stages of 16,
+// the loads of the next three stages to LDS in flight behind the products of the present one.
 // Where there are too few tiles for the device, several workgroups share a tile's k axis and a third launch adds their sums in a fixed order.
 #pragma once
 
@@ -28,7 +28,7 @@ struct PackJob {
     int    kind;
     uint4 *halves;              // [row blocks][k steps][1 or 2][64 lanes]
     int   *exponent;            // of each row (null: packed bits, which are not scaled)
-    int    k_steps;             // of 16, even
+    int    k_steps;             // of 16
     int    blocks;              // workgroups
     float *line;                // gradients as rows: their sums (null: not wanted), added with accumulate
     int    accumulate;
@@ -199,70 +199,88 @@ __device__ __forceinline__ float element_again(Operand const &a, int kind_a, Ope
 }
 
 
-// four elements of a row of D that lie side by side, n a multiple of 4; `all`: the four exist and may be moved with 16-byte accesses
-__device__ __forceinline__ void finish_four(DenseOutput const &o, float (&d)[4], int m, int n, bool all)
+// What a launch is for: y or its bits, products as they are (or a slab's sums), logits.
+enum PackedUse : int { kUseForward = 0, kUseStore = 1, kUseLogits = 2 };
+
+// 32 x 64 elements of a wavefront lie in LDS as rows of kTilePitch floats.
+constexpr int kTilePitch = 68;
+
+// v[step]: four neighbours of row 4 step + lane / 16 of such a tile, and what they become.  `all`: the four may be moved with 16-byte accesses.
+template <int USE>
+__device__ __forceinline__ void finish_tile(DenseOutput const &o, float const *tile, float const *bias, int m0, int n0, int lane)
 {
-    if (o.kind == kOutForward || o.kind == kOutLogits) {
-        float r[4] = {};
-        float const b = o.bias ? o.bias[m] : 0.0f;
-        if (o.residual) {
-            float const *from = o.residual + m * o.residual_stride + n;
-            if (all) { load_floats(from, true, r); }
+    int const n = n0 + (lane & 15) * 4, row0 = lane >> 4;
+    bool const all = n + 4 <= o.columns && o.stride % 4 == 0 && (reinterpret_cast<uintptr_t>(o.out) & 15) == 0 &&
+                     (USE != kUseForward || !o.residual || (o.residual_stride % 4 == 0 && (reinterpret_cast<uintptr_t>(o.residual) & 15) == 0));
+    if (n >= o.columns) { return; }
+    // what is added is asked for at once, ahead of the first use
+    float more[8][4] = {};
+    float const *from = USE == kUseForward ? o.residual : o.accumulate ? static_cast<float const *>(o.out) : nullptr;
+    long long const pitch = USE == kUseForward ? o.residual_stride : o.stride;
+    if (from) {
+#pragma unroll
+        for (int step = 0; step < 8; ++step) {
+            int const m = m0 + step * 4 + row0;
+            if (m >= o.rows) { continue; }
+            if (all) { load_floats(from + m * pitch + n, true, more[step]); }
             else {
 #pragma unroll
-                for (int q = 0; q < 4; ++q) { if (n + q < o.columns) { r[q] = from[q]; } }
+                for (int q = 0; q < 4; ++q) { if (n + q < o.columns) { more[step][q] = from[m * pitch + n + q]; } }
             }
         }
-#pragma unroll
-        for (int q = 0; q < 4; ++q) { d[q] = activated(d[q] + b + r[q], o.activation); }
-    }
-    float *to = static_cast<float *>(o.out) + m * o.stride + n;
-    if (all) {
-        float4 v = make_float4(d[0], d[1], d[2], d[3]);
-        if (o.accumulate) {
-            float4 const w = *reinterpret_cast<float4 const *>(to);
-            v = make_float4(w.x + v.x, w.y + v.y, w.z + v.z, w.w + v.w);
-        }
-        *reinterpret_cast<float4 *>(to) = v;
-        return;
     }
 #pragma unroll
-    for (int q = 0; q < 4; ++q) { if (n + q < o.columns) { to[q] = o.accumulate ? to[q] + d[q] : d[q]; } }
-}
-
-// 32 x 64 elements of a wavefront, in LDS (rows of kTilePitch floats), become what they are for: 16 lanes across a row
-constexpr int kTilePitch = 68;
-__device__ __forceinline__ void finish_tile(DenseOutput const &o, float const *tile, int m0, int n0, int lane)
-{
-    int const n = n0 + (lane & 15) * 4;
-    bool const vec = n + 4 <= o.columns && o.stride % 4 == 0 && (reinterpret_cast<uintptr_t>(o.out) & 15) == 0 &&
-                     (!o.residual || (o.residual_stride % 4 == 0 && (reinterpret_cast<uintptr_t>(o.residual) & 15) == 0));
     for (int step = 0; step < 8; ++step) {
-        int const row = step * 4 + (lane >> 4), m = m0 + row;
-        if (m >= o.rows || n >= o.columns) { continue; }
+        int const row = step * 4 + row0, m = m0 + row;
+        if (m >= o.rows) { continue; }
         float d[4];
         load_floats(tile + row * kTilePitch + (lane & 15) * 4, true, d);
-        finish_four(o, d, m, n, vec);
+        if (USE != kUseStore) {
+            float const b = bias[row];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) { d[q] += b; }
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) { d[q] += more[step][q]; }
+        if (USE == kUseForward && o.activation != kActNone) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) { d[q] = activated(d[q], o.activation); }
+        }
+        float *to = static_cast<float *>(o.out) + m * o.stride + n;
+        if (all) { *reinterpret_cast<float4 *>(to) = make_float4(d[0], d[1], d[2], d[3]); }
+        else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) { if (n + q < o.columns) { to[q] = d[q]; } }
+        }
     }
 }
 
 // the same to packed bits: a row of 64 columns is two words
-__device__ __forceinline__ void finish_tile_bits(DenseOutput const &o, float const *tile, int m0, int n0, int lane)
+__device__ __forceinline__ void finish_tile_bits(DenseOutput const &o, float const *tile, float const *bias, int m0, int n0, int lane)
 {
     int const n = n0 + lane;
+    bool const inside = n < o.columns;
     for (int row = 0; row < 32 && m0 + row < o.rows; ++row) {
-        bool const inside = n < o.columns;
-        uint64_t const bits = __ballot(inside && before_activation(o, tile[row * kTilePitch + lane], m0 + row, inside ? n : 0) > 0.0f);
+        float z = tile[row * kTilePitch + lane] + bias[row];
+        if (o.residual && inside) { z += o.residual[(m0 + row) * o.residual_stride + n]; }
+        uint64_t const bits = __ballot(inside && z > 0.0f);
         if ((lane & 31) == 0 && inside) { static_cast<uint32_t *>(o.out)[(m0 + row) * o.stride + (n >> 5)] = (uint32_t)(bits >> (lane & 32)); }
     }
 }
 
-template <int TM, int WM, int WN, int PB>
-__device__ __forceinline__ void packed_tile(PackedProduct const &p, int id, char *lds)
+// Waits until at most N of this wavefront's loads are on their way (loads arrive in order) and its reads of LDS are done, then for the workgroup.
+template <int N>
+__device__ __forceinline__ void arrived(void)
+{
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(N) : "memory");
+}
+
+template <int USE, int TM, int WM, int WN, int PB, int BUFFERS>
+__device__ __forceinline__ void packed_tile(PackedProduct const &p, int id, char *lds, int *scales, float *bias)
 {
     constexpr int TN = 2, kWaves = WM * WN, kBM = TM * WM, kBN = TN * WN;           // blocks of 32 rows
     static_assert(kBM == kWaves && kBN == kWaves, "each wavefront loads one row block of either operand");
-    constexpr int kStageA = kBM * 4096, kStage = kStageA + kBN * 2048 * PB;
+    constexpr int kStageA = kBM * 2048, kStage = kStageA + kBN * 1024 * PB, kLoads = 2 + PB, kAhead = BUFFERS - 1;
     int const lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int const tiles = p.m_tiles * p.n_tiles;
     int const slab = id / tiles;
@@ -271,141 +289,188 @@ __device__ __forceinline__ void packed_tile(PackedProduct const &p, int id, char
     int const band = t / (8 * p.n_tiles), rest = t - band * 8 * p.n_tiles, high = min(8, p.m_tiles - band * 8);
     int const m_tile = band * 8 + rest % high, n_tile = rest / high;
     int const rb_a = m_tile * kBM, rb_b = n_tile * kBN;
-    int const first = slab * p.slab_stages, last = min(first + p.slab_stages, p.k_steps / 2);
+    int const first = slab * p.slab_stages, stages = min(p.slab_stages, p.k_steps - first);
 
-    // a stage is 32 k: of each row block four (packed bits: two) neighbouring blocks of 1 KiB, which a wavefront moves to LDS as they are
-    char const *from_a = reinterpret_cast<char const *>(p.a) + ((long long)min(rb_a + wave, p.a_blocks - 1) * p.k_steps + 2 * first) * 2048;
-    char const *from_b = reinterpret_cast<char const *>(p.b) + ((long long)min(rb_b + wave, p.b_blocks - 1) * p.k_steps + 2 * first) * (1024 * PB);
+    // a stage is 16 k: of each row block two (packed bits: one) blocks of 1 KiB, which a wavefront moves to LDS as they are
+    char const *from_a = reinterpret_cast<char const *>(p.a) + ((long long)min(rb_a + wave, p.a_blocks - 1) * p.k_steps + first) * 2048;
+    char const *from_b = reinterpret_cast<char const *>(p.b) + ((long long)min(rb_b + wave, p.b_blocks - 1) * p.k_steps + first) * (1024 * PB);
+    uint32_t const at_lds = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds);
     auto const fetch = [&](int buffer) {
-        typedef const __attribute__((address_space(1))) void *Global;
-        typedef __attribute__((address_space(3))) void *Shared;
-        Global const a = (Global)(from_a + lane * 16), b = (Global)(from_b + lane * 16);
-        Shared const to_a = (Shared)(lds + buffer * kStage + wave * 4096), to_b = (Shared)(lds + buffer * kStage + kStageA + wave * 2048 * PB);
-        __builtin_amdgcn_global_load_lds(a, to_a, 16, 0, 0);
-        __builtin_amdgcn_global_load_lds(a, to_a, 16, 1024, 0);
-        __builtin_amdgcn_global_load_lds(a, to_a, 16, 2048, 0);
-        __builtin_amdgcn_global_load_lds(a, to_a, 16, 3072, 0);
-        __builtin_amdgcn_global_load_lds(b, to_b, 16, 0, 0);
-        __builtin_amdgcn_global_load_lds(b, to_b, 16, 1024, 0);
+        // (as assembly: the compiler would wait for all of them ahead of every read of LDS, whichever buffer it reads.  Each lane's sixteen bytes go to M0 + offset + 16 lane.)
+        uint32_t const to_a = at_lds + buffer * kStage + wave * 2048, to_b = at_lds + buffer * kStage + kStageA + wave * 1024 * PB;
+        char const *const a = from_a + lane * 16, *const b = from_b + lane * 16;
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\tglobal_load_lds_dwordx4 %1, off offset:1024" :: "s"(to_a), "v"(a) : "memory", "m0");
         if constexpr (PB == 2) {
-            __builtin_amdgcn_global_load_lds(b, to_b, 16, 2048, 0);
-            __builtin_amdgcn_global_load_lds(b, to_b, 16, 3072, 0);
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\tglobal_load_lds_dwordx4 %1, off offset:1024" :: "s"(to_b), "v"(b) : "memory", "m0");
         }
-        from_a += 4096; from_b += 2048 * PB;
+        else { asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(to_b), "v"(b) : "memory", "m0"); }
+        from_a += 2048; from_b += 1024 * PB;
     };
+
+    // what is needed behind the products: the scales and biases of the tile's rows (the barriers of the stages are between this and its use)
+    DenseOutput o = p.out;
+    int const *const scale_a = scales, *const scale_b = scales + kBM * 32;
+    for (int i = threadIdx.x; i < kBM * 32; i += kWaves * 64) {
+        scales[i] = p.ea[min(rb_a * 32 + i, p.a_blocks * 32 - 1)];
+        if (USE != kUseStore) { bias[i] = o.bias && rb_a * 32 + i < o.rows ? o.bias[rb_a * 32 + i] : 0.0f; }
+    }
+    for (int i = threadIdx.x; i < kBN * 32; i += kWaves * 64) { scales[kBM * 32 + i] = PB == 2 ? p.eb[min(rb_b * 32 + i, p.b_blocks * 32 - 1)] : 0; }
 
     int const wm = wave / WN, wn = wave % WN;
     DenseAcc16 acc[TM][TN] = {};
-    fetch(0);
-    for (int stage = first; stage < last; ++stage) {
-        int const buffer = (stage - first) & 1;
-        // this wavefront's loads of the stage have arrived; behind the barrier all wavefronts' have, and nobody reads the other buffer any more
-        __builtin_amdgcn_s_waitcnt(0x0f70);
-        __syncthreads();
-        if (stage + 1 < last) { fetch(buffer ^ 1); }
+    auto const multiply = [&](int buffer) {
         char const *from = lds + buffer * kStage + lane * 16;
+        DenseHalf8 a[TM][2], b[TN][PB];
 #pragma unroll
-        for (int step = 0; step < 2; ++step) {
-            DenseHalf8 a[TM][2], b[TN][PB];
+        for (int i = 0; i < TM; ++i) {
 #pragma unroll
-            for (int i = 0; i < TM; ++i) {
-#pragma unroll
-                for (int q = 0; q < 2; ++q) { a[i][q] = *reinterpret_cast<DenseHalf8 const *>(from + (((wm * TM + i) * 2 + step) * 2 + q) * 1024); }
-            }
-#pragma unroll
-            for (int j = 0; j < TN; ++j) {
-#pragma unroll
-                for (int q = 0; q < PB; ++q) { b[j][q] = *reinterpret_cast<DenseHalf8 const *>(from + kStageA + (((wn * TN + j) * 2 + step) * PB + q) * 1024); }
-            }
-#pragma unroll
-            for (int i = 0; i < TM; ++i) {
-#pragma unroll
-                for (int j = 0; j < TN; ++j) {
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][1], b[j][0], acc[i][j], 0, 0, 0);
-                    if constexpr (PB == 2) { acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][0], b[j][1], acc[i][j], 0, 0, 0); }
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][0], b[j][0], acc[i][j], 0, 0, 0);
-                }
-            }
+            for (int q = 0; q < 2; ++q) { a[i][q] = *reinterpret_cast<DenseHalf8 const *>(from + ((wm * TM + i) * 2 + q) * 1024); }
         }
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+#pragma unroll
+            for (int q = 0; q < PB; ++q) { b[j][q] = *reinterpret_cast<DenseHalf8 const *>(from + kStageA + ((wn * TN + j) * PB + q) * 1024); }
+        }
+        __builtin_amdgcn_sched_barrier(0);          // (all reads are asked for ahead of the first product: with two wavefronts per SIMD what one waits for the other hides)
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+#pragma unroll
+            for (int j = 0; j < TN; ++j) { acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][1], b[j][0], acc[i][j], 0, 0, 0); }
+            if constexpr (PB == 2) {
+#pragma unroll
+                for (int j = 0; j < TN; ++j) { acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][0], b[j][1], acc[i][j], 0, 0, 0); }
+            }
+#pragma unroll
+            for (int j = 0; j < TN; ++j) { acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][0], b[j][0], acc[i][j], 0, 0, 0); }
+        }
+    };
+    // A stage's loads are asked for kAhead stages before.  Behind the barrier all wavefronts' loads of the stage have arrived, and nobody reads the buffer of the stage before any more,
+    // which the next loads go to.
+    int const ahead = min(kAhead, stages);
+    for (int s = 0; s < ahead; ++s) { fetch(s); }
+    int buffer = 0, free = kAhead;
+    int s = 0;
+    for (; s + kAhead < stages; ++s) {
+        arrived<(kAhead - 1) * kLoads>();
+        fetch(free);
+        multiply(buffer);
+        free = buffer;
+        buffer = buffer + 1 == BUFFERS ? 0 : buffer + 1;
+    }
+    for (; s < stages; ++s) {
+        arrived<0>();
+        multiply(buffer);
+        buffer = buffer + 1 == BUFFERS ? 0 : buffer + 1;
     }
 
     // 32 x 64 elements at a time go through LDS, so that a lane has neighbours of a row to store, or the rows of a column to sum
-    DenseOutput o = p.out;
-    if (p.slabs > 1) {
-        o.kind = kOutStore; o.out = p.sums + slab * p.sums_slab; o.stride = p.sums_pitch; o.accumulate = 0; o.line = nullptr;
+    if (USE != kUseLogits && p.slabs > 1) {
+        o.kind = kOutStore; o.out = p.sums + slab * p.sums_slab; o.stride = p.sums_pitch; o.accumulate = 0;
     }
     float *const tile = reinterpret_cast<float *>(lds) + wave * 32 * kTilePitch;
     int const n0 = (rb_b + wn * TN) * 32;
     int eb[TN];
-#pragma unroll
-    for (int j = 0; j < TN; ++j) { eb[j] = p.eb ? p.eb[min(n0 + j * 32 + (lane & 31), p.b_blocks * 32 - 1)] : 0; }
-    float2 column = make_float2(-INFINITY, 0.0f);
     __syncthreads();                            // (the stages are done with LDS)
 #pragma unroll
+    for (int j = 0; j < TN; ++j) { eb[j] = scale_b[(wn * TN + j) * 32 + (lane & 31)]; }
+    float2 column = make_float2(-INFINITY, 0.0f);
+#pragma nounroll
     for (int i = 0; i < TM; ++i) {
         int const rb = rb_a + wm * TM + i, m0 = rb * 32;
-        if (rb >= p.a_blocks) { continue; }
+        if (rb >= p.a_blocks) { break; }
         bool odd = false;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            int const row = acc_row(r, lane), ea = p.ea[m0 + row];
+        for (int u = 0; u < TM; ++u) {              // (registers have no index)
+            if (u != i) { continue; }
 #pragma unroll
-            for (int j = 0; j < TN; ++j) {
-                float const d = ldexpf(acc[i][j][r], -(ea + eb[j]));           // the scales come off
-                odd = odd || d != d;
-                tile[row * kTilePitch + j * 32 + (lane & 31)] = d;
+            for (int r = 0; r < 16; ++r) {
+                int const row = acc_row(r, lane), ea = scale_a[(wm * TM + i) * 32 + row];
+#pragma unroll
+                for (int j = 0; j < TN; ++j) {
+                    float const d = ldexpf(acc[u][j][r], -(ea + eb[j]));           // the scales come off
+                    odd = odd || d != d;
+                    tile[row * kTilePitch + j * 32 + (lane & 31)] = d;
+                }
             }
         }
-        if (p.kind_a >= 0 && p.slabs == 1 && __any(odd)) {
+        float const *const b = bias + (wm * TM + i) * 32;
+        if (USE != kUseLogits && p.kind_a >= 0 && p.slabs == 1 && __any(odd)) {
             for (int row = 0; row < 32; ++row) {
                 if (m0 + row < o.rows && n0 + lane < o.columns) { tile[row * kTilePitch + lane] = element_again(p.src_a, p.kind_a, p.src_b, p.kind_b, m0 + row, n0 + lane); }
             }
         }
-        if (o.kind == kOutBits) { finish_tile_bits(o, tile, m0, n0, lane); continue; }
-        if (o.kind == kOutLogits && n0 + lane < o.columns) {
+        if (USE == kUseLogits && n0 + lane < o.columns) {
             // (largest, sum of exponents) of the 32 rows of this lane's column
             int const n = n0 + lane, rows = min(32, o.rows - m0), label = o.label[n] - o.first_channel - m0;
+            float z[32];
             float2 s = make_float2(-INFINITY, 0.0f);
-            for (int row = 0; row < rows; ++row) { s.x = fmaxf(s.x, tile[row * kTilePitch + lane] + (o.bias ? o.bias[m0 + row] : 0.0f)); }
-            for (int row = 0; row < rows; ++row) {
-                float const z = tile[row * kTilePitch + lane] + (o.bias ? o.bias[m0 + row] : 0.0f);
-                s.y += z == -INFINITY ? 0.0f : exp_of_nonpositive(z - s.x);
-                if (row == label) { o.label_logit[n] = z; }
+#pragma unroll
+            for (int row = 0; row < 32; ++row) {
+                z[row] = row < rows ? tile[row * kTilePitch + lane] + b[row] : -INFINITY;
+                s.x = fmaxf(s.x, z[row]);
             }
+#pragma unroll
+            for (int row = 0; row < 32; ++row) { s.y += z[row] == -INFINITY ? 0.0f : exp_of_nonpositive(z[row] - s.x); }
+            if (label >= 0 && label < rows) { o.label_logit[n] = tile[label * kTilePitch + lane] + b[label]; }
             column = joined(column, s);
         }
-        if (o.out) { finish_tile(o, tile, m0, n0, lane); }
+        if (USE == kUseForward && o.kind == kOutBits)         { finish_tile_bits(o, tile, b, m0, n0, lane); }
+        else if (USE == kUseForward && o.kind == kOutForward) { finish_tile<kUseForward>(o, tile, b, m0, n0, lane); }
+        else if (USE != kUseLogits || o.out)                  { finish_tile<USE == kUseLogits ? kUseLogits : kUseStore>(o, tile, b, m0, n0, lane); }
     }
-    if (o.kind == kOutLogits && n0 + lane < o.columns && rb_a + wm * TM < p.a_blocks) {
+    if (USE == kUseLogits && n0 + lane < o.columns && rb_a + wm * TM < p.a_blocks) {
         o.partial[(long long)((rb_a + wm * TM) / TM) * o.columns + n0 + lane] = column;
     }
 }
 
-// one product, and behind it another (workgroups 0: none)
-template <int TM, int WM, int WN, int PB>
-__global__ __launch_bounds__(WM * WN * 64) void dense_packed_kernel(PackedProduct p, PackedProduct q)
+template <int TM, int WM, int WN, int BUFFERS>
+constexpr int packed_lds(void)
 {
-    __shared__ __attribute__((aligned(1024))) char lds[2 * (TM * WM + 2 * WN) * 4096];
-    if ((int)blockIdx.x < p.workgroups) { packed_tile<TM, WM, WN, PB>(p, blockIdx.x, lds); }
-    else                                { packed_tile<TM, WM, WN, 2>(q, blockIdx.x - p.workgroups, lds); }
+    constexpr int kStages = BUFFERS * (TM * WM + 2 * WN) * 2048, kTiles = WM * WN * 32 * kTilePitch * 4;
+    return kStages > kTiles ? kStages : kTiles;
 }
 
-// the slabs' sums of a product, in order, and what becomes of them: a thread per element, a wavefront within a row
-__device__ __forceinline__ void join_slabs(PackedProduct const &p, long long id)
+template <int USE, int TM, int WM, int WN, int PB, int BUFFERS>
+__global__ __launch_bounds__(WM * WN * 64) void dense_packed_kernel(PackedProduct p)
+{
+    __shared__ __attribute__((aligned(1024))) char lds[packed_lds<TM, WM, WN, BUFFERS>()];
+    __shared__ int scales[(TM * WM + 2 * WN) * 32];
+    __shared__ float bias[TM * WM * 32];
+    packed_tile<USE, TM, WM, WN, PB, BUFFERS>(p, blockIdx.x, lds, scales, bias);
+}
+
+// one product, and behind it another whose operands are not packed bits (either may have no workgroups)
+template <int TM, int WM, int WN, int PB, int BUFFERS>
+__global__ __launch_bounds__(WM * WN * 64) void dense_packed_pair_kernel(PackedProduct p, PackedProduct q)
+{
+    __shared__ __attribute__((aligned(1024))) char lds[packed_lds<TM, WM, WN, BUFFERS>()];
+    __shared__ int scales[(TM * WM + 2 * WN) * 32];
+    if ((int)blockIdx.x < p.workgroups) { packed_tile<kUseStore, TM, WM, WN, PB, BUFFERS>(p, blockIdx.x, lds, scales, nullptr); }
+    else                                { packed_tile<kUseStore, TM, WM, WN, 2, BUFFERS>(q, blockIdx.x - p.workgroups, lds, scales, nullptr); }
+}
+
+// The slabs' sums of a product, in order, and what becomes of them: a wavefront takes 64 neighbours of a row.
+__device__ __forceinline__ void join_slabs(PackedProduct const &p, unsigned id)
 {
     DenseOutput const &o = p.out;
-    int const pitch = (o.columns + 63) / 64 * 64, lane = threadIdx.x & 63;
-    int const m = (int)(id / pitch), n = (int)(id % pitch);
+    unsigned const across = (unsigned)(p.sums_pitch / 64), unit = id * 4 + threadIdx.x / 64;
+    int const lane = threadIdx.x & 63, m = (int)(unit / across), n = (int)(unit % across) * 64 + lane;
     if (m >= o.rows) { return; }
     bool const inside = n < o.columns;
     float d = 0.0f;
     if (inside) {
-        for (int s = 0; s < p.slabs; ++s) { d += p.sums[s * p.sums_slab + m * p.sums_pitch + n]; }
+        float const *from = p.sums + m * p.sums_pitch + n;
+        int s = 0;
+        for (; s + 4 <= p.slabs; s += 4) {
+            float const a = from[s * p.sums_slab], b = from[(s + 1) * p.sums_slab], c = from[(s + 2) * p.sums_slab], e = from[(s + 3) * p.sums_slab];
+            d = (((d + a) + b) + c) + e;
+        }
+        for (; s < p.slabs; ++s) { d += from[s * p.sums_slab]; }
         if (d != d && p.kind_a >= 0) { d = element_again(p.src_a, p.kind_a, p.src_b, p.kind_b, m, n); }
     }
     if (o.kind == kOutForward) { if (inside) { static_cast<float *>(o.out)[m * o.stride + n] = activated(before_activation(o, d, m, n), o.activation); } }
     else if (o.kind == kOutBits) {
-        uint64_t const bits = __ballot(inside && before_activation(o, d, m, n) > 0.0f);
+        uint64_t const bits = __ballot(inside && before_activation(o, d, m, inside ? n : 0) > 0.0f);
         if ((lane & 31) == 0 && inside) { static_cast<uint32_t *>(o.out)[m * o.stride + (n >> 5)] = (uint32_t)(bits >> (lane & 32)); }
     }
     else if (inside) { store_element(o, d, m, n); }
@@ -413,8 +478,8 @@ __device__ __forceinline__ void join_slabs(PackedProduct const &p, long long id)
 
 __global__ __launch_bounds__(256) void dense_join_kernel(PackedProduct p, PackedProduct q, unsigned first_blocks)
 {
-    if (blockIdx.x < first_blocks) { join_slabs(p, (long long)blockIdx.x * 256 + threadIdx.x); }
-    else                           { join_slabs(q, (long long)(blockIdx.x - first_blocks) * 256 + threadIdx.x); }
+    if (blockIdx.x < first_blocks) { join_slabs(p, blockIdx.x); }
+    else                           { join_slabs(q, blockIdx.x - first_blocks); }
 }
 
 }  // namespace bbhip

@@ -1,6 +1,8 @@
 // Rules by which the entries of dense layers and of the loss on top of one divide their work, apart from the code that launches: plain C++.
 #pragma once
 
+#include <initializer_list>
+
 #include "launch_rules.hpp"
 
 namespace bbhip {
@@ -21,7 +23,7 @@ struct PackedShape {
     int  tile_rows(void) const { return large ? 128 : 64; }         // that a wavefront owns
 };
 
-inline int pack_steps(int depth) { return ceil_div(depth, 32) * 2; }
+inline int pack_steps(int depth) { return ceil_div(depth, 16); }
 
 inline PackedShape packed_shape(bool large, int slabs, int m, int n, int k)
 {
@@ -30,60 +32,59 @@ inline PackedShape packed_shape(bool large, int slabs, int m, int n, int k)
     s.large = large;
     s.m_tiles = ceil_div(m, side); s.n_tiles = ceil_div(n, side);
     s.k_steps = pack_steps(k);
-    s.slab_stages = ceil_div(s.k_steps / 2, slabs);
-    s.slabs = ceil_div(s.k_steps / 2, s.slab_stages);
+    s.slab_stages = ceil_div(s.k_steps, slabs);
+    s.slabs = ceil_div(s.k_steps, s.slab_stages);
     return s;
 }
 
-// Time of a launch in stages of a small tile on a compute unit (768 cycles of matrix instructions with two halves per operand): a large tile's stage is four of them.  Workgroups of one
-// length run in rounds of 256; small tiles two on a compute unit, each at half the speed.
-inline double packed_cost(PackedShape const &s, int m, int n)
+// Time of a launch in stages of a small tile on a compute unit (384 cycles of matrix instructions with two halves per operand, 0.16 us).  A large tile's stage is four of them; small tiles
+// run two on a compute unit, each at half the speed.  Six stages' worth are a workgroup's beginning and end.
+constexpr double kStageLarge = 4.0 / 0.75, kStageSmall = 1.0 / 0.6;
+inline double packed_length(PackedShape const &s) { return (s.slab_stages + 6) * (s.large ? kStageLarge : 2 * kStageSmall); }
+inline int    packed_at_once(PackedShape const &s) { return s.large ? 256 : 512; }
+
+// sums written and read again at about 4 TB/s, and a launch
+inline double join_cost(PackedShape const &s, int m, int n) { return s.slabs > 1 ? (double)s.slabs * m * n * 8.0 / 4.0e6 / 0.16 : 0.0; }
+constexpr double kJoinLaunch = 25.0;
+
+// Two kinds of workgroups dealt out in order to whoever is free: when the last one ends.
+inline double packed_end(PackedShape const &x, PackedShape const &y)
 {
-    long long const wgs = s.workgroups();
-    double const stage = s.large ? 4.0 / 0.75 : 1.0 / 0.6, at_once = s.large ? 256 : 512;
-    double const rounds = (double)((wgs + (long long)at_once - 1) / (long long)at_once) * (s.large ? 1 : 2);
-    double cost = (s.slab_stages + 3) * rounds * stage;
-    // sums written and read again at about 4 TB/s, and a launch: a unit is 0.32 us
-    if (s.slabs > 1) { cost += 10 + (double)s.slabs * m * n * 8.0 / 4.0e6 / 0.32; }
-    return cost;
+    long long const at_once = packed_at_once(x), n1 = x.workgroups(), n2 = y.workgroups();
+    double const l1 = packed_length(x), l2 = packed_length(y);
+    long long const full = n1 / at_once, more = n1 % at_once;           // `more` places are taken once more than the others
+    double const free0 = full * l1, free1 = more ? free0 + l1 : free0;
+    if (n2 == 0) { return free1; }
+    // the places that are free first take `head` workgroups each before the others join in
+    long long const head = more ? (long long)(l1 / l2) : 0, first = at_once - more;
+    if (n2 <= first * head) { double const end = free0 + (double)((n2 + first - 1) / first) * l2; return end > free1 ? end : free1; }
+    long long const left = n2 - first * head;
+    return (more ? free1 : free0) + (double)((left + at_once - 1) / at_once) * l2;
+}
+
+// The division of one product (n1 = 0) or of two in one launch, tiles of one size: a length of the k axis for all workgroups is tried, halved from the longest on.
+inline void best_shapes(int m0, int n0, int k0, int m1, int n1, int k1, PackedShape &s0, PackedShape &s1, bool only_whole = false)
+{
+    int const longest = pack_steps(k0 > k1 ? k0 : k1);
+    double least = -1.0;
+    for (int large = 0; large < 2; ++large) {
+        for (int parts : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
+            int const length = ceil_div(longest, parts);
+            if (parts > 1 && (only_whole || length < 8)) { break; }
+            PackedShape const x = packed_shape(large != 0, ceil_div(pack_steps(k0), length), m0, n0, k0);
+            PackedShape const y = m1 ? packed_shape(large != 0, ceil_div(pack_steps(k1), length), m1, n1, k1) : PackedShape{large != 0, 0, 0, 0, 1, 0};
+            double const join = join_cost(x, m0, n0) + (m1 ? join_cost(y, m1, n1) : 0.0);
+            double const cost = packed_end(x, y) + join + (join > 0 ? kJoinLaunch : 0.0);
+            if (least < 0 || cost < least) { least = cost; s0 = x; s1 = y; }
+        }
+    }
 }
 
 inline PackedShape best_shape(int m, int n, int k, bool only_whole = false)
 {
-    PackedShape best = packed_shape(true, 1, m, n, k);
-    for (int large = 0; large < 2; ++large) {
-        for (int slabs : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
-            if (slabs > 1 && (only_whole || pack_steps(k) / 2 / slabs < 4)) { break; }
-            PackedShape const s = packed_shape(large != 0, slabs, m, n, k);
-            if (packed_cost(s, m, n) < packed_cost(best, m, n)) { best = s; }
-        }
-    }
-    return best;
-}
-
-// Two products in one launch: tiles of one size, each with its own division of the k axis so that the longest workgroup does not outlast the rest.
-inline void best_shapes(int m0, int n0, int k0, int m1, int n1, int k1, PackedShape &s0, PackedShape &s1)
-{
-    double least = -1.0;
-    for (int large = 0; large < 2; ++large) {
-        for (int a : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
-            if (a > 1 && pack_steps(k0) / 2 / a < 4) { break; }
-            for (int b : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
-                if (b > 1 && pack_steps(k1) / 2 / b < 4) { break; }
-                PackedShape const x = packed_shape(large != 0, a, m0, n0, k0), y = packed_shape(large != 0, b, m1, n1, k1);
-                double const stage = large ? 4.0 / 0.75 : 1.0 / 0.6;
-                double const total = (double)x.workgroups() * (x.slab_stages + 3) + (double)y.workgroups() * (y.slab_stages + 3);
-                int const longest = x.slab_stages > y.slab_stages ? x.slab_stages : y.slab_stages;
-                double cost = (total / 256 + 0.5 * (longest + 3) * (large ? 1 : 2)) * stage;
-                if (cost < (longest + 3) * stage * (large ? 1 : 2)) { cost = (longest + 3) * stage * (large ? 1 : 2); }
-                if (x.slabs > 1 || y.slabs > 1) {
-                    double const moved = (x.slabs > 1 ? (double)x.slabs * m0 * n0 : 0.0) + (y.slabs > 1 ? (double)y.slabs * m1 * n1 : 0.0);
-                    cost += 10 + moved * 8.0 / 4.0e6 / 0.32;
-                }
-                if (least < 0 || cost < least) { least = cost; s0 = x; s1 = y; }
-            }
-        }
-    }
+    PackedShape s{}, none{};
+    best_shapes(m, n, k, 0, 0, 0, s, none, only_whole);
+    return s;
 }
 
 // The channels of a loss are taken in pieces, so that what is held of the logits does not grow with their number.

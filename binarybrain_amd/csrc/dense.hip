@@ -40,85 +40,6 @@ int check_tiles(long long tiles, int threads, char const *name)
     return 0;
 }
 
-// ---- products straight from the operands ----
-int direct(DirectProduct &d, Product const &p, int columns, char const *name, int waves)
-{
-    d.a = p.a; d.b = p.b; d.out = p.out;
-    d.n_tiles = ceil_div(columns, kDirectTile);
-    long long const tiles = p.wanted ? (long long)ceil_div(p.out.rows, kDirectTile) * d.n_tiles : 0;
-    if (check_tiles(tiles, waves * 64, name)) { return 1; }
-    d.tiles = (int)tiles;
-    return 0;
-}
-
-int direct_forward(Product const &p, bool bit, hipStream_t st, char const *name)
-{
-    if (p.out.columns <= kFewFrames && p.out.kind != kOutLogits) {
-        DirectProduct d{};
-        d.a = p.a; d.b = p.b; d.out = p.out;
-        long long const blocks = ceil_div(p.out.rows, kFewWaves);
-        if (check_tiles(blocks, kFewWaves * 64, name)) { return 1; }
-        dim3 const grid((unsigned)blocks), block(kFewWaves * 64);
-        if (p.out.columns == 1) {
-            if (bit) { launch((dense_few_frames_kernel<kBitColumns, 1>), grid, block, 0, st, d); }
-            else     { launch((dense_few_frames_kernel<kColumns, 1>), grid, block, 0, st, d); }
-        }
-        else {
-            if (bit) { launch((dense_few_frames_kernel<kBitColumns, kFewFrames>), grid, block, 0, st, d); }
-            else     { launch((dense_few_frames_kernel<kColumns, kFewFrames>), grid, block, 0, st, d); }
-        }
-        BBHIP_LAUNCH_CHECK();
-        return 0;
-    }
-    int const waves = direct_waves(p.a.depth);
-    DirectProduct d;
-    if (direct(d, p, p.out.columns, name, waves)) { return 1; }
-    dim3 const grid((unsigned)d.tiles), block((unsigned)waves * 64);
-    if (waves == 8) {
-        if (bit) { launch((dense_direct_kernel<kRows, kBitColumns, 8>), grid, block, 0, st, d); }
-        else     { launch((dense_direct_kernel<kRows, kColumns, 8>), grid, block, 0, st, d); }
-    }
-    else {
-        if (bit) { launch((dense_direct_kernel<kRows, kBitColumns, 4>), grid, block, 0, st, d); }
-        else     { launch((dense_direct_kernel<kRows, kColumns, 4>), grid, block, 0, st, d); }
-    }
-    BBHIP_LAUNCH_CHECK();
-    return 0;
-}
-
-// dw.a and dx.b are gradients; where these are more than dy itself, or wanted, they are formed first and lie in `dz`
-int direct_backward(Product const &dw, Product const &dx, float *dz, long long dz_stride, bool bit, hipStream_t st, char const *name)
-{
-    int const waves = direct_waves(dw.wanted && dw.a.depth > dx.a.depth ? dw.a.depth : dx.a.depth);
-    DirectProduct w, x;
-    Product with_line = dw, from_dz = dx;
-    if (dz) {
-        DzArgs z{dw.a, dz, dz_stride, ceil_div(dw.a.depth, 1024)};
-        long long const blocks = (long long)z.per_row * dw.a.rows;
-        if (check_tiles(blocks, 256, name)) { return 1; }
-        launch(dense_dz_kernel, dim3((unsigned)blocks), dim3(256), 0, st, z);
-        BBHIP_LAUNCH_CHECK();
-        with_line.a = rows_of(dz, dz_stride, dw.a.rows, dw.a.depth);
-        from_dz.b = rows_of(dz, dz_stride, dx.b.rows, dx.b.depth);
-    }
-    if (dw.out.line) { with_line.b.ones = dw.b.rows; }
-    if (direct(w, with_line, dw.out.columns + (dw.out.line ? 1 : 0), name, waves) || direct(x, from_dz, dx.out.columns, name, waves) ||
-        check_tiles((long long)w.tiles + x.tiles, waves * 64, name)) { return 1; }
-    if (w.tiles + x.tiles == 0) { return 0; }
-    dim3 const grid((unsigned)(w.tiles + x.tiles)), block((unsigned)waves * 64);
-    if (waves == 8) {
-        if (bit) { launch((dense_direct_backward_kernel<kBitRows, 8>), grid, block, 0, st, w, x); }
-        else     { launch((dense_direct_backward_kernel<kRows, 8>), grid, block, 0, st, w, x); }
-    }
-    else {
-        if (bit) { launch((dense_direct_backward_kernel<kBitRows, 4>), grid, block, 0, st, w, x); }
-        else     { launch((dense_direct_backward_kernel<kRows, 4>), grid, block, 0, st, w, x); }
-    }
-    BBHIP_LAUNCH_CHECK();
-    return 0;
-}
-
-// ---- products by way of packed halves ----
 // Takes pieces of a workspace, or counts them (base null)
 struct Carver {
     char *base;
@@ -131,6 +52,139 @@ struct Carver {
     }
 };
 
+// the sums of workgroups that share a product's k axis (columns and perhaps one more)
+long long sums_pitch(int columns) { return ceil_div(columns, 64) * 64LL; }
+float *sums_of(Carver &c, int slabs, int rows, int columns) { return slabs > 1 ? c.take<float>((size_t)slabs * rows * sums_pitch(columns)) : nullptr; }
+
+// added up, and what becomes of them; q may have none
+int join(PackedProduct const &p, PackedProduct const &q, hipStream_t st, char const *name)
+{
+    if (p.slabs > 1 && p.out.kind == kOutLogits) {
+        long long const blocks = ceil_div(p.out.rows, 32) * (p.sums_pitch / 64);
+        if (check_tiles(blocks, 256, name)) { return 1; }
+        launch(dense_join_logits_kernel, dim3((unsigned)blocks), dim3(256), 0, st, p);
+        BBHIP_LAUNCH_CHECK();
+        return 0;
+    }
+    auto const blocks = [](PackedProduct const &d) { return d.slabs > 1 ? ((long long)d.out.rows * d.sums_pitch + 255) / 256 : 0; };
+    long long const first = blocks(p), second = blocks(q);
+    if (first + second == 0) { return 0; }
+    if (check_tiles(first + second, 256, name)) { return 1; }
+    launch(dense_join_kernel, dim3((unsigned)(first + second)), dim3(256), 0, st, p, q, (unsigned)first);
+    BBHIP_LAUNCH_CHECK();
+    return 0;
+}
+
+// ---- products straight from the operands ----
+int direct(DirectProduct &d, Product const &p, DirectShape const &s, float *sums, int columns, char const *name)
+{
+    d = DirectProduct{};
+    d.slabs = 1;
+    if (!p.wanted) { return 0; }
+    d.a = p.a; d.b = p.b; d.out = p.out;
+    d.n_tiles = s.n_tiles; d.slabs = s.slabs; d.slab_chunks = s.slab_chunks;
+    d.sums = sums; d.sums_pitch = sums_pitch(columns); d.sums_slab = d.sums_pitch * p.out.rows;
+    if (check_tiles(s.tiles * s.slabs, s.waves * 64, name)) { return 1; }
+    d.tiles = (int)s.tiles;
+    return 0;
+}
+
+PackedProduct sums_to_join(DirectProduct const &d)
+{
+    PackedProduct p{};
+    p.slabs = d.tiles ? d.slabs : 1; p.sums = d.sums; p.sums_pitch = d.sums_pitch; p.sums_slab = d.sums_slab; p.out = d.out; p.kind_a = -1;
+    return p;
+}
+
+bool few_frames(Product const &p) { return p.out.columns <= kFewFrames && p.out.kind != kOutLogits; }
+
+int few_frames_forward(Product const &p, bool bit, hipStream_t st, char const *name)
+{
+    DirectProduct d{};
+    d.a = p.a; d.b = p.b; d.out = p.out;
+    // four rows for a wavefront where that leaves two workgroups for a compute unit
+    bool const four = p.out.rows >= 512 * kFewWaves * 4;
+    long long const blocks = ceil_div(p.out.rows, kFewWaves * (four ? 4 : 1));
+    if (check_tiles(blocks, kFewWaves * 64, name)) { return 1; }
+    dim3 const grid((unsigned)blocks), block(kFewWaves * 64);
+#define BBHIP_FEW(KIND, FRAMES)                                                                                         \
+    do {                                                                                                                \
+        if (four) { if (p.a.vec) { launch((dense_few_frames_kernel<KIND, FRAMES, 4, true>), grid, block, 0, st, d); }   \
+                    else         { launch((dense_few_frames_kernel<KIND, FRAMES, 4, false>), grid, block, 0, st, d); } } \
+        else      { if (p.a.vec) { launch((dense_few_frames_kernel<KIND, FRAMES, 1, true>), grid, block, 0, st, d); }   \
+                    else         { launch((dense_few_frames_kernel<KIND, FRAMES, 1, false>), grid, block, 0, st, d); } } \
+    } while (0)
+    if (p.out.columns == 1) { if (bit) { BBHIP_FEW(kBitColumns, 1); } else { BBHIP_FEW(kColumns, 1); } }
+    else                    { if (bit) { BBHIP_FEW(kBitColumns, kFewFrames); } else { BBHIP_FEW(kColumns, kFewFrames); } }
+#undef BBHIP_FEW
+    BBHIP_LAUNCH_CHECK();
+    return 0;
+}
+
+int direct_forward(Product const &p, bool bit, float *sums, hipStream_t st, char const *name)
+{
+    DirectShape const s = direct_shape(p.out.rows, p.out.columns, p.a.depth);
+    DirectProduct d;
+    if (direct(d, p, s, sums, p.out.columns, name)) { return 1; }
+    dim3 const grid((unsigned)d.workgroups()), block((unsigned)s.waves * 64);
+    if (s.waves == 16) {
+        if (bit) { launch((dense_direct_kernel<kRows, kBitColumns, 16>), grid, block, 0, st, d); }
+        else     { launch((dense_direct_kernel<kRows, kColumns, 16>), grid, block, 0, st, d); }
+    }
+    else {
+        if (bit) { launch((dense_direct_kernel<kRows, kBitColumns, 4>), grid, block, 0, st, d); }
+        else     { launch((dense_direct_kernel<kRows, kColumns, 4>), grid, block, 0, st, d); }
+    }
+    BBHIP_LAUNCH_CHECK();
+    return join(sums_to_join(d), PackedProduct{}, st, name);
+}
+
+// of a small backward pass: how it is divided, and its places in a workspace
+struct DirectBackwardSpace {
+    DirectShape w, x;
+    float *dz, *w_sums, *x_sums;
+    DirectBackwardSpace(Carver &c, int inputs, int outputs, int frames, bool with_dz)
+        : w(direct_shape(outputs, inputs + 1, frames)), x(direct_shape(inputs, frames, outputs))
+    {
+        if (w.waves != x.waves) { w.waves = x.waves = 16; }
+        dz = with_dz ? c.take<float>((size_t)outputs * (ceil_div(frames, 64) * 64)) : nullptr;
+        w_sums = sums_of(c, w.slabs, outputs, inputs + 1);
+        x_sums = sums_of(c, x.slabs, inputs, frames);
+    }
+};
+
+// dw.a and dx.b are gradients; where these are more than dy itself, or wanted, they are formed first and lie in `dz`
+int direct_backward(Product const &dw, Product const &dx, DirectBackwardSpace const &s, float *dz, long long dz_stride, bool bit, hipStream_t st, char const *name)
+{
+    DirectProduct w, x;
+    Product with_line = dw, from_dz = dx;
+    if (dz) {
+        DzArgs z{dw.a, dz, dz_stride, ceil_div(dw.a.depth, 1024)};
+        long long const blocks = (long long)z.per_row * dw.a.rows;
+        if (check_tiles(blocks, 256, name)) { return 1; }
+        launch(dense_dz_kernel, dim3((unsigned)blocks), dim3(256), 0, st, z);
+        BBHIP_LAUNCH_CHECK();
+        with_line.a = rows_of(dz, dz_stride, dw.a.rows, dw.a.depth);
+        from_dz.b = rows_of(dz, dz_stride, dx.b.rows, dx.b.depth);
+    }
+    with_line.b.ones = dw.out.line ? dw.b.rows : -1;
+    if (direct(w, with_line, s.w, s.w_sums, dw.out.columns + 1, name) || direct(x, from_dz, s.x, s.x_sums, dx.out.columns, name) ||
+        check_tiles((long long)w.workgroups() + x.workgroups(), s.w.waves * 64, name)) { return 1; }
+    if (w.tiles + x.tiles == 0) { return 0; }
+    dim3 const grid((unsigned)(w.workgroups() + x.workgroups())), block((unsigned)s.w.waves * 64);
+    if (s.w.waves == 16) {
+        if (bit) { launch((dense_direct_backward_kernel<kBitRows, 16>), grid, block, 0, st, w, x); }
+        else     { launch((dense_direct_backward_kernel<kRows, 16>), grid, block, 0, st, w, x); }
+    }
+    else {
+        if (bit) { launch((dense_direct_backward_kernel<kBitRows, 4>), grid, block, 0, st, w, x); }
+        else     { launch((dense_direct_backward_kernel<kRows, 4>), grid, block, 0, st, w, x); }
+    }
+    BBHIP_LAUNCH_CHECK();
+    return join(sums_to_join(w), sums_to_join(x), st, name);
+}
+
+// ---- products by way of packed halves ----
 bool is_bits(int kind) { return kind == kBitRows || kind == kBitColumns; }
 
 // an operand's halves and scales in a workspace, and the job that writes them
@@ -155,20 +209,24 @@ struct Packed {
 
 struct Jobs {
     PackArgs a{};
-    int count = 0;
-    void add(PackJob const &j) { a.job[count++] = j; }
+    int count = 0, deepest = 0;
+    void add(PackJob const &j)
+    {
+        a.job[count++] = j;
+        if (j.exponent && j.src.depth > deepest) { deepest = j.src.depth; }
+    }
     int run(hipStream_t st, char const *name) const
     {
         long long total = 0;
         for (int i = 0; i < count; ++i) { total += a.job[i].blocks; }
-        if (check_tiles(total, kPackBlock, name)) { return 1; }
-        launch(dense_pack_kernel, dim3((unsigned)total), dim3(kPackBlock), 0, st, a);
+        bool const wide = deepest > kPackHeld * 512;
+        if (check_tiles(total, wide ? 1024 : 512, name)) { return 1; }
+        if (wide) { launch(dense_pack_kernel<1024>, dim3((unsigned)total), dim3(1024), 0, st, a); }
+        else      { launch(dense_pack_kernel<512>, dim3((unsigned)total), dim3(512), 0, st, a); }
         BBHIP_LAUNCH_CHECK();
         return 0;
     }
 };
-
-float *sums_of(Carver &c, PackedShape const &s, int m, int n) { return s.slabs > 1 ? c.take<float>((size_t)s.slabs * m * (ceil_div(n, 64) * 64)) : nullptr; }
 
 int packed_product(PackedProduct &d, Product const &p, PackedShape const &s, Packed const &a, Packed const &b, float *sums, char const *name)
 {
@@ -177,63 +235,54 @@ int packed_product(PackedProduct &d, Product const &p, PackedShape const &s, Pac
     d.a = a.halves; d.ea = a.exponent; d.a_blocks = a.blocks;
     d.b = b.halves; d.eb = b.exponent; d.b_blocks = b.blocks; d.b_pieces = b.pieces;
     d.k_steps = s.k_steps; d.m_tiles = s.m_tiles; d.n_tiles = s.n_tiles; d.slabs = s.slabs; d.slab_stages = s.slab_stages;
-    if (check_tiles(s.workgroups(), s.large ? 512 : 256, name)) { return 1; }
+    if (check_tiles(s.workgroups(), kTileThreads[s.size], name)) { return 1; }
     d.workgroups = (int)s.workgroups();
-    d.sums = sums; d.sums_pitch = ceil_div(p.out.columns, 64) * 64; d.sums_slab = d.sums_pitch * p.out.rows;
+    d.sums = sums; d.sums_pitch = sums_pitch(p.out.columns); d.sums_slab = d.sums_pitch * p.out.rows;
     d.out = p.out;
+    d.out.line = nullptr;               // (summed where the halves are written)
     d.src_a = p.a; d.src_b = p.b; d.kind_a = p.again ? p.kind_a : -1; d.kind_b = p.kind_b;
     return 0;
 }
 
-// the sums of the products whose k axis workgroups share
-int packed_join(PackedProduct const &p, PackedProduct const &q, hipStream_t st, char const *name)
+int packed_run(PackedProduct const &p, int size, hipStream_t st, char const *name)
 {
-    auto const blocks = [](PackedProduct const &d) { return d.slabs > 1 ? ((long long)d.out.rows * d.sums_pitch + 255) / 256 : 0; };
-    long long const first = blocks(p), second = blocks(q);
-    if (first + second == 0) { return 0; }
-    if (check_tiles(first + second, 256, name)) { return 1; }
-    launch(dense_join_kernel, dim3((unsigned)(first + second)), dim3(256), 0, st, p, q, (unsigned)first);
-    BBHIP_LAUNCH_CHECK();
-    return 0;
-}
-
-int packed_run(PackedProduct const &p, bool large, hipStream_t st, char const *name)
-{
-    dim3 const grid((unsigned)p.workgroups), block(large ? 512 : 256);
-#define BBHIP_PACKED(USE)                                                                               \
+    dim3 const grid((unsigned)p.workgroups), block((unsigned)kTileThreads[size]);
+#define BBHIP_PACKED(USE, ...)                                                                          \
     do {                                                                                                \
-        if (large) {                                                                                    \
-            if (p.b_pieces == 1) { launch((dense_packed_kernel<USE, 4, 2, 4, 1, 4>), grid, block, 0, st, p); } \
-            else                 { launch((dense_packed_kernel<USE, 4, 2, 4, 2, 4>), grid, block, 0, st, p); } \
-        }                                                                                               \
-        else {                                                                                          \
-            if (p.b_pieces == 1) { launch((dense_packed_kernel<USE, 2, 2, 2, 1, 4>), grid, block, 0, st, p); } \
-            else                 { launch((dense_packed_kernel<USE, 2, 2, 2, 2, 4>), grid, block, 0, st, p); } \
-        }                                                                                               \
+        if (p.b_pieces == 1) { launch((dense_packed_kernel<USE, __VA_ARGS__, 1, kTileBuffers[size_]>), grid, block, 0, st, p); } \
+        else                 { launch((dense_packed_kernel<USE, __VA_ARGS__, 2, kTileBuffers[size_]>), grid, block, 0, st, p); } \
     } while (0)
-    if (p.out.kind == kOutLogits) { BBHIP_PACKED(kUseLogits); }
-    else                          { BBHIP_PACKED(kUseForward); }
+#define BBHIP_PACKED_SIZES(USE)                                                                         \
+    do {                                                                                                \
+        if (size == kTileLarge)       { constexpr int size_ = kTileLarge;  BBHIP_PACKED(USE, 4, 2, 4); } \
+        else if (size == kTileMiddle) { constexpr int size_ = kTileMiddle; BBHIP_PACKED(USE, 4, 2, 2); } \
+        else                          { constexpr int size_ = kTileSmall;  BBHIP_PACKED(USE, 2, 2, 2); } \
+    } while (0)
+    if (p.out.kind == kOutLogits) { BBHIP_PACKED_SIZES(kUseLogits); }
+    else                          { BBHIP_PACKED_SIZES(kUseForward); }
+#undef BBHIP_PACKED_SIZES
 #undef BBHIP_PACKED
     BBHIP_LAUNCH_CHECK();
-    return packed_join(p, PackedProduct{}, st, name);
+    return join(p, PackedProduct{}, st, name);
 }
 
 // p and behind it q, whose operands are not packed bits
-int packed_run(PackedProduct const &p, PackedProduct const &q, bool large, hipStream_t st, char const *name)
+int packed_run(PackedProduct const &p, PackedProduct const &q, int size, hipStream_t st, char const *name)
 {
-    if (check_tiles((long long)p.workgroups + q.workgroups, large ? 512 : 256, name)) { return 1; }
+    if (check_tiles((long long)p.workgroups + q.workgroups, kTileThreads[size], name)) { return 1; }
     if (p.workgroups + q.workgroups == 0) { return 0; }
-    dim3 const grid((unsigned)(p.workgroups + q.workgroups)), block(large ? 512 : 256);
-    if (large) {
-        if (p.b_pieces == 1) { launch((dense_packed_pair_kernel<4, 2, 4, 1, 4>), grid, block, 0, st, p, q); }
-        else                 { launch((dense_packed_pair_kernel<4, 2, 4, 2, 4>), grid, block, 0, st, p, q); }
-    }
-    else {
-        if (p.b_pieces == 1) { launch((dense_packed_pair_kernel<2, 2, 2, 1, 4>), grid, block, 0, st, p, q); }
-        else                 { launch((dense_packed_pair_kernel<2, 2, 2, 2, 4>), grid, block, 0, st, p, q); }
-    }
+    dim3 const grid((unsigned)(p.workgroups + q.workgroups)), block((unsigned)kTileThreads[size]);
+#define BBHIP_PACKED(...)                                                                               \
+    do {                                                                                                \
+        if (p.b_pieces == 1) { launch((dense_packed_pair_kernel<__VA_ARGS__, 1, kTileBuffers[size_]>), grid, block, 0, st, p, q); } \
+        else                 { launch((dense_packed_pair_kernel<__VA_ARGS__, 2, kTileBuffers[size_]>), grid, block, 0, st, p, q); } \
+    } while (0)
+    if (size == kTileLarge)       { constexpr int size_ = kTileLarge;  BBHIP_PACKED(4, 2, 4); }
+    else if (size == kTileMiddle) { constexpr int size_ = kTileMiddle; BBHIP_PACKED(4, 2, 2); }
+    else                          { constexpr int size_ = kTileSmall;  BBHIP_PACKED(2, 2, 2); }
+#undef BBHIP_PACKED
     BBHIP_LAUNCH_CHECK();
-    return packed_join(p, q, st, name);
+    return join(p, q, st, name);
 }
 
 // of a layer's forward pass
@@ -242,7 +291,7 @@ struct ForwardSpace {
     Packed W, x;
     float *sums;
     ForwardSpace(Carver &c, int inputs, int outputs, int frames, bool bit)
-        : shape(best_shape(outputs, frames, inputs)), W(c, outputs, inputs, false), x(c, frames, inputs, bit), sums(sums_of(c, shape, outputs, frames)) {}
+        : shape(best_shape(outputs, frames, inputs)), W(c, outputs, inputs, false), x(c, frames, inputs, bit), sums(sums_of(c, shape.slabs, outputs, frames)) {}
 };
 
 // of its backward pass
@@ -257,14 +306,14 @@ struct BackwardSpace {
         x = Packed(c, inputs, frames, bit);
         W = Packed(c, inputs, outputs, false);
         dz_columns = Packed(c, frames, outputs, false);
-        dw_sums = sums_of(c, dw, outputs, inputs);
-        dx_sums = sums_of(c, dx, inputs, frames);
+        dw_sums = sums_of(c, dw.slabs, outputs, inputs);
+        dx_sums = sums_of(c, dx.slabs, inputs, frames);
     }
     // the last piece of a loss, of fewer channels: the same places, the same divisions of the k axis or fewer
     void cut(int inputs, int outputs, int frames)
     {
-        dw = packed_shape(dw.large, dw.slabs, outputs, inputs, frames);
-        dx = packed_shape(dx.large, dx.slabs, inputs, frames, outputs);
+        dw = packed_shape(dw.size, dw.slabs, outputs, inputs, frames);
+        dx = packed_shape(dx.size, dx.slabs, inputs, frames, outputs);
         dz_rows.blocks = ceil_div(outputs, 32);
         W.steps = dz_columns.steps = pack_steps(outputs);
     }
@@ -283,12 +332,9 @@ struct BackwardSpace {
     {
         PackedProduct p, q;
         if (packed_product(p, w, dw, dz_rows, x, dw_sums, name) || packed_product(q, i, dx, W, dz_columns, dx_sums, name)) { return 1; }
-        return packed_run(p, q, dw.large, st, name);
+        return packed_run(p, q, dw.size, st, name);
     }
 };
-
-// dz of a small backward pass
-float *small_dz(Carver &c, int outputs, int frames) { return c.take<float>((size_t)outputs * (ceil_div(frames, 64) * 64)); }
 
 // ---- what an entry checks ----
 int check_sizes(int inputs, int outputs, int frames, char const *name)
@@ -337,11 +383,17 @@ int dense_forward(void const *x, bool bit, void *y, bool bit_out, float const *W
     p.out.rows = outputs; p.out.columns = frames; p.out.out = y; p.out.stride = y_stride;
     p.out.bias = b; p.out.residual = residual; p.out.residual_stride = residual_stride; p.out.activation = activation;
     hipStream_t const st = static_cast<hipStream_t>(stream);
-    if (!product_packed(outputs, frames, inputs)) {
-        ScopedTimer tm(kTimeOther, st);
-        return direct_forward(p, bit, st, name);
-    }
     Carver c{static_cast<char *>(workspace)};
+    if (few_frames(p)) {
+        ScopedTimer tm(kTimeOther, st);
+        return few_frames_forward(p, bit, st, name);
+    }
+    if (!product_packed(outputs, frames, inputs)) {
+        float *const sums = sums_of(c, direct_shape(outputs, frames, inputs).slabs, outputs, frames);
+        if (check_workspace(workspace, workspace_size, c.at, name)) { return 1; }
+        ScopedTimer tm(kTimeOther, st);
+        return direct_forward(p, bit, sums, st, name);
+    }
     ForwardSpace const s(c, inputs, outputs, frames, bit);
     if (check_workspace(workspace, workspace_size, c.at, name)) { return 1; }
     ScopedTimer tm(kTimeOther, st);
@@ -349,7 +401,7 @@ int dense_forward(void const *x, bool bit, void *y, bool bit_out, float const *W
     jobs.add(s.W.job(p.a, p.kind_a));
     jobs.add(s.x.job(p.b, p.kind_b));
     PackedProduct d;
-    return jobs.run(st, name) || packed_product(d, p, s.shape, s.W, s.x, s.sums, name) || packed_run(d, s.shape.large, st, name);
+    return jobs.run(st, name) || packed_product(d, p, s.shape, s.W, s.x, s.sums, name) || packed_run(d, s.shape.size, st, name);
 }
 
 int dense_backward(void const *x, bool bit, float const *dy, float const *y, float const *W, float *dx, float *dW, float *db, float *dr, int activation,
@@ -390,18 +442,19 @@ int dense_backward(void const *x, bool bit, float const *dy, float const *y, flo
         return jobs.run(st, name) || s.run(w, i, st, name);
     }
     Carver c{static_cast<char *>(workspace)};
-    float *dz = small_dz(c, outputs, frames);
-    if (dr || activation == kActNone) { dz = dr; }
-    else if (check_workspace(workspace, workspace_size, c.at, name)) { return 1; }
+    bool const own = !dr && activation != kActNone;
+    DirectBackwardSpace const d(c, inputs, outputs, frames, own);
+    if (check_workspace(workspace, workspace_size, c.at, name)) { return 1; }
     ScopedTimer tm(kTimeOther, st);
-    return direct_backward(w, i, dz, dr ? stride : ceil_div(frames, 64) * 64, bit, st, name);
+    return direct_backward(w, i, d, own ? d.dz : dr, own ? ceil_div(frames, 64) * 64 : stride, bit, st, name);
 }
 
 // ---- the loss on top of a dense layer ----
 struct LossSpace {
     LossPlan plan;
     float2 *partial;
-    float *label_logit, *top = nullptr, *share = nullptr, *coef = nullptr, *logits = nullptr;
+    float *label_logit, *top = nullptr, *share = nullptr, *coef = nullptr, *logits = nullptr, *logit_sums = nullptr;
+    char *direct_space = nullptr;       // not packed: of a piece's gradients
     Packed W, x;                        // packed: of a piece's logits
     alignas(BackwardSpace) char backward_space[sizeof(BackwardSpace)];
     size_t total;
@@ -420,7 +473,22 @@ struct LossSpace {
         if (plan.packed) {
             W = Packed(c, plan.piece, inputs, false);
             x = Packed(c, frames, inputs, bit);
+            logit_sums = sums_of(c, plan.logits.slabs, plan.piece, frames);
             if (gradients) { new (backward_space) BackwardSpace(c, inputs, plan.piece, frames, bit); }
+        }
+        else {
+            // (the last piece, of fewer channels, may be divided otherwise)
+            int const last = channels - (channels - 1) / plan.piece * plan.piece;
+            size_t most = 0, most_sums = 0;
+            for (int count : {plan.piece, last}) {
+                Carver d{nullptr}, e{nullptr};
+                DirectBackwardSpace const space(d, inputs, count, frames, false);
+                sums_of(e, direct_shape(count, frames, inputs).slabs, count, frames);
+                most = d.at > most ? d.at : most;
+                most_sums = e.at > most_sums ? e.at : most_sums;
+            }
+            logit_sums = c.take<float>(most_sums / sizeof(float));
+            if (gradients) { direct_space = c.take<char>(most); }
         }
         total = c.at;
     }
@@ -453,15 +521,15 @@ int dense_loss(void const *x, bool bit, float const *W, float const *b, int cons
         p.out.bias = b ? b + first : nullptr;
         p.out.partial = s.partial + (size_t)(first / s.plan.tile) * frames;
         p.out.label = label; p.out.label_logit = s.label_logit; p.out.first_channel = first;
-        if (!s.plan.packed) { return direct_forward(p, bit, st, name); }
+        if (!s.plan.packed) { return direct_forward(p, bit, s.logit_sums, st, name); }
         Jobs jobs;
         jobs.add(s.W.job(p.a, kRows));
         if (!x_packed) { jobs.add(s.x.job(p.b, bit ? kBitColumns : kColumns)); x_packed = true; }
-        PackedShape const shape = packed_shape(s.plan.logits.large, 1, count, frames, inputs);
+        PackedShape const shape = packed_shape(s.plan.logits.size, s.plan.logits.slabs, count, frames, inputs);
         PackedProduct d;
         Packed W_piece = s.W;
         W_piece.blocks = ceil_div(count, 32);
-        return (int)(jobs.run(st, name) || packed_product(d, p, shape, W_piece, s.x, nullptr, name) || packed_run(d, shape.large, st, name));
+        return (int)(jobs.run(st, name) || packed_product(d, p, shape, W_piece, s.x, s.logit_sums, name) || packed_run(d, shape.size, st, name));
     };
     // the pieces' largest logits and sums; the last piece's logits stay for its gradient
     for (int piece = 0; piece < pieces; ++piece) { if (logit_piece(piece, gradients && piece == pieces - 1)) { return 1; } }
@@ -497,7 +565,9 @@ int dense_loss(void const *x, bool bit, float const *W, float const *b, int cons
         i.out.kind = kOutStore; i.out.rows = inputs; i.out.columns = frames; i.out.out = dx; i.out.stride = dx_stride; i.out.accumulate = piece != pieces - 1;
         if (!s.plan.packed) {
             // (in the place of the logits)
-            if (direct_backward(w, i, logits, s.plan.stride, bit, st, name)) { return 1; }
+            Carver c{s.direct_space};
+            DirectBackwardSpace const d(c, inputs, count, frames, false);
+            if (direct_backward(w, i, d, logits, s.plan.stride, bit, st, name)) { return 1; }
             continue;
         }
         Jobs jobs;
@@ -533,8 +603,9 @@ size_t bbhip_DenseAffine_WorkspaceBytes(int input_node_size, int output_node_siz
     if (check_sizes(input_node_size, output_node_size, frame_size, __func__)) { return 0; }
     Carver forward{nullptr}, backward{nullptr};
     if (!product_packed(output_node_size, frame_size, input_node_size)) {
-        small_dz(backward, output_node_size, frame_size);
-        return backward.at;
+        sums_of(forward, direct_shape(output_node_size, frame_size, input_node_size).slabs, output_node_size, frame_size);
+        DirectBackwardSpace const d(backward, input_node_size, output_node_size, frame_size, true);
+        return forward.at > backward.at ? forward.at : backward.at;
     }
     ForwardSpace const f(forward, input_node_size, output_node_size, frame_size, false);
     BackwardSpace const b(backward, input_node_size, output_node_size, frame_size, false);

@@ -4,7 +4,9 @@
 // v_mfma_f32_32x32x2_f32 takes one value per lane and operand: lane l holds row l & 31 at the k of its half, l >> 5, so a lane loads 16 consecutive k of one row
 // (64 bytes where these are neighbours in memory, 16 times 128 bytes of a half wavefront where rows are) and the 16 instructions of a chunk each take one of them:
 // which k meets which in an instruction does not matter as long as both operands agree.  Every product and sum is fp32; no operand is written anywhere.
-// One launch, and what it costs is the latency of a chunk's loads and 16 x 64 cycles of matrix instructions per chunk and wavefront.
+// What a launch costs is the latency of a chunk's loads and 16 x 64 cycles of matrix instructions per chunk and wavefront; other wavefronts cover the latency (with the next chunk
+// held in registers sixteen wavefronts do not fit a compute unit without spilling).  Where there are few tiles and a long k axis several workgroups share it (slabs), and dense_join_kernel
+// adds their sums in order.
 //
 // dense_few_frames_kernel: up to eight frames, where a tile of 32 would be mostly empty and the weights are all there is to read.  A wavefront owns an output node and
 // walks its row of W 1 KiB at a time, the frames lie in LDS.
@@ -23,6 +25,10 @@ struct DirectProduct {
     DenseOutput out;
     int n_tiles;                    // tiles side by side
     int tiles;
+    int slabs, slab_chunks;         // workgroups that share a tile's k axis
+    float *sums;                    // slabs > 1: [slab][m][pitch]
+    long long sums_pitch, sums_slab;
+    __host__ __device__ int workgroups(void) const { return tiles * slabs; }
 };
 
 // What a lane loads of an operand for a chunk, as it comes from memory: a loop holds the next chunk's while the present one's is multiplied, so nothing is computed of it before.
@@ -82,28 +88,25 @@ struct RawRun {
 };
 
 template <int KA, int KB, int WAVES>
-__device__ __forceinline__ void direct_product(DirectProduct const &t, int tile, float *lds)
+__device__ __forceinline__ void direct_product(DirectProduct const &t, int id, float *lds)
 {
+    int const slab = id / t.tiles, tile = id - slab * t.tiles;
     int const m0 = tile / t.n_tiles * kDirectTile, n0 = (tile % t.n_tiles) * kDirectTile;
     int const lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int const r = lane & 31, half = lane >> 5;
     // (rows behind the last one read the last one: their elements are not stored; so does the row of ones)
     int const row_a = min(m0 + r, t.a.rows - 1), row_b = min(n0 + r, t.b.rows - 1);
     bool const ones = n0 + r == t.b.ones;
-    int const chunks = (t.a.depth + kDirectChunk - 1) / kDirectChunk;
+    int const first = slab * t.slab_chunks, chunks = min(first + t.slab_chunks, (t.a.depth + kDirectChunk - 1) / kDirectChunk);
     DenseAcc acc = {};
-    RawRun<KA> a, an;
-    RawRun<KB> b, bn;
-    auto const fetch = [&](RawRun<KA> &u, RawRun<KB> &v, int c) {
-        bool const whole = (c + 1) * kDirectChunk <= t.a.depth;
-        u.load(t.a, row_a, c * kDirectChunk + half * kDirectRun, whole);
-        v.load(t.b, row_b, c * kDirectChunk + half * kDirectRun, whole);
-    };
-    if (wave < chunks) { fetch(a, b, wave); }
-    for (int c = wave; c < chunks; c += WAVES) {
+#pragma nounroll
+    for (int c = first + wave; c < chunks; c += WAVES) {
+        RawRun<KA> a;
+        RawRun<KB> b;
         bool const whole = (c + 1) * kDirectChunk <= t.a.depth;
         int const k = c * kDirectChunk + half * kDirectRun;
-        if (c + WAVES < chunks) { fetch(an, bn, c + WAVES); }
+        a.load(t.a, row_a, k, whole);
+        b.load(t.b, row_b, k, whole);
         if (whole) {
 #pragma unroll
             for (int j = 0; j < kDirectRun; ++j) {
@@ -116,7 +119,6 @@ __device__ __forceinline__ void direct_product(DirectProduct const &t, int tile,
                 acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a.value(t.a, row_a, k, j, false, false), b.value(t.b, row_b, k, j, false, ones), acc, 0, 0, 0);
             }
         }
-        a = an; b = bn;
     }
 #pragma unroll
     for (int j = 0; j < 16; ++j) { lds[(wave * 16 + j) * 64 + lane] = acc[j]; }
@@ -125,15 +127,19 @@ __device__ __forceinline__ void direct_product(DirectProduct const &t, int tile,
     DenseOutput const &o = t.out;
     constexpr int kPer = 16 / WAVES;
     float z[kPer];
+    int const n = n0 + r;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
         int const reg = e * WAVES + wave;
         float d = 0.0f;
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) { d += lds[(w * 16 + reg) * 64 + lane]; }
-        int const m = m0 + acc_row(reg, lane), n = n0 + r;
+        int const m = m0 + acc_row(reg, lane);
         bool const inside = m < o.rows && n < o.columns;
-        if (o.kind == kOutForward) {
+        if (t.slabs > 1) {
+            if (m < o.rows && (n < o.columns || (n == o.columns && o.line))) { t.sums[slab * t.sums_slab + m * t.sums_pitch + n] = d; }
+        }
+        else if (o.kind == kOutForward) {
             if (inside) { static_cast<float *>(o.out)[m * o.stride + n] = activated(before_activation(o, d, m, n), o.activation); }
         }
         else if (o.kind == kOutBits) {
@@ -144,28 +150,29 @@ __device__ __forceinline__ void direct_product(DirectProduct const &t, int tile,
             if (m < o.rows && (n < o.columns || (n == o.columns && o.line))) { store_element(o, d, m, n); }
         }
         else {
-            z[e] = inside ? before_activation(o, d, m, n) : 0.0f;
+            z[e] = inside ? before_activation(o, d, m, n) : -INFINITY;
             if (inside) {
                 if (o.out) { static_cast<float *>(o.out)[m * o.stride + n] = z[e]; }
                 if (o.label[n] == m + o.first_channel) { o.label_logit[n] = z[e]; }
             }
         }
     }
-    if (o.kind == kOutLogits) {
-        __syncthreads();
+    if (o.kind == kOutLogits && t.slabs == 1) {
+        // (largest, sum of exponents) of the tile's rows: of this lane's, the other half's, the other wavefronts'
+        float2 s = make_float2(-INFINITY, 0.0f);
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) { lds[(e * WAVES + wave) * 64 + lane] = z[e]; }
+        for (int e = 0; e < kPer; ++e) { s.x = fmaxf(s.x, z[e]); }
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) { s.y += z[e] == -INFINITY ? 0.0f : exp_of_nonpositive(z[e] - s.x); }
+        s = joined(s, make_float2(__shfl_xor(s.x, 32), __shfl_xor(s.y, 32)));
         __syncthreads();
-        int const n = n0 + r;
+        float2 *const part = reinterpret_cast<float2 *>(lds);
+        if (half == 0) { part[wave * 32 + r] = s; }
+        __syncthreads();
         if (threadIdx.x < 32 && n < o.columns) {
-            int const rows = min(kDirectTile, o.rows - m0);
-            float top = -INFINITY, sum = 0.0f;
-            for (int i = 0; i < rows; ++i) { top = fmaxf(top, lds[((i & 3) + 4 * (i >> 3)) * 64 + ((i >> 2) & 1) * 32 + r]); }
-            for (int i = 0; i < rows; ++i) {
-                float const v = lds[((i & 3) + 4 * (i >> 3)) * 64 + ((i >> 2) & 1) * 32 + r];
-                sum += v == -INFINITY ? 0.0f : exp_of_nonpositive(v - top);
-            }
-            o.partial[(long long)(m0 / kDirectTile) * o.columns + n] = make_float2(top, sum);
+#pragma unroll
+            for (int w = 1; w < WAVES; ++w) { s = joined(s, part[w * 32 + r]); }
+            o.partial[(long long)(m0 / kDirectTile) * o.columns + n] = s;
         }
     }
 }
@@ -182,8 +189,8 @@ template <int KX, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void dense_direct_backward_kernel(DirectProduct dw, DirectProduct dx)
 {
     __shared__ float lds[WAVES * 16 * 64];
-    if ((int)blockIdx.x < dw.tiles) { direct_product<kRows, KX, WAVES>(dw, blockIdx.x, lds); }
-    else                            { direct_product<kColumns, kColumns, WAVES>(dx, blockIdx.x - dw.tiles, lds); }
+    if ((int)blockIdx.x < dw.workgroups()) { direct_product<kRows, KX, WAVES>(dw, blockIdx.x, lds); }
+    else                            { direct_product<kColumns, kColumns, WAVES>(dx, blockIdx.x - dw.workgroups(), lds); }
 }
 
 // dz of a call, written: 1024 elements of a row per workgroup, units of a row dealt out by a flat list
@@ -201,29 +208,19 @@ __global__ __launch_bounds__(256) void dense_dz_kernel(DzArgs a)
 // ---- up to eight frames ---------------------------------------------------------------------------------------------------------------------
 constexpr int kFewFrames = 8, kFewWaves = 4, kFewPiece = 1024;             // values of k in LDS at a time
 
-// p.b: columns or packed bits.  A wavefront owns one row of p.a: lane l takes four values of every 256.
-template <int KB, int FRAMES>
+// t.b: columns or packed bits.  A wavefront owns ROWS rows of t.a: what it reads of the frames in LDS serves all of them, and so does what the workgroup reads of the frames, whose values lie
+// a row pitch apart.  VEC: lane l takes four neighbouring values of every 256, with one load; else four that lie 64 apart.
+template <int KB, int FRAMES, int ROWS, bool VEC>
 __global__ __launch_bounds__(kFewWaves * 64) void dense_few_frames_kernel(DirectProduct t)
 {
     __shared__ __attribute__((aligned(16))) float x[FRAMES][kFewPiece];
-    int const lane = threadIdx.x & 63, m = blockIdx.x * kFewWaves + (threadIdx.x >> 6);
+    int const lane = threadIdx.x & 63, m0 = (blockIdx.x * kFewWaves + (threadIdx.x >> 6)) * ROWS;
     Operand const &a = t.a, &b = t.b;
-    float const *w = static_cast<float const *>(a.p) + min(m, a.rows - 1) * a.stride;
     int const frames = min(FRAMES, b.rows);
-    float acc[FRAMES] = {};
+    float acc[ROWS][FRAMES] = {};
     for (int k0 = 0; k0 < a.depth; k0 += kFewPiece) {
         int const here = min(kFewPiece, a.depth - k0);
         if (k0) { __syncthreads(); }
-        float v[kFewPiece / 256][4];
-#pragma unroll
-        for (int i = 0; i < kFewPiece / 256; ++i) {
-            int const k = k0 + i * 256 + lane * 4;
-            if (a.vec && k + 4 <= a.depth) { load_floats(w + k, true, v[i]); }
-            else {
-#pragma unroll
-                for (int q = 0; q < 4; ++q) { v[i][q] = k + q < a.depth ? w[k + q] : 0.0f; }
-            }
-        }
         for (int i = threadIdx.x; i < kFewPiece; i += kFewWaves * 64) {
             if constexpr (KB == kBitColumns) {
                 uint32_t const bits = i < here ? static_cast<uint32_t const *>(b.p)[(k0 + i) * b.stride] : 0u;
@@ -236,34 +233,53 @@ __global__ __launch_bounds__(kFewWaves * 64) void dense_few_frames_kernel(Direct
             }
         }
         __syncthreads();
+        for (int i = 0; i < here; i += 256) {
+            float v[ROWS][4];
 #pragma unroll
-        for (int i = 0; i < kFewPiece / 256; ++i) {
-            if (i * 256 >= here) { continue; }
+            for (int q = 0; q < ROWS; ++q) {
+                float const *w = static_cast<float const *>(a.p) + min(m0 + q, a.rows - 1) * a.stride + k0 + i;
+                if (VEC && i + lane * 4 + 4 <= here) { load_floats(w + lane * 4, true, v[q]); }
+                else {
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) { int const at = VEC ? lane * 4 + u : u * 64 + lane; v[q][u] = i + at < here ? w[at] : 0.0f; }
+                }
+            }
 #pragma unroll
             for (int f = 0; f < FRAMES; ++f) {
                 float u[4];
-                load_floats(&x[f][i * 256 + lane * 4], true, u);
+                if (VEC) { load_floats(&x[f][i + lane * 4], true, u); }
+                else {
 #pragma unroll
-                for (int q = 0; q < 4; ++q) { acc[f] = fmaf(v[i][q], u[q], acc[f]); }
+                    for (int h = 0; h < 4; ++h) { u[h] = x[f][i + h * 64 + lane]; }
+                }
+#pragma unroll
+                for (int q = 0; q < ROWS; ++q) {
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) { acc[q][f] = fmaf(v[q][h], u[h], acc[q][f]); }
+                }
             }
         }
     }
-#pragma unroll
-    for (int f = 0; f < FRAMES; ++f) {
-#pragma unroll
-        for (int step = 32; step > 0; step /= 2) { acc[f] += __shfl_xor(acc[f], step); }
-    }
-    // lane f finishes frame f
-    float d = acc[0];
-#pragma unroll
-    for (int f = 1; f < FRAMES; ++f) { d = lane == f ? acc[f] : d; }
     DenseOutput const &o = t.out;
-    bool const inside = m < o.rows && lane < o.columns && lane < FRAMES;
-    if (o.kind == kOutBits) {
-        uint64_t const bits = __ballot(inside && before_activation(o, d, inside ? m : 0, inside ? lane : 0) > 0.0f);
-        if (lane == 0 && m < o.rows) { static_cast<uint32_t *>(o.out)[m * o.stride] = (uint32_t)bits; }
+#pragma unroll
+    for (int q = 0; q < ROWS; ++q) {
+        int const m = m0 + q;
+#pragma unroll
+        for (int f = 0; f < FRAMES; ++f) {
+#pragma unroll
+            for (int step = 32; step > 0; step /= 2) { acc[q][f] += __shfl_xor(acc[q][f], step); }
+        }
+        // lane f finishes frame f
+        float d = acc[q][0];
+#pragma unroll
+        for (int f = 1; f < FRAMES; ++f) { d = lane == f ? acc[q][f] : d; }
+        bool const inside = m < o.rows && lane < o.columns && lane < FRAMES;
+        if (o.kind == kOutBits) {
+            uint64_t const bits = __ballot(inside && before_activation(o, d, inside ? m : 0, inside ? lane : 0) > 0.0f);
+            if (lane == 0 && m < o.rows) { static_cast<uint32_t *>(o.out)[m * o.stride] = (uint32_t)bits; }
+        }
+        else if (inside) { static_cast<float *>(o.out)[m * o.stride + lane] = activated(before_activation(o, d, m, lane), o.activation); }
     }
-    else if (inside) { static_cast<float *>(o.out)[m * o.stride + lane] = activated(before_activation(o, d, m, lane), o.activation); }
 }
 
 }  // namespace bbhip

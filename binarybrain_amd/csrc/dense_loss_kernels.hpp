@@ -9,7 +9,7 @@
 
 namespace bbhip {
 
-constexpr int kFinishFrames = 32, kFinishGroups = 16;
+constexpr int kFinishFrames = 8, kFinishGroups = 64;
 
 struct LossFinishArgs {
     float2 const *partial;          // [tiles][frames]
@@ -22,7 +22,7 @@ struct LossFinishArgs {
     int    tiles, frames, channels;
 };
 
-// 32 frames per workgroup; sixteen threads of a frame take its tiles in turn (neighbouring lanes neighbouring frames) and are joined through LDS in a fixed order
+// Eight frames per workgroup; 64 threads of a frame take its tiles in turn (neighbouring lanes neighbouring frames) and are joined two by two through LDS
 __global__ __launch_bounds__(kFinishFrames * kFinishGroups) void dense_loss_finish_kernel(LossFinishArgs a)
 {
     __shared__ float2 part[kFinishGroups][kFinishFrames];
@@ -32,9 +32,11 @@ __global__ __launch_bounds__(kFinishFrames * kFinishGroups) void dense_loss_fini
         for (int t = group; t < a.tiles; t += kFinishGroups) { s = joined(s, a.partial[(long long)t * a.frames + f]); }
     }
     part[group][at] = s;
-    __syncthreads();
+    for (int step = kFinishGroups / 2; step > 0; step /= 2) {
+        __syncthreads();
+        if (group < step) { s = joined(s, part[group + step][at]); part[group][at] = s; }
+    }
     if (group != 0 || f >= a.frames) { return; }
-    for (int g = 1; g < kFinishGroups; ++g) { s = joined(s, part[g][at]); }
     int const label = a.label[f];
     float const w = a.weight ? a.weight[f] : 1.0f;
     bool const counts = label >= 0 && label < a.channels && w != 0.0f;

@@ -20,7 +20,7 @@ namespace bbhip {
 typedef _Float16 DenseHalf8 __attribute__((ext_vector_type(8)));
 typedef float    DenseAcc16 __attribute__((ext_vector_type(16)));
 
-constexpr int kPackBlock = 512, kPackRows = 8;
+constexpr int kPackRows = 8;
 constexpr int kPackHeld = 8;                    // groups of eight values that a thread keeps between finding the largest and splitting
 
 struct PackJob {
@@ -59,10 +59,10 @@ __device__ __forceinline__ float magnitude(float v) { float const a = fabsf(v); 
 // Eight rows and all their k per workgroup: what it writes are whole lines of 128 bytes (eight rows' 16), and with 64 groups of eight k side by side a thread holds all values of a row of up to 4096
 // between finding the largest and splitting.  Where rows are columns of the buffer it reads 32 bytes at a time; workgroups that share a line run on one XCD (xcd_run).  With 32 rows per
 // workgroup a batch of 65 frames of 6144 bits and as many weights took 30 us.
-template <int KIND>
+template <int KIND, int THREADS>
 __device__ __forceinline__ void pack_rows(PackJob const &j, int block, float *share)
 {
-    constexpr int ROWS = kPackRows, kOctets = kPackBlock / ROWS;      // side by side
+    constexpr int ROWS = kPackRows, kOctets = THREADS / ROWS;      // side by side
     constexpr bool kBits = KIND == kBitRows || KIND == kBitColumns;
     constexpr int kPieces = kBits ? 1 : 2;
     int const at = threadIdx.x % ROWS, octet0 = threadIdx.x / ROWS, row = block * ROWS + at;
@@ -93,7 +93,7 @@ __device__ __forceinline__ void pack_rows(PackJob const &j, int block, float *sh
         // over the threads of a row: within the wavefront, then through LDS in a fixed order
 #pragma unroll
         for (int step = ROWS; step < 64; step *= 2) { top = fmaxf(top, __shfl_xor(top, step)); sum += __shfl_xor(sum, step); }
-        constexpr int kWaves = kPackBlock / 64;
+        constexpr int kWaves = THREADS / 64;
         int const wave = threadIdx.x / 64;
         if ((threadIdx.x & 63) < ROWS) { share[wave * ROWS + at] = top; share[(kWaves + wave) * ROWS + at] = sum; }
         __syncthreads();
@@ -137,33 +137,39 @@ __device__ __forceinline__ void pack_rows(PackJob const &j, int block, float *sh
             }
         }
     };
-    int const from = kBits ? 0 : kPackHeld;
     if (!kBits) {
 #pragma unroll
         for (int u = 0; u < kPackHeld; ++u) { if (octet0 + u * kOctets < octets) { write(octet0 + u * kOctets, held[u]); } }
     }
-    for (int i = from; octet0 + i * kOctets < octets; ++i) {
-        int const o = octet0 + i * kOctets;
-        float v[8] = {};
-        if (there && o * 8 < j.src.depth) { load_values<KIND, 8>(j.src, row, o * 8, v); }
-        write(o, v);
+    // what is not held (packed bits: four groups asked for at a time, which are few registers)
+    constexpr int kAtATime = kBits ? 4 : 1;
+    for (int i = kBits ? 0 : kPackHeld; octet0 + i * kOctets < octets; i += kAtATime) {
+        float v[kAtATime][8] = {};
+#pragma unroll
+        for (int u = 0; u < kAtATime; ++u) {
+            int const o = octet0 + (i + u) * kOctets;
+            if (there && o * 8 < j.src.depth) { load_values<KIND, 8>(j.src, row, o * 8, v[u]); }
+        }
+#pragma unroll
+        for (int u = 0; u < kAtATime; ++u) { if (octet0 + (i + u) * kOctets < octets) { write(octet0 + (i + u) * kOctets, v[u]); } }
     }
 }
 
-__global__ __launch_bounds__(kPackBlock) void dense_pack_kernel(PackArgs a)
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void dense_pack_kernel(PackArgs a)
 {
-    __shared__ float share[2 * kPackBlock / 64 * kPackRows];
+    __shared__ float share[2 * THREADS / 64 * kPackRows];
     int block = blockIdx.x, which = 0;
     while (block >= a.job[which].blocks) { block -= a.job[which].blocks; ++which; }
     PackJob const &j = a.job[which];
     block = xcd_run(block, j.blocks);
     switch (j.kind) {
-    case kRows:       pack_rows<kRows>(j, block, share); break;
-    case kColumns:    pack_rows<kColumns>(j, block, share); break;
-    case kBitRows:    pack_rows<kBitRows>(j, block, share); break;
-    case kBitColumns: pack_rows<kBitColumns>(j, block, share); break;
-    case kGradRows:   pack_rows<kGradRows>(j, block, share); break;
-    default:          pack_rows<kGradColumns>(j, block, share); break;
+    case kRows:       pack_rows<kRows, THREADS>(j, block, share); break;
+    case kColumns:    pack_rows<kColumns, THREADS>(j, block, share); break;
+    case kBitRows:    pack_rows<kBitRows, THREADS>(j, block, share); break;
+    case kBitColumns: pack_rows<kBitColumns, THREADS>(j, block, share); break;
+    case kGradRows:   pack_rows<kGradRows, THREADS>(j, block, share); break;
+    default:          pack_rows<kGradColumns, THREADS>(j, block, share); break;
     }
 }
 
@@ -279,8 +285,9 @@ template <int USE, int TM, int WM, int WN, int PB, int BUFFERS>
 __device__ __forceinline__ void packed_tile(PackedProduct const &p, int id, char *lds, int *scales, float *bias)
 {
     constexpr int TN = 2, kWaves = WM * WN, kBM = TM * WM, kBN = TN * WN;           // blocks of 32 rows
-    static_assert(kBM == kWaves && kBN == kWaves, "each wavefront loads one row block of either operand");
-    constexpr int kStageA = kBM * 2048, kStage = kStageA + kBN * 1024 * PB, kLoads = 2 + PB, kAhead = BUFFERS - 1;
+    constexpr int kOwn = kBM / kWaves;              // row blocks of a that a wavefront loads; of b it loads one
+    static_assert(kBM == kWaves * kOwn && kBN == kWaves, "the wavefronts share the loads evenly");
+    constexpr int kStageA = kBM * 2048, kStage = kStageA + kBN * 1024 * PB, kLoads = 2 * kOwn + PB, kAhead = BUFFERS - 1;
     int const lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int const tiles = p.m_tiles * p.n_tiles;
     int const slab = id / tiles;
@@ -292,19 +299,26 @@ __device__ __forceinline__ void packed_tile(PackedProduct const &p, int id, char
     int const first = slab * p.slab_stages, stages = min(p.slab_stages, p.k_steps - first);
 
     // a stage is 16 k: of each row block two (packed bits: one) blocks of 1 KiB, which a wavefront moves to LDS as they are
-    char const *from_a = reinterpret_cast<char const *>(p.a) + ((long long)min(rb_a + wave, p.a_blocks - 1) * p.k_steps + first) * 2048;
+    char const *from_a[kOwn];
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) { from_a[i] = reinterpret_cast<char const *>(p.a) + ((long long)min(rb_a + wave * kOwn + i, p.a_blocks - 1) * p.k_steps + first) * 2048; }
     char const *from_b = reinterpret_cast<char const *>(p.b) + ((long long)min(rb_b + wave, p.b_blocks - 1) * p.k_steps + first) * (1024 * PB);
     uint32_t const at_lds = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds);
     auto const fetch = [&](int buffer) {
         // (as assembly: the compiler would wait for all of them ahead of every read of LDS, whichever buffer it reads.  Each lane's sixteen bytes go to M0 + offset + 16 lane.)
-        uint32_t const to_a = at_lds + buffer * kStage + wave * 2048, to_b = at_lds + buffer * kStage + kStageA + wave * 1024 * PB;
-        char const *const a = from_a + lane * 16, *const b = from_b + lane * 16;
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\tglobal_load_lds_dwordx4 %1, off offset:1024" :: "s"(to_a), "v"(a) : "memory", "m0");
+        uint32_t const to_a = at_lds + buffer * kStage + wave * kOwn * 2048, to_b = at_lds + buffer * kStage + kStageA + wave * 1024 * PB;
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i) {
+            char const *const a = from_a[i] + lane * 16;
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\tglobal_load_lds_dwordx4 %1, off offset:1024" :: "s"(to_a + i * 2048), "v"(a) : "memory", "m0");
+            from_a[i] += 2048;
+        }
+        char const *const b = from_b + lane * 16;
         if constexpr (PB == 2) {
             asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\tglobal_load_lds_dwordx4 %1, off offset:1024" :: "s"(to_b), "v"(b) : "memory", "m0");
         }
         else { asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(to_b), "v"(b) : "memory", "m0"); }
-        from_a += 2048; from_b += 1024 * PB;
+        from_b += 1024 * PB;
     };
 
     // what is needed behind the products: the scales and biases of the tile's rows (the barriers of the stages are between this and its use)
@@ -322,16 +336,17 @@ __device__ __forceinline__ void packed_tile(PackedProduct const &p, int id, char
         char const *from = lds + buffer * kStage + lane * 16;
         DenseHalf8 a[TM][2], b[TN][PB];
 #pragma unroll
-        for (int i = 0; i < TM; ++i) {
-#pragma unroll
-            for (int q = 0; q < 2; ++q) { a[i][q] = *reinterpret_cast<DenseHalf8 const *>(from + ((wm * TM + i) * 2 + q) * 1024); }
-        }
-#pragma unroll
         for (int j = 0; j < TN; ++j) {
 #pragma unroll
             for (int q = 0; q < PB; ++q) { b[j][q] = *reinterpret_cast<DenseHalf8 const *>(from + kStageA + ((wn * TN + j) * PB + q) * 1024); }
         }
-        __builtin_amdgcn_sched_barrier(0);          // (all reads are asked for ahead of the first product: with two wavefronts per SIMD what one waits for the other hides)
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) { a[i][q] = *reinterpret_cast<DenseHalf8 const *>(from + ((wm * TM + i) * 2 + q) * 1024); }
+            // (all reads are asked for ahead of the first product, in the order in which the products want them: a product waits for no read behind its own)
+            __builtin_amdgcn_sched_barrier(0);
+        }
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
 #pragma unroll
@@ -342,11 +357,13 @@ __device__ __forceinline__ void packed_tile(PackedProduct const &p, int id, char
             }
 #pragma unroll
             for (int j = 0; j < TN; ++j) { acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][0], b[j][0], acc[i][j], 0, 0, 0); }
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
     // A stage's loads are asked for kAhead stages before.  Behind the barrier all wavefronts' loads of the stage have arrived, and nobody reads the buffer of the stage before any more,
     // which the next loads go to.
     int const ahead = min(kAhead, stages);
+    __builtin_amdgcn_s_waitcnt(0xc07f);         // (no scalar load on its way: with one the compiler could not count reads of LDS and would wait for all of them at once)
     for (int s = 0; s < ahead; ++s) { fetch(s); }
     int buffer = 0, free = kAhead;
     int s = 0;
@@ -364,7 +381,7 @@ __device__ __forceinline__ void packed_tile(PackedProduct const &p, int id, char
     }
 
     // 32 x 64 elements at a time go through LDS, so that a lane has neighbours of a row to store, or the rows of a column to sum
-    if (USE != kUseLogits && p.slabs > 1) {
+    if (p.slabs > 1) {
         o.kind = kOutStore; o.out = p.sums + slab * p.sums_slab; o.stride = p.sums_pitch; o.accumulate = 0;
     }
     float *const tile = reinterpret_cast<float *>(lds) + wave * 32 * kTilePitch;
@@ -399,7 +416,7 @@ __device__ __forceinline__ void packed_tile(PackedProduct const &p, int id, char
                 if (m0 + row < o.rows && n0 + lane < o.columns) { tile[row * kTilePitch + lane] = element_again(p.src_a, p.kind_a, p.src_b, p.kind_b, m0 + row, n0 + lane); }
             }
         }
-        if (USE == kUseLogits && n0 + lane < o.columns) {
+        if (USE == kUseLogits && p.slabs == 1 && n0 + lane < o.columns) {
             // (largest, sum of exponents) of the 32 rows of this lane's column
             int const n = n0 + lane, rows = min(32, o.rows - m0), label = o.label[n] - o.first_channel - m0;
             float z[32];
@@ -416,9 +433,10 @@ __device__ __forceinline__ void packed_tile(PackedProduct const &p, int id, char
         }
         if (USE == kUseForward && o.kind == kOutBits)         { finish_tile_bits(o, tile, b, m0, n0, lane); }
         else if (USE == kUseForward && o.kind == kOutForward) { finish_tile<kUseForward>(o, tile, b, m0, n0, lane); }
-        else if (USE != kUseLogits || o.out)                  { finish_tile<USE == kUseLogits ? kUseLogits : kUseStore>(o, tile, b, m0, n0, lane); }
+        else if (USE == kUseLogits && p.slabs == 1)           { if (o.out) { finish_tile<kUseLogits>(o, tile, b, m0, n0, lane); } }
+        else                                                  { finish_tile<kUseStore>(o, tile, b, m0, n0, lane); }
     }
-    if (USE == kUseLogits && n0 + lane < o.columns && rb_a + wm * TM < p.a_blocks) {
+    if (USE == kUseLogits && p.slabs == 1 && n0 + lane < o.columns && rb_a + wm * TM < p.a_blocks) {
         o.partial[(long long)((rb_a + wm * TM) / TM) * o.columns + n0 + lane] = column;
     }
 }
@@ -431,7 +449,7 @@ constexpr int packed_lds(void)
 }
 
 template <int USE, int TM, int WM, int WN, int PB, int BUFFERS>
-__global__ __launch_bounds__(WM * WN * 64) void dense_packed_kernel(PackedProduct p)
+__global__ __launch_bounds__(WM * WN * 64, 2) void dense_packed_kernel(PackedProduct p)
 {
     __shared__ __attribute__((aligned(1024))) char lds[packed_lds<TM, WM, WN, BUFFERS>()];
     __shared__ int scales[(TM * WM + 2 * WN) * 32];
@@ -441,12 +459,25 @@ __global__ __launch_bounds__(WM * WN * 64) void dense_packed_kernel(PackedProduc
 
 // one product, and behind it another whose operands are not packed bits (either may have no workgroups)
 template <int TM, int WM, int WN, int PB, int BUFFERS>
-__global__ __launch_bounds__(WM * WN * 64) void dense_packed_pair_kernel(PackedProduct p, PackedProduct q)
+__global__ __launch_bounds__(WM * WN * 64, 2) void dense_packed_pair_kernel(PackedProduct p, PackedProduct q)
 {
     __shared__ __attribute__((aligned(1024))) char lds[packed_lds<TM, WM, WN, BUFFERS>()];
     __shared__ int scales[(TM * WM + 2 * WN) * 32];
     if ((int)blockIdx.x < p.workgroups) { packed_tile<kUseStore, TM, WM, WN, PB, BUFFERS>(p, blockIdx.x, lds, scales, nullptr); }
     else                                { packed_tile<kUseStore, TM, WM, WN, 2, BUFFERS>(q, blockIdx.x - p.workgroups, lds, scales, nullptr); }
+}
+
+__device__ __forceinline__ float sum_of_slabs(PackedProduct const &p, int m, int n)
+{
+    float const *from = p.sums + m * p.sums_pitch + n;
+    float d = 0.0f;
+    int s = 0;
+    for (; s + 4 <= p.slabs; s += 4) {
+        float const a = from[s * p.sums_slab], b = from[(s + 1) * p.sums_slab], c = from[(s + 2) * p.sums_slab], e = from[(s + 3) * p.sums_slab];
+        d = (((d + a) + b) + c) + e;
+    }
+    for (; s < p.slabs; ++s) { d += from[s * p.sums_slab]; }
+    return d;
 }
 
 // The slabs' sums of a product, in order, and what becomes of them: a wavefront takes 64 neighbours of a row.
@@ -456,16 +487,10 @@ __device__ __forceinline__ void join_slabs(PackedProduct const &p, unsigned id)
     unsigned const across = (unsigned)(p.sums_pitch / 64), unit = id * 4 + threadIdx.x / 64;
     int const lane = threadIdx.x & 63, m = (int)(unit / across), n = (int)(unit % across) * 64 + lane;
     if (m >= o.rows) { return; }
-    bool const inside = n < o.columns;
+    bool const inside = n < o.columns || (n == o.columns && o.line && o.kind == kOutStore);
     float d = 0.0f;
     if (inside) {
-        float const *from = p.sums + m * p.sums_pitch + n;
-        int s = 0;
-        for (; s + 4 <= p.slabs; s += 4) {
-            float const a = from[s * p.sums_slab], b = from[(s + 1) * p.sums_slab], c = from[(s + 2) * p.sums_slab], e = from[(s + 3) * p.sums_slab];
-            d = (((d + a) + b) + c) + e;
-        }
-        for (; s < p.slabs; ++s) { d += from[s * p.sums_slab]; }
+        d = sum_of_slabs(p, m, n);
         if (d != d && p.kind_a >= 0) { d = element_again(p.src_a, p.kind_a, p.src_b, p.kind_b, m, n); }
     }
     if (o.kind == kOutForward) { if (inside) { static_cast<float *>(o.out)[m * o.stride + n] = activated(before_activation(o, d, m, n), o.activation); } }
@@ -480,6 +505,38 @@ __global__ __launch_bounds__(256) void dense_join_kernel(PackedProduct p, Packed
 {
     if (blockIdx.x < first_blocks) { join_slabs(p, blockIdx.x); }
     else                           { join_slabs(q, blockIdx.x - first_blocks); }
+}
+
+// the same for logits: a workgroup takes 32 rows of 64 columns, each wavefront eight of the rows
+__global__ __launch_bounds__(256) void dense_join_logits_kernel(PackedProduct p)
+{
+    __shared__ float2 part[4][64];
+    DenseOutput const &o = p.out;
+    unsigned const across = (unsigned)(p.sums_pitch / 64);
+    int const lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tile = (int)(blockIdx.x / across), n = (int)(blockIdx.x % across) * 64 + lane;
+    bool const inside = n < o.columns;
+    int const label = inside ? o.label[n] - o.first_channel : -1;
+    float z[8];
+    float2 s = make_float2(-INFINITY, 0.0f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        int const m = tile * 32 + wave * 8 + i;
+        z[i] = -INFINITY;
+        if (!inside || m >= o.rows) { continue; }
+        z[i] = sum_of_slabs(p, m, n) + (o.bias ? o.bias[m] : 0.0f);
+        if (o.out) { static_cast<float *>(o.out)[m * o.stride + n] = z[i]; }
+        if (label == m) { o.label_logit[n] = z[i]; }
+        s.x = fmaxf(s.x, z[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) { s.y += z[i] == -INFINITY ? 0.0f : exp_of_nonpositive(z[i] - s.x); }
+    part[wave][lane] = s;
+    __syncthreads();
+    if (wave == 0 && inside) {
+#pragma unroll
+        for (int w = 1; w < 4; ++w) { s = joined(s, part[w][lane]); }
+        o.partial[(long long)tile * o.columns + n] = s;
+    }
 }
 
 }  // namespace bbhip

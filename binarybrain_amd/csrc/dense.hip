@@ -61,8 +61,8 @@ int join(PackedProduct const &p, PackedProduct const &q, hipStream_t st, char co
 {
     if (p.slabs > 1 && p.out.kind == kOutLogits) {
         long long const blocks = ceil_div(p.out.rows, 32) * (p.sums_pitch / 64);
-        if (check_tiles(blocks, 256, name)) { return 1; }
-        launch(dense_join_logits_kernel, dim3((unsigned)blocks), dim3(256), 0, st, p);
+        if (check_tiles(blocks, kJoinLogitWaves * 64, name)) { return 1; }
+        launch(dense_join_logits_kernel, dim3((unsigned)blocks), dim3(kJoinLogitWaves * 64), 0, st, p);
         BBHIP_LAUNCH_CHECK();
         return 0;
     }
@@ -102,8 +102,8 @@ int few_frames_forward(Product const &p, bool bit, hipStream_t st, char const *n
 {
     DirectProduct d{};
     d.a = p.a; d.b = p.b; d.out = p.out;
-    // four rows for a wavefront where that leaves two workgroups for a compute unit
-    bool const four = p.out.rows >= 512 * kFewWaves * 4;
+    // four rows for a wavefront where that leaves a workgroup for every other compute unit: the frames, a row pitch apart, are read by each workgroup
+    bool const four = p.out.rows >= 128 * kFewWaves * 4;
     long long const blocks = ceil_div(p.out.rows, kFewWaves * (four ? 4 : 1));
     if (check_tiles(blocks, kFewWaves * 64, name)) { return 1; }
     dim3 const grid((unsigned)blocks), block(kFewWaves * 64);
@@ -127,14 +127,15 @@ int direct_forward(Product const &p, bool bit, float *sums, hipStream_t st, char
     DirectProduct d;
     if (direct(d, p, s, sums, p.out.columns, name)) { return 1; }
     dim3 const grid((unsigned)d.workgroups()), block((unsigned)s.waves * 64);
-    if (s.waves == 16) {
-        if (bit) { launch((dense_direct_kernel<kRows, kBitColumns, 16>), grid, block, 0, st, d); }
-        else     { launch((dense_direct_kernel<kRows, kColumns, 16>), grid, block, 0, st, d); }
-    }
-    else {
-        if (bit) { launch((dense_direct_kernel<kRows, kBitColumns, 4>), grid, block, 0, st, d); }
-        else     { launch((dense_direct_kernel<kRows, kColumns, 4>), grid, block, 0, st, d); }
-    }
+#define BBHIP_DIRECT(WAVES)                                                                             \
+    do {                                                                                                \
+        if (bit) { launch((dense_direct_kernel<kRows, kBitColumns, WAVES>), grid, block, 0, st, d); }   \
+        else     { launch((dense_direct_kernel<kRows, kColumns, WAVES>), grid, block, 0, st, d); }      \
+    } while (0)
+    if (s.waves == 8)      { BBHIP_DIRECT(8); }
+    else if (s.waves == 4) { BBHIP_DIRECT(4); }
+    else                   { BBHIP_DIRECT(1); }
+#undef BBHIP_DIRECT
     BBHIP_LAUNCH_CHECK();
     return join(sums_to_join(d), PackedProduct{}, st, name);
 }
@@ -144,9 +145,8 @@ struct DirectBackwardSpace {
     DirectShape w, x;
     float *dz, *w_sums, *x_sums;
     DirectBackwardSpace(Carver &c, int inputs, int outputs, int frames, bool with_dz)
-        : w(direct_shape(outputs, inputs + 1, frames)), x(direct_shape(inputs, frames, outputs))
     {
-        if (w.waves != x.waves) { w.waves = x.waves = 16; }
+        direct_shapes(outputs, inputs + 1, frames, inputs, frames, outputs, w, x);
         dz = with_dz ? c.take<float>((size_t)outputs * (ceil_div(frames, 64) * 64)) : nullptr;
         w_sums = sums_of(c, w.slabs, outputs, inputs + 1);
         x_sums = sums_of(c, x.slabs, inputs, frames);
@@ -168,19 +168,27 @@ int direct_backward(Product const &dw, Product const &dx, DirectBackwardSpace co
         from_dz.b = rows_of(dz, dz_stride, dx.b.rows, dx.b.depth);
     }
     with_line.b.ones = dw.out.line ? dw.b.rows : -1;
-    if (direct(w, with_line, s.w, s.w_sums, dw.out.columns + 1, name) || direct(x, from_dz, s.x, s.x_sums, dx.out.columns, name) ||
-        check_tiles((long long)w.workgroups() + x.workgroups(), s.w.waves * 64, name)) { return 1; }
-    if (w.tiles + x.tiles == 0) { return 0; }
-    dim3 const grid((unsigned)(w.workgroups() + x.workgroups())), block((unsigned)s.w.waves * 64);
-    if (s.w.waves == 16) {
-        if (bit) { launch((dense_direct_backward_kernel<kBitRows, 16>), grid, block, 0, st, w, x); }
-        else     { launch((dense_direct_backward_kernel<kRows, 16>), grid, block, 0, st, w, x); }
+    if (direct(w, with_line, s.w, s.w_sums, dw.out.columns + 1, name) || direct(x, from_dz, s.x, s.x_sums, dx.out.columns, name)) { return 1; }
+    // in one launch where both take as many wavefronts
+    bool const together = s.w.waves == s.x.waves && launch_holds((long long)w.workgroups() + x.workgroups() + 1, s.w.waves * 64);
+    DirectProduct none{};
+    none.slabs = 1;
+    for (int part = together ? 1 : 0; part < 2; ++part) {
+        DirectProduct const &a = together || part == 0 ? w : none, &b = together || part == 1 ? x : none;
+        int const waves = part == 0 ? s.w.waves : s.x.waves;
+        if (a.workgroups() + b.workgroups() == 0) { continue; }
+        dim3 const grid((unsigned)(a.workgroups() + b.workgroups())), block((unsigned)waves * 64);
+#define BBHIP_DIRECT(WAVES)                                                                             \
+        do {                                                                                            \
+            if (bit) { launch((dense_direct_backward_kernel<kBitRows, WAVES>), grid, block, 0, st, a, b); } \
+            else     { launch((dense_direct_backward_kernel<kRows, WAVES>), grid, block, 0, st, a, b); }    \
+        } while (0)
+        if (waves == 8)      { BBHIP_DIRECT(8); }
+        else if (waves == 4) { BBHIP_DIRECT(4); }
+        else                 { BBHIP_DIRECT(1); }
+#undef BBHIP_DIRECT
+        BBHIP_LAUNCH_CHECK();
     }
-    else {
-        if (bit) { launch((dense_direct_backward_kernel<kBitRows, 4>), grid, block, 0, st, w, x); }
-        else     { launch((dense_direct_backward_kernel<kRows, 4>), grid, block, 0, st, w, x); }
-    }
-    BBHIP_LAUNCH_CHECK();
     return join(sums_to_join(w), sums_to_join(x), st, name);
 }
 
@@ -341,7 +349,7 @@ int check_sizes(int inputs, int outputs, int frames, char const *name)
 {
     if (!(inputs > 0 && outputs > 0 && frames > 0)) { return fail("%s: sizes must be positive", name); }
     if (inputs > kDenseNodesMost || outputs > kDenseNodesMost || frames > kDenseFramesMost) {
-        return fail("%s: more than 2^%d nodes or 2^%d frames", name, 24, 26);
+        return fail("%s: more than 2^24 nodes or 2^25 frames", name);
     }
     return 0;
 }
@@ -349,6 +357,7 @@ int check_sizes(int inputs, int outputs, int frames, char const *name)
 int check_stride(bool bit, int stride, int frames, char const *name)
 {
     if ((bit ? (long long)stride * 32 : stride) < frames) { return fail("%s: frame stride shorter than the frames", name); }
+    if (stride > kDenseStrideMost) { return fail("%s: a frame stride of %d: at most %d", name, stride, kDenseStrideMost); }
     return 0;
 }
 
@@ -356,6 +365,7 @@ Operand frames_as_columns(void const *x, int stride, int inputs, int frames)
 {
     Operand o{};
     o.p = x; o.stride = stride; o.rows = frames; o.depth = inputs; o.ones = -1;
+    o.vec = starts_on_16_bytes(x) && stride % 4 == 0;
     return o;
 }
 

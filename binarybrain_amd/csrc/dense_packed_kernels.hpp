@@ -507,36 +507,50 @@ __global__ __launch_bounds__(256) void dense_join_kernel(PackedProduct p, Packed
     else                           { join_slabs(q, blockIdx.x - first_blocks); }
 }
 
-// the same for logits: a workgroup takes 32 rows of 64 columns, each wavefront eight of the rows
-__global__ __launch_bounds__(256) void dense_join_logits_kernel(PackedProduct p)
+// The same for logits: a workgroup takes 32 rows of 64 columns, each of its sixteen wavefronts two of the rows, four slabs of both at a time.
+constexpr int kJoinLogitWaves = 16;
+__global__ __launch_bounds__(kJoinLogitWaves * 64) void dense_join_logits_kernel(PackedProduct p)
 {
-    __shared__ float2 part[4][64];
+    __shared__ float2 part[kJoinLogitWaves][64];
     DenseOutput const &o = p.out;
     unsigned const across = (unsigned)(p.sums_pitch / 64);
     int const lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tile = (int)(blockIdx.x / across), n = (int)(blockIdx.x % across) * 64 + lane;
+    int const m0 = tile * 32 + wave * 2;
     bool const inside = n < o.columns;
     int const label = inside ? o.label[n] - o.first_channel : -1;
-    float z[8];
+    float z[2] = {};
+    if (inside) {
+        // (a row behind the last one reads the last one)
+        float const *const a = p.sums + min(m0, o.rows - 1) * p.sums_pitch + n, *const b = p.sums + min(m0 + 1, o.rows - 1) * p.sums_pitch + n;
+        for (int s = 0; s < p.slabs; s += 4) {
+            float u[4], v[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                long long const at = min(s + q, p.slabs - 1) * p.sums_slab;
+                u[q] = a[at]; v[q] = b[at];
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) { z[0] += s + q < p.slabs ? u[q] : 0.0f; z[1] += s + q < p.slabs ? v[q] : 0.0f; }
+        }
+    }
     float2 s = make_float2(-INFINITY, 0.0f);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        int const m = tile * 32 + wave * 8 + i;
-        z[i] = -INFINITY;
-        if (!inside || m >= o.rows) { continue; }
-        z[i] = sum_of_slabs(p, m, n) + (o.bias ? o.bias[m] : 0.0f);
+    for (int i = 0; i < 2; ++i) {
+        int const m = m0 + i;
+        if (!inside || m >= o.rows) { z[i] = -INFINITY; continue; }
+        z[i] += o.bias ? o.bias[m] : 0.0f;
         if (o.out) { static_cast<float *>(o.out)[m * o.stride + n] = z[i]; }
         if (label == m) { o.label_logit[n] = z[i]; }
         s.x = fmaxf(s.x, z[i]);
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) { s.y += z[i] == -INFINITY ? 0.0f : exp_of_nonpositive(z[i] - s.x); }
+    for (int i = 0; i < 2; ++i) { s.y += z[i] == -INFINITY ? 0.0f : exp_of_nonpositive(z[i] - s.x); }
     part[wave][lane] = s;
-    __syncthreads();
-    if (wave == 0 && inside) {
-#pragma unroll
-        for (int w = 1; w < 4; ++w) { s = joined(s, part[w][lane]); }
-        o.partial[(long long)tile * o.columns + n] = s;
+    for (int step = kJoinLogitWaves / 2; step > 0; step /= 2) {
+        __syncthreads();
+        if (wave < step) { s = joined(s, part[wave + step][lane]); part[wave][lane] = s; }
     }
+    if (wave == 0 && inside) { o.partial[(long long)tile * o.columns + n] = s; }
 }
 
 }  // namespace bbhip

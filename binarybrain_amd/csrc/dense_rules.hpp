@@ -7,22 +7,23 @@
 
 namespace bbhip {
 
-constexpr int kDenseNodesMost = 1 << 24, kDenseFramesMost = 1 << 26;
+// (31 rows of the largest stride are less than 2^32 bytes: what dense_direct_kernel's 32-bit offsets hold)
+constexpr int kDenseNodesMost = 1 << 24, kDenseFramesMost = 1 << 25, kDenseStrideMost = 33 << 20;
 
 // How a product straight from its operands is divided: tiles of 32 x 32, wavefronts that share a tile's k axis (chunks of 32), and workgroups that do.
 struct DirectShape { int waves, n_tiles, slabs, slab_chunks; long long tiles; };
-inline DirectShape direct_shape(int m, int n, int k)
+inline DirectShape direct_shape(int m, int n, int k, int waves = 0)
 {
     DirectShape s;
     int const chunks = ceil_div(k, 32);
-    s.waves = chunks >= 8 ? 16 : 4;
+    s.waves = waves ? waves : chunks > 16 ? 8 : chunks > 2 ? 4 : 1;
     s.n_tiles = ceil_div(n, 32);
     s.tiles = (long long)ceil_div(m, 32) * s.n_tiles;
-    // two chunks for a wavefront are what a join is worth from four on
+    // two chunks for a wavefront are what a join is worth from six on
     int slabs = 1;
-    if (s.tiles < 256 && chunks >= 4 * s.waves) {
-        slabs = ceil_div(chunks, 2 * s.waves);
-        int const most = (int)(512 / s.tiles);
+    if (s.tiles < 512 && chunks >= 6 * s.waves) {
+        slabs = chunks / (2 * s.waves);
+        int const most = (int)(1024 / s.tiles);
         if (slabs > most) { slabs = most; }
     }
     s.slab_chunks = ceil_div(chunks, slabs);
@@ -30,8 +31,21 @@ inline DirectShape direct_shape(int m, int n, int k)
     return s;
 }
 
+// Both products of a backward pass: as many wavefronts for either, and so one launch, while the device holds all of them at once or nearly so; beyond that a short k axis leaves most of
+// the longer one's wavefronts without work (9932 x 6136 x 25 frames 1143 us, with a launch each 470; 191 x 227 x 56 frames 8.3 and 16.8).
+inline void direct_shapes(int m0, int n0, int k0, int m1, int n1, int k1, DirectShape &s0, DirectShape &s1)
+{
+    s0 = direct_shape(m0, n0, k0);
+    s1 = direct_shape(m1, n1, k1);
+    if (s0.tiles + s1.tiles <= 1024 && s0.waves != s1.waves) {
+        int const waves = s0.waves > s1.waves ? s0.waves : s1.waves;
+        s0 = direct_shape(m0, n0, k0, waves);
+        s1 = direct_shape(m1, n1, k1, waves);
+    }
+}
+
 // Whether a product goes by way of packed halves (two launches at least, and both operands are written once more) instead of straight from its operands.
-inline bool product_packed(int m, int n, int k) { return (long long)m * n * k >= 1LL << 26 && m >= 32 && n >= 32 && k >= 32; }
+inline bool product_packed(int m, int n, int k) { return (long long)m * n * k >= 1LL << 29 && m >= 32 && n >= 32 && k >= 32; }
 
 // Tiles of a packed product: 256 x 256 by eight wavefronts, 256 x 128 or 128 x 128 by four (two such workgroups on a compute unit); stages that lie in LDS.
 enum PackedTile : int { kTileLarge = 0, kTileMiddle = 1, kTileSmall = 2, kTileSizes = 3 };
@@ -62,7 +76,12 @@ inline PackedShape packed_shape(int size, int slabs, int m, int n, int k)
 // Time of a launch in stages of a small tile on a compute unit (384 cycles of matrix instructions with two halves per operand, 0.16 us).  A large tile's stage is four of them, a middle
 // one's two; of the tiles of four wavefronts two are on a compute unit, each at half the speed.  Six stages' worth are a workgroup's beginning and end.
 constexpr double kTileStage[kTileSizes] = {4.0 / 0.75, 2 * 2.0 / 0.7, 2 * 1.0 / 0.55};
-inline double packed_length(PackedShape const &s) { return (s.slab_stages + 6) * kTileStage[s.size]; }
+inline double packed_length(PackedShape const &s, long long workgroups)
+{
+    // (where each has a compute unit of its own it is not half as fast, though nothing covers what it waits for)
+    bool const alone = s.size != kTileLarge && workgroups <= 256;
+    return (s.slab_stages + 6) * kTileStage[s.size] * (alone ? 0.65 : 1.0);
+}
 inline int    packed_at_once(PackedShape const &s) { return kTileAtOnce[s.size]; }
 
 // sums written and read again at about 4 TB/s, and a launch
@@ -73,7 +92,7 @@ constexpr double kJoinLaunch = 25.0;
 inline double packed_end(PackedShape const &x, PackedShape const &y)
 {
     long long const at_once = packed_at_once(x), n1 = x.workgroups(), n2 = y.workgroups();
-    double const l1 = packed_length(x), l2 = packed_length(y);
+    double const l1 = packed_length(x, n1 + n2), l2 = packed_length(y, n1 + n2);
     long long const full = n1 / at_once, more = n1 % at_once;           // `more` places are taken once more than the others
     double const free0 = full * l1, free1 = more ? free0 + l1 : free0;
     if (n2 == 0) { return free1; }

@@ -529,7 +529,7 @@ int bbhip_fp32_CategoricalSampling(float const *dev_y_buf, float const *dev_u_bu
  *     y[o][f] = activation(sum over i of W[o][i] * x[i][f] + b[o] + residual[o][f])
  * activation: 0 none, 1 relu, 2 sigmoid, 3 hard tanh (limits -1 and 1).  bit_...: x is packed bits, read as 0 and 1; ..._bit: y is packed bits, set where the sum is above 0 (the bits
  * behind the last frame of its word are 0; further words of a row are left alone). 
- * At most 2^24 nodes and 2^26 frames. */
+ * At most 2^24 nodes, 2^25 frames and strides of 33 * 2^20. */
 size_t bbhip_DenseAffine_WorkspaceBytes(int input_node_size, int output_node_size, int frame_size);
 int bbhip_fp32_DenseAffine_Forward(float const *dev_x_buf, float *dev_y_buf, float const *dev_W, float const *dev_b, float const *dev_residual_buf, int activation,
                                    int input_node_size, int output_node_size, int frame_size, int x_frame_stride, int y_frame_stride, int residual_frame_stride,

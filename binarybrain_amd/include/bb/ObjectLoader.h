@@ -1,6 +1,6 @@
 // Reconstruct a serialized object from its recorded type name (reference: include/bb/ObjectLoader.h:407-447
 // `Object_Load` / `Object_LoadFromFile`).  Known here: the LUT layers of widths 2..6 on fp32 or packed-bit frames,
-// BinaryLut6, StochasticBatchNormalization, LayerNormalization, AverageLut, MaxLut, Reduce, Binarize, HardTanh, RealToBinary, BinaryToReal, BinaryModulation, DifferentiableLutDiscreteN (the LUT layer put together from its parts), MaxPooling, UpSampling, Shuffle, the convolution wrapper with its Im2Col / Col2Im, the layer list, and tensors.  An unknown name yields an empty pointer, as in the reference.
+// BinaryLut6, StochasticBatchNormalization, LayerNormalization, DenseAffine, AverageLut, MaxLut, Reduce, Binarize, HardTanh, RealToBinary, BinaryToReal, BinaryModulation, DifferentiableLutDiscreteN (the LUT layer put together from its parts), MaxPooling, UpSampling, Shuffle, the convolution wrapper with its Im2Col / Col2Im, the layer list, and tensors.  An unknown name yields an empty pointer, as in the reference.
 #pragma once
 
 #include "bb/StochasticLutN.h"
@@ -12,6 +12,7 @@
 #include "bb/Sequential.h"
 #include "bb/StochasticBatchNormalization.h"
 #include "bb/LayerNormalization.h"
+#include "bb/DenseAffine.h"
 #include "bb/MaxLut.h"
 #include "bb/AverageLut.h"
 #include "bb/Reduce.h"
@@ -56,6 +57,8 @@ inline std::shared_ptr<Object> CreateByName(std::string const &name)
     if (name == StochasticBatchNormalization<float>::ObjectName()) { return StochasticBatchNormalization<float>::Create(); }
     if (name == LayerNormalization<float, float>::ObjectName())   { return LayerNormalization<float, float>::Create(); }
     if (name == LayerNormalization<Bit, float>::ObjectName())     { return LayerNormalization<Bit, float>::Create(); }
+    if (name == DenseAffine<float, float>::ObjectName())          { return DenseAffine<float, float>::Create((index_t)1); }
+    if (name == DenseAffine<Bit, float>::ObjectName())            { return DenseAffine<Bit, float>::Create((index_t)1); }
     if (name == AverageLut<float, float>::ObjectName())           { return AverageLut<float, float>::Create(); }
     if (name == AverageLut<Bit, float>::ObjectName())             { return AverageLut<Bit, float>::Create(); }
     if (name == MaxLut<float, float>::ObjectName())               { return MaxLut<float, float>::Create(); }

@@ -7,6 +7,7 @@
 
 #include "bb/Core.h"
 #include "bb/Tensor.h"
+#include "bb/Workspace.h"
 
 namespace bb {
 
@@ -32,6 +33,10 @@ class OptimizerAdam : public Optimizer {
     std::vector<std::shared_ptr<Tensor>> m_m, m_v;
     // device tables of the call: element counts and the four pointer lists
     std::shared_ptr<Memory> m_size_table, m_param_table, m_grad_table, m_m_table, m_v_table;
+
+    T         m_max_norm = (T)-1;               // negative: gradients are taken as they are
+    std::shared_ptr<Memory> m_norm;             // (norm, scale) of the last clipped step
+    Workspace m_work;
 
     OptimizerAdam(T learning_rate, T beta1, T beta2)
         : m_learning_rate(learning_rate), m_beta1(beta1), m_beta2(beta2), m_b1(beta1), m_b2(beta2) {}
@@ -62,6 +67,16 @@ public:
     std::string GetOptimizerName(void) const override { return "OptimizerAdam"; }
 
     void SetLearningRate(double learning_rate) override { m_learning_rate = (T)learning_rate; }
+
+    // From now on gradients count scaled to this norm where theirs, as one vector, is larger (they stay as they are until ZeroGrad); a negative value ends it.  No tensor may be in the
+    // list twice.  (The reference's optimizer does not clip.)
+    void SetGradientClipping(double max_norm)
+    {
+        m_max_norm = (T)max_norm;
+        if (!m_norm) { m_norm = Memory::Create(2 * sizeof(float)); }
+    }
+    // the norm that the gradients had in the last clipped step
+    double GetGradientNorm(void) const { return m_norm ? ((float const *)m_norm->LockConst())[0] : 0.0; }
 
     // Binds the parameter list; the moment estimates start at zero (reference: OptimizerAdam.h:120-130).
     // The tensors must keep their storage (no Resize) while the optimizer is in use.
@@ -116,6 +131,16 @@ private:
             m_v[(std::size_t)i]->LockDeviceMemory();
         }
         T const lr_t = m_learning_rate * std::sqrt((T)1.0 - m_b2) / ((T)1.0 - m_b1);        // OptimizerAdam.h:171
+        if (m_max_norm >= (T)0) {
+            std::size_t const size = bbhip_GradientNorm_WorkspaceBytes();
+            CheckDevice(bbhip_fp32_OptimizerAdam_Clipped((int)n, (int const *)m_size_table->LockDeviceConst(), (float *const *)m_param_table->LockDeviceConst(),
+                            (float *const *)m_grad_table->LockDeviceConst(), (float *const *)m_m_table->LockDeviceConst(), (float *const *)m_v_table->LockDeviceConst(), lr_t,
+                            (double)m_beta1, (double)m_beta2, m_max_norm, (float *)m_norm->LockDevice(true), zero_grads, m_work.Get(size), size, nullptr),
+                        "bbhip_fp32_OptimizerAdam_Clipped");
+            m_b1 *= m_beta1;
+            m_b2 *= m_beta2;
+            return;
+        }
         auto const entry = zero_grads ? bbhip_fp32_OptimizerAdam_Update : bbhip_fp32_OptimizerAdam;
         CheckDevice(entry((int)n, (int const *)m_size_table->LockDeviceConst(),
                           (float *const *)m_param_table->LockDeviceConst(), (float *const *)m_grad_table->LockDeviceConst(),

@@ -132,7 +132,8 @@ int direct_forward(Product const &p, bool bit, float *sums, hipStream_t st, char
         if (bit) { launch((dense_direct_kernel<kRows, kBitColumns, WAVES>), grid, block, 0, st, d); }   \
         else     { launch((dense_direct_kernel<kRows, kColumns, WAVES>), grid, block, 0, st, d); }      \
     } while (0)
-    if (s.waves == 8)      { BBHIP_DIRECT(8); }
+    if (s.waves == 16)     { BBHIP_DIRECT(16); }
+    else if (s.waves == 8) { BBHIP_DIRECT(8); }
     else if (s.waves == 4) { BBHIP_DIRECT(4); }
     else                   { BBHIP_DIRECT(1); }
 #undef BBHIP_DIRECT

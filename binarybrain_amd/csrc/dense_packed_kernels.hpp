@@ -278,7 +278,8 @@ __device__ __forceinline__ void finish_tile_bits(DenseOutput const &o, float con
 template <int N>
 __device__ __forceinline__ void arrived(void)
 {
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(N) : "memory");
+    __builtin_amdgcn_s_waitcnt(0xc07f);         // (lgkmcnt 0, where the compiler sees it: it need not wait for these reads again)
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" :: "n"(N) : "memory");
 }
 
 template <int USE, int TM, int WM, int WN, int PB, int BUFFERS>
@@ -332,52 +333,93 @@ __device__ __forceinline__ void packed_tile(PackedProduct const &p, int id, char
 
     int const wm = wave / WN, wn = wave % WN;
     DenseAcc16 acc[TM][TN] = {};
-    auto const multiply = [&](int buffer) {
+    struct Halves { DenseHalf8 a[TM][2], b[TN][PB]; };
+    auto const read = [&](int buffer, Halves &h) {
         char const *from = lds + buffer * kStage + lane * 16;
-        DenseHalf8 a[TM][2], b[TN][PB];
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
 #pragma unroll
-            for (int q = 0; q < PB; ++q) { b[j][q] = *reinterpret_cast<DenseHalf8 const *>(from + kStageA + ((wn * TN + j) * PB + q) * 1024); }
+            for (int q = 0; q < PB; ++q) { h.b[j][q] = *reinterpret_cast<DenseHalf8 const *>(from + kStageA + ((wn * TN + j) * PB + q) * 1024); }
         }
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
 #pragma unroll
-            for (int q = 0; q < 2; ++q) { a[i][q] = *reinterpret_cast<DenseHalf8 const *>(from + ((wm * TM + i) * 2 + q) * 1024); }
+            for (int q = 0; q < 2; ++q) { h.a[i][q] = *reinterpret_cast<DenseHalf8 const *>(from + ((wm * TM + i) * 2 + q) * 1024); }
             // (all reads are asked for ahead of the first product, in the order in which the products want them: a product waits for no read behind its own)
             __builtin_amdgcn_sched_barrier(0);
         }
+    };
+    auto const multiply = [&](Halves const &h) {
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
 #pragma unroll
-            for (int j = 0; j < TN; ++j) { acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][1], b[j][0], acc[i][j], 0, 0, 0); }
+            for (int j = 0; j < TN; ++j) { acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(h.a[i][1], h.b[j][0], acc[i][j], 0, 0, 0); }
             if constexpr (PB == 2) {
 #pragma unroll
-                for (int j = 0; j < TN; ++j) { acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][0], b[j][1], acc[i][j], 0, 0, 0); }
+                for (int j = 0; j < TN; ++j) { acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(h.a[i][0], h.b[j][1], acc[i][j], 0, 0, 0); }
             }
 #pragma unroll
-            for (int j = 0; j < TN; ++j) { acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][0], b[j][0], acc[i][j], 0, 0, 0); }
+            for (int j = 0; j < TN; ++j) { acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(h.a[i][0], h.b[j][0], acc[i][j], 0, 0, 0); }
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    // A stage's loads are asked for kAhead stages before.  Behind the barrier all wavefronts' loads of the stage have arrived, and nobody reads the buffer of the stage before any more,
-    // which the next loads go to.
-    int const ahead = min(kAhead, stages);
     __builtin_amdgcn_s_waitcnt(0xc07f);         // (no scalar load on its way: with one the compiler could not count reads of LDS and would wait for all of them at once)
-    for (int s = 0; s < ahead; ++s) { fetch(s); }
-    int buffer = 0, free = kAhead;
-    int s = 0;
-    for (; s + kAhead < stages; ++s) {
-        arrived<(kAhead - 1) * kLoads>();
-        fetch(free);
-        multiply(buffer);
-        free = buffer;
-        buffer = buffer + 1 == BUFFERS ? 0 : buffer + 1;
+    if constexpr (TM == 2) {
+        // A small tile's halves fit the registers twice: the next stage's are read behind the present one's products, which nothing else would cover where a compute unit has one such
+        // workgroup.  A stage's buffer is free as soon as its halves are in registers, so the loads are four stages ahead.
+        static_assert(BUFFERS == 4, "the stage's buffer is its number modulo four");
+        Halves even, odd;
+        int const ahead = min(BUFFERS, stages);
+        for (int s = 0; s < ahead; ++s) { fetch(s); }
+        if (stages >= 4) { arrived<3 * kLoads>(); } else { arrived<0>(); }
+        read(0, even);
+        auto const step = [&](int s, Halves const &now, Halves &next) {
+            if (s + 1 < stages) {
+                if (s + 3 < stages) { arrived<2 * kLoads>(); } else { arrived<0>(); }
+                if (s + 4 < stages) { fetch(s & 3); }
+                read((s + 1) & 3, next);
+            }
+            multiply(now);
+        };
+        auto const full_step = [&](int s, Halves const &now, Halves &next) {           // (without a branch between the reads and the products, so that these wait for none of them)
+            arrived<2 * kLoads>();
+            fetch(s & 3);
+            read((s + 1) & 3, next);
+            multiply(now);
+        };
+        int s = 0;
+        for (; s + 5 < stages; s += 2) {
+            full_step(s, even, odd);
+            full_step(s + 1, odd, even);
+        }
+#pragma nounroll
+        for (; s < stages; s += 2) {
+            step(s, even, odd);
+            if (s + 1 < stages) { step(s + 1, odd, even); }
+        }
     }
-    for (; s < stages; ++s) {
-        arrived<0>();
-        multiply(buffer);
-        buffer = buffer + 1 == BUFFERS ? 0 : buffer + 1;
+    else {
+        // A stage's loads are asked for kAhead stages before.  Behind the barrier all wavefronts' loads of the stage have arrived, and nobody reads the buffer of the stage before any
+        // more, which the next loads go to.
+        Halves h;
+        int const ahead = min(kAhead, stages);
+        for (int s = 0; s < ahead; ++s) { fetch(s); }
+        int buffer = 0, free = kAhead;
+        int s = 0;
+        for (; s + kAhead < stages; ++s) {
+            arrived<(kAhead - 1) * kLoads>();
+            fetch(free);
+            read(buffer, h);
+            multiply(h);
+            free = buffer;
+            buffer = buffer + 1 == BUFFERS ? 0 : buffer + 1;
+        }
+        for (; s < stages; ++s) {
+            arrived<0>();
+            read(buffer, h);
+            multiply(h);
+            buffer = buffer + 1 == BUFFERS ? 0 : buffer + 1;
+        }
     }
 
     // 32 x 64 elements at a time go through LDS, so that a lane has neighbours of a row to store, or the rows of a column to sum

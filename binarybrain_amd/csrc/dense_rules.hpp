@@ -16,9 +16,9 @@ inline DirectShape direct_shape(int m, int n, int k, int waves = 0)
 {
     DirectShape s;
     int const chunks = ceil_div(k, 32);
-    s.waves = waves ? waves : chunks > 16 ? 8 : chunks > 2 ? 4 : 1;
     s.n_tiles = ceil_div(n, 32);
     s.tiles = (long long)ceil_div(m, 32) * s.n_tiles;
+    s.waves = waves ? waves : chunks > 16 ? (s.tiles <= 64 && chunks <= 64 ? 16 : 8) : chunks > 2 || s.tiles < 2048 ? 4 : 1;
     // two chunks for a wavefront are what a join is worth from six on
     int slabs = 1;
     if (s.tiles < 512 && chunks >= 6 * s.waves) {
@@ -37,8 +37,10 @@ inline void direct_shapes(int m0, int n0, int k0, int m1, int n1, int k1, Direct
 {
     s0 = direct_shape(m0, n0, k0);
     s1 = direct_shape(m1, n1, k1);
+    if (s0.waves > 8) { s0 = direct_shape(m0, n0, k0, 8); }
+    if (s1.waves > 8) { s1 = direct_shape(m1, n1, k1, 8); }
     if (s0.tiles + s1.tiles <= 1024 && s0.waves != s1.waves) {
-        int const waves = s0.waves > s1.waves ? s0.waves : s1.waves;
+        int const more = s0.waves > s1.waves ? s0.waves : s1.waves, waves = more < 8 ? more : 8;
         s0 = direct_shape(m0, n0, k0, waves);
         s1 = direct_shape(m1, n1, k1, waves);
     }

@@ -17,21 +17,26 @@ constexpr int kNormBlock = 256, kNormPiece = 4096, kNormGrid = 1024;
 template <bool BACKWARDS, class F>
 __device__ __forceinline__ void for_each_piece(int size, int const *size_table, F const &f)
 {
-    __shared__ int scan[kNormBlock];            // pieces up to and with each tensor of the batch
+    __shared__ int scan[kNormBlock], waves[kNormBlock / 64];            // pieces up to and with each tensor of the batch
     int const batches = (size + kNormBlock - 1) / kNormBlock;
     // (pieces of the batches before; a list of many batches is walked in order, a short one may be walked backwards)
     long long before = 0;
     for (int batch = 0; batch < batches; ++batch) {
         int const t0 = batch * kNormBlock, t = t0 + threadIdx.x;
         int mine = t < size ? (size_table[t] > 0 ? (size_table[t] - 1) / kNormPiece + 1 : 0) : 0;
+        // running sum: within the wavefront, then the wavefronts'
+        int const lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+        for (int step = 1; step < 64; step *= 2) {
+            int const add = __shfl_up(mine, step);
+            mine += lane >= step ? add : 0;
+        }
+        if (lane == 63) { waves[wave] = mine; }
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kNormBlock / 64 - 1; ++w) { mine += w < wave ? waves[w] : 0; }
         scan[threadIdx.x] = mine;
         __syncthreads();
-        for (int step = 1; step < kNormBlock; step *= 2) {
-            int const add = (int)threadIdx.x >= step ? scan[threadIdx.x - step] : 0;
-            __syncthreads();
-            scan[threadIdx.x] += add;
-            __syncthreads();
-        }
         int const total = scan[kNormBlock - 1];
         int const first = (int)((blockIdx.x + gridDim.x - before % gridDim.x) % gridDim.x);
         int const count = first < total ? (total - first - 1) / (int)gridDim.x + 1 : 0;

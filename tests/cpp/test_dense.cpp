@@ -35,7 +35,7 @@ static void test_rules(void)
         int const chunks = (k + 31) / 32;
         check(d.slabs >= 1 && (long long)d.slabs * d.slab_chunks >= chunks && (long long)(d.slabs - 1) * d.slab_chunks < chunks, "direct slabs", m, k);
         check(d.slabs == 1 || d.tiles * d.slabs <= 1024, "direct workgroups", m, n);
-        check((d.waves == 1 || d.waves == 4 || d.waves == 8) && d.tiles == (long long)((m + 31) / 32) * ((n + 31) / 32), "direct tiles", m, n);
+        check((d.waves == 1 || d.waves == 4 || d.waves == 8 || d.waves == 16) && d.tiles == (long long)((m + 31) / 32) * ((n + 31) / 32), "direct tiles", m, n);
         bbhip::PackedShape s{}, t{}, one = bbhip::best_shape(m, n, k);
         bbhip::best_shapes(m, n, k, m1, n, k1, s, t);
         for (auto const &p : {s, t, one}) {

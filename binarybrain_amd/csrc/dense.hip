@@ -102,8 +102,9 @@ int few_frames_forward(Product const &p, bool bit, hipStream_t st, char const *n
 {
     DirectProduct d{};
     d.a = p.a; d.b = p.b; d.out = p.out;
-    // four rows for a wavefront where that leaves a workgroup for every other compute unit: the frames, a row pitch apart, are read by each workgroup
-    bool const four = p.out.rows >= 128 * kFewWaves * 4;
+    // Four rows for a wavefront, which read a frame's value once, where wavefronts of one row would not run all at once (32 KB of LDS per workgroup: five on a compute unit).  1024 inputs, one frame:
+    // 4096 outputs 5.3 us with one row and 7.1 with four, 8192 10.2 and 8.4; eight frames: 9.6 and 10.8, 20.2 and 13.4; 8192 x 8192 x 8 frames 131 and 68.
+    bool const four = p.out.rows > 5 * 256 * kFewWaves;
     long long const blocks = ceil_div(p.out.rows, kFewWaves * (four ? 4 : 1));
     if (check_tiles(blocks, kFewWaves * 64, name)) { return 1; }
     dim3 const grid((unsigned)blocks), block(kFewWaves * 64);
@@ -123,7 +124,7 @@ int few_frames_forward(Product const &p, bool bit, hipStream_t st, char const *n
 
 int direct_forward(Product const &p, bool bit, float *sums, hipStream_t st, char const *name)
 {
-    DirectShape const s = direct_shape(p.out.rows, p.out.columns, p.a.depth);
+    DirectShape const s = p.out.kind == kOutLogits ? logits_shape(p.out.rows, p.out.columns, p.a.depth) : direct_shape(p.out.rows, p.out.columns, p.a.depth);
     DirectProduct d;
     if (direct(d, p, s, sums, p.out.columns, name)) { return 1; }
     dim3 const grid((unsigned)d.workgroups()), block((unsigned)s.waves * 64);
@@ -132,8 +133,7 @@ int direct_forward(Product const &p, bool bit, float *sums, hipStream_t st, char
         if (bit) { launch((dense_direct_kernel<kRows, kBitColumns, WAVES>), grid, block, 0, st, d); }   \
         else     { launch((dense_direct_kernel<kRows, kColumns, WAVES>), grid, block, 0, st, d); }      \
     } while (0)
-    if (s.waves == 16)     { BBHIP_DIRECT(16); }
-    else if (s.waves == 8) { BBHIP_DIRECT(8); }
+    if (s.waves == 8)      { BBHIP_DIRECT(8); }
     else if (s.waves == 4) { BBHIP_DIRECT(4); }
     else                   { BBHIP_DIRECT(1); }
 #undef BBHIP_DIRECT
@@ -194,8 +194,6 @@ int direct_backward(Product const &dw, Product const &dx, DirectBackwardSpace co
 }
 
 // ---- products by way of packed halves ----
-bool is_bits(int kind) { return kind == kBitRows || kind == kBitColumns; }
-
 // an operand's halves and scales in a workspace, and the job that writes them
 struct Packed {
     uint4 *halves;
@@ -399,7 +397,7 @@ int dense_forward(void const *x, bool bit, void *y, bool bit_out, float const *W
         ScopedTimer tm(kTimeOther, st);
         return few_frames_forward(p, bit, st, name);
     }
-    if (!product_packed(outputs, frames, inputs)) {
+    if (!forward_packed(inputs, outputs, frames)) {
         float *const sums = sums_of(c, direct_shape(outputs, frames, inputs).slabs, outputs, frames);
         if (check_workspace(workspace, workspace_size, c.at, name)) { return 1; }
         ScopedTimer tm(kTimeOther, st);
@@ -443,7 +441,7 @@ int dense_backward(void const *x, bool bit, float const *dy, float const *y, flo
     i.out = DenseOutput{};
     i.out.kind = kOutStore; i.out.rows = inputs; i.out.columns = frames; i.out.out = dx; i.out.stride = dx_stride;
     hipStream_t const st = static_cast<hipStream_t>(stream);
-    if (product_packed(outputs, frames, inputs)) {
+    if (backward_packed(inputs, outputs, frames)) {
         Carver c{static_cast<char *>(workspace)};
         BackwardSpace const s(c, inputs, outputs, frames, bit);
         if (check_workspace(workspace, workspace_size, c.at, name)) { return 1; }
@@ -494,7 +492,7 @@ struct LossSpace {
             for (int count : {plan.piece, last}) {
                 Carver d{nullptr}, e{nullptr};
                 DirectBackwardSpace const space(d, inputs, count, frames, false);
-                sums_of(e, direct_shape(count, frames, inputs).slabs, count, frames);
+                sums_of(e, logits_shape(count, frames, inputs).slabs, count, frames);
                 most = d.at > most ? d.at : most;
                 most_sums = e.at > most_sums ? e.at : most_sums;
             }
@@ -613,13 +611,10 @@ size_t bbhip_DenseAffine_WorkspaceBytes(int input_node_size, int output_node_siz
 {
     if (check_sizes(input_node_size, output_node_size, frame_size, __func__)) { return 0; }
     Carver forward{nullptr}, backward{nullptr};
-    if (!product_packed(output_node_size, frame_size, input_node_size)) {
-        sums_of(forward, direct_shape(output_node_size, frame_size, input_node_size).slabs, output_node_size, frame_size);
-        DirectBackwardSpace const d(backward, input_node_size, output_node_size, frame_size, true);
-        return forward.at > backward.at ? forward.at : backward.at;
-    }
-    ForwardSpace const f(forward, input_node_size, output_node_size, frame_size, false);
-    BackwardSpace const b(backward, input_node_size, output_node_size, frame_size, false);
+    if (forward_packed(input_node_size, output_node_size, frame_size)) { ForwardSpace const f(forward, input_node_size, output_node_size, frame_size, false); }
+    else { sums_of(forward, direct_shape(output_node_size, frame_size, input_node_size).slabs, output_node_size, frame_size); }
+    if (backward_packed(input_node_size, output_node_size, frame_size)) { BackwardSpace const b(backward, input_node_size, output_node_size, frame_size, false); }
+    else { DirectBackwardSpace const d(backward, input_node_size, output_node_size, frame_size, true); }
     return forward.at > backward.at ? forward.at : backward.at;
 }
 

@@ -22,7 +22,8 @@ struct LossFinishArgs {
     int    tiles, frames, channels;
 };
 
-// Eight frames per workgroup; 64 threads of a frame take its tiles in turn (neighbouring lanes neighbouring frames) and are joined two by two through LDS
+// Eight frames per workgroup; 64 threads of a frame take its tiles in turn (neighbouring lanes neighbouring frames) and are joined two by two through LDS (3.9 us for 1001
+// channels x 1000 frames, 7.4 for 32768 x 4096: a chain of loads and joins)
 __global__ __launch_bounds__(kFinishFrames * kFinishGroups) void dense_loss_finish_kernel(LossFinishArgs a)
 {
     __shared__ float2 part[kFinishGroups][kFinishFrames];

@@ -8,9 +8,13 @@
 //
 // Two launches.  The first reads each operand as it lies and leaves its halves in the order in which the matrix instructions want them: blocks of 32 rows x 16 k,
 // 1 KiB each, lane l's sixteen bytes (row l & 31, k 8 (l >> 5) .. + 8) at 16 l, so that the second launch moves them to LDS and from there to registers with 16-byte accesses
-// that meet no bank twice, without a transposition anywhere.  In the second, a workgroup of eight wavefronts owns 256 x 256 elements (128 x 128: four) and walks k in stages of 16,
-// the loads of the next three stages to LDS in flight behind the products of the present one.
+// that meet no bank twice, without a transposition anywhere.  In the second, a workgroup of eight wavefronts owns 256 x 256 elements (256 x 128 or 128 x 128: four) and walks k in stages of
+// 16, the loads of the next three stages to LDS in flight behind the products of the present one (the small tile: of the next four, and its halves one stage ahead in registers).
 // Where there are too few tiles for the device, several workgroups share a tile's k axis and a third launch adds their sums in a fixed order.
+//
+// What bounds it: the matrix instructions and the power they take.  4096 x 4096 x 8192 with packed bits is 550 GFLOP of halves in 451 to 501 us, both products of its backward pass on real
+// values 1650 in 1345 to 1500: 1.1 to 1.2 PFLOP/s, where a plain product of halves by the library reaches 1.17 to 1.26.  Five or seven stages ahead changed nothing.  Packing is
+// bound by memory: 205 MB in 57 us and 1.2 GB in 370, 3.3 to 3.6 TB/s.  Small problems are bound by two launches of 12 us and more whose workgroups run once.
 #pragma once
 
 #include "dense_operands.hpp"
@@ -58,7 +62,8 @@ __device__ __forceinline__ float magnitude(float v) { float const a = fabsf(v); 
 
 // Eight rows and all their k per workgroup: what it writes are whole lines of 128 bytes (eight rows' 16), and with 64 groups of eight k side by side a thread holds all values of a row of up to 4096
 // between finding the largest and splitting.  Where rows are columns of the buffer it reads 32 bytes at a time; workgroups that share a line run on one XCD (xcd_run).  With 32 rows per
-// workgroup a batch of 65 frames of 6144 bits and as many weights took 30 us.
+// workgroup a batch of 65 frames of 6144 bits and as many weights took 14 us longer.  1024 threads instead of 512 where a row is longer than these hold: 6144 inputs x 1024 x 1024 70 us and 74,
+// 16384 x 512 x 512 90 and 95; where they do hold it 92.6 and 88.3 (a backward pass over 1024 x 1024 x 4096 frames).
 template <int KIND, int THREADS>
 __device__ __forceinline__ void pack_rows(PackJob const &j, int block, float *share)
 {

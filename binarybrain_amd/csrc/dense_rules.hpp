@@ -11,45 +11,77 @@ namespace bbhip {
 constexpr int kDenseNodesMost = 1 << 24, kDenseFramesMost = 1 << 25, kDenseStrideMost = 33 << 20;
 
 // How a product straight from its operands is divided: tiles of 32 x 32, wavefronts that share a tile's k axis (chunks of 32), and workgroups that do.
+// Wavefronts: 512 x 512 (256 tiles) over 128 inputs take 4.5 us with eight and 5.0 with four, over 512 6.5 and 9.0; 1024 x 600 (608 tiles) over 128 6.8 with four and 7.7 with eight,
+// over 512 13.2 and 13.7; 4096 x 1024 over 64 17.1 with one and 19.9 with four, 2048 x 1024 over 64 12.6 and 11.9.  (Sixteen are within 0.3 us of eight.)
+// Slabs: a chunk for every wavefront while there is a compute unit for each workgroup, four chunks and twice as many workgroups otherwise.  128 x 128 over 512 inputs 6.3 us whole and 7.3 in
+// two, over 1024 9.0 and (in four) 7.2, over 8192 48.5 and (in sixteen) 10.1; 1024 x 64 over 2048 15.0 whole, 9.3 in four, 9.9 in eight; 1024 x 128 over 4096 29.2 whole, 19.9 in four,
+// 21.3 in eight; 512 x 512 over 4096 30.1 whole and 30.8 in two.  A slab is whole rounds of the wavefronts' chunks: 1024 x 65 over 6144 takes 23.9 in eight and 27.2 in six.
 struct DirectShape { int waves, n_tiles, slabs, slab_chunks; long long tiles; };
-inline DirectShape direct_shape(int m, int n, int k, int waves = 0)
+inline DirectShape direct_shape(int m, int n, int k, int waves = 0, int shared_from = 24)
 {
     DirectShape s;
     int const chunks = ceil_div(k, 32);
     s.n_tiles = ceil_div(n, 32);
     s.tiles = (long long)ceil_div(m, 32) * s.n_tiles;
-    s.waves = waves ? waves : chunks > 16 ? (s.tiles <= 64 && chunks <= 64 ? 16 : 8) : chunks > 2 || s.tiles < 2048 ? 4 : 1;
-    // two chunks for a wavefront are what a join is worth from six on
+    s.waves = waves ? waves : s.tiles <= 512 || chunks > 16 ? 8 : chunks > 2 || s.tiles <= 2048 ? 4 : 1;
     int slabs = 1;
-    if (s.tiles < 512 && chunks >= 6 * s.waves) {
-        slabs = chunks / (2 * s.waves);
-        int const most = (int)(1024 / s.tiles);
-        if (slabs > most) { slabs = most; }
+    if (s.tiles < 256 && chunks >= shared_from) {
+        auto const least = [](int a, long long b) { return a < b ? a : (int)b; };
+        int const one = least(chunks / s.waves, 256 / s.tiles), four = least(chunks / (4 * s.waves), 512 / s.tiles);
+        slabs = one > four ? one : four;
+        slabs = slabs < 1 ? 1 : slabs > 16 ? 16 : slabs;
     }
-    s.slab_chunks = ceil_div(chunks, slabs);
+    s.slab_chunks = slabs > 1 ? ceil_div(ceil_div(chunks, slabs), s.waves) * s.waves : chunks;
     s.slabs = ceil_div(chunks, s.slab_chunks);
     return s;
 }
 
+// Logits: the launch that joins slabs is one more of a loss's four, so a longer axis is whole (a loss of ten classes, 1024 inputs, 64 frames takes 20 us whole and 22 shared).
+inline DirectShape logits_shape(int channels, int frames, int inputs) { return direct_shape(channels, frames, inputs, 0, 48); }
+
 // Both products of a backward pass: as many wavefronts for either, and so one launch, while the device holds all of them at once or nearly so; beyond that a short k axis leaves most of
-// the longer one's wavefronts without work (9932 x 6136 x 25 frames 1143 us, with a launch each 470; 191 x 227 x 56 frames 8.3 and 16.8).
+// the longer one's wavefronts without work (9932 x 6136 x 25 frames 1143 us, with a launch each 470; 191 x 227 x 56 frames 8.3 and 16.8).  256 x 256 x 256 (136 tiles) 8.1 us with eight and
+// 9.4 with four, 1024 x 256 x 64 frames (328) 9.3 and 8.1, 512 x 512 x 512 (528) 20.7 and 18.1; 256 x 256 x 4096 frames (1096) 35.0 with four and 44.6 with a launch each.
 inline void direct_shapes(int m0, int n0, int k0, int m1, int n1, int k1, DirectShape &s0, DirectShape &s1)
 {
     s0 = direct_shape(m0, n0, k0);
     s1 = direct_shape(m1, n1, k1);
-    if (s0.waves > 8) { s0 = direct_shape(m0, n0, k0, 8); }
-    if (s1.waves > 8) { s1 = direct_shape(m1, n1, k1, 8); }
-    if (s0.tiles + s1.tiles <= 1024 && s0.waves != s1.waves) {
-        int const more = s0.waves > s1.waves ? s0.waves : s1.waves, waves = more < 8 ? more : 8;
+    if (s0.tiles + s1.tiles <= 2048) {
+        int const waves = s0.tiles + s1.tiles <= 256 ? 8 : 4;
         s0 = direct_shape(m0, n0, k0, waves);
         s1 = direct_shape(m1, n1, k1, waves);
     }
 }
 
-// Whether a product goes by way of packed halves (two launches at least, and both operands are written once more) instead of straight from its operands.
-inline bool product_packed(int m, int n, int k) { return (long long)m * n * k >= 1LL << 29 && m >= 32 && n >= 32 && k >= 32; }
+// Whether a product goes by way of packed halves (two launches at least, and both operands are read and written once more) instead of straight from its operands: the products saved
+// against the launch and the values packed.  A forward pass, us straight and packed: 1001 x 500 x 777 inputs 22 and 27, 1001 x 1000 x 777 39 and 29, 1024 x 1024 x 1024 30 and 30,
+// 2048 x 1024 x 256 20 and 22, 4096 x 64 x 4096 35 and 52 (the weights are all there is to read), 4096 x 4096 x 64 55 and 35, 8192 x 1024 x 128 47 and 28.
+inline bool long_enough(int a, int b, int c) { return a >= 32 && b >= 32 && c >= 32; }
+inline double volume(int a, int b, int c) { return (double)a * b * c; }
+inline bool forward_packed(int inputs, int outputs, int frames)
+{
+    return long_enough(inputs, outputs, frames) && volume(inputs, outputs, frames) >= (1 << 29) + 80.0 * inputs * ((double)outputs + frames);
+}
 
-// Tiles of a packed product: 256 x 256 by eight wavefronts, 256 x 128 or 128 x 128 by four (two such workgroups on a compute unit); stages that lie in LDS.
+// A backward pass, which packs dz as rows and as columns, inputs x outputs x frames: 512 x 512 x 512 18 and 26, 512 x 512 x 1024 31 and 30, 777 x 1001 x 500 44 and 35, 1024 x 1024 x 1024 82
+// and 39, 256 x 2048 x 1024 53 and 43, 96 x 4096 x 1024 48 and 65, 64 x 8192 x 1024 70 and 90, 128 x 8192 x 1024 100 and 95, 4096 x 4096 x 32 74 and 100, x 64 96 and 104.
+inline bool backward_packed(int inputs, int outputs, int frames)
+{
+    return long_enough(inputs, outputs, frames) &&
+           volume(inputs, outputs, frames) >= (3 << 26) + 48.0 * (2.0 * outputs * frames + (double)inputs * frames + (double)inputs * outputs);
+}
+
+// A loss, with its gradients or alone (a frame's loss has the same bits either way): with gradients 512 inputs x 512 channels x 1024 frames 47 and 54, 777 x 1001 x 500 73 and 57, 784 x 512 x 1024 62 and 59, 64 x 8192 x 1024 115 and 115, 128 x 8192 x 1024 168 and
+// 121, 4096 x 64 x 1024 61 and 72, 4096 x 4096 x 32 104 and 160, x 64 138 and 166.
+inline bool loss_packed(int inputs, int channels, int frames)
+{
+    return long_enough(inputs, channels, frames) &&
+           volume(inputs, channels, frames) >= 2.5e8 + 25.0 * ((double)channels * frames + 4.0 * inputs * ((double)channels + frames));
+}
+
+// Tiles of a packed product: 256 x 256 by eight wavefronts, 256 x 128 or 128 x 128 by four (two such workgroups on a compute unit); stages that lie in LDS.  Large, middle and small tiles, us:
+// 4096 x 4096 x 8192 with packed bits 494, 493, 548, its backward pass on real values 1550, 1611, 1737; 784 inputs x 6144 x 1024 82, 61, 56; backward 1024 x 1001 x 1000 55, 51, 44;
+// 10007 channels x 513 frames x 1024 bits 78, 62, 55.
 enum PackedTile : int { kTileLarge = 0, kTileMiddle = 1, kTileSmall = 2, kTileSizes = 3 };
 constexpr int kTileRows[kTileSizes] = {256, 256, 128}, kTileColumns[kTileSizes] = {256, 128, 128}, kTileThreads[kTileSizes] = {512, 256, 256};
 constexpr int kTileBuffers[kTileSizes] = {4, 3, 4}, kTileWaveRows[kTileSizes] = {128, 128, 64}, kTileAtOnce[kTileSizes] = {256, 512, 512};
@@ -86,7 +118,8 @@ inline double packed_length(PackedShape const &s, long long workgroups)
 }
 inline int    packed_at_once(PackedShape const &s) { return kTileAtOnce[s.size]; }
 
-// sums written and read again at about 4 TB/s, and a launch
+// Sums written and read again at about 4 TB/s, and a launch: 1024 outputs x 1024 frames x 2048 inputs take 54 us with no tile shared and 39 with its k axis in three parts, 784 x 6144 x 1024 55
+// whole and 79 in two, a backward pass 1024 x 1001 x 1000 40 and 44.
 inline double join_cost(PackedShape const &s, int m, int n) { return s.slabs > 1 ? (double)s.slabs * m * n * 8.0 / 4.0e6 / 0.16 : 0.0; }
 constexpr double kJoinLaunch = 25.0;
 
@@ -130,7 +163,8 @@ inline PackedShape best_shape(int m, int n, int k)
     return s;
 }
 
-// The channels of a loss are taken in pieces, so that what is held of the logits does not grow with their number.
+// The channels of a loss are taken in pieces, so that what is held of the logits does not grow with their number: 256 MiB of them: 32768 channels x 4096 frames take 3.31 ms
+// (64 MiB: 3.72, more launches of fewer tiles).
 constexpr int kLossTile = 32;               // channels per (largest, sum of exponents) of the direct products and of joined sums
 struct LossPlan {
     bool packed;
@@ -144,7 +178,7 @@ struct LossPlan {
 inline LossPlan loss_plan(int inputs, int channels, int frames)
 {
     LossPlan p;
-    p.packed = product_packed(channels, frames, inputs);
+    p.packed = loss_packed(inputs, channels, frames);
     p.stride = ceil_div(frames, 64) * 64;
     long long const most = (64ll << 20) / p.stride / 256 * 256;
     p.piece = most < 256 ? 256 : (int)(most < (1 << 24) ? most : (1 << 24));

@@ -4,7 +4,8 @@
 // Sizes and addresses lie in device tables, as the optimizer has them, so the host does not know how much there is: a fixed number of workgroups walks pieces of
 // 4096 elements of whatever tensors there are, piece c of the whole list going to workgroup c mod gridDim.  Each workgroup finds its pieces by a running sum of the
 // tensors' piece counts, 256 tensors at a time.  Squares are summed in 64 bits: the kernel waits for memory, and a sum in 64 bits neither overflows nor loses small
-// gradients beside large ones.  The order of the sums is fixed by the sizes alone.  What bounds it: HBM (4 bytes per element).
+// gradients beside large ones.  The order of the sums is fixed by the sizes alone.  What bounds it: HBM (4 bytes per element), or the
+// latency of two launches: three tensors of 463 thousand values 4.3 + 2.5 us; 2^26 values 80 us, and the Adam step on them 345 (1.9 GB at 5.4 TB/s).
 #pragma once
 
 #include "vector_kernels.hpp"

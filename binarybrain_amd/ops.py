@@ -87,6 +87,8 @@ class AdamState:
             for tensor in (p, *others):
                 if not tensor.is_cuda or not tensor.is_contiguous() or tensor.dtype != torch.float32 or tensor.numel() != p.numel():
                     raise capi.BbhipError("AdamState: contiguous float32 device tensors, those of a parameter of one size")
+        held = [t.data_ptr() for t in (*self.params, *self.grads, *self.m, *self.v) if t.numel()]
+        self.twice = len(set(held)) != len(held)
         dev = params[0].device
         table = lambda ts: torch.tensor([t.data_ptr() for t in ts], dtype=torch.int64, device=dev)
         self.t_params, self.t_grads, self.t_m, self.t_v = table(self.params), table(self.grads), table(self.m), table(self.v)
@@ -101,6 +103,8 @@ class AdamState:
         return np.float32(native.adam_rate(self.lr, self.b1, self.b2))
 
     def _clipped(self, max_norm, zero_grads):
+        if self.twice:
+            raise capi.BbhipError("AdamState: a tensor is listed twice, which a step with clipped gradients cannot have")
         norm = native.adam_clipped(self.t_size, self.t_params, self.t_grads, self.t_m, self.t_v, self.lr_t(), *self.betas, float(max_norm), zero_grads)
         self.b1 = self.b1 * self.beta1
         self.b2 = self.b2 * self.beta2

@@ -112,3 +112,14 @@ def test_lists_that_are_refused():
     for bad in (-1.0, float("nan")):
         with pytest.raises(BbhipError, match="max_norm"):
             ops.GradientTable([t]).norm(bad)
+
+
+def test_a_clipped_step_refuses_a_tensor_twice():
+    import torch
+    from binarybrain_amd import ops
+    from binarybrain_amd.capi import BbhipError
+    p, q, g, h = (torch.ones(8, device="cuda") for _ in range(4))
+    for params, grads in (([p, p], [g, h]), ([p, q], [g, g]), ([p], [p])):
+        for step in ("step", "update"):
+            with pytest.raises(BbhipError, match="twice"):
+                getattr(ops.AdamState(params, grads), step)(max_norm=1.0)

@@ -116,65 +116,96 @@ __device__ __forceinline__ void load_floats(float const *p, bool vec, float (&v)
     for (int j = 0; j < N; ++j) { v[j] = p[j]; }
 }
 
-// N values from k on, k a multiple of N (4, 8 or 16); 0 behind the last one.  The row exists.
+// Values at k, k + 1, ... of a row; behind the last one the last one again, whose use the caller undoes.  `vec`: all exist, and 16-byte loads are aligned.
+template <class T, int N>
+__device__ __forceinline__ void load_run(T const *p, int k, int depth, bool vec, T (&v)[N])
+{
+    if (vec) {
+#pragma unroll
+        for (int j = 0; j < N; j += 4) {
+            uint4 const q = *reinterpret_cast<uint4 const *>(p + k + j);
+            v[j] = __builtin_bit_cast(T, q.x); v[j + 1] = __builtin_bit_cast(T, q.y); v[j + 2] = __builtin_bit_cast(T, q.z); v[j + 3] = __builtin_bit_cast(T, q.w);
+        }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) { v[j] = p[min(k + j, depth - 1)]; }
+}
+
+// the same where consecutive k are a row pitch apart
+template <class T, int N>
+__device__ __forceinline__ void load_column(T const *p, long long stride, int left, T (&v)[N])
+{
+    if (left >= N) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) { v[j] = p[j * stride]; }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) { v[j] = *p; p += j + 1 < left ? stride : 0; }
+}
+
+// gradient_through without a branch (the activation is the same for all)
+__device__ __forceinline__ float gradient_of(float dy, float y, int activation)
+{
+    bool const closed = (activation == kActRelu && y <= 0.0f) || (activation == kActHardTanh && (y <= -1.0f || y >= 1.0f));
+    float const slope = activation == kActSigmoid ? y * (1.0f - y) : 1.0f;
+    return closed ? 0.0f : dy * slope;
+}
+
+// N values from k on, k a multiple of N (8); 0 behind the last one.  The row and the first value exist.  Gradients through an activation take one path for whole and cut runs: the callers unroll this, and a launch
+// waits for its code first (with a path per value for cut runs and a branch per value for the activation the packing of a backward pass over 1024 x 1001 x 1000 took 15.0 us instead of 12.0, of
+// 4096 x 4096 x 8192 369 instead of 355; values that are only read lose more by the bounds, 14.9 us and 13.4 for 784 x 6144 x 1024).
 template <int KIND, int N>
 __device__ __forceinline__ void load_values(Operand const &o, int row, int k, float (&v)[N])
 {
-    if (k + N > o.depth) {
+    int const left = o.depth - k;
+    bool const whole = left >= N;
+    if (!whole && ((KIND != kGradRows && KIND != kGradColumns) || o.mode == kGradSoftmax)) {
 #pragma unroll
         for (int j = 0; j < N; ++j) { v[j] = k + j < o.depth ? operand_at<KIND>(o, row, k + j) : 0.0f; }
         return;
     }
     if constexpr (KIND == kRows) {
-        if (row == o.ones) {
-#pragma unroll
-            for (int j = 0; j < N; ++j) { v[j] = 1.0f; }
-            return;
-        }
-        load_floats(static_cast<float const *>(o.p) + row * o.stride + k, o.vec, v);
+        load_run(static_cast<float const *>(o.p) + row * o.stride, k, o.depth, o.vec, v);
         if (o.coef) {
             float c[N];
-            load_floats(o.coef + k, true, c);
+            load_run(o.coef, k, o.depth, true, c);
 #pragma unroll
             for (int j = 0; j < N; ++j) { v[j] = c[j] == 0.0f ? 0.0f : v[j]; }
         }
     }
-    if constexpr (KIND == kColumns) {
-        float const *p = static_cast<float const *>(o.p) + k * o.stride + row;
-#pragma unroll
-        for (int j = 0; j < N; ++j) { v[j] = p[j * o.stride]; }
-    }
+    if constexpr (KIND == kColumns) { load_column(static_cast<float const *>(o.p) + k * o.stride + row, o.stride, N, v); }
     if constexpr (KIND == kBitRows) {
-        uint32_t const w = row == o.ones ? 0xffffffffu : static_cast<uint32_t const *>(o.p)[row * o.stride + (k >> 5)] >> (k & 31);
+        uint32_t const w = static_cast<uint32_t const *>(o.p)[row * o.stride + (k >> 5)] >> (k & 31);
 #pragma unroll
         for (int j = 0; j < N; ++j) { v[j] = (float)((w >> j) & 1u); }
     }
     if constexpr (KIND == kBitColumns) {
-        uint32_t const *p = static_cast<uint32_t const *>(o.p) + k * o.stride + (row >> 5);
+        uint32_t w[N];
+        load_column(static_cast<uint32_t const *>(o.p) + k * o.stride + (row >> 5), o.stride, N, w);
 #pragma unroll
-        for (int j = 0; j < N; ++j) { v[j] = (float)((p[j * o.stride] >> (row & 31)) & 1u); }
+        for (int j = 0; j < N; ++j) { v[j] = (float)((w[j] >> (row & 31)) & 1u); }
     }
     if constexpr (KIND == kGradRows) {
-        long long const at = row * o.stride + k;
-        load_floats(static_cast<float const *>(o.p) + at, o.vec, v);
+        long long const at = row * o.stride;
+        load_run(static_cast<float const *>(o.p) + at, k, o.depth, o.vec && whole, v);
         if (o.mode == kGradSoftmax) {
             float top[N], share[N], coef[N];
-            load_floats(o.top + k, true, top); load_floats(o.share + k, true, share); load_floats(o.coef + k, true, coef);
+            load_run(o.top, k, o.depth, true, top); load_run(o.share, k, o.depth, true, share); load_run(o.coef, k, o.depth, true, coef);
 #pragma unroll
             for (int j = 0; j < N; ++j) { v[j] = softmax_gradient(v[j], top[j], share[j], coef[j], o.label[k + j], row + o.first); }
         }
         else if (o.mode != kActNone) {
             float y[N];
-            load_floats(o.y + at, o.vec, y);
+            load_run(o.y + at, k, o.depth, o.vec && whole, y);
 #pragma unroll
-            for (int j = 0; j < N; ++j) { v[j] = gradient_through(v[j], y[j], o.mode); }
+            for (int j = 0; j < N; ++j) { v[j] = gradient_of(v[j], y[j], o.mode); }
         }
     }
     if constexpr (KIND == kGradColumns) {
         long long const at = k * o.stride + row;
-        float const *p = static_cast<float const *>(o.p) + at;
-#pragma unroll
-        for (int j = 0; j < N; ++j) { v[j] = p[j * o.stride]; }
+        load_column(static_cast<float const *>(o.p) + at, o.stride, left, v);
         if (o.mode == kGradSoftmax) {
             float const top = o.top[row], share = o.share[row], coef = o.coef[row];
             int const label = o.label[row];
@@ -182,9 +213,15 @@ __device__ __forceinline__ void load_values(Operand const &o, int row, int k, fl
             for (int j = 0; j < N; ++j) { v[j] = softmax_gradient(v[j], top, share, coef, label, k + j + o.first); }
         }
         else if (o.mode != kActNone) {
+            float y[N];
+            load_column(o.y + at, o.stride, left, y);
 #pragma unroll
-            for (int j = 0; j < N; ++j) { v[j] = gradient_through(v[j], o.y[at + j * o.stride], o.mode); }
+            for (int j = 0; j < N; ++j) { v[j] = gradient_of(v[j], y[j], o.mode); }
         }
+    }
+    if (!whole) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) { v[j] = j < left ? v[j] : 0.0f; }
     }
 }
 

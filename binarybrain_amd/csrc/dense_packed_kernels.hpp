@@ -14,7 +14,7 @@
 //
 // What bounds it: the matrix instructions and the power they take.  4096 x 4096 x 8192 with packed bits is 550 GFLOP of halves in 451 to 501 us, both products of its backward pass on real
 // values 1650 in 1345 to 1500: 1.1 to 1.2 PFLOP/s, where a plain product of halves by the library reaches 1.17 to 1.26.  Five or seven stages ahead changed nothing.  Packing is
-// bound by memory and by its two phases, loads and then stores: 205 MB in 57 us, 1.34 GB in 369, 3.6 TB/s.  Small problems are bound by two launches of 12 us and more whose workgroups run once.
+// bound by memory and by its two phases, loads and then stores: 205 MB in 57 us, 1.34 GB in 355, 3.6 to 3.8 TB/s.  Small problems are bound by two launches of 12 us and more whose workgroups run once.
 #pragma once
 
 #include "dense_operands.hpp"
@@ -161,7 +161,7 @@ __device__ __forceinline__ void pack_rows(PackJob const &j, int block, float *sh
 }
 
 template <int THREADS>
-__global__ __launch_bounds__(THREADS) void dense_pack_kernel(PackArgs a)
+__global__ __launch_bounds__(THREADS, 4) void dense_pack_kernel(PackArgs a)
 {
     __shared__ float share[2 * THREADS / 64 * kPackRows];
     int block = blockIdx.x, which = 0;

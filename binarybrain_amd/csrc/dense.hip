@@ -135,7 +135,8 @@ int direct_forward(Product const &p, bool bit, float *sums, hipStream_t st, char
     } while (0)
     if (s.waves == 8)      { BBHIP_DIRECT(8); }
     else if (s.waves == 4) { BBHIP_DIRECT(4); }
-    else                   { BBHIP_DIRECT(1); }
+    else if (s.waves == 1) { BBHIP_DIRECT(1); }
+    else                   { return fail("%s: no kernel of %d wavefronts", name, s.waves); }
 #undef BBHIP_DIRECT
     BBHIP_LAUNCH_CHECK();
     return join(sums_to_join(d), PackedProduct{}, st, name);
@@ -186,7 +187,8 @@ int direct_backward(Product const &dw, Product const &dx, DirectBackwardSpace co
         } while (0)
         if (waves == 8)      { BBHIP_DIRECT(8); }
         else if (waves == 4) { BBHIP_DIRECT(4); }
-        else                 { BBHIP_DIRECT(1); }
+        else if (waves == 1) { BBHIP_DIRECT(1); }
+        else                 { return fail("%s: no kernel of %d wavefronts", name, waves); }
 #undef BBHIP_DIRECT
         BBHIP_LAUNCH_CHECK();
     }
@@ -226,7 +228,7 @@ struct Jobs {
     {
         long long total = 0;
         for (int i = 0; i < count; ++i) { total += a.job[i].blocks; }
-        bool const wide = deepest > kPackHeld * 512;
+        bool const wide = pack_is_wide(deepest);
         if (check_tiles(total, wide ? 1024 : 512, name)) { return 1; }
         if (wide) { launch(dense_pack_kernel<1024>, dim3((unsigned)total), dim3(1024), 0, st, a); }
         else      { launch(dense_pack_kernel<512>, dim3((unsigned)total), dim3(512), 0, st, a); }

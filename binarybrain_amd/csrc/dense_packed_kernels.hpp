@@ -18,14 +18,12 @@
 #pragma once
 
 #include "dense_operands.hpp"
+#include "dense_rules.hpp"
 
 namespace bbhip {
 
 typedef _Float16 DenseHalf8 __attribute__((ext_vector_type(8)));
 typedef float    DenseAcc16 __attribute__((ext_vector_type(16)));
-
-constexpr int kPackRows = 8;
-constexpr int kPackHeld = 8;                    // groups of eight values that a thread keeps between finding the largest and splitting
 
 struct PackJob {
     Operand src;
@@ -62,8 +60,7 @@ __device__ __forceinline__ float magnitude(float v) { float const a = fabsf(v); 
 
 // Eight rows and all their k per workgroup: what it writes are whole lines of 128 bytes (eight rows' 16), and with 64 groups of eight k side by side a thread holds all values of a row of up to 4096
 // between finding the largest and splitting.  Where rows are columns of the buffer it reads 32 bytes at a time; workgroups that share a line run on one XCD (xcd_run).  With 32 rows per
-// workgroup a batch of 65 frames of 6144 bits and as many weights took 14 us longer.  1024 threads instead of 512 where a row is longer than these hold: 6144 inputs x 1024 x 1024 70 us and 74,
-// 16384 x 512 x 512 90 and 95; where they do hold it 92.6 and 88.3 (a backward pass over 1024 x 1024 x 4096 frames).
+// workgroup a batch of 65 frames of 6144 bits and as many weights took 14 us longer.
 template <int KIND, int THREADS>
 __device__ __forceinline__ void pack_rows(PackJob const &j, int block, float *share)
 {

@@ -1,0 +1,20 @@
+"""CPU suite: which form (straight or packed, wavefronts, tiles, shared k axes, pieces) a size of a dense layer or of the loss on top of one takes (tests/cpp/test_dense_forms.cpp)."""
+import os
+import subprocess
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def tool(*args):
+    exe = os.path.join(ROOT, "tests", "cpp", "test_dense_forms")
+    if not os.path.exists(exe):
+        from binarybrain_amd.build import build_cpp_tests
+        build_cpp_tests()
+    res = subprocess.run([exe, *map(str, args)], stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=120)
+    assert res.returncode == 0, res.stdout
+    return res.stdout.strip()
+
+
+def test_rules():
+    """no rule asks for a number of wavefronts that no kernel has"""
+    tool("--rules")

@@ -23,7 +23,7 @@ struct Product {
     Operand     a, b;
     int         kind_a, kind_b;
     DenseOutput out;
-    bool wanted = true, again = false;          // again: elements that come out as no number are formed again
+    bool wanted = true;
 };
 
 Operand rows_of(float const *p, long long stride, int rows, int depth)
@@ -249,7 +249,7 @@ int packed_product(PackedProduct &d, Product const &p, PackedShape const &s, Pac
     d.sums = sums; d.sums_pitch = sums_pitch(p.out.columns); d.sums_slab = d.sums_pitch * p.out.rows;
     d.out = p.out;
     d.out.line = nullptr;               // (summed where the halves are written)
-    d.src_a = p.a; d.src_b = p.b; d.kind_a = p.again ? p.kind_a : -1; d.kind_b = p.kind_b;
+    d.src_a = p.a; d.src_b = p.b; d.kind_a = p.kind_a; d.kind_b = p.kind_b;
     return 0;
 }
 
@@ -388,7 +388,7 @@ int dense_forward(void const *x, bool bit, void *y, bool bit_out, float const *W
     Product p;
     p.a = rows_of(W, inputs, outputs, inputs);
     p.b = frames_as_columns(x, x_stride, inputs, frames);
-    p.kind_a = kRows; p.kind_b = bit ? kBitColumns : kColumns; p.again = true;
+    p.kind_a = kRows; p.kind_b = bit ? kBitColumns : kColumns;
     p.out = DenseOutput{};
     p.out.kind = bit_out ? kOutBits : kOutForward;
     p.out.rows = outputs; p.out.columns = frames; p.out.out = y; p.out.stride = y_stride;
@@ -439,7 +439,7 @@ int dense_backward(void const *x, bool bit, float const *dy, float const *y, flo
     i.wanted = dx != nullptr;
     i.a = rows_of(W, inputs, inputs, outputs);
     i.b = g; i.b.rows = frames; i.b.depth = outputs;
-    i.kind_a = kColumns; i.kind_b = kGradColumns; w.again = i.again = true;
+    i.kind_a = kColumns; i.kind_b = kGradColumns;
     i.out = DenseOutput{};
     i.out.kind = kOutStore; i.out.rows = inputs; i.out.columns = frames; i.out.out = dx; i.out.stride = dx_stride;
     hipStream_t const st = static_cast<hipStream_t>(stream);
@@ -527,15 +527,17 @@ int dense_loss(void const *x, bool bit, float const *W, float const *b, int cons
         Product p;
         p.a = rows_of(W + (size_t)first * inputs, inputs, count, inputs);
         p.b = frames_as_columns(x, x_stride, inputs, frames);
+        p.kind_a = kRows; p.kind_b = bit ? kBitColumns : kColumns;
         p.out = DenseOutput{};
         p.out.kind = kOutLogits; p.out.rows = count; p.out.columns = frames; p.out.out = store ? logits : nullptr; p.out.stride = s.plan.stride;
         p.out.bias = b ? b + first : nullptr;
         p.out.partial = s.partial + (size_t)(first / s.plan.tile) * frames;
         p.out.label = label; p.out.label_logit = s.label_logit; p.out.first_channel = first;
+        p.out.channels = channels; p.out.weight = weight;
         if (!s.plan.packed) { return direct_forward(p, bit, s.logit_sums, st, name); }
         Jobs jobs;
-        jobs.add(s.W.job(p.a, kRows));
-        if (!x_packed) { jobs.add(s.x.job(p.b, bit ? kBitColumns : kColumns)); x_packed = true; }
+        jobs.add(s.W.job(p.a, p.kind_a));
+        if (!x_packed) { jobs.add(s.x.job(p.b, p.kind_b)); x_packed = true; }
         PackedShape const shape = packed_shape(s.plan.logits.size, s.plan.logits.slabs, count, frames, inputs);
         PackedProduct d;
         Packed W_piece = s.W;

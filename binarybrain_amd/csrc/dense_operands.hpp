@@ -251,7 +251,16 @@ struct DenseOutput {
     int const *label;
     float *label_logit;
     int   first_channel;            // kOutLogits: channel of row 0 (a piece of the channels)
+    int   channels;                 // kOutLogits: of all pieces
+    float const *weight;            // kOutLogits: of the frames (null: 1)
 };
+
+// kOutLogits: whether anything is made of a frame's logits
+__device__ __forceinline__ bool frame_counts(DenseOutput const &o, int n)
+{
+    int const label = o.label[n];
+    return label >= 0 && label < o.channels && !(o.weight && o.weight[n] == 0.0f);
+}
 
 __device__ __forceinline__ float before_activation(DenseOutput const &o, float d, int m, int n)
 {

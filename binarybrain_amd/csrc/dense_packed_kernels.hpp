@@ -17,7 +17,7 @@
 // bound by memory and by its two phases, loads and then stores: 205 MB in 57 us, 1.34 GB in 355, 3.6 to 3.8 TB/s.  Small problems are bound by two launches of 12 us and more whose workgroups run once.
 #pragma once
 
-#include "dense_operands.hpp"
+#include "dense_direct_kernels.hpp"
 #include "dense_rules.hpp"
 
 namespace bbhip {
@@ -189,33 +189,199 @@ struct PackedProduct {
     long long sums_pitch, sums_slab;
     DenseOutput out;
     Operand src_a, src_b;           // where an element is formed again if it is no number
-    int   kind_a, kind_b;           // (kind_a negative: not asked for)
+    int   kind_a, kind_b;           // (sums of products straight from the operands: kind_a negative, there is nothing to form again)
 };
-
-// An element straight from the operands.  The halves of an infinity times a lower half of 0 are no number where the value's product is infinite: elements that come out as no number are
-// formed again in fp32, value by value, so that infinities and NaN are what the formula says.  (Slow, and only for operands that hold some.)
-__device__ __forceinline__ float element_again(Operand const &a, int kind_a, Operand const &b, int kind_b, int m, int n)
-{
-    float d = 0.0f;
-    for (int k = 0; k < a.depth && d == d; ++k) {
-        float const u = kind_a == kRows ? operand_at<kRows>(a, m, k) : kind_a == kColumns ? operand_at<kColumns>(a, m, k) : operand_at<kGradRows>(a, m, k);
-        float const v = kind_b == kRows ? operand_at<kRows>(b, n, k) : kind_b == kColumns ? operand_at<kColumns>(b, n, k) :
-                        kind_b == kBitRows ? operand_at<kBitRows>(b, n, k) : kind_b == kBitColumns ? operand_at<kBitColumns>(b, n, k) : operand_at<kGradColumns>(b, n, k);
-        d = fmaf(u, v, d);
-    }
-    return d;
-}
-
 
 // What a launch is for: y or its bits, products as they are (or a slab's sums), logits.
 enum PackedUse : int { kUseForward = 0, kUseStore = 1, kUseLogits = 2 };
 
 // 32 x 64 elements of a wavefront lie in LDS as rows of kTilePitch floats.
 constexpr int kTilePitch = 68;
+// What such a tile has in the place of an element that is not to be stored: a NaN of its own (`marks`: there may be some).  The elements that are stored are never this one: NaN are formed
+// again, and plain_nan() is what they are then.
+constexpr uint32_t kNotStored = 0x7fb0a5a5u;
+__device__ __forceinline__ bool stored(float v) { return __builtin_bit_cast(uint32_t, v) != kNotStored; }
+__device__ __forceinline__ float plain_nan(float v) { return v == v ? v : __builtin_bit_cast(float, 0x7fc00000u); }
+
+// ---- elements formed again ----------------------------------------------------------------------------------------------------------------
+// The halves of an infinity times a lower half of 0 are no number where the value's product is infinite: an element that comes out as no number is formed again in fp32 straight from the
+// operands, so that infinities and NaN are what the formula says; its neighbours keep the bits that they have.
+
+// By a wavefront: its lanes take the k in turn, four at a time so that their loads overlap.
+template <int KA, int KB>
+__device__ __forceinline__ float element_again(Operand const &a, Operand const &b, int m, int n, int lane)
+{
+    float d = 0.0f;
+#pragma nounroll
+    for (int k0 = lane; k0 < a.depth; k0 += 4 * 64) {
+        float u[4], v[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            int const k = min(k0 + q * 64, a.depth - 1);
+            u[q] = operand_at<KA>(a, m, k);
+            v[q] = operand_at<KB>(b, n, k);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) { if (k0 + q * 64 < a.depth) { d = fmaf(u[q], v[q], d); } }
+    }
+#pragma unroll
+    for (int step = 32; step > 0; step /= 2) { d += __shfl_xor(d, step); }
+    return d;
+}
+
+// Values of row row0 + r at k0 + 8 half and the seven behind it, 0 behind the last k (row0 a multiple of 32, k0 of 16; rows behind the last one hold anything)
+template <int KIND>
+__device__ __forceinline__ void load_eight(Operand const &o, int row0, int k0, int r, int half, float (&v)[8])
+{
+    constexpr bool kGrad = KIND == kGradRows || KIND == kGradColumns;
+    constexpr int kAs = KIND == kGradRows ? kRows : KIND == kGradColumns ? kColumns : KIND;
+    constexpr bool kAlong = kAs == kRows || kAs == kBitRows;
+    TileBuffer const from = RawRun<kAs>::buffer(o, row0, k0);
+    uint32_t const pitch = (uint32_t)o.stride * 4, step = kAlong ? 4 : pitch;
+    uint32_t const at = kAlong ? r * pitch + half * 32 : half * 8 * pitch + (kAs == kColumns ? r * 4 : 0);
+    int const k = k0 + half * 8;
+    if constexpr (KIND == kBitRows) {
+        uint32_t const w = load_word(from, r * pitch) >> (k & 31);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) { v[j] = (float)((w >> j) & 1u); }
+    }
+    else if (kAs == kRows && o.vec) {
+#pragma unroll
+        for (int j = 0; j < 8; j += 4) {
+            uint4 const q = load_words(from, at + j * 4);
+            v[j] = __builtin_bit_cast(float, q.x); v[j + 1] = __builtin_bit_cast(float, q.y); v[j + 2] = __builtin_bit_cast(float, q.z); v[j + 3] = __builtin_bit_cast(float, q.w);
+        }
+    }
+    else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            uint32_t const w = load_word(from, at + j * step);
+            v[j] = KIND == kBitColumns ? (float)((w >> r) & 1u) : __builtin_bit_cast(float, w);
+        }
+    }
+    // (values of the frames k: zero behind the last)
+    auto const of_frames = [&](void const *p, int j) { return load_word(tile_buffer(static_cast<uint32_t const *>(p) + k0, (o.depth - k0) * 4LL), (half * 8 + j) * 4); };
+    if constexpr (KIND == kRows) {
+        if (o.coef) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) { v[j] = __builtin_bit_cast(float, of_frames(o.coef, j)) == 0.0f ? 0.0f : v[j]; }
+        }
+    }
+    if constexpr (kGrad) {
+        if (o.mode == kGradSoftmax) {
+            int const frame = min(row0 + r, o.rows - 1);
+            float top = KIND == kGradColumns ? o.top[frame] : 0.0f, share = KIND == kGradColumns ? o.share[frame] : 0.0f, coef = KIND == kGradColumns ? o.coef[frame] : 0.0f;
+            int label = KIND == kGradColumns ? o.label[frame] : 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if constexpr (KIND == kGradRows) {
+                    top = __builtin_bit_cast(float, of_frames(o.top, j)); share = __builtin_bit_cast(float, of_frames(o.share, j));
+                    coef = __builtin_bit_cast(float, of_frames(o.coef, j)); label = (int)of_frames(o.label, j);
+                }
+                v[j] = softmax_gradient(v[j], top, share, coef, label, (KIND == kGradRows ? row0 + r : k + j) + o.first);
+            }
+        }
+        else if (o.mode != kActNone) {
+            Operand y = o;
+            y.p = o.y;
+            TileBuffer const values = RawRun<kAs>::buffer(y, row0, k0);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) { v[j] = gradient_of(v[j], __builtin_bit_cast(float, load_word(values, at + j * step)), o.mode); }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) { v[j] = k + j < o.depth ? v[j] : 0.0f; }
+}
+
+// 32 x 32 of them by a wavefront, on the fp32 matrix instructions
+template <int KA, int KB>
+__device__ __forceinline__ DenseAcc16 block_again(Operand const &a, Operand const &b, int m0, int n0, int lane)
+{
+    DenseAcc16 acc = {};
+#pragma nounroll
+    for (int k0 = 0; k0 < a.depth; k0 += 16) {
+        float u[8], v[8];
+        load_eight<KA>(a, m0, k0, lane & 31, lane >> 5, u);
+        load_eight<KB>(b, n0, k0, lane & 31, lane >> 5, v);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) { acc = __builtin_amdgcn_mfma_f32_32x32x2f32(u[q], v[q], acc, 0, 0, 0); }
+    }
+    return acc;
+}
+
+// Those of a tile of 32 x 64 in LDS, rows of `pitch`: bit 16 j + r of a lane's word is element r of block j as a matrix instruction leaves it.  Few by the element (4096 k: about 10 us each, which
+// a launch that waits for one wavefront pays), more by the block.
+constexpr int kFewAgain = 16;
+template <int KA, int KB>
+__device__ __forceinline__ void tile_again(Operand const &a, Operand const &b, float *tile, int pitch, uint32_t which, int m0, int n0, int lane)
+{
+    asm volatile("" : "+v"(lane));              // (so that nothing of this is computed ahead, in registers that the accumulators need)
+#pragma nounroll
+    for (int j = 0; j < 2; ++j) {
+        uint32_t mine = (which >> (16 * j)) & 0xffffu;
+        int count = __popc(mine);
+#pragma unroll
+        for (int step = 32; step > 0; step /= 2) { count += __shfl_xor(count, step); }
+        if (count > kFewAgain) {
+            DenseAcc16 const acc = block_again<KA, KB>(a, b, m0, n0 + j * 32, lane);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) { if ((mine >> r) & 1u) { tile[acc_row(r, lane) * pitch + j * 32 + (lane & 31)] = plain_nan(acc[r]); } }
+            continue;
+        }
+        for (uint64_t lanes = __ballot(mine != 0u); lanes != 0; lanes = __ballot(mine != 0u)) {
+            int const from = __ffsll((unsigned long long)lanes) - 1, r = __ffs(__builtin_amdgcn_readlane((int)mine, from)) - 1;
+            int const row = acc_row(r, from), column = j * 32 + (from & 31);
+            float const d = element_again<KA, KB>(a, b, m0 + row, n0 + column, lane);
+            if (lane == from) { tile[row * pitch + column] = plain_nan(d); mine &= mine - 1; }
+        }
+    }
+}
+
+// The same for the elements (m, n0 + lane) of a row, d, where `again`: few by the element, more by a lane each.
+template <int KA, int KB>
+__device__ __forceinline__ void row_again(Operand const &a, Operand const &b, float &d, bool again, int m, int n0, int lane)
+{
+    uint64_t lanes = __ballot(again);
+    if (__popcll(lanes) > kFewAgain) {
+        if (!again) { return; }
+        d = 0.0f;
+#pragma nounroll
+        for (int k0 = 0; k0 < a.depth; k0 += 4) {
+            float u[4], v[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                int const k = min(k0 + q, a.depth - 1);
+                u[q] = operand_at<KA>(a, m, k);
+                v[q] = operand_at<KB>(b, n0 + lane, k);
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) { if (k0 + q < a.depth) { d = fmaf(u[q], v[q], d); } }
+        }
+        return;
+    }
+    for (; lanes != 0; lanes &= lanes - 1) {
+        int const from = __ffsll((unsigned long long)lanes) - 1;
+        float const e = element_again<KA, KB>(a, b, m, n0 + from, lane);
+        if (lane == from) { d = e; }
+    }
+}
+
+// whichever kinds the operands are of
+__device__ __forceinline__ void logit_again(Operand const &a, Operand const &b, int kind_b, float &d, bool again, int m, int n0, int lane)
+{
+    if (kind_b == kColumns) { row_again<kRows, kColumns>(a, b, d, again, m, n0, lane); }
+    else                    { row_again<kRows, kBitColumns>(a, b, d, again, m, n0, lane); }
+}
+__device__ __forceinline__ void row_again(Operand const &a, int kind_a, Operand const &b, int kind_b, float &d, bool again, int m, int n0, int lane)
+{
+    if (kind_a == kRows)           { logit_again(a, b, kind_b, d, again, m, n0, lane); }
+    else if (kind_a == kGradRows)  { if (kind_b == kRows) { row_again<kGradRows, kRows>(a, b, d, again, m, n0, lane); }    else { row_again<kGradRows, kBitRows>(a, b, d, again, m, n0, lane); } }
+    else                           { row_again<kColumns, kGradColumns>(a, b, d, again, m, n0, lane); }
+}
 
 // v[step]: four neighbours of row 4 step + lane / 16 of such a tile, and what they become.  `all`: the four may be moved with 16-byte accesses.
 template <int USE>
-__device__ __forceinline__ void finish_tile(DenseOutput const &o, float const *tile, float const *bias, int m0, int n0, int lane)
+__device__ __forceinline__ void finish_tile(DenseOutput const &o, float const *tile, float const *bias, int m0, int n0, int lane, bool marks)
 {
     int const n = n0 + (lane & 15) * 4, row0 = lane >> 4;
     bool const all = n + 4 <= o.columns && o.stride % 4 == 0 && (reinterpret_cast<uintptr_t>(o.out) & 15) == 0 &&
@@ -243,6 +409,12 @@ __device__ __forceinline__ void finish_tile(DenseOutput const &o, float const *t
         if (m >= o.rows) { continue; }
         float d[4];
         load_floats(tile + row * kTilePitch + (lane & 15) * 4, true, d);
+        bool whole = all;
+        uint32_t keep = 0xfu;
+        if (__builtin_expect(marks, 0)) {
+            keep = (stored(d[0]) ? 1u : 0u) | (stored(d[1]) ? 2u : 0u) | (stored(d[2]) ? 4u : 0u) | (stored(d[3]) ? 8u : 0u);
+            whole = whole && keep == 0xfu;
+        }
         if (USE != kUseStore) {
             float const b = bias[row];
 #pragma unroll
@@ -255,16 +427,16 @@ __device__ __forceinline__ void finish_tile(DenseOutput const &o, float const *t
             for (int q = 0; q < 4; ++q) { d[q] = activated(d[q], o.activation); }
         }
         float *to = static_cast<float *>(o.out) + m * o.stride + n;
-        if (all) { *reinterpret_cast<float4 *>(to) = make_float4(d[0], d[1], d[2], d[3]); }
+        if (whole) { *reinterpret_cast<float4 *>(to) = make_float4(d[0], d[1], d[2], d[3]); }
         else {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) { if (n + q < o.columns) { to[q] = d[q]; } }
+            for (int q = 0; q < 4; ++q) { if (n + q < o.columns && ((keep >> q) & 1u)) { to[q] = d[q]; } }
         }
     }
 }
 
-// the same to packed bits: a row of 64 columns is two words
-__device__ __forceinline__ void finish_tile_bits(DenseOutput const &o, float const *tile, float const *bias, int m0, int n0, int lane)
+// The same to packed bits: a row of 64 columns is two words.  What is not to be stored is 0 in them; `more`: the bits are added to those of a first pass.
+__device__ __forceinline__ void finish_tile_bits(DenseOutput const &o, float const *tile, float const *bias, int m0, int n0, int lane, bool more)
 {
     int const n = n0 + lane;
     bool const inside = n < o.columns;
@@ -272,8 +444,43 @@ __device__ __forceinline__ void finish_tile_bits(DenseOutput const &o, float con
         float z = tile[row * kTilePitch + lane] + bias[row];
         if (o.residual && inside) { z += o.residual[(m0 + row) * o.residual_stride + n]; }
         uint64_t const bits = __ballot(inside && z > 0.0f);
-        if ((lane & 31) == 0 && inside) { static_cast<uint32_t *>(o.out)[(m0 + row) * o.stride + (n >> 5)] = (uint32_t)(bits >> (lane & 32)); }
+        if ((lane & 31) == 0 && inside) {
+            uint32_t *const to = static_cast<uint32_t *>(o.out) + (m0 + row) * o.stride + (n >> 5);
+            *to = (uint32_t)(bits >> (lane & 32)) | (more ? *to : 0u);
+        }
     }
+}
+
+// What becomes of a tile of 32 x 64; logits: (largest, sum of exponents) of its rows join `column`, this lane's.
+template <int USE>
+__device__ __forceinline__ void finish(DenseOutput const &o, bool partial_sums, float const *tile, float const *bias, int m0, int n0, int lane, float2 &column, bool marks, bool more)
+{
+    if (USE == kUseLogits && !partial_sums && n0 + lane < o.columns) {
+        int const n = n0 + lane, rows = min(32, o.rows - m0), label = o.label[n] - o.first_channel - m0;
+        float z[32];
+        float2 s = make_float2(-INFINITY, 0.0f);
+#pragma unroll
+        for (int row = 0; row < 32; ++row) {
+            z[row] = row < rows ? tile[row * kTilePitch + lane] + bias[row] : -INFINITY;
+            s.x = fmaxf(s.x, z[row]);
+        }
+        if (__builtin_expect(marks, 0)) {
+            s.x = -INFINITY;
+#pragma unroll
+            for (int row = 0; row < 32; ++row) {
+                z[row] = stored(tile[row * kTilePitch + lane]) ? z[row] : -INFINITY;
+                s.x = fmaxf(s.x, z[row]);
+            }
+        }
+#pragma unroll
+        for (int row = 0; row < 32; ++row) { s.y += z[row] == -INFINITY ? 0.0f : exp_of_nonpositive(z[row] - s.x); }
+        if (label >= 0 && label < rows && stored(tile[label * kTilePitch + lane])) { o.label_logit[n] = tile[label * kTilePitch + lane] + bias[label]; }
+        column = joined(column, s);
+    }
+    if (USE == kUseForward && o.kind == kOutBits)         { finish_tile_bits(o, tile, bias, m0, n0, lane, more); }
+    else if (USE == kUseForward && o.kind == kOutForward) { finish_tile<kUseForward>(o, tile, bias, m0, n0, lane, marks); }
+    else if (USE == kUseLogits && !partial_sums)          { if (o.out) { finish_tile<kUseLogits>(o, tile, bias, m0, n0, lane, marks); } }
+    else                                                  { finish_tile<kUseStore>(o, tile, bias, m0, n0, lane, marks); }
 }
 
 // Waits until at most N of this wavefront's loads are on their way (loads arrive in order) and its reads of LDS are done, then for the workgroup.
@@ -284,7 +491,7 @@ __device__ __forceinline__ void arrived(void)
     asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" :: "n"(N) : "memory");
 }
 
-template <int USE, int TM, int WM, int WN, int PB, int BUFFERS>
+template <int USE, int KA, int KB, int TM, int WM, int WN, int PB, int BUFFERS>
 __device__ __forceinline__ void packed_tile(PackedProduct const &p, int id, char *lds, int *scales, float *bias)
 {
     constexpr int TN = 2, kWaves = WM * WN, kBM = TM * WM, kBN = TN * WN;           // blocks of 32 rows
@@ -430,19 +637,21 @@ __device__ __forceinline__ void packed_tile(PackedProduct const &p, int id, char
     }
     float *const tile = reinterpret_cast<float *>(lds) + wave * 32 * kTilePitch;
     int const n0 = (rb_b + wn * TN) * 32;
-    int eb[TN];
     __syncthreads();                            // (the stages are done with LDS)
-#pragma unroll
-    for (int j = 0; j < TN; ++j) { eb[j] = scale_b[(wn * TN + j) * 32 + (lane & 31)]; }
     float2 column = make_float2(-INFINITY, 0.0f);
+    uint32_t again[TM] = {};                    // of the elements that are formed again, bit 16 j + r
 #pragma nounroll
     for (int i = 0; i < TM; ++i) {
         int const rb = rb_a + wm * TM + i, m0 = rb * 32;
         if (rb >= p.a_blocks) { break; }
-        bool odd = false;
+        int eb[TN];
+#pragma unroll
+        for (int j = 0; j < TN; ++j) { eb[j] = scale_b[(wn * TN + j) * 32 + (lane & 31)]; }
+        bool marks = false;
 #pragma unroll
         for (int u = 0; u < TM; ++u) {              // (registers have no index)
             if (u != i) { continue; }
+            bool odd = false;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 int const row = acc_row(r, lane), ea = scale_a[(wm * TM + i) * 32 + row];
@@ -453,32 +662,45 @@ __device__ __forceinline__ void packed_tile(PackedProduct const &p, int id, char
                     tile[row * kTilePitch + j * 32 + (lane & 31)] = d;
                 }
             }
-        }
-        float const *const b = bias + (wm * TM + i) * 32;
-        if (USE != kUseLogits && p.kind_a >= 0 && p.slabs == 1 && __any(odd)) {
-            for (int row = 0; row < 32; ++row) {
-                if (m0 + row < o.rows && n0 + lane < o.columns) { tile[row * kTilePitch + lane] = element_again(p.src_a, p.kind_a, p.src_b, p.kind_b, m0 + row, n0 + lane); }
+            marks = p.slabs == 1 && __any(odd);
+            if (__builtin_expect(marks, 0)) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+#pragma unroll
+                    for (int j = 0; j < TN; ++j) {
+                        float *const d = tile + acc_row(r, lane) * kTilePitch + j * 32 + (lane & 31);
+                        if (*d != *d) {
+                            again[u] |= 1u << (j * 16 + r);
+                            *d = __builtin_bit_cast(float, kNotStored);
+                        }
+                    }
+                }
             }
         }
-        if (USE == kUseLogits && p.slabs == 1 && n0 + lane < o.columns) {
-            // (largest, sum of exponents) of the 32 rows of this lane's column
-            int const n = n0 + lane, rows = min(32, o.rows - m0), label = o.label[n] - o.first_channel - m0;
-            float z[32];
-            float2 s = make_float2(-INFINITY, 0.0f);
+        finish<USE>(o, p.slabs > 1, tile, bias + (wm * TM + i) * 32, m0, n0, lane, column, marks, false);
+    }
+    // A second time round for what is formed again (its code needs the registers that the accumulators have had)
+    uint32_t any = 0;
 #pragma unroll
-            for (int row = 0; row < 32; ++row) {
-                z[row] = row < rows ? tile[row * kTilePitch + lane] + b[row] : -INFINITY;
-                s.x = fmaxf(s.x, z[row]);
+    for (int u = 0; u < TM; ++u) { any |= again[u]; }
+    if (__builtin_expect(p.slabs == 1 && __any(any != 0u), 0)) {
+#pragma nounroll
+        for (int i = 0; i < TM; ++i) {
+            int const m0 = (rb_a + wm * TM + i) * 32;
+            uint32_t here = 0;
+#pragma unroll
+            for (int u = 0; u < TM; ++u) { here = u == i ? again[u] : here; }
+            // (not those outside, nor of frames that nothing is made of)
+            for (int r = 0; r < 16; ++r) { if (m0 + acc_row(r, lane) >= o.rows) { here &= ~(0x10001u << r); } }
+            for (int j = 0; j < TN; ++j) {
+                int const n = n0 + j * 32 + (lane & 31);
+                if (n >= o.columns || (USE == kUseLogits && !frame_counts(o, n))) { here &= ~(0xffffu << (16 * j)); }
             }
-#pragma unroll
-            for (int row = 0; row < 32; ++row) { s.y += z[row] == -INFINITY ? 0.0f : exp_of_nonpositive(z[row] - s.x); }
-            if (label >= 0 && label < rows) { o.label_logit[n] = tile[label * kTilePitch + lane] + b[label]; }
-            column = joined(column, s);
+            if (!__any(here != 0u)) { continue; }
+            for (int row = 0; row < 32; ++row) { tile[row * kTilePitch + lane] = __builtin_bit_cast(float, kNotStored); }
+            tile_again<KA, KB>(p.src_a, p.src_b, tile, kTilePitch, here, m0, n0, lane);
+            finish<USE>(o, false, tile, bias + (wm * TM + i) * 32, m0, n0, lane, column, true, true);
         }
-        if (USE == kUseForward && o.kind == kOutBits)         { finish_tile_bits(o, tile, b, m0, n0, lane); }
-        else if (USE == kUseForward && o.kind == kOutForward) { finish_tile<kUseForward>(o, tile, b, m0, n0, lane); }
-        else if (USE == kUseLogits && p.slabs == 1)           { if (o.out) { finish_tile<kUseLogits>(o, tile, b, m0, n0, lane); } }
-        else                                                  { finish_tile<kUseStore>(o, tile, b, m0, n0, lane); }
     }
     if (USE == kUseLogits && p.slabs == 1 && n0 + lane < o.columns && rb_a + wm * TM < p.a_blocks) {
         o.partial[(long long)((rb_a + wm * TM) / TM) * o.columns + n0 + lane] = column;
@@ -498,17 +720,17 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void dense_packed_kernel(PackedPro
     __shared__ __attribute__((aligned(1024))) char lds[packed_lds<TM, WM, WN, BUFFERS>()];
     __shared__ int scales[(TM * WM + 2 * WN) * 32];
     __shared__ float bias[TM * WM * 32];
-    packed_tile<USE, TM, WM, WN, PB, BUFFERS>(p, blockIdx.x, lds, scales, bias);
+    packed_tile<USE, kRows, PB == 1 ? kBitColumns : kColumns, TM, WM, WN, PB, BUFFERS>(p, blockIdx.x, lds, scales, bias);
 }
 
-// one product, and behind it another whose operands are not packed bits (either may have no workgroups)
+// the weights' gradient, and behind it the input's (either may have no workgroups)
 template <int TM, int WM, int WN, int PB, int BUFFERS>
 __global__ __launch_bounds__(WM * WN * 64, 2) void dense_packed_pair_kernel(PackedProduct p, PackedProduct q)
 {
     __shared__ __attribute__((aligned(1024))) char lds[packed_lds<TM, WM, WN, BUFFERS>()];
     __shared__ int scales[(TM * WM + 2 * WN) * 32];
-    if ((int)blockIdx.x < p.workgroups) { packed_tile<kUseStore, TM, WM, WN, PB, BUFFERS>(p, blockIdx.x, lds, scales, nullptr); }
-    else                                { packed_tile<kUseStore, TM, WM, WN, 2, BUFFERS>(q, blockIdx.x - p.workgroups, lds, scales, nullptr); }
+    if ((int)blockIdx.x < p.workgroups) { packed_tile<kUseStore, kGradRows, PB == 1 ? kBitRows : kRows, TM, WM, WN, PB, BUFFERS>(p, blockIdx.x, lds, scales, nullptr); }
+    else                                { packed_tile<kUseStore, kColumns, kGradColumns, TM, WM, WN, 2, BUFFERS>(q, blockIdx.x - p.workgroups, lds, scales, nullptr); }
 }
 
 __device__ __forceinline__ float sum_of_slabs(PackedProduct const &p, int m, int n)
@@ -533,10 +755,8 @@ __device__ __forceinline__ void join_slabs(PackedProduct const &p, unsigned id)
     if (m >= o.rows) { return; }
     bool const inside = n < o.columns || (n == o.columns && o.line && o.kind == kOutStore);
     float d = 0.0f;
-    if (inside) {
-        d = sum_of_slabs(p, m, n);
-        if (d != d && p.kind_a >= 0) { d = element_again(p.src_a, p.kind_a, p.src_b, p.kind_b, m, n); }
-    }
+    if (inside) { d = sum_of_slabs(p, m, n); }
+    if (__builtin_expect(p.kind_a >= 0 && __any(inside && d != d), 0)) { row_again(p.src_a, p.kind_a, p.src_b, p.kind_b, d, inside && d != d, m, n - lane, lane); }
     if (o.kind == kOutForward) { if (inside) { static_cast<float *>(o.out)[m * o.stride + n] = activated(before_activation(o, d, m, n), o.activation); } }
     else if (o.kind == kOutBits) {
         uint64_t const bits = __ballot(inside && before_activation(o, d, m, inside ? n : 0) > 0.0f);
@@ -553,7 +773,7 @@ __global__ __launch_bounds__(256) void dense_join_kernel(PackedProduct p, Packed
 
 // The same for logits: a workgroup takes 32 rows of 64 columns, each of its sixteen wavefronts two of the rows, four slabs of both at a time.
 constexpr int kJoinLogitWaves = 16;
-__global__ __launch_bounds__(kJoinLogitWaves * 64) void dense_join_logits_kernel(PackedProduct p)
+__global__ __launch_bounds__(kJoinLogitWaves * 64, 8) void dense_join_logits_kernel(PackedProduct p)
 {
     __shared__ float2 part[kJoinLogitWaves][64];
     DenseOutput const &o = p.out;
@@ -575,6 +795,14 @@ __global__ __launch_bounds__(kJoinLogitWaves * 64) void dense_join_logits_kernel
             }
 #pragma unroll
             for (int q = 0; q < 4; ++q) { z[0] += s + q < p.slabs ? u[q] : 0.0f; z[1] += s + q < p.slabs ? v[q] : 0.0f; }
+        }
+    }
+    if (__builtin_expect(p.kind_a >= 0 && __any(inside && (z[0] != z[0] || z[1] != z[1])), 0)) {
+#pragma nounroll
+        for (int i = 0; i < 2; ++i) {
+            float d = i ? z[1] : z[0];
+            if (m0 + i < o.rows) { logit_again(p.src_a, p.src_b, p.kind_b, d, inside && d != d && frame_counts(o, n), m0 + i, n - lane, lane); }
+            if (i) { z[1] = d; } else { z[0] = d; }
         }
     }
     float2 s = make_float2(-INFINITY, 0.0f);

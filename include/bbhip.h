@@ -559,8 +559,8 @@ int bbhip_bit_fp32_DenseAffine_Backward(int const *dev_x_buf, float const *dev_d
  *     dev_loss_buf[f] = -w * log p_label,   dz[c] = w / weight_sum * (p_c - [c is the label]),   dx = W^T dz,   dW = dz x^T,   db = sum over frames of dz.
  * The caller passes weight_sum = the sum of the weights that count and reports sum(dev_loss_buf) / weight_sum, whose gradients these are.  A frame whose label is negative or not below ch_size, or
  * whose weight is 0, does not count: loss 0, dx 0 and no part of dW and db, whatever it holds.  dx, dW and db (which is formed with dW) may be NULL: without any of them the loss alone is
- * computed, in half the time or less.  dW and db are added to what they hold with accumulate.  gradients: whether there will be any.  A bias of minus infinity closes a channel.  W and the
- * frames that count must be finite: DenseAffine forms elements with infinities again in fp32, the products here do not. */
+ * computed, in half the time or less.  dW and db are added to what they hold with accumulate.  gradients: whether there will be any.  A bias of minus infinity closes a channel.
+ * Infinities and NaN in W and in the frames that count come out as the formulas have them, in any product and at any size, as in DenseAffine. */
 size_t bbhip_LossDenseSoftmaxCrossEntropy_WorkspaceBytes(int input_node_size, int ch_size, int frame_size, int gradients);
 int bbhip_fp32_LossDenseSoftmaxCrossEntropy(float const *dev_x_buf, float const *dev_W, float const *dev_b, int const *dev_label_buf, float const *dev_weight_buf,
                                             float *dev_dx_buf, float *dev_dW, float *dev_db, float *dev_loss_buf, float weight_sum, int accumulate, int input_node_size,

@@ -200,17 +200,21 @@ int direct_backward(Product const &dw, Product const &dx, DirectBackwardSpace co
 struct Packed {
     uint4 *halves;
     int   *exponent;
+    float *lost;
+    uint4 *tails = nullptr;
     int    blocks, steps, pieces;
     Packed() = default;
-    Packed(Carver &c, int rows, int depth, bool bits) : blocks(ceil_div(rows, 32)), steps(pack_steps(depth)), pieces(bits ? 1 : 2)
+    Packed(Carver &c, int rows, int depth, bool bits, bool with_tails = false) : blocks(ceil_div(rows, 32)), steps(pack_steps(depth)), pieces(bits ? 1 : 2)
     {
         halves = c.take<uint4>((size_t)blocks * steps * pieces * 64);
         exponent = bits ? nullptr : c.take<int>((size_t)blocks * 32);
+        lost = c.take<float>((size_t)blocks * 32);
+        if (with_tails) { tails = c.take<uint4>((size_t)blocks * steps * 64); }
     }
     PackJob job(Operand const &o, int kind) const
     {
         PackJob j{};
-        j.src = o; j.kind = kind; j.halves = halves; j.exponent = exponent; j.k_steps = steps;
+        j.src = o; j.kind = kind; j.halves = halves; j.exponent = exponent; j.lost = lost; j.tails = tails; j.k_steps = steps;
         j.blocks = blocks * (32 / kPackRows);
         return j;
     }
@@ -241,8 +245,8 @@ int packed_product(PackedProduct &d, Product const &p, PackedShape const &s, Pac
 {
     d = PackedProduct{};
     if (!p.wanted) { d.b_pieces = 2; return 0; }
-    d.a = a.halves; d.ea = a.exponent; d.a_blocks = a.blocks;
-    d.b = b.halves; d.eb = b.exponent; d.b_blocks = b.blocks; d.b_pieces = b.pieces;
+    d.a = a.halves; d.ea = a.exponent; d.lost_a = a.lost; d.a_blocks = a.blocks;
+    d.b = b.halves; d.eb = b.exponent; d.lost_b = b.lost; d.tails = a.tails ? a.tails : b.tails; d.b_blocks = b.blocks; d.b_pieces = b.pieces;
     d.k_steps = s.k_steps; d.m_tiles = s.m_tiles; d.n_tiles = s.n_tiles; d.slabs = s.slabs; d.slab_stages = s.slab_stages;
     if (check_tiles(s.workgroups(), kTileThreads[s.size], name)) { return 1; }
     d.workgroups = (int)s.workgroups();
@@ -281,10 +285,17 @@ int packed_run(PackedProduct const &p, PackedProduct const &q, int size, hipStre
     if (check_tiles((long long)p.workgroups + q.workgroups, kTileThreads[size], name)) { return 1; }
     if (p.workgroups + q.workgroups == 0) { return 0; }
     dim3 const grid((unsigned)(p.workgroups + q.workgroups)), block((unsigned)kTileThreads[size]);
+    bool const tails = p.tails || q.tails;
 #define BBHIP_PACKED(...)                                                                               \
     do {                                                                                                \
-        if (p.b_pieces == 1) { launch((dense_packed_pair_kernel<__VA_ARGS__, 1, kTileBuffers[size_]>), grid, block, 0, st, p, q); } \
-        else                 { launch((dense_packed_pair_kernel<__VA_ARGS__, 2, kTileBuffers[size_]>), grid, block, 0, st, p, q); } \
+        if (tails) {                                                                                    \
+            if (p.b_pieces == 1) { launch((dense_packed_pair_kernel<true, __VA_ARGS__, 1, kTileBuffers[size_]>), grid, block, 0, st, p, q); } \
+            else                 { launch((dense_packed_pair_kernel<true, __VA_ARGS__, 2, kTileBuffers[size_]>), grid, block, 0, st, p, q); } \
+        }                                                                                               \
+        else {                                                                                          \
+            if (p.b_pieces == 1) { launch((dense_packed_pair_kernel<false, __VA_ARGS__, 1, kTileBuffers[size_]>), grid, block, 0, st, p, q); } \
+            else                 { launch((dense_packed_pair_kernel<false, __VA_ARGS__, 2, kTileBuffers[size_]>), grid, block, 0, st, p, q); } \
+        }                                                                                               \
     } while (0)
     if (size == kTileLarge)       { constexpr int size_ = kTileLarge;  BBHIP_PACKED(4, 2, 4); }
     else if (size == kTileMiddle) { constexpr int size_ = kTileMiddle; BBHIP_PACKED(4, 2, 2); }
@@ -308,13 +319,13 @@ struct BackwardSpace {
     PackedShape dw, dx;
     Packed dz_rows, x, W, dz_columns;
     float *dw_sums, *dx_sums;
-    BackwardSpace(Carver &c, int inputs, int outputs, int frames, bool bit)
+    BackwardSpace(Carver &c, int inputs, int outputs, int frames, bool bit, bool tails)
     {
         best_shapes(outputs, inputs, frames, inputs, frames, outputs, dw, dx);
-        dz_rows = Packed(c, outputs, frames, false);
+        dz_rows = Packed(c, outputs, frames, false, tails);
         x = Packed(c, inputs, frames, bit);
         W = Packed(c, inputs, outputs, false);
-        dz_columns = Packed(c, frames, outputs, false);
+        dz_columns = Packed(c, frames, outputs, false, tails);
         dw_sums = sums_of(c, dw.slabs, outputs, inputs);
         dx_sums = sums_of(c, dx.slabs, inputs, frames);
     }
@@ -445,7 +456,7 @@ int dense_backward(void const *x, bool bit, float const *dy, float const *y, flo
     hipStream_t const st = static_cast<hipStream_t>(stream);
     if (backward_packed(inputs, outputs, frames)) {
         Carver c{static_cast<char *>(workspace)};
-        BackwardSpace const s(c, inputs, outputs, frames, bit);
+        BackwardSpace const s(c, inputs, outputs, frames, bit, false);
         if (check_workspace(workspace, workspace_size, c.at, name)) { return 1; }
         ScopedTimer tm(kTimeOther, st);
         Jobs jobs;
@@ -485,7 +496,7 @@ struct LossSpace {
             W = Packed(c, plan.piece, inputs, false);
             x = Packed(c, frames, inputs, bit);
             logit_sums = sums_of(c, plan.logits.slabs, plan.piece, frames);
-            if (gradients) { new (backward_space) BackwardSpace(c, inputs, plan.piece, frames, bit); }
+            if (gradients) { new (backward_space) BackwardSpace(c, inputs, plan.piece, frames, bit, true); }
         }
         else {
             // (the last piece, of fewer channels, may be divided otherwise)
@@ -617,7 +628,7 @@ size_t bbhip_DenseAffine_WorkspaceBytes(int input_node_size, int output_node_siz
     Carver forward{nullptr}, backward{nullptr};
     if (forward_packed(input_node_size, output_node_size, frame_size)) { ForwardSpace const f(forward, input_node_size, output_node_size, frame_size, false); }
     else { sums_of(forward, direct_shape(output_node_size, frame_size, input_node_size).slabs, output_node_size, frame_size); }
-    if (backward_packed(input_node_size, output_node_size, frame_size)) { BackwardSpace const b(backward, input_node_size, output_node_size, frame_size, false); }
+    if (backward_packed(input_node_size, output_node_size, frame_size)) { BackwardSpace const b(backward, input_node_size, output_node_size, frame_size, false, false); }
     else { DirectBackwardSpace const d(backward, input_node_size, output_node_size, frame_size, true); }
     return forward.at > backward.at ? forward.at : backward.at;
 }

@@ -1,10 +1,18 @@
 // Products of dense layers on the fp16 matrix instructions, to the accuracy of fp32: large problems.
 //
-// A value v of an operand's row is scaled by a power of two that brings the largest of its row into [2^14, 2^15), and split into two halves, v 2^e = h + l with
+// A value v of an operand's row is scaled by a power of two that brings the largest of its row to 2^15 and more, as far as halves hold it, and split into two halves, v 2^e = h + l with
 // h = fp16(v 2^e), l = fp16(v 2^e - h): 22 bits, so that  a b = (ah bh + ah bl + al bh) 2^-(ea + eb)  up to 3 * 2^-22 of a product at most (the product of the two lower halves is left
 // out) and about 2^-24 on the average: what rounding the factors to fp32 would cost.  The matrix instruction multiplies halves exactly and sums in fp32.  Three fp16 products run
-// at 2.5 PFLOP/s / 3 where the fp32 matrix instructions have 0.157; a packed-bit operand is one half without any error, so its products are two.  What the scaling
-// costs: a value more than 2^15 times smaller than the largest of its row keeps fewer bits, and is off by at most 2^-40 of that one.
+// at 2.5 PFLOP/s / 3 where the fp32 matrix instructions have 0.157; a packed-bit operand is one half without any error, so its products are two.
+//
+// What the scaling costs, and how it is made good: a value below 2^-18 of the largest of its row keeps fewer bits, one below 2^-41 none, where fp32 would keep all.  That matters where the other
+// operand is as much larger there (an input that is not normalised, whose weights are small) or 0 where this one is large (gradients over sparse bits).  So the first launch also leaves what each row lost,
+// the sum of what its halves leave of such values, and an element of the product whose sum never got 2^20 times as large as its row and its column can have changed it
+//     |sum| < 2^20 * (lost of the row * largest of the column + largest of the row * lost of the column)
+// is formed again in fp32 straight from the operands, as one that is no number is (an infinity times a lower half of 0).  What fp32 sums of that length round away is as much.  Sums are looked
+// at on the way too (a number that has been large has lost as much in fp32, however small it ends): ordinary operands have next to none of these elements.  The gradients of a softmax do, with
+// magnitudes spread over more than 2^18: over 32768 channels a twentieth of dx.  So the first launch leaves these operands' tails too, what the halves leave of small values, 2^39 times as large, as halves
+// once more, and tails times the other operand's upper halves are added ahead of everything else: what is lost is 2^11 times less then, for a third more work in these two products.
 //
 // Two launches.  The first reads each operand as it lies and leaves its halves in the order in which the matrix instructions want them: blocks of 32 rows x 16 k,
 // 1 KiB each, lane l's sixteen bytes (row l & 31, k 8 (l >> 5) .. + 8) at 16 l, so that the second launch moves them to LDS and from there to registers with 16-byte accesses
@@ -30,13 +38,17 @@ struct PackJob {
     int    kind;
     uint4 *halves;              // [row blocks][k steps][1 or 2][64 lanes]
     int   *exponent;            // of each row (null: packed bits, which are not scaled)
+    float *lost;                // of each row: the magnitudes, scaled, of what its halves leave of values that they do not hold to 22 bits; minus infinity: it has no value but 0
     int    k_steps;             // of 16
     int    blocks;              // workgroups
     float *line;                // gradients as rows: their sums (null: not wanted), added with accumulate
     int    accumulate;
     float *dz;                  // gradients as rows: themselves (null: not wanted), rows of dz_stride
     long long dz_stride;
+    uint4 *tails;               // gradients: what the halves leave of small values, 2^39 times as large, in halves once more: [row blocks][k steps][64 lanes] (null: not wanted)
 };
+
+constexpr float kTailScale = 549755813888.0f;           // 2^39: what is left of a value, 2^-25 at most, becomes 2^14
 
 constexpr int kPackJobs = 4;
 struct PackArgs { PackJob job[kPackJobs]; };
@@ -71,7 +83,7 @@ __device__ __forceinline__ void pack_rows(PackJob const &j, int block, float *sh
     int const octets = j.k_steps * 2;
     bool const there = row < j.src.rows;
     float held[kPackHeld][8];
-    float top = 0.0f, sum = 0.0f;
+    float top = 0.0f, sum = 0.0f, lost = 0.0f;
     int e = 0;
     if (!kBits) {
         int i = 0;
@@ -102,7 +114,8 @@ __device__ __forceinline__ void pack_rows(PackJob const &j, int block, float *sh
         top = 0.0f; sum = 0.0f;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) { top = fmaxf(top, share[w * ROWS + at]); sum += share[(kWaves + w) * ROWS + at]; }
-        e = top > 0.0f ? 14 - ilogbf(top) : 0;
+        e = top > 0.0f ? 15 - ilogbf(top) : 0;
+        if (ldexpf(top, e) >= 65520.0f) { --e; }            // (which halves would round to infinity)
         if (threadIdx.x < ROWS) {
             j.exponent[row] = e;
             if constexpr (KIND == kGradRows) { if (j.line && there) { j.line[row] = j.accumulate ? j.line[row] + sum : sum; } }
@@ -114,13 +127,30 @@ __device__ __forceinline__ void pack_rows(PackJob const &j, int block, float *sh
             to[0] = make_uint4(two_halves(v[0], v[1]), two_halves(v[2], v[3]), two_halves(v[4], v[5]), two_halves(v[6], v[7]));
         }
         else {
-            float h[8], l[8];
+            float h[8], l[8], left[8];
 #pragma unroll
             for (int q = 0; q < 8; ++q) {
                 h[q] = ldexpf(v[q], e);
                 float const upper = (float)(_Float16)h[q];
                 // (the difference of an infinity to itself is no number, its lower half 0)
                 l[q] = fabsf(upper) < INFINITY ? h[q] - upper : 0.0f;
+                // (below 1/8 the lower half's steps, 2^-24, are more than 2^-21 of the value)
+                left[q] = fabsf(h[q]) < 0.125f ? l[q] - (float)(_Float16)l[q] : 0.0f;
+            }
+            if ((KIND == kGradRows || KIND == kGradColumns) && j.tails) {
+                float t[8];
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    t[q] = left[q] * kTailScale;
+                    // (a tail meets the other operand's upper half only: what the lower one is of a value, 2^-11, counts as lost)
+                    lost += fabsf(left[q]) * 4.8828125e-4f + fabsf(t[q] - (float)(_Float16)t[q]) * (1.0f / kTailScale);
+                }
+                uint4 *const tail = j.tails + ((long long)(row >> 5) * j.k_steps + (o >> 1)) * 64 + (o & 1) * 32 + (row & 31);
+                *tail = make_uint4(two_halves(t[0], t[1]), two_halves(t[2], t[3]), two_halves(t[4], t[5]), two_halves(t[6], t[7]));
+            }
+            else {
+#pragma unroll
+                for (int q = 0; q < 8; ++q) { lost += fabsf(left[q]); }
             }
             to[0]  = make_uint4(two_halves(h[0], h[1]), two_halves(h[2], h[3]), two_halves(h[4], h[5]), two_halves(h[6], h[7]));
             to[64] = make_uint4(two_halves(l[0], l[1]), two_halves(l[2], l[3]), two_halves(l[4], l[5]), two_halves(l[6], l[7]));
@@ -153,14 +183,34 @@ __device__ __forceinline__ void pack_rows(PackJob const &j, int block, float *sh
             if (there && o * 8 < j.src.depth) { load_values<KIND, 8>(j.src, row, o * 8, v[u]); }
         }
 #pragma unroll
-        for (int u = 0; u < kAtATime; ++u) { if (octet0 + (i + u) * kOctets < octets) { write(octet0 + (i + u) * kOctets, v[u]); } }
+        for (int u = 0; u < kAtATime; ++u) {
+            if (octet0 + (i + u) * kOctets < octets) { write(octet0 + (i + u) * kOctets, v[u]); }
+            if constexpr (kBits) {
+#pragma unroll
+                for (int q = 0; q < 8; ++q) { top = fmaxf(top, v[u][q]); }
+            }
+        }
+    }
+    // (of packed bits only whether any is set; of others every thread has the row's largest)
+    constexpr int kWaves = THREADS / 64;
+    float mine = kBits ? top : lost;
+#pragma unroll
+    for (int step = ROWS; step < 64; step *= 2) { mine += __shfl_xor(mine, step); }
+    float *const part = share + 2 * kWaves * ROWS;
+    if ((threadIdx.x & 63) < ROWS) { part[threadIdx.x / 64 * ROWS + at] = mine; }
+    __syncthreads();
+    if (threadIdx.x < ROWS) {
+        mine = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) { mine += part[w * ROWS + at]; }
+        j.lost[row] = kBits ? (mine > 0.0f ? 0.0f : -INFINITY) : top > 0.0f ? mine : -INFINITY;
     }
 }
 
 template <int THREADS>
 __global__ __launch_bounds__(THREADS, 4) void dense_pack_kernel(PackArgs a)
 {
-    __shared__ float share[2 * THREADS / 64 * kPackRows];
+    __shared__ float share[3 * THREADS / 64 * kPackRows];
     int block = blockIdx.x, which = 0;
     while (block >= a.job[which].blocks) { block -= a.job[which].blocks; ++which; }
     PackJob const &j = a.job[which];
@@ -179,6 +229,8 @@ __global__ __launch_bounds__(THREADS, 4) void dense_pack_kernel(PackArgs a)
 struct PackedProduct {
     uint4 const *a, *b;             // halves
     int   const *ea, *eb;           // exponents of the rows (eb null: 0)
+    float const *lost_a, *lost_b;   // what the rows lost
+    uint4 const *tails;             // of a or of b (null: neither)
     int   a_blocks, b_blocks;       // row blocks of 32
     int   k_steps;
     int   b_pieces;
@@ -204,25 +256,30 @@ __device__ __forceinline__ bool stored(float v) { return __builtin_bit_cast(uint
 __device__ __forceinline__ float plain_nan(float v) { return v == v ? v : __builtin_bit_cast(float, 0x7fc00000u); }
 
 // ---- elements formed again ----------------------------------------------------------------------------------------------------------------
-// The halves of an infinity times a lower half of 0 are no number where the value's product is infinite: an element that comes out as no number is formed again in fp32 straight from the
-// operands, so that infinities and NaN are what the formula says; its neighbours keep the bits that they have.
+// The halves of an infinity times a lower half of 0 are no number where the value's product is infinite, and halves lose small values beside large ones: such elements are formed again in fp32
+// straight from the operands, so that they are what the formula says; their neighbours keep the bits that they have.
 
-// By a wavefront: its lanes take the k in turn, four at a time so that their loads overlap.
-template <int KA, int KB>
+// An element stands where its scaled sum got as large as the limits of its row and its column together: what they lost, times the other's largest (below 2^16; bits: 1), times 2^20.  (Where
+// either has no value but 0 nothing is lost: minus infinity.)
+template <int PB>
+__device__ __forceinline__ float limit_of(float lost) { return lost * (PB == 2 ? 68719476736.0f : 1048576.0f); }
+
+// By a wavefront: its lanes take the k in turn, N at a time, whose loads overlap.
+template <int KA, int KB, int N>
 __device__ __forceinline__ float element_again(Operand const &a, Operand const &b, int m, int n, int lane)
 {
     float d = 0.0f;
 #pragma nounroll
-    for (int k0 = lane; k0 < a.depth; k0 += 4 * 64) {
-        float u[4], v[4];
+    for (int k0 = lane; k0 < a.depth; k0 += N * 64) {
+        float u[N], v[N];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
+        for (int q = 0; q < N; ++q) {
             int const k = min(k0 + q * 64, a.depth - 1);
             u[q] = operand_at<KA>(a, m, k);
             v[q] = operand_at<KB>(b, n, k);
         }
 #pragma unroll
-        for (int q = 0; q < 4; ++q) { if (k0 + q * 64 < a.depth) { d = fmaf(u[q], v[q], d); } }
+        for (int q = 0; q < N; ++q) { if (k0 + q * 64 < a.depth) { d = fmaf(u[q], v[q], d); } }
     }
 #pragma unroll
     for (int step = 32; step > 0; step /= 2) { d += __shfl_xor(d, step); }
@@ -331,7 +388,7 @@ __device__ __forceinline__ void tile_again(Operand const &a, Operand const &b, f
         for (uint64_t lanes = __ballot(mine != 0u); lanes != 0; lanes = __ballot(mine != 0u)) {
             int const from = __ffsll((unsigned long long)lanes) - 1, r = __ffs(__builtin_amdgcn_readlane((int)mine, from)) - 1;
             int const row = acc_row(r, from), column = j * 32 + (from & 31);
-            float const d = element_again<KA, KB>(a, b, m0 + row, n0 + column, lane);
+            float const d = element_again<KA, KB, 16>(a, b, m0 + row, n0 + column, lane);
             if (lane == from) { tile[row * pitch + column] = plain_nan(d); mine &= mine - 1; }
         }
     }
@@ -344,7 +401,7 @@ __device__ __forceinline__ void row_again(Operand const &a, Operand const &b, fl
     uint64_t lanes = __ballot(again);
     if (__popcll(lanes) > kFewAgain) {
         if (!again) { return; }
-        d = 0.0f;
+        float sum[4] = {};                      // (shorter chains of roundings than one sum)
 #pragma nounroll
         for (int k0 = 0; k0 < a.depth; k0 += 4) {
             float u[4], v[4];
@@ -355,13 +412,14 @@ __device__ __forceinline__ void row_again(Operand const &a, Operand const &b, fl
                 v[q] = operand_at<KB>(b, n0 + lane, k);
             }
 #pragma unroll
-            for (int q = 0; q < 4; ++q) { if (k0 + q < a.depth) { d = fmaf(u[q], v[q], d); } }
+            for (int q = 0; q < 4; ++q) { if (k0 + q < a.depth) { sum[q] = fmaf(u[q], v[q], sum[q]); } }
         }
+        d = (sum[0] + sum[1]) + (sum[2] + sum[3]);
         return;
     }
     for (; lanes != 0; lanes &= lanes - 1) {
         int const from = __ffsll((unsigned long long)lanes) - 1;
-        float const e = element_again<KA, KB>(a, b, m, n0 + from, lane);
+        float const e = element_again<KA, KB, 4>(a, b, m, n0 + from, lane);
         if (lane == from) { d = e; }
     }
 }
@@ -491,8 +549,9 @@ __device__ __forceinline__ void arrived(void)
     asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" :: "n"(N) : "memory");
 }
 
-template <int USE, int KA, int KB, int TM, int WM, int WN, int PB, int BUFFERS>
-__device__ __forceinline__ void packed_tile(PackedProduct const &p, int id, char *lds, int *scales, float *bias)
+// TAILS: 1 a has tails, 2 b has, 0 neither
+template <int USE, int KA, int KB, int TAILS, int TM, int WM, int WN, int PB, int BUFFERS>
+__device__ __forceinline__ void packed_tile(PackedProduct const &p, int id, char *lds, int *scales, float *limits, float *bias)
 {
     constexpr int TN = 2, kWaves = WM * WN, kBM = TM * WM, kBN = TN * WN;           // blocks of 32 rows
     constexpr int kOwn = kBM / kWaves;              // row blocks of a that a wavefront loads; of b it loads one
@@ -534,14 +593,75 @@ __device__ __forceinline__ void packed_tile(PackedProduct const &p, int id, char
     // what is needed behind the products: the scales and biases of the tile's rows (the barriers of the stages are between this and its use)
     DenseOutput o = p.out;
     int const *const scale_a = scales, *const scale_b = scales + kBM * 32;
+    float const *const limit_a = limits, *const limit_b = limits + kBM * 32;
     for (int i = threadIdx.x; i < kBM * 32; i += kWaves * 64) {
         scales[i] = p.ea[min(rb_a * 32 + i, p.a_blocks * 32 - 1)];
+        limits[i] = limit_of<PB>(p.lost_a[min(rb_a * 32 + i, p.a_blocks * 32 - 1)]);
         if (USE != kUseStore) { bias[i] = o.bias && rb_a * 32 + i < o.rows ? o.bias[rb_a * 32 + i] : 0.0f; }
     }
-    for (int i = threadIdx.x; i < kBN * 32; i += kWaves * 64) { scales[kBM * 32 + i] = PB == 2 ? p.eb[min(rb_b * 32 + i, p.b_blocks * 32 - 1)] : 0; }
+    for (int i = threadIdx.x; i < kBN * 32; i += kWaves * 64) {
+        scales[kBM * 32 + i] = PB == 2 ? p.eb[min(rb_b * 32 + i, p.b_blocks * 32 - 1)] : 0;
+        limits[kBM * 32 + i] = limit_of<PB>(p.lost_b[min(rb_b * 32 + i, p.b_blocks * 32 - 1)]);
+    }
 
     int const wm = wave / WN, wn = wave % WN;
     DenseAcc16 acc[TM][TN] = {};
+    if constexpr (TAILS != 0) {
+        // One operand's tails times the other's upper halves ahead of everything else, two steps of k at a time, and the sums brought to scale.
+        constexpr int kTailStage = (kBM + kBN) * 2048, kTailLoads = 2 * kOwn + 2;
+        constexpr long long kStepA = TAILS == 1 ? 1024 : 2048, kStepB = TAILS == 2 ? 1024 : 1024 * PB;          // bytes from step to step
+        char const *tail_a[kOwn];
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i) {
+            tail_a[i] = reinterpret_cast<char const *>(TAILS == 1 ? p.tails : p.a) + ((long long)min(rb_a + wave * kOwn + i, p.a_blocks - 1) * p.k_steps + first) * kStepA + lane * 16;
+        }
+        char const *tail_b = reinterpret_cast<char const *>(TAILS == 2 ? p.tails : p.b) + ((long long)min(rb_b + wave, p.b_blocks - 1) * p.k_steps + first) * kStepB + lane * 16;
+        auto const fetch_tails = [&](int buffer, int s) {
+            bool const both = 2 * s + 1 < stages;           // (else the first step once more, which is not used)
+            auto const two = [&](uint32_t to, char const *from, long long step) {
+                asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(to), "v"(from) : "memory", "m0");
+                asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(to + 1024), "v"(from + (both ? step : 0)) : "memory", "m0");
+            };
+#pragma unroll
+            for (int i = 0; i < kOwn; ++i) { two(at_lds + buffer * kTailStage + (wave * kOwn + i) * 2048, tail_a[i], kStepA); tail_a[i] += 2 * kStepA; }
+            two(at_lds + buffer * kTailStage + (kBM + wave) * 2048, tail_b, kStepB);
+            tail_b += 2 * kStepB;
+        };
+        int const pairs = (stages + 1) / 2;
+        for (int s = 0; s < min(kAhead, pairs); ++s) { fetch_tails(s, s); }
+        int buffer = 0, free = kAhead;
+#pragma nounroll
+        for (int s = 0; s < pairs; ++s) {
+            if (s + kAhead < pairs) { arrived<(kAhead - 1) * kTailLoads>(); fetch_tails(free, s + kAhead); }
+            else                    { arrived<0>(); }
+            char const *const from = lds + buffer * kTailStage + lane * 16;
+            DenseHalf8 u[TM][2], v[TN][2];
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+#pragma unroll
+                for (int j = 0; j < TN; ++j) { v[j][q] = *reinterpret_cast<DenseHalf8 const *>(from + (kBM + wn * TN + j) * 2048 + q * 1024); }
+#pragma unroll
+                for (int i = 0; i < TM; ++i) { u[i][q] = *reinterpret_cast<DenseHalf8 const *>(from + (wm * TM + i) * 2048 + q * 1024); }
+            }
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                if (q == 1 && 2 * s + 1 >= stages) { break; }
+#pragma unroll
+                for (int i = 0; i < TM; ++i) {
+#pragma unroll
+                    for (int j = 0; j < TN; ++j) { acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(u[i][q], v[j][q], acc[i][j], 0, 0, 0); }
+                }
+            }
+            free = buffer;
+            buffer = buffer + 1 == BUFFERS ? 0 : buffer + 1;
+        }
+        __syncthreads();                        // (nobody reads LDS any more, where the first stages go)
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+#pragma unroll
+            for (int j = 0; j < TN; ++j) { acc[i][j] *= 1.0f / kTailScale; }
+        }
+    }
     struct Halves { DenseHalf8 a[TM][2], b[TN][PB]; };
     auto const read = [&](int buffer, Halves &h) {
         char const *from = lds + buffer * kStage + lane * 16;
@@ -572,6 +692,34 @@ __device__ __forceinline__ void packed_tile(PackedProduct const &p, int id, char
             __builtin_amdgcn_sched_barrier(0);
         }
     };
+    // Of each element whether its sum has not been as large as its limit yet, bit 16 j + r; later whether it is formed again.  Looked at up to eight times on the way, and not ahead of 1024 k: with
+    // fewer a sum is seldom that small at the end.  Nor where the limits are below 2^12 (sums of scaled values are 2^27 and more): all rows of a wavefront have that in common.
+    uint32_t again[TM];
+#pragma unroll
+    for (int i = 0; i < TM; ++i) { again[i] = 0xffffffffu; }
+    int const look_every = max(64, (stages / 8 + 1) & ~1);
+    int look = look_every;
+    auto const look_at_sums = [&] {
+        look += look_every;
+        float lb[TN], most = 0.0f;
+#pragma unroll
+        for (int j = 0; j < TN; ++j) { lb[j] = limit_b[(wn * TN + j) * 32 + (lane & 31)]; most = fmaxf(most, lb[j]); }
+#pragma unroll
+        for (int i = 0; i < TM; ++i) { most = fmaxf(most, limit_a[(wm * TM + i) * 32 + (lane & 31)]); }
+        if (!__any(most >= 4096.0f)) { look = 0x7fffffff; return; }
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+            // (the sign of the difference goes in at the bottom, from the last element to the first)
+            uint32_t small = 0;
+#pragma unroll
+            for (int e = 16 * TN - 1; e >= 0; --e) {
+                float const left = fabsf(acc[i][e / 16][e % 16]) - (limit_a[(wm * TM + i) * 32 + acc_row(e % 16, lane)] + lb[e / 16]);
+                small = __builtin_amdgcn_alignbit(small, __builtin_bit_cast(uint32_t, left), 31);
+                if (e % 4 == 0) { __builtin_amdgcn_sched_barrier(0); }
+            }
+            again[i] &= small;
+        }
+    };
     __builtin_amdgcn_s_waitcnt(0xc07f);         // (no scalar load on its way: with one the compiler could not count reads of LDS and would wait for all of them at once)
     if constexpr (TM == 2) {
         // A small tile's halves fit the registers twice: the next stage's are read behind the present one's products, which nothing else would cover where a compute unit has one such
@@ -597,9 +745,13 @@ __device__ __forceinline__ void packed_tile(PackedProduct const &p, int id, char
             multiply(now);
         };
         int s = 0;
-        for (; s + 5 < stages; s += 2) {
-            full_step(s, even, odd);
-            full_step(s + 1, odd, even);
+        for (;;) {
+            for (int const end = min(stages - 5, look); s < end; s += 2) {
+                full_step(s, even, odd);
+                full_step(s + 1, odd, even);
+            }
+            if (s < look) { break; }
+            look_at_sums();
         }
 #pragma nounroll
         for (; s < stages; s += 2) {
@@ -615,13 +767,17 @@ __device__ __forceinline__ void packed_tile(PackedProduct const &p, int id, char
         for (int s = 0; s < ahead; ++s) { fetch(s); }
         int buffer = 0, free = kAhead;
         int s = 0;
-        for (; s + kAhead < stages; ++s) {
-            arrived<(kAhead - 1) * kLoads>();
-            fetch(free);
-            read(buffer, h);
-            multiply(h);
-            free = buffer;
-            buffer = buffer + 1 == BUFFERS ? 0 : buffer + 1;
+        for (;;) {
+            for (int const end = min(stages - kAhead, look); s < end; ++s) {
+                arrived<(kAhead - 1) * kLoads>();
+                fetch(free);
+                read(buffer, h);
+                multiply(h);
+                free = buffer;
+                buffer = buffer + 1 == BUFFERS ? 0 : buffer + 1;
+            }
+            if (s < look) { break; }
+            look_at_sums();
         }
         for (; s < stages; ++s) {
             arrived<0>();
@@ -639,45 +795,66 @@ __device__ __forceinline__ void packed_tile(PackedProduct const &p, int id, char
     int const n0 = (rb_b + wn * TN) * 32;
     __syncthreads();                            // (the stages are done with LDS)
     float2 column = make_float2(-INFINITY, 0.0f);
-    uint32_t again[TM] = {};                    // of the elements that are formed again, bit 16 j + r
+#pragma unroll
+    for (int i = 0; i < TM; ++i) { if (rb_a + wm * TM + i >= p.a_blocks) { again[i] = 0; } }
 #pragma nounroll
     for (int i = 0; i < TM; ++i) {
         int const rb = rb_a + wm * TM + i, m0 = rb * 32;
         if (rb >= p.a_blocks) { break; }
         int eb[TN];
+        float lb[TN];
 #pragma unroll
-        for (int j = 0; j < TN; ++j) { eb[j] = scale_b[(wn * TN + j) * 32 + (lane & 31)]; }
-        bool marks = false;
+        for (int j = 0; j < TN; ++j) { eb[j] = scale_b[(wn * TN + j) * 32 + (lane & 31)]; lb[j] = limit_b[(wn * TN + j) * 32 + (lane & 31)]; }
+        // (registers have no index; `which` is i, and the compiler does not know it: it would write the loop out, with all its addresses in registers at once)
+        int which = i;
+        asm volatile("" : "+s"(which));
+        DenseAcc16 now[TN];
+        uint32_t small = 0;
 #pragma unroll
-        for (int u = 0; u < TM; ++u) {              // (registers have no index)
-            if (u != i) { continue; }
-            bool odd = false;
+        for (int u = 0; u < TM; ++u) {
+            if (u != which) { continue; }
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                int const row = acc_row(r, lane), ea = scale_a[(wm * TM + i) * 32 + row];
+            for (int j = 0; j < TN; ++j) { now[j] = acc[u][j]; }
+            small = again[u];
+        }
+        bool odd = false;                           // some sum is below its limit, or no number
 #pragma unroll
-                for (int j = 0; j < TN; ++j) {
-                    float const d = ldexpf(acc[u][j][r], -(ea + eb[j]));           // the scales come off
-                    odd = odd || d != d;
-                    tile[row * kTilePitch + j * 32 + (lane & 31)] = d;
-                }
+        for (int r = 0; r < 16; ++r) {
+            int const row = acc_row(r, lane), ea = scale_a[(wm * TM + i) * 32 + row];
+            float const la = limit_a[(wm * TM + i) * 32 + row];
+#pragma unroll
+            for (int j = 0; j < TN; ++j) {
+                odd = odd | !(fabsf(now[j][r]) >= la + lb[j]);
+                tile[row * kTilePitch + j * 32 + (lane & 31)] = ldexpf(now[j][r], -(ea + eb[j]));           // the scales come off
             }
-            marks = p.slabs == 1 && __any(odd);
-            if (__builtin_expect(marks, 0)) {
+        }
+        bool const marks = p.slabs == 1 && __any(odd);
+        uint32_t formed = 0;
+        if (__builtin_expect(marks, 0)) {
+            int at = lane;
+            asm volatile("" : "+v"(at));            // (or the sums of limits from above stay in registers)
+            uint32_t below = 0;                     // as look_at_sums has it
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
+            for (int e = 16 * TN - 1; e >= 0; --e) {
+                float const left = fabsf(now[e / 16][e % 16]) - (limit_a[(wm * TM + i) * 32 + acc_row(e % 16, at)] + limit_b[(wn * TN + e / 16) * 32 + (at & 31)]);
+                below = __builtin_amdgcn_alignbit(below, __builtin_bit_cast(uint32_t, left), 31);
+                if (e % 4 == 0) { __builtin_amdgcn_sched_barrier(0); }
+            }
+            below &= small;
 #pragma unroll
-                    for (int j = 0; j < TN; ++j) {
-                        float *const d = tile + acc_row(r, lane) * kTilePitch + j * 32 + (lane & 31);
-                        if (*d != *d) {
-                            again[u] |= 1u << (j * 16 + r);
-                            *d = __builtin_bit_cast(float, kNotStored);
-                        }
-                    }
+            for (int e = 0; e < 16 * TN; ++e) {
+                float *const d = tile + acc_row(e % 16, at) * kTilePitch + e / 16 * 32 + (at & 31);
+                if (*d != *d || ((below >> e) & 1u)) {
+                    formed |= 1u << e;
+                    *d = __builtin_bit_cast(float, kNotStored);
                 }
             }
         }
-        finish<USE>(o, p.slabs > 1, tile, bias + (wm * TM + i) * 32, m0, n0, lane, column, marks, false);
+#pragma unroll
+        for (int u = 0; u < TM; ++u) { again[u] = u == which ? formed : again[u]; }
+        int at = lane;
+        asm volatile("" : "+v"(at));                // (nor are its addresses kept from one round to the next)
+        finish<USE>(o, p.slabs > 1, tile, bias + (wm * TM + i) * 32, m0, n0, at, column, marks, false);
     }
     // A second time round for what is formed again (its code needs the registers that the accumulators have had)
     uint32_t any = 0;
@@ -719,21 +896,24 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void dense_packed_kernel(PackedPro
 {
     __shared__ __attribute__((aligned(1024))) char lds[packed_lds<TM, WM, WN, BUFFERS>()];
     __shared__ int scales[(TM * WM + 2 * WN) * 32];
+    __shared__ float limits[(TM * WM + 2 * WN) * 32];
     __shared__ float bias[TM * WM * 32];
-    packed_tile<USE, kRows, PB == 1 ? kBitColumns : kColumns, TM, WM, WN, PB, BUFFERS>(p, blockIdx.x, lds, scales, bias);
+    packed_tile<USE, kRows, PB == 1 ? kBitColumns : kColumns, 0, TM, WM, WN, PB, BUFFERS>(p, blockIdx.x, lds, scales, limits, bias);
 }
 
 // the weights' gradient, and behind it the input's (either may have no workgroups)
-template <int TM, int WM, int WN, int PB, int BUFFERS>
+template <bool TAILS, int TM, int WM, int WN, int PB, int BUFFERS>
 __global__ __launch_bounds__(WM * WN * 64, 2) void dense_packed_pair_kernel(PackedProduct p, PackedProduct q)
 {
     __shared__ __attribute__((aligned(1024))) char lds[packed_lds<TM, WM, WN, BUFFERS>()];
     __shared__ int scales[(TM * WM + 2 * WN) * 32];
-    if ((int)blockIdx.x < p.workgroups) { packed_tile<kUseStore, kGradRows, PB == 1 ? kBitRows : kRows, TM, WM, WN, PB, BUFFERS>(p, blockIdx.x, lds, scales, nullptr); }
-    else                                { packed_tile<kUseStore, kColumns, kGradColumns, TM, WM, WN, 2, BUFFERS>(q, blockIdx.x - p.workgroups, lds, scales, nullptr); }
+    __shared__ float limits[(TM * WM + 2 * WN) * 32];
+    if ((int)blockIdx.x < p.workgroups) { packed_tile<kUseStore, kGradRows, PB == 1 ? kBitRows : kRows, TAILS ? 1 : 0, TM, WM, WN, PB, BUFFERS>(p, blockIdx.x, lds, scales, limits, nullptr); }
+    else                                { packed_tile<kUseStore, kColumns, kGradColumns, TAILS ? 2 : 0, TM, WM, WN, 2, BUFFERS>(q, blockIdx.x - p.workgroups, lds, scales, limits, nullptr); }
 }
 
-__device__ __forceinline__ float sum_of_slabs(PackedProduct const &p, int m, int n)
+// `top`: the largest magnitude of the sums
+__device__ __forceinline__ float sum_of_slabs(PackedProduct const &p, int m, int n, float &top)
 {
     float const *from = p.sums + m * p.sums_pitch + n;
     float d = 0.0f;
@@ -741,9 +921,17 @@ __device__ __forceinline__ float sum_of_slabs(PackedProduct const &p, int m, int
     for (; s + 4 <= p.slabs; s += 4) {
         float const a = from[s * p.sums_slab], b = from[(s + 1) * p.sums_slab], c = from[(s + 2) * p.sums_slab], e = from[(s + 3) * p.sums_slab];
         d = (((d + a) + b) + c) + e;
+        top = fmaxf(fmaxf(fmaxf(fmaxf(top, fabsf(a)), fabsf(b)), fabsf(c)), fabsf(e));
     }
-    for (; s < p.slabs; ++s) { d += from[s * p.sums_slab]; }
+    for (; s < p.slabs; ++s) { float const a = from[s * p.sums_slab]; d += a; top = fmaxf(top, fabsf(a)); }
+    top = fmaxf(top, fabsf(d));
     return d;
+}
+
+// as the tiles have it, with the scales off
+__device__ __forceinline__ float limit_at(PackedProduct const &p, int m, int n)
+{
+    return p.b_pieces == 2 ? ldexpf(limit_of<2>(p.lost_a[m] + p.lost_b[n]), -(p.ea[m] + p.eb[n])) : ldexpf(limit_of<1>(p.lost_a[m] + p.lost_b[n]), -p.ea[m]);
 }
 
 // The slabs' sums of a product, in order, and what becomes of them: a wavefront takes 64 neighbours of a row.
@@ -755,8 +943,14 @@ __device__ __forceinline__ void join_slabs(PackedProduct const &p, unsigned id)
     if (m >= o.rows) { return; }
     bool const inside = n < o.columns || (n == o.columns && o.line && o.kind == kOutStore);
     float d = 0.0f;
-    if (inside) { d = sum_of_slabs(p, m, n); }
-    if (__builtin_expect(p.kind_a >= 0 && __any(inside && d != d), 0)) { row_again(p.src_a, p.kind_a, p.src_b, p.kind_b, d, inside && d != d, m, n - lane, lane); }
+    bool again = false;
+    if (inside) {
+        float const limit = p.kind_a >= 0 ? limit_at(p, m, n) : -INFINITY;
+        float top = 0.0f;
+        d = sum_of_slabs(p, m, n, top);
+        again = p.kind_a >= 0 && (d != d || top < limit);
+    }
+    if (__builtin_expect(__any(again), 0)) { row_again(p.src_a, p.kind_a, p.src_b, p.kind_b, d, again, m, n - lane, lane); }
     if (o.kind == kOutForward) { if (inside) { static_cast<float *>(o.out)[m * o.stride + n] = activated(before_activation(o, d, m, n), o.activation); } }
     else if (o.kind == kOutBits) {
         uint64_t const bits = __ballot(inside && before_activation(o, d, m, inside ? n : 0) > 0.0f);
@@ -782,7 +976,11 @@ __global__ __launch_bounds__(kJoinLogitWaves * 64, 8) void dense_join_logits_ker
     int const m0 = tile * 32 + wave * 2;
     bool const inside = n < o.columns;
     int const label = inside ? o.label[n] - o.first_channel : -1;
-    float z[2] = {};
+    float z[2] = {}, top[2] = {}, limit[2] = {-INFINITY, -INFINITY};
+    if (inside && p.kind_a >= 0) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) { limit[i] = limit_at(p, min(m0 + i, o.rows - 1), n); }
+    }
     if (inside) {
         // (a row behind the last one reads the last one)
         float const *const a = p.sums + min(m0, o.rows - 1) * p.sums_pitch + n, *const b = p.sums + min(m0 + 1, o.rows - 1) * p.sums_pitch + n;
@@ -794,14 +992,22 @@ __global__ __launch_bounds__(kJoinLogitWaves * 64, 8) void dense_join_logits_ker
                 u[q] = a[at]; v[q] = b[at];
             }
 #pragma unroll
-            for (int q = 0; q < 4; ++q) { z[0] += s + q < p.slabs ? u[q] : 0.0f; z[1] += s + q < p.slabs ? v[q] : 0.0f; }
+            for (int q = 0; q < 4; ++q) {
+                z[0] += s + q < p.slabs ? u[q] : 0.0f; z[1] += s + q < p.slabs ? v[q] : 0.0f;
+                top[0] = fmaxf(top[0], fabsf(u[q])); top[1] = fmaxf(top[1], fabsf(v[q]));
+            }
         }
     }
-    if (__builtin_expect(p.kind_a >= 0 && __any(inside && (z[0] != z[0] || z[1] != z[1])), 0)) {
+    bool again[2] = {};
+    if (inside && p.kind_a >= 0) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) { again[i] = z[i] != z[i] || fmaxf(top[i], fabsf(z[i])) < limit[i]; }
+    }
+    if (__builtin_expect(__any(again[0] || again[1]), 0)) {
 #pragma nounroll
         for (int i = 0; i < 2; ++i) {
             float d = i ? z[1] : z[0];
-            if (m0 + i < o.rows) { logit_again(p.src_a, p.src_b, p.kind_b, d, inside && d != d && frame_counts(o, n), m0 + i, n - lane, lane); }
+            if (m0 + i < o.rows) { logit_again(p.src_a, p.src_b, p.kind_b, d, (i ? again[1] : again[0]) && frame_counts(o, n), m0 + i, n - lane, lane); }
             if (i) { z[1] = d; } else { z[0] = d; }
         }
     }

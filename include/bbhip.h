@@ -529,6 +529,8 @@ int bbhip_fp32_CategoricalSampling(float const *dev_y_buf, float const *dev_u_bu
  *     y[o][f] = activation(sum over i of W[o][i] * x[i][f] + b[o] + residual[o][f])
  * activation: 0 none, 1 relu, 2 sigmoid, 3 hard tanh (limits -1 and 1).  bit_...: x is packed bits, read as 0 and 1; ..._bit: y is packed bits, set where the sum is above 0 (the bits
  * behind the last frame of its word are 0; further words of a row are left alone). 
+ * At any size and for operands of any scales an element is as accurate as a sum of fp32 products in fp32: what it is off by goes by the magnitudes of its own products, not by other values of its
+ * row or column (large products are made of halves; elements that these do not hold are formed again in fp32, and a call most of whose elements are such takes that much longer).
  * At most 2^24 nodes, 2^25 frames and strides of 33 * 2^20. */
 size_t bbhip_DenseAffine_WorkspaceBytes(int input_node_size, int output_node_size, int frame_size);
 int bbhip_fp32_DenseAffine_Forward(float const *dev_x_buf, float *dev_y_buf, float const *dev_W, float const *dev_b, float const *dev_residual_buf, int activation,

@@ -24,9 +24,10 @@ class GradientNorm {
     }
 
 public:
-    // The tensors must keep their storage (no Resize) while they are bound, and none may be in the list twice.
+    // The tensors must keep their storage (no Resize) while they are bound.  One that is in the list twice is refused: it would be counted and scaled twice, by two workgroups at once.
     explicit GradientNorm(Variables grads) : m_grads(grads), m_norm(Memory::Create(2 * sizeof(float)))
     {
+        if (grads.HasOneTwice()) { throw Exception("GradientNorm: a tensor is in the list twice"); }
         index_t const n = grads.GetSize();
         std::vector<std::int32_t> sizes;
         std::vector<void *> addresses;

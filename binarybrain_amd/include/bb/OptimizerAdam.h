@@ -35,11 +35,17 @@ class OptimizerAdam : public Optimizer {
     std::shared_ptr<Memory> m_size_table, m_param_table, m_grad_table, m_m_table, m_v_table;
 
     T         m_max_norm = (T)-1;               // negative: gradients are taken as they are
+    bool      m_twice = false;                  // a tensor is in the lists twice
     std::shared_ptr<Memory> m_norm;             // (norm, scale) of the last clipped step
     Workspace m_work;
 
     OptimizerAdam(T learning_rate, T beta1, T beta2)
         : m_learning_rate(learning_rate), m_beta1(beta1), m_beta2(beta2), m_b1(beta1), m_b2(beta2) {}
+
+    static void RefuseTwice(double max_norm, bool twice)
+    {
+        if (max_norm >= 0 && twice) { throw Exception("OptimizerAdam: a tensor is in the lists twice, which a step with clipped gradients cannot have"); }
+    }
 
     static std::shared_ptr<Memory> pointer_table(std::vector<void *> const &ptrs)
     {
@@ -68,14 +74,19 @@ public:
 
     void SetLearningRate(double learning_rate) override { m_learning_rate = (T)learning_rate; }
 
-    // From now on gradients count scaled to this norm where theirs, as one vector, is larger (they stay as they are until ZeroGrad); a negative value ends it.  No tensor may be in the
-    // list twice.  (The reference's optimizer does not clip.)
+    // From now on gradients count scaled to this norm where theirs, as one vector, is larger (they stay as they are until ZeroGrad); a negative value ends it, and infinity only measures.  A list in
+    // which a tensor is twice cannot be clipped.  (The reference's optimizer does not clip.)
     void SetGradientClipping(double max_norm)
     {
+        if (max_norm != max_norm) { throw Exception("OptimizerAdam: the norm to clip to is not a number"); }
+        RefuseTwice(max_norm, m_twice);
         m_max_norm = (T)max_norm;
-        if (!m_norm) { m_norm = Memory::Create(2 * sizeof(float)); }
+        if (!m_norm) {
+            m_norm = Memory::Create(2 * sizeof(float));
+            std::memset(m_norm->Lock(true), 0, 2 * sizeof(float));
+        }
     }
-    // the norm that the gradients had in the last clipped step
+    // the norm that the gradients had in the last clipped step, 0 ahead of the first
     double GetGradientNorm(void) const { return m_norm ? ((float const *)m_norm->LockConst())[0] : 0.0; }
 
     // Binds the parameter list; the moment estimates start at zero (reference: OptimizerAdam.h:120-130).
@@ -83,6 +94,11 @@ public:
     void SetVariables(Variables params, Variables grads) override
     {
         BB_ASSERT(params.GetSize() == grads.GetSize());
+        Variables all = params;
+        all.PushBack(grads);
+        bool const twice = all.HasOneTwice();
+        RefuseTwice(m_max_norm, twice);
+        m_twice  = twice;
         m_params = params;
         m_grads  = grads;
         m_m.clear(); m_v.clear();

@@ -65,6 +65,9 @@ public:
 
     std::string GetObjectName(void) const override { return "Tensor"; }
 
+    // whether both have elements, and the same ones (a copy shares them)
+    bool SharesElements(Tensor const &other) const { return m_size > 0 && m_mem == other.m_mem; }
+
 protected:
     // the layout of the reference's typed tensor (include/bb/Tensor.h:614-651): version, parent version, element offset,
     // element count, shape, row-major strides, elements
@@ -201,6 +204,14 @@ public:
     Tensor &operator[](index_t i) { return *m_tensors[(std::size_t)i]; }
     Tensor const &operator[](index_t i) const { return *m_tensors[(std::size_t)i]; }
     void FillZero(void) { for (auto &t : m_tensors) { t->FillZero(); } }
+    // whether two of its tensors have the same elements
+    bool HasOneTwice(void) const
+    {
+        for (std::size_t i = 0; i < m_tensors.size(); ++i) {
+            for (std::size_t j = 0; j < i; ++j) { if (m_tensors[i]->SharesElements(*m_tensors[j])) { return true; } }
+        }
+        return false;
+    }
 };
 
 }  // namespace bb

@@ -1,12 +1,12 @@
-"""CPU suite: which form (straight or packed, wavefronts, tiles, shared k axes, pieces) a size of a dense layer or of the loss on top of one takes (tests/cpp/test_dense_forms.cpp)."""
+"""CPU suite: what the host classes of clipped gradients refuse (tests/cpp/test_dense_objects.cpp); which form (straight or packed, wavefronts, tiles, shared k axes, pieces) a size of a dense layer or of the loss on top of one takes (tests/cpp/test_dense_forms.cpp)."""
 import os
 import subprocess
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
-def tool(*args):
-    exe = os.path.join(ROOT, "tests", "cpp", "test_dense_forms")
+def tool(*args, name="test_dense_forms"):
+    exe = os.path.join(ROOT, "tests", "cpp", name)
     if not os.path.exists(exe):
         from binarybrain_amd.build import build_cpp_tests
         build_cpp_tests()
@@ -18,3 +18,7 @@ def tool(*args):
 def test_rules():
     """no rule asks for a number of wavefronts that no kernel has"""
     tool("--rules")
+
+
+def test_objects():
+    tool(name="test_dense_objects")

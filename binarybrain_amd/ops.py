@@ -74,7 +74,7 @@ def vector_minmax(name, src0, src1, out=None):
 
 class AdamState:
     """Device-side tables of one parameter list for bbhip_fp32_OptimizerAdam, with the bias-correction products kept
-    on the host as the reference does (include/bb/OptimizerAdam.h:104-110, 166-180)."""
+    on the host as the reference does (include/bb/OptimizerAdam.h:104-110, 166-180).  Gradients behind the last parameter's are not looked at."""
 
     def __init__(self, params, grads, learning_rate=0.001, beta1=0.9, beta2=0.999, m=None, v=None):
         for tensor in (*params, *grads):
@@ -83,15 +83,17 @@ class AdamState:
         self.params, self.grads = list(params), list(grads)
         self.m = [torch.zeros_like(p) for p in params] if m is None else list(m)
         self.v = [torch.zeros_like(p) for p in params] if v is None else list(v)
-        for p, *others in zip(self.params, self.grads, self.m, self.v, strict=True):
+        if len(self.grads) < len(self.params) or len(self.m) != len(self.params) or len(self.v) != len(self.params):
+            raise capi.BbhipError("AdamState: %d parameters, %d gradients, %d and %d moments" % (len(self.params), len(self.grads), len(self.m), len(self.v)))
+        for p, *others in zip(self.params, self.grads, self.m, self.v):
             for tensor in (p, *others):
                 if not tensor.is_cuda or not tensor.is_contiguous() or tensor.dtype != torch.float32 or tensor.numel() != p.numel():
                     raise capi.BbhipError("AdamState: contiguous float32 device tensors, those of a parameter of one size")
-        held = [t.data_ptr() for t in (*self.params, *self.grads, *self.m, *self.v) if t.numel()]
+        held = [t.data_ptr() for t in (*self.params, *self.grads[:len(self.params)], *self.m, *self.v) if t.numel()]
         self.twice = len(set(held)) != len(held)
         dev = params[0].device
         table = lambda ts: torch.tensor([t.data_ptr() for t in ts], dtype=torch.int64, device=dev)
-        self.t_params, self.t_grads, self.t_m, self.t_v = table(self.params), table(self.grads), table(self.m), table(self.v)
+        self.t_params, self.t_grads, self.t_m, self.t_v = table(self.params), table(self.grads[:len(self.params)]), table(self.m), table(self.v)
         self.t_size = torch.tensor([p.numel() for p in params], dtype=torch.int32, device=dev)
         f32 = np.float32
         self.lr, self.beta1, self.beta2 = f32(learning_rate), f32(beta1), f32(beta2)

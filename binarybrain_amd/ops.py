@@ -74,7 +74,10 @@ def vector_minmax(name, src0, src1, out=None):
 
 class AdamState:
     """Device-side tables of one parameter list for bbhip_fp32_OptimizerAdam, with the bias-correction products kept
-    on the host as the reference does (include/bb/OptimizerAdam.h:104-110, 166-180).  Gradients behind the last parameter's are not looked at."""
+    on the host as the reference does (include/bb/OptimizerAdam.h:104-110, 166-180).  Gradients behind the last parameter's are not looked at.
+
+    The plain step takes its betas as the reference does, rounded to float32; a step with clipped gradients takes 1 - beta of the values given, in 64 bits.  With betas that are float32 values
+    (np.float32(0.999)) both have the same bits where nothing is clipped."""
 
     def __init__(self, params, grads, learning_rate=0.001, beta1=0.9, beta2=0.999, m=None, v=None):
         for tensor in (*params, *grads):

@@ -1,4 +1,5 @@
-"""GPU: the lists that AdamState takes."""
+"""GPU: the lists that AdamState takes, and the plain step beside one whose gradients are not clipped."""
+import numpy as np
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -27,3 +28,19 @@ def test_lists_of_unequal_length():
             a.step(max_norm=max_norm)
             b.step(max_norm=max_norm)
         assert all(torch.equal(p, q) for p, q in zip(more, same)) and len(a.grads) == 3
+
+
+def test_a_step_that_clips_nothing_is_the_plain_one():
+    """of betas that are float32 values"""
+    import torch
+    from binarybrain_amd import ops
+    sizes = [4096, 33, 100_001, 1]
+    plain, measured = tensors(1, sizes), tensors(1, sizes)
+    grads = tensors(2, sizes)
+    betas = dict(beta1=np.float32(0.9), beta2=np.float32(0.999))
+    a, b = ops.AdamState(plain, grads, **betas), ops.AdamState(measured, grads, **betas)
+    for _ in range(3):
+        a.step()
+        assert b.step(max_norm=float("inf"))[1].item() == 1.0
+        for p, q in zip(plain + a.m + a.v, measured + b.m + b.v):
+            assert torch.equal(p, q)

@@ -2,6 +2,10 @@
 import os
 import subprocess
 
+import pytest
+
+import dense_sizes
+
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
@@ -22,3 +26,8 @@ def test_rules():
 
 def test_objects():
     tool(name="test_dense_objects")
+
+
+@pytest.mark.parametrize("what,size", [(what, size) for what, sizes in (("forward", dense_sizes.FORWARD), ("backward", dense_sizes.BACKWARD), ("loss", dense_sizes.LOSS)) for size in sizes])
+def test_sizes_take_the_forms_that_they_are_there_for(what, size):
+    assert tool(what, *size) == getattr(dense_sizes, what.upper())[size]

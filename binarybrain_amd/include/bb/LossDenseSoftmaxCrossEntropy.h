@@ -1,4 +1,4 @@
-// The softmax cross entropy on top of a dense layer, in pieces of its channels: neither the logits nor their gradient are ever held whole.  CalculateLoss takes the layer's INPUT and the
+// The softmax cross entropy on top of a dense layer, in pieces of its channels: at most 64 Mi logits (or those of 256 channels) are held at a time.  CalculateLoss takes the layer's INPUT and the
 // labels, adds to the layer's gradients and returns the input's; accumulated over batches like the other losses.  (The reference has no such loss: there the layer's
 // output goes through LossSoftmaxCrossEntropy.)
 #pragma once

@@ -594,8 +594,8 @@ def _loss_weight_sum(label, weight, weight_sum, channels, frame_size):
 
 
 def loss_dense_softmax_cross_entropy(x, W, b, label, frame_size, weight=None, weight_sum=None, dW=None, db=None, want_gradients=True, want_dx=True, want_weights=True):
-    """The cross entropy of softmax(W x + b) against label (int32 [1, at least frame_size]; negative, or no channel: the frame does not count), and its gradients, without ever holding the
-    logits of all channels: (loss [1, stride of x], dx, dW, db), None for what is not wanted.  The loss of the batch is loss[:, :frame_size].sum() / weight_sum, whose gradient they are.
+    """The cross entropy of softmax(W x + b) against label (int32 [1, at least frame_size]; negative, or no channel: the frame does not count), and its gradients, with
+    at most 64 Mi logits (or those of 256 channels) held at a time: (loss [1, stride of x], dx, dW, db), None for what is not wanted.  The loss of the batch is loss[:, :frame_size].sum() / weight_sum, whose gradient they are.
     weight [1, ...]: of each frame (None: 1); weight_sum defaults to the sum of the weights that count, read by the host (a captured step gives its own).  dW and db given: added to in place."""
     return native.loss_dense_softmax_cross_entropy(x, W, b, label, frame_size, x.shape[-1], weight, _loss_weight_sum(label, weight, weight_sum, W.shape[0], frame_size), dW, db,
                                                    want_gradients and want_dx, want_gradients and want_weights)

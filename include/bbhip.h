@@ -557,7 +557,8 @@ int bbhip_bit_fp32_DenseAffine_Backward(int const *dev_x_buf, float const *dev_d
                                         int x_frame_stride, int dx_frame_stride, int frame_stride, void *dev_workspace, size_t workspace_size, void *stream);
 
 /* LossDenseSoftmaxCrossEntropy: the cross entropy of p = softmax(W x + b) over ch_size channels (W [ch][input]) against one label per frame, and its gradients, in pieces of the
- * channels: the logits are never held whole, the workspace does not grow with the channels beyond a piece's.  With w the frame's weight (dev_weight_buf, NULL: 1)
+ * channels.  With gradients the logits of one piece are held at a time, at most 64 Mi of them or those of 256 channels, which is all of a smaller call's; beyond that the workspace grows with
+ * the channels only by 8 bytes for every 32 or more of them and frame.  With w the frame's weight (dev_weight_buf, NULL: 1)
  *     dev_loss_buf[f] = -w * log p_label,   dz[c] = w / weight_sum * (p_c - [c is the label]),   dx = W^T dz,   dW = dz x^T,   db = sum over frames of dz.
  * The caller passes weight_sum = the sum of the weights that count and reports sum(dev_loss_buf) / weight_sum, whose gradients these are.  A frame whose label is negative or not below ch_size, or
  * whose weight is 0, does not count: loss 0, dx 0 and no part of dW and db, whatever it holds.  dx, dW and db (which is formed with dW) may be NULL: without any of them the loss alone is

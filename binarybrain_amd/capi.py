@@ -116,6 +116,7 @@ _SIGNATURES = {
     "bbhip_LossDistillation_WorkspaceBytes": (C.c_size_t, [_i] * 3),
     "bbhip_fp32_LossDistillation": (C.c_int, [_vp] * 6 + [_f, _f] + [_i] * 6 + [_vp, C.c_size_t, _vp]),
     "bbhip_DenseAffine_WorkspaceBytes": (C.c_size_t, [_i] * 3),
+    "bbhip_DenseAffine_Forward_WorkspaceBytes": (C.c_size_t, [_i] * 4),
     "bbhip_fp32_DenseAffine_Forward": (C.c_int, [_vp] * 5 + [_i] * 7 + [_vp, C.c_size_t, _vp]),
     "bbhip_bit_fp32_DenseAffine_Forward": (C.c_int, [_vp] * 5 + [_i] * 7 + [_vp, C.c_size_t, _vp]),
     "bbhip_fp32_bit_DenseAffine_Forward": (C.c_int, [_vp] * 5 + [_i] * 6 + [_vp, C.c_size_t, _vp]),

@@ -622,15 +622,24 @@ int squares(int size, int const *sizes, float *const *grads, void *workspace, si
 
 }  // namespace
 
+size_t bbhip_DenseAffine_Forward_WorkspaceBytes(int input_node_size, int output_node_size, int frame_size, int bit_input)
+{
+    if (check_sizes(input_node_size, output_node_size, frame_size, __func__)) { return 0; }
+    Carver forward{nullptr};
+    if (frame_size <= kFewFrames) { return 0; }
+    if (forward_packed(input_node_size, output_node_size, frame_size)) { ForwardSpace const f(forward, input_node_size, output_node_size, frame_size, bit_input != 0); }
+    else { sums_of(forward, direct_shape(output_node_size, frame_size, input_node_size).slabs, output_node_size, frame_size); }
+    return forward.at;
+}
+
 size_t bbhip_DenseAffine_WorkspaceBytes(int input_node_size, int output_node_size, int frame_size)
 {
     if (check_sizes(input_node_size, output_node_size, frame_size, __func__)) { return 0; }
-    Carver forward{nullptr}, backward{nullptr};
-    if (forward_packed(input_node_size, output_node_size, frame_size)) { ForwardSpace const f(forward, input_node_size, output_node_size, frame_size, false); }
-    else { sums_of(forward, direct_shape(output_node_size, frame_size, input_node_size).slabs, output_node_size, frame_size); }
+    size_t const forward = bbhip_DenseAffine_Forward_WorkspaceBytes(input_node_size, output_node_size, frame_size, 0);
+    Carver backward{nullptr};
     if (backward_packed(input_node_size, output_node_size, frame_size)) { BackwardSpace const b(backward, input_node_size, output_node_size, frame_size, false, false); }
     else { DirectBackwardSpace const d(backward, input_node_size, output_node_size, frame_size, true); }
-    return forward.at > backward.at ? forward.at : backward.at;
+    return forward > backward.at ? forward : backward.at;
 }
 
 int bbhip_fp32_DenseAffine_Forward(float const *dev_x_buf, float *dev_y_buf, float const *dev_W, float const *dev_b, float const *dev_residual_buf, int activation,

@@ -637,7 +637,7 @@ at::Tensor dense_affine_forward_as(bool bit, bool bit_out, char const *name, T x
     if ((bit_out ? (int64_t)y_stride * 32 : y_stride) < frames) { c.refuse("the output's rows are shorter than the frames"); }
     if (residual) { c.rows("residual", *residual, at::kFloat, outputs, frames); }
     at::Tensor y = bit_out ? zeros_i32(x, outputs, y_stride) : rows_f32(x, outputs, y_stride);
-    at::Tensor const work = c.workspace(x, bbhip_DenseAffine_WorkspaceBytes(inputs, outputs, frames));
+    at::Tensor const work = c.workspace(x, bbhip_DenseAffine_Forward_WorkspaceBytes(inputs, outputs, frames, (int)bit));
     int const r_stride = residual ? stride_of(*residual) : 0;
     if (bit_out) {
         if (bit) {

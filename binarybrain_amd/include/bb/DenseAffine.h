@@ -77,6 +77,7 @@ protected:
         if (!buf.IsDeviceAvailable()) { throw Exception("DenseAffine: host-only execution is not provided by this library (device path only)"); }
     }
     static int Stride(FrameBuffer const &buf) { return (int)(buf.GetFrameStride() / 4); }
+    std::size_t ForwardWorkspaceSize(index_t frames) const { return bbhip_DenseAffine_Forward_WorkspaceBytes((int)GetInputNodeSize(), (int)GetOutputNodeSize(), (int)frames, kBit); }
     std::size_t WorkspaceSize(index_t frames) const { return bbhip_DenseAffine_WorkspaceBytes((int)GetInputNodeSize(), (int)GetOutputNodeSize(), (int)frames); }
 
 public:
@@ -154,7 +155,7 @@ public:
         bool const more = !residual_buf.Empty();
         BB_ASSERT(!more || (residual_buf.GetType() == BB_TYPE_FP32 && residual_buf.GetNodeSize() == y_buf.GetNodeSize() && residual_buf.GetFrameSize() == x_buf.GetFrameSize()));
         int const in = (int)x_buf.GetNodeSize(), out = (int)y_buf.GetNodeSize(), frames = (int)x_buf.GetFrameSize();
-        std::size_t const size = WorkspaceSize(frames);
+        std::size_t const size = ForwardWorkspaceSize(frames);
         {
             auto px = x_buf.LockDeviceMemoryConst();
             auto py = y_buf.LockDeviceMemory(true);

@@ -532,7 +532,8 @@ int bbhip_fp32_CategoricalSampling(float const *dev_y_buf, float const *dev_u_bu
  * At any size and for operands of any scales an element is as accurate as a sum of fp32 products in fp32: what it is off by goes by the magnitudes of its own products, not by other values of its
  * row or column (large products are made of halves; elements that these do not hold are formed again in fp32, and a call most of whose elements are such takes that much longer).
  * At most 2^24 nodes, 2^25 frames and strides of 33 * 2^20. */
-size_t bbhip_DenseAffine_WorkspaceBytes(int input_node_size, int output_node_size, int frame_size);
+size_t bbhip_DenseAffine_WorkspaceBytes(int input_node_size, int output_node_size, int frame_size);         /* of either pass */
+size_t bbhip_DenseAffine_Forward_WorkspaceBytes(int input_node_size, int output_node_size, int frame_size, int bit_input);   /* of the forward pass alone */
 int bbhip_fp32_DenseAffine_Forward(float const *dev_x_buf, float *dev_y_buf, float const *dev_W, float const *dev_b, float const *dev_residual_buf, int activation,
                                    int input_node_size, int output_node_size, int frame_size, int x_frame_stride, int y_frame_stride, int residual_frame_stride,
                                    void *dev_workspace, size_t workspace_size, void *stream);

@@ -142,8 +142,8 @@ __device__ __forceinline__ void pack_rows(PackJob const &j, int block, float *sh
 #pragma unroll
                 for (int q = 0; q < 8; ++q) {
                     t[q] = left[q] * kTailScale;
-                    // (a tail meets the other operand's upper half only: what the lower one is of a value, 2^-11, counts as lost)
-                    lost += fabsf(left[q]) * 4.8828125e-4f + fabsf(t[q] - (float)(_Float16)t[q]) * (1.0f / kTailScale);
+                    // (a tail meets the other operand's upper half only: what the lower one can be of the other's largest, 2^-12, counts as lost)
+                    lost += fabsf(left[q]) * 2.44140625e-4f + fabsf(t[q] - (float)(_Float16)t[q]) * (1.0f / kTailScale);
                 }
                 uint4 *const tail = j.tails + ((long long)(row >> 5) * j.k_steps + (o >> 1)) * 64 + (o & 1) * 32 + (row & 31);
                 *tail = make_uint4(two_halves(t[0], t[1]), two_halves(t[2], t[3]), two_halves(t[4], t[5]), two_halves(t[6], t[7]));
@@ -701,12 +701,12 @@ __device__ __forceinline__ void packed_tile(PackedProduct const &p, int id, char
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    // Of each element whether its sum has not been as large as its limit yet, bit 16 j + r; later whether it is formed again.  Looked at up to eight times on the way, and not ahead of 1024 k: with
-    // fewer a sum is seldom that small at the end.  Nor where the limits are below 2^12 (sums of scaled values are 2^27 and more): all rows of a wavefront have that in common.
+    // Of each element whether its sum has not been as large as its limit yet, bit 16 j + r; later whether it is formed again.  Looked at up to eight times on the way, every 1024 k or more: with
+    // fewer a sum is seldom that small at the end, but for gradients of a softmax, every 256.  Nor where the limits are below 2^12 (sums of scaled values are 2^27 and more): all rows of a wavefront have that in common.
     uint32_t again[TM];
 #pragma unroll
     for (int i = 0; i < TM; ++i) { again[i] = 0xffffffffu; }
-    int const look_every = max(64, (stages / 8 + 1) & ~1);
+    int const look_every = max(TAILS ? 16 : 64, (stages / 8 + 1) & ~1);
     int look = look_every;
     auto const look_at_sums = [&] {
         look += look_every;

@@ -54,29 +54,33 @@ inline void direct_shapes(int m0, int n0, int k0, int m1, int n1, int k1, Direct
 }
 
 // Whether a product goes by way of packed halves (two launches at least, and both operands are read and written once more) instead of straight from its operands: the products saved
-// against the launch and the values packed.  A forward pass, us straight and packed: 1001 x 500 x 777 inputs 22 and 27, 1001 x 1000 x 777 39 and 29, 1024 x 1024 x 1024 30 and 30,
-// 2048 x 1024 x 256 20 and 22, 4096 x 64 x 4096 35 and 52 (the weights are all there is to read), 4096 x 4096 x 64 55 and 35, 8192 x 1024 x 128 47 and 28.
+// against the launch and the values packed.  A forward pass, inputs x outputs x frames, us straight and packed: 777 x 1001 x 500 23 and 30, 777 x 1001 x 1000 41 and 32, 64 x 4096 x 4096 53 and
+// 41, 128 x 8192 x 1024 46 and 32, 4096 x 4096 x 64 32 and 60 (the weights are all there is to read).  Straight products read rows of a multiple of four weights sixteen bytes at a time, which
+// counts up to 1024 inputs: 784 x 1024 x 1024 22 and 32, 1024 x 1024 x 1024 30 and 33, 512 x 2048 x 1024 30 and 31, 784 x 1024 x 2048 40 and 35; 1536 x 1024 x 1024 38 and 37, 2048 x 1024 x 1024 47 and
+// 41 (2048 x 1024 x 512 29 and 34).
 inline bool long_enough(int a, int b, int c) { return a >= 32 && b >= 32 && c >= 32; }
 inline double volume(int a, int b, int c) { return (double)a * b * c; }
 inline bool forward_packed(int inputs, int outputs, int frames)
 {
-    return long_enough(inputs, outputs, frames) && volume(inputs, outputs, frames) >= (1 << 29) + 80.0 * inputs * ((double)outputs + frames);
+    return long_enough(inputs, outputs, frames) && volume(inputs, outputs, frames) >= ((1 << 29) + 80.0 * inputs * ((double)outputs + frames)) * (inputs % 4 == 0 && inputs <= 1024 ? 1.6 : 1.0);
 }
 
-// A backward pass, which packs dz as rows and as columns, inputs x outputs x frames: 512 x 512 x 512 18 and 26, 512 x 512 x 1024 31 and 30, 777 x 1001 x 500 44 and 35, 1024 x 1024 x 1024 82
-// and 39, 256 x 2048 x 1024 53 and 43, 96 x 4096 x 1024 48 and 65, 64 x 8192 x 1024 70 and 90, 128 x 8192 x 1024 100 and 95, 4096 x 4096 x 32 74 and 100, x 64 96 and 104.
+// A backward pass, which packs dz as rows and as columns, inputs x outputs x frames: 512 x 512 x 1024 29 and 34, 256 x 1024 x 1024 31 and 31, 777 x 1001 x 500 35 and 39, 384 x 1000 x 1000 35 and 35,
+// 784 x 512 x 1024 34 and 38, 256 x 2048 x 1024 51 and 43, 1024 x 1024 x 1024 82 and 41, 96 x 4096 x 1024 43 and 57, 64 x 8192 x 1024 58 and 94, 128 x 8192 x 1024 93 and 102, 4096 x 4096 x 32 70
+// and 95, x 64 88 and 101.
 inline bool backward_packed(int inputs, int outputs, int frames)
 {
     return long_enough(inputs, outputs, frames) &&
-           volume(inputs, outputs, frames) >= (3 << 26) + 48.0 * (2.0 * outputs * frames + (double)inputs * frames + (double)inputs * outputs);
+           volume(inputs, outputs, frames) >= 2.9e8 + 48.0 * (2.0 * outputs * frames + (double)inputs * frames + (double)inputs * outputs);
 }
 
-// A loss, with its gradients or alone (a frame's loss has the same bits either way): with gradients 512 inputs x 512 channels x 1024 frames 47 and 54, 777 x 1001 x 500 73 and 57, 784 x 512 x 1024 62 and 59, 64 x 8192 x 1024 115 and 115, 128 x 8192 x 1024 168 and
-// 121, 4096 x 64 x 1024 61 and 72, 4096 x 4096 x 32 104 and 160, x 64 138 and 166.
+// A loss, with its gradients or alone (a frame's loss has the same bits either way); packed gradients have tails.  With gradients, inputs x channels x frames: 512 x 512 x 1024 47 and 66,
+// 784 x 512 x 1024 51 and 71, 777 x 1001 x 500 60 and 70, 512 x 1000 x 1000 63 and 78, 256 x 2048 x 1024 77 and 79, 1024 x 1001 x 700 87 and 91, 777 x 1001 x 1000 105 and 86, 64 x 8192 x 1024 103
+// and 139, 128 x 8192 x 1024 156 and 151, 64 x 4096 x 4096 187 and 203, 4096 x 64 x 1024 61 and 82, 4096 x 4096 x 32 97 and 186, x 64 127 and 191.
 inline bool loss_packed(int inputs, int channels, int frames)
 {
     return long_enough(inputs, channels, frames) &&
-           volume(inputs, channels, frames) >= 2.5e8 + 25.0 * ((double)channels * frames + 4.0 * inputs * ((double)channels + frames));
+           volume(inputs, channels, frames) >= (1 << 29) + 25.0 * ((double)channels * frames + 4.0 * inputs * ((double)channels + frames));
 }
 
 // Tiles of a packed product: 256 x 256 by eight wavefronts, 256 x 128 or 128 x 128 by four (two such workgroups on a compute unit); stages that lie in LDS.  Large, middle and small tiles, us:

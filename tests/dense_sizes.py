@@ -6,7 +6,7 @@ FORWARD = {
     (300, 200, 40): "straight waves 8 slabs 1",
     (2048, 40, 70): "straight waves 8 slabs 8",
     (300, 2600, 2500): "packed small slabs 1 narrow",
-    (1100, 640, 1300): "packed small slabs 4 narrow",
+    (1103, 640, 1300): "packed small slabs 4 narrow",
     (145, 21806, 548): "packed middle slabs 1 narrow",
     (8300, 700, 1100): "packed small slabs 8 wide",          # rows longer than the packing threads hold
 }
@@ -14,8 +14,8 @@ FORWARD = {
 # (the weights' gradient and the input's; wide: frames or outputs beyond what the packing threads hold)
 BACKWARD = {
     (64, 64, 1030): "straight waves 8 slabs 3 and waves 8 slabs 1",
-    (1068, 455, 575): "packed small slabs 1 narrow and slabs 1",
-    (640, 530, 1100): "packed small slabs 4 narrow and slabs 2",
+    (992, 579, 681): "packed small slabs 1 narrow and slabs 1",
+    (700, 600, 1200): "packed small slabs 4 narrow and slabs 2",
     (4897, 1036, 1833): "packed middle slabs 1 narrow and slabs 1",
     (5000, 644, 814): "packed large slabs 1 narrow and slabs 1",
     (300, 2600, 1100): "packed large slabs 5 narrow and slabs 12",
@@ -28,7 +28,7 @@ LOSS = {
     (24, 701, 100000): "straight pieces 2 last 189",
     (64, 701, 100000): "packed pieces 2 last 189 logits large slabs 1",
     (40, 9001, 9000): "packed pieces 2 last 1577 logits large slabs 1",
-    (44, 3312, 4888): "packed pieces 1 last 3312 logits middle slabs 1",
-    (249, 1300, 1072): "packed pieces 1 last 1300 logits small slabs 1",
-    (1600, 640, 700): "packed pieces 1 last 640 logits small slabs 6",
+    (67, 3097, 4890): "packed pieces 1 last 3097 logits middle slabs 1",
+    (395, 1378, 1260): "packed pieces 1 last 1378 logits small slabs 1",
+    (2000, 700, 700): "packed pieces 1 last 700 logits small slabs 6",
 }

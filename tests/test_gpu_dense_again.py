@@ -11,7 +11,7 @@ pytestmark = pytest.mark.gpu
 
 F32 = np.float32
 # (inputs, outputs, frames): tiles of each size, whole and with a shared k axis, odd ends
-SIZES = [(300, 2600, 2500), (640, 530, 1100), (1100, 640, 1300), (145, 21806, 548)]
+SIZES = [(300, 2600, 2500), (640, 530, 1100), (1103, 640, 1300), (145, 21806, 548)]
 
 
 def differ_only_at(a, b, where):
@@ -71,7 +71,7 @@ def test_forward_to_bits_leaves_the_others_alone(size, bit):
 
 
 @pytest.mark.parametrize("bit", [False, True])
-@pytest.mark.parametrize("size", [(300, 2600, 1100), (640, 530, 1100), (1024, 1001, 1000), (2048, 4300, 1500)])
+@pytest.mark.parametrize("size", [(300, 2600, 1100), (700, 600, 1200), (1024, 1001, 1000), (2048, 4300, 1500)])
 def test_backward_leaves_the_others_alone(size, bit):
     """NaN in one gradient: its output's row of dW, db and its frame's column of dx; gradients are added to what is there"""
     from binarybrain_amd import ops
@@ -101,7 +101,7 @@ def test_backward_leaves_the_others_alone(size, bit):
 
 
 # (inputs, channels, frames): straight, packed whole and with a shared k axis for the logits
-LOSS_SIZES = [(40, 50, 60), (300, 1500, 1030), (1600, 640, 700), (64, 2500, 2000)]
+LOSS_SIZES = [(40, 50, 60), (395, 1378, 1260), (2000, 700, 700), (64, 2500, 2000)]
 
 
 @pytest.mark.parametrize("size", LOSS_SIZES)

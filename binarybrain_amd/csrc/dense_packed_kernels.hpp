@@ -20,9 +20,10 @@
 // 16, the loads of the next three stages to LDS in flight behind the products of the present one (the small tile: of the next four, and its halves one stage ahead in registers).
 // Where there are too few tiles for the device, several workgroups share a tile's k axis and a third launch adds their sums in a fixed order.
 //
-// What bounds it: the matrix instructions and the power they take.  4096 x 4096 x 8192 with packed bits is 550 GFLOP of halves in 451 to 501 us, both products of its backward pass on real
-// values 1650 in 1345 to 1500: 1.1 to 1.2 PFLOP/s, where a plain product of halves by the library reaches 1.17 to 1.26.  Five or seven stages ahead changed nothing.  Packing is
-// bound by memory and by its two phases, loads and then stores: 205 MB in 57 us, 1.34 GB in 355, 3.6 to 3.8 TB/s.  Small problems are bound by two launches of 12 us and more whose workgroups run once.
+// What bounds it: the matrix instructions and the power they take.  4096 x 4096 x 8192 with packed bits is 550 GFLOP of halves in 442 to 481 us, both products of its backward pass on real
+// values 1650 in 1320 to 1500: 1.1 to 1.2 PFLOP/s, where a plain product of halves by the library reaches 1.17 to 1.26.  Five or seven stages ahead changed nothing.  Packing is
+// bound by memory and by its two phases, loads and then stores: 207 MB in 60 us, 1.35 GB in 366, 3.5 to 3.7 TB/s.  Small problems are bound by two launches of 13 us and more whose workgroups run once.  Summing what rows lose and looking for
+// it costs a large product 1 % and a small one 2 to 3 us of 40; with the tails it is 15 us of 85 for a loss over 777 x 1001 x 1000 and 0.7 ms of 4.1 over 1024 x 32768 x 4096.
 #pragma once
 
 #include "dense_direct_kernels.hpp"

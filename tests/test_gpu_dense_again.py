@@ -157,3 +157,25 @@ def test_operands_full_of_nan_cost_no_multiple(size, bit):
     plain, odd = seconds(W), seconds(V)
     assert np.isnan(odd[1][::3]).all() and np.array_equal(odd[1][1::3], plain[1][1::3])
     assert odd[0] <= 10 * plain[0] + 3, (plain[0], odd[0])
+
+
+@pytest.mark.parametrize("size", [(1024, 4096, 4096), (1500, 1024, 1024)])
+def test_operands_that_are_all_nan_are_done_at_once(size):
+    """whole tiles, and a shared k axis: at most twice a plain call and what the launches behind it take"""
+    import torch
+    from binarybrain_amd import ops
+    inputs, outputs, frames = size
+    x, W = torch.randn((inputs, frames), device="cuda"), torch.randn((outputs, inputs), device="cuda")
+
+    def milliseconds(W):
+        best = 1e9
+        for _ in range(3):
+            a, z = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            y = ops.dense_affine_forward(x, W, None, frames)
+            z.record()
+            torch.cuda.synchronize()
+            best = min(best, a.elapsed_time(z))
+        return best, y
+    plain, odd = milliseconds(W)[0], milliseconds(torch.full_like(W, float("nan")))
+    assert bool(odd[1].isnan().all()) and odd[0] <= 2 * plain + 0.3, (plain, odd[0])

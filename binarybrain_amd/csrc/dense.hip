@@ -201,20 +201,20 @@ struct Packed {
     uint4 *halves;
     int   *exponent;
     float *lost;
-    uint4 *tails = nullptr;
-    int    blocks, steps, pieces;
+    uint4 *thirds = nullptr;
+    int    blocks, steps, pieces, triple;
     Packed() = default;
-    Packed(Carver &c, int rows, int depth, bool bits, bool with_tails = false) : blocks(ceil_div(rows, 32)), steps(pack_steps(depth)), pieces(bits ? 1 : 2)
+    Packed(Carver &c, int rows, int depth, bool bits, bool as_triple = false) : blocks(ceil_div(rows, 32)), steps(pack_steps(depth)), pieces(bits ? 1 : 2), triple(as_triple)
     {
         halves = c.take<uint4>((size_t)blocks * steps * pieces * 64);
         exponent = bits ? nullptr : c.take<int>((size_t)blocks * 32);
         lost = c.take<float>((size_t)blocks * 32);
-        if (with_tails) { tails = c.take<uint4>((size_t)blocks * steps * 64); }
+        if (as_triple && !bits) { thirds = c.take<uint4>((size_t)blocks * steps * 64); }
     }
     PackJob job(Operand const &o, int kind) const
     {
         PackJob j{};
-        j.src = o; j.kind = kind; j.halves = halves; j.exponent = exponent; j.lost = lost; j.tails = tails; j.k_steps = steps;
+        j.src = o; j.kind = kind; j.halves = halves; j.exponent = exponent; j.lost = lost; j.triple = triple; j.thirds = thirds; j.k_steps = steps;
         j.blocks = blocks * (32 / kPackRows);
         return j;
     }
@@ -246,7 +246,7 @@ int packed_product(PackedProduct &d, Product const &p, PackedShape const &s, Pac
     d = PackedProduct{};
     if (!p.wanted) { d.b_pieces = 2; return 0; }
     d.a = a.halves; d.ea = a.exponent; d.lost_a = a.lost; d.a_blocks = a.blocks;
-    d.b = b.halves; d.eb = b.exponent; d.lost_b = b.lost; d.tails = a.tails ? a.tails : b.tails; d.b_blocks = b.blocks; d.b_pieces = b.pieces;
+    d.b = b.halves; d.eb = b.exponent; d.lost_b = b.lost; d.thirds_a = a.thirds; d.thirds_b = b.thirds; d.triple = a.triple; d.b_blocks = b.blocks; d.b_pieces = b.pieces;
     d.k_steps = s.k_steps; d.m_tiles = s.m_tiles; d.n_tiles = s.n_tiles; d.slabs = s.slabs; d.slab_stages = s.slab_stages;
     if (check_tiles(s.workgroups(), kTileThreads[s.size], name)) { return 1; }
     d.workgroups = (int)s.workgroups();
@@ -285,10 +285,10 @@ int packed_run(PackedProduct const &p, PackedProduct const &q, int size, hipStre
     if (check_tiles((long long)p.workgroups + q.workgroups, kTileThreads[size], name)) { return 1; }
     if (p.workgroups + q.workgroups == 0) { return 0; }
     dim3 const grid((unsigned)(p.workgroups + q.workgroups)), block((unsigned)kTileThreads[size]);
-    bool const tails = p.tails || q.tails;
+    bool const triple = p.triple || q.triple;
 #define BBHIP_PACKED(...)                                                                               \
     do {                                                                                                \
-        if (tails) {                                                                                    \
+        if (triple) {                                                                                   \
             if (p.b_pieces == 1) { launch((dense_packed_pair_kernel<true, __VA_ARGS__, 1, kTileBuffers[size_]>), grid, block, 0, st, p, q); } \
             else                 { launch((dense_packed_pair_kernel<true, __VA_ARGS__, 2, kTileBuffers[size_]>), grid, block, 0, st, p, q); } \
         }                                                                                               \
@@ -319,13 +319,13 @@ struct BackwardSpace {
     PackedShape dw, dx;
     Packed dz_rows, x, W, dz_columns;
     float *dw_sums, *dx_sums;
-    BackwardSpace(Carver &c, int inputs, int outputs, int frames, bool bit, bool tails)
+    BackwardSpace(Carver &c, int inputs, int outputs, int frames, bool bit, bool triple)
     {
         best_shapes(outputs, inputs, frames, inputs, frames, outputs, dw, dx);
-        dz_rows = Packed(c, outputs, frames, false, tails);
-        x = Packed(c, inputs, frames, bit);
-        W = Packed(c, inputs, outputs, false);
-        dz_columns = Packed(c, frames, outputs, false, tails);
+        dz_rows = Packed(c, outputs, frames, false, triple);
+        x = Packed(c, inputs, frames, bit, triple);
+        W = Packed(c, inputs, outputs, false, triple);
+        dz_columns = Packed(c, frames, outputs, false, triple);
         dw_sums = sums_of(c, dw.slabs, outputs, inputs);
         dx_sums = sums_of(c, dx.slabs, inputs, frames);
     }

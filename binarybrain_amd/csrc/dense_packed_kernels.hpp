@@ -10,9 +10,12 @@
 // the sum of what its halves leave of such values, and an element of the product whose sum never got 2^20 times as large as its row and its column can have changed it
 //     |sum| < 2^20 * (lost of the row * largest of the column + largest of the row * lost of the column)
 // is formed again in fp32 straight from the operands, as one that is no number is (an infinity times a lower half of 0).  What fp32 sums of that length round away is as much.  Sums are looked
-// at on the way too (a number that has been large has lost as much in fp32, however small it ends): ordinary operands have next to none of these elements.  The gradients of a softmax do, with
-// magnitudes spread over more than 2^18: over 32768 channels a twentieth of dx.  So the first launch leaves these operands' tails too, what the halves leave of small values, 2^39 times as large, as halves
-// once more, and tails times the other operand's upper halves are added ahead of everything else: what is lost is 2^11 times less then, for a third more work in these two products.
+// at on the way too (a number that has been large has lost as much in fp32, however small it ends): ordinary operands have next to none of these elements.
+//
+// The gradients of a softmax do have them, with magnitudes spread over more than 2^100: a twentieth of dx over 32768 channels as training begins, most of all elements as it ends (1024 inputs x 1024
+// channels x 4096 frames then took 1.7 to 2.2 ms).  So the products of a loss's gradients take their operands as three pieces of bf16, 24 bits in the
+// range of fp32: six products instead of three (three instead of two over packed bits), the smallest first, whatever the values are. The thirds lie apart from the first two pieces and are walked
+// ahead of these.  A layer's backward pass keeps halves even where its gradient is a softmax's: 1024 x 1024 x 4096 takes 93 us then, 149 with confident logits, and as triples 139 for any gradient.
 //
 // Two launches.  The first reads each operand as it lies and leaves its halves in the order in which the matrix instructions want them: blocks of 32 rows x 16 k,
 // 1 KiB each, lane l's sixteen bytes (row l & 31, k 8 (l >> 5) .. + 8) at 16 l, so that the second launch moves them to LDS and from there to registers with 16-byte accesses
@@ -23,8 +26,10 @@
 // What bounds it: the matrix instructions and the power they take.  4096 x 4096 x 8192 with packed bits is 550 GFLOP of halves in 442 to 481 us, both products of its backward pass on real
 // values 1650 in 1320 to 1500: 1.1 to 1.2 PFLOP/s, where a plain product of halves by the library reaches 1.17 to 1.26.  Five or seven stages ahead changed nothing.  Packing is
 // bound by memory and by its two phases, loads and then stores: 207 MB in 60 us, 1.35 GB in 366, 3.5 to 3.7 TB/s.  Small problems are bound by two launches of 13 us and more whose workgroups run once.  Summing what rows lose and looking for
-// it costs a large product 1 % and a small one 2 to 3 us of 40; with the tails it is 15 us of 85 for a loss over 777 x 1001 x 1000 and 0.7 ms of 4.1 over 1024 x 32768 x 4096.
+// it costs a large product 1 % and a small one 2 to 3 us of 40; with its triples a loss over 777 x 1001 x 1000 takes 94 us (70 with halves that lose), over 1024 x 32768 x 4096 4.74 ms (3.39).
 #pragma once
+
+#include <type_traits>
 
 #include "dense_direct_kernels.hpp"
 #include "dense_rules.hpp"
@@ -46,10 +51,13 @@ struct PackJob {
     int    accumulate;
     float *dz;                  // gradients as rows: themselves (null: not wanted), rows of dz_stride
     long long dz_stride;
-    uint4 *tails;               // gradients: what the halves leave of small values, 2^39 times as large, in halves once more: [row blocks][k steps][64 lanes] (null: not wanted)
+    int    triple;              // three pieces of bf16 instead of halves
+    uint4 *thirds;              // the last of them: [row blocks][k steps][64 lanes]; the others lie where halves do
 };
 
-constexpr float kTailScale = 549755813888.0f;           // 2^39: what is left of a value, 2^-25 at most, becomes 2^14
+// Triples: the largest of a row is brought to 2^40, so that a value 2^-140 as large still has all its pieces (2^-100, and 2^-126 is the least of a third).
+constexpr int   kTripleTop = 40;
+constexpr float kTripleLeast = 7.88860905e-31f;         // 2^-100
 
 constexpr int kPackJobs = 4;
 struct PackArgs { PackJob job[kPackJobs]; };
@@ -59,6 +67,14 @@ __device__ __forceinline__ uint32_t two_halves(float a, float b)
     typedef _Float16 Half2 __attribute__((ext_vector_type(2)));
     Half2 const h = {(_Float16)a, (_Float16)b};
     return __builtin_bit_cast(uint32_t, h);
+}
+
+__device__ __forceinline__ float to_bf16(float v) { return (float)(__bf16)v; }
+__device__ __forceinline__ uint32_t two_bf16(float a, float b)
+{
+    typedef __bf16 Two __attribute__((ext_vector_type(2)));
+    Two const t = {(__bf16)a, (__bf16)b};
+    return __builtin_bit_cast(uint32_t, t);
 }
 
 // workgroup -> place in the list of tiles: workgroups go round the eight XCDs, each of which gets a run of neighbours
@@ -115,8 +131,8 @@ __device__ __forceinline__ void pack_rows(PackJob const &j, int block, float *sh
         top = 0.0f; sum = 0.0f;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) { top = fmaxf(top, share[w * ROWS + at]); sum += share[(kWaves + w) * ROWS + at]; }
-        e = top > 0.0f ? 15 - ilogbf(top) : 0;
-        if (ldexpf(top, e) >= 65520.0f) { --e; }            // (which halves would round to infinity)
+        e = top > 0.0f ? (j.triple ? kTripleTop : 15) - ilogbf(top) : 0;
+        if (!j.triple && ldexpf(top, e) >= 65520.0f) { --e; }           // (which halves would round to infinity)
         if (threadIdx.x < ROWS) {
             j.exponent[row] = e;
             if constexpr (KIND == kGradRows) { if (j.line && there) { j.line[row] = j.accumulate ? j.line[row] + sum : sum; } }
@@ -125,10 +141,28 @@ __device__ __forceinline__ void pack_rows(PackJob const &j, int block, float *sh
     auto const write = [&](int o, float const (&v)[8]) {
         uint4 *to = j.halves + (((long long)(row >> 5) * j.k_steps + (o >> 1)) * kPieces) * 64 + (o & 1) * 32 + (row & 31);
         if constexpr (kBits) {
-            to[0] = make_uint4(two_halves(v[0], v[1]), two_halves(v[2], v[3]), two_halves(v[4], v[5]), two_halves(v[6], v[7]));
+            if (j.triple) { to[0] = make_uint4(two_bf16(v[0], v[1]), two_bf16(v[2], v[3]), two_bf16(v[4], v[5]), two_bf16(v[6], v[7])); }
+            else          { to[0] = make_uint4(two_halves(v[0], v[1]), two_halves(v[2], v[3]), two_halves(v[4], v[5]), two_halves(v[6], v[7])); }
+        }
+        else if (j.triple) {
+            float h[8], m[8], l[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                float const a = ldexpf(v[q], e);
+                h[q] = to_bf16(a);
+                float const rest = fabsf(h[q]) < INFINITY ? a - h[q] : 0.0f;
+                m[q] = to_bf16(rest);
+                l[q] = rest - m[q];
+                // (whose pieces might leave the range of bf16)
+                lost += fabsf(a) < kTripleLeast ? fabsf(a) : 0.0f;
+            }
+            to[0]  = make_uint4(two_bf16(h[0], h[1]), two_bf16(h[2], h[3]), two_bf16(h[4], h[5]), two_bf16(h[6], h[7]));
+            to[64] = make_uint4(two_bf16(m[0], m[1]), two_bf16(m[2], m[3]), two_bf16(m[4], m[5]), two_bf16(m[6], m[7]));
+            j.thirds[((long long)(row >> 5) * j.k_steps + (o >> 1)) * 64 + (o & 1) * 32 + (row & 31)] =
+                make_uint4(two_bf16(l[0], l[1]), two_bf16(l[2], l[3]), two_bf16(l[4], l[5]), two_bf16(l[6], l[7]));
         }
         else {
-            float h[8], l[8], left[8];
+            float h[8], l[8];
 #pragma unroll
             for (int q = 0; q < 8; ++q) {
                 h[q] = ldexpf(v[q], e);
@@ -136,22 +170,7 @@ __device__ __forceinline__ void pack_rows(PackJob const &j, int block, float *sh
                 // (the difference of an infinity to itself is no number, its lower half 0)
                 l[q] = fabsf(upper) < INFINITY ? h[q] - upper : 0.0f;
                 // (below 1/8 the lower half's steps, 2^-24, are more than 2^-21 of the value)
-                left[q] = fabsf(h[q]) < 0.125f ? l[q] - (float)(_Float16)l[q] : 0.0f;
-            }
-            if ((KIND == kGradRows || KIND == kGradColumns) && j.tails) {
-                float t[8];
-#pragma unroll
-                for (int q = 0; q < 8; ++q) {
-                    t[q] = left[q] * kTailScale;
-                    // (a tail meets the other operand's upper half only: what the lower one can be of the other's largest, 2^-12, counts as lost)
-                    lost += fabsf(left[q]) * 2.44140625e-4f + fabsf(t[q] - (float)(_Float16)t[q]) * (1.0f / kTailScale);
-                }
-                uint4 *const tail = j.tails + ((long long)(row >> 5) * j.k_steps + (o >> 1)) * 64 + (o & 1) * 32 + (row & 31);
-                *tail = make_uint4(two_halves(t[0], t[1]), two_halves(t[2], t[3]), two_halves(t[4], t[5]), two_halves(t[6], t[7]));
-            }
-            else {
-#pragma unroll
-                for (int q = 0; q < 8; ++q) { lost += fabsf(left[q]); }
+                lost += fabsf(h[q]) < 0.125f ? fabsf(l[q] - (float)(_Float16)l[q]) : 0.0f;
             }
             to[0]  = make_uint4(two_halves(h[0], h[1]), two_halves(h[2], h[3]), two_halves(h[4], h[5]), two_halves(h[6], h[7]));
             to[64] = make_uint4(two_halves(l[0], l[1]), two_halves(l[2], l[3]), two_halves(l[4], l[5]), two_halves(l[6], l[7]));
@@ -231,7 +250,8 @@ struct PackedProduct {
     uint4 const *a, *b;             // halves
     int   const *ea, *eb;           // exponents of the rows (eb null: 0)
     float const *lost_a, *lost_b;   // what the rows lost
-    uint4 const *tails;             // of a or of b (null: neither)
+    uint4 const *thirds_a, *thirds_b;           // triples: their last pieces (packed bits: null)
+    int   triple;
     int   a_blocks, b_blocks;       // row blocks of 32
     int   k_steps;
     int   b_pieces;
@@ -260,10 +280,10 @@ __device__ __forceinline__ float plain_nan(float v) { return v == v ? v : __buil
 // The halves of an infinity times a lower half of 0 are no number where the value's product is infinite, and halves lose small values beside large ones: such elements are formed again in fp32
 // straight from the operands, so that they are what the formula says; their neighbours keep the bits that they have.
 
-// An element stands where its scaled sum got as large as the limits of its row and its column together: what they lost, times the other's largest (below 2^16; bits: 1), times 2^20.  (Where
+// An element stands where its scaled sum got as large as the limits of its row and its column together: what they lost, times the other's largest (below 2^16, of triples 2^41; bits: 1), times 2^20.  (Where
 // either has no value but 0 nothing is lost: minus infinity.)
-template <int PB>
-__device__ __forceinline__ float limit_of(float lost) { return lost * (PB == 2 ? 68719476736.0f : 1048576.0f); }
+template <int PB, bool TRIPLE>
+__device__ __forceinline__ float limit_of(float lost) { return lost * (PB == 1 ? 1048576.0f : TRIPLE ? 2305843009213693952.0f : 68719476736.0f); }
 
 // By a wavefront: its lanes take the k in turn, N at a time, whose loads overlap.
 template <int KA, int KB, int N>
@@ -565,8 +585,15 @@ __device__ __forceinline__ void arrived(void)
     asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" :: "n"(N) : "memory");
 }
 
-// TAILS: 1 a has tails, 2 b has, 0 neither
-template <int USE, int KA, int KB, int TAILS, int TM, int WM, int WN, int PB, int BUFFERS>
+template <bool TRIPLE>
+__device__ __forceinline__ DenseAcc16 product_of(DenseHalf8 a, DenseHalf8 b, DenseAcc16 c)
+{
+    typedef __bf16 Bf8 __attribute__((ext_vector_type(8)));
+    if constexpr (TRIPLE) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(Bf8, a), __builtin_bit_cast(Bf8, b), c, 0, 0, 0); }
+    else                  { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+}
+
+template <int USE, int KA, int KB, bool TRIPLE, int TM, int WM, int WN, int PB, int BUFFERS>
 __device__ __forceinline__ void packed_tile(PackedProduct const &p, int id, char *lds, int *scales, float *limits, float *bias)
 {
     constexpr int TN = 2, kWaves = WM * WN, kBM = TM * WM, kBN = TN * WN;           // blocks of 32 rows
@@ -612,71 +639,71 @@ __device__ __forceinline__ void packed_tile(PackedProduct const &p, int id, char
     float const *const limit_a = limits, *const limit_b = limits + kBM * 32;
     for (int i = threadIdx.x; i < kBM * 32; i += kWaves * 64) {
         scales[i] = p.ea[min(rb_a * 32 + i, p.a_blocks * 32 - 1)];
-        limits[i] = limit_of<PB>(p.lost_a[min(rb_a * 32 + i, p.a_blocks * 32 - 1)]);
+        limits[i] = limit_of<PB, TRIPLE>(p.lost_a[min(rb_a * 32 + i, p.a_blocks * 32 - 1)]);
         if (USE != kUseStore) { bias[i] = o.bias && rb_a * 32 + i < o.rows ? o.bias[rb_a * 32 + i] : 0.0f; }
     }
     for (int i = threadIdx.x; i < kBN * 32; i += kWaves * 64) {
         scales[kBM * 32 + i] = PB == 2 ? p.eb[min(rb_b * 32 + i, p.b_blocks * 32 - 1)] : 0;
-        limits[kBM * 32 + i] = limit_of<PB>(p.lost_b[min(rb_b * 32 + i, p.b_blocks * 32 - 1)]);
+        limits[kBM * 32 + i] = limit_of<PB, TRIPLE>(p.lost_b[min(rb_b * 32 + i, p.b_blocks * 32 - 1)]);
     }
 
     int const wm = wave / WN, wn = wave % WN;
     DenseAcc16 acc[TM][TN] = {};
-    if constexpr (TAILS != 0) {
-        // One operand's tails times the other's upper halves ahead of everything else, two steps of k at a time, and the sums brought to scale.
-        constexpr int kTailStage = (kBM + kBN) * 2048, kTailLoads = 2 * kOwn + 2;
-        constexpr long long kStepA = TAILS == 1 ? 1024 : 2048, kStepB = TAILS == 2 ? 1024 : 1024 * PB;          // bytes from step to step
-        char const *tail_a[kOwn];
+    if constexpr (TRIPLE) {
+        // Thirds of one operand times firsts of the other ahead of everything else, two steps of k at a time.
+        auto const thirds = [&](auto of_a) {
+            constexpr bool kOfA = decltype(of_a)::value;
+            constexpr int kThirdStage = (kBM + kBN) * 2048, kThirdLoads = 2 * kOwn + 2;
+            constexpr long long kStepA = kOfA ? 1024 : 2048, kStepB = kOfA ? 1024 * PB : 1024;          // bytes from step to step
+            char const *third_a[kOwn];
 #pragma unroll
-        for (int i = 0; i < kOwn; ++i) {
-            tail_a[i] = reinterpret_cast<char const *>(TAILS == 1 ? p.tails : p.a) + ((long long)min(rb_a + wave * kOwn + i, p.a_blocks - 1) * p.k_steps + first) * kStepA + lane * 16;
-        }
-        char const *tail_b = reinterpret_cast<char const *>(TAILS == 2 ? p.tails : p.b) + ((long long)min(rb_b + wave, p.b_blocks - 1) * p.k_steps + first) * kStepB + lane * 16;
-        auto const fetch_tails = [&](int buffer, int s) {
-            bool const both = 2 * s + 1 < stages;           // (else the first step once more, which is not used)
-            auto const two = [&](uint32_t to, char const *from, long long step) {
-                asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(to), "v"(from) : "memory", "m0");
-                asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(to + 1024), "v"(from + (both ? step : 0)) : "memory", "m0");
+            for (int i = 0; i < kOwn; ++i) {
+                third_a[i] = reinterpret_cast<char const *>(kOfA ? p.thirds_a : p.a) + ((long long)min(rb_a + wave * kOwn + i, p.a_blocks - 1) * p.k_steps + first) * kStepA + lane * 16;
+            }
+            char const *third_b = reinterpret_cast<char const *>(kOfA ? p.b : p.thirds_b) + ((long long)min(rb_b + wave, p.b_blocks - 1) * p.k_steps + first) * kStepB + lane * 16;
+            auto const fetch_two = [&](int buffer, int s) {
+                bool const both = 2 * s + 1 < stages;           // (else the first step once more, which is not used)
+                auto const two = [&](uint32_t to, char const *from, long long step) {
+                    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(to), "v"(from) : "memory", "m0");
+                    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(to + 1024), "v"(from + (both ? step : 0)) : "memory", "m0");
+                };
+#pragma unroll
+                for (int i = 0; i < kOwn; ++i) { two(at_lds + buffer * kThirdStage + (wave * kOwn + i) * 2048, third_a[i], kStepA); third_a[i] += 2 * kStepA; }
+                two(at_lds + buffer * kThirdStage + (kBM + wave) * 2048, third_b, kStepB);
+                third_b += 2 * kStepB;
             };
-#pragma unroll
-            for (int i = 0; i < kOwn; ++i) { two(at_lds + buffer * kTailStage + (wave * kOwn + i) * 2048, tail_a[i], kStepA); tail_a[i] += 2 * kStepA; }
-            two(at_lds + buffer * kTailStage + (kBM + wave) * 2048, tail_b, kStepB);
-            tail_b += 2 * kStepB;
-        };
-        int const pairs = (stages + 1) / 2;
-        for (int s = 0; s < min(kAhead, pairs); ++s) { fetch_tails(s, s); }
-        int buffer = 0, free = kAhead;
+            int const pairs = (stages + 1) / 2;
+            for (int s = 0; s < min(kAhead, pairs); ++s) { fetch_two(s, s); }
+            int buffer = 0, free = kAhead;
 #pragma nounroll
-        for (int s = 0; s < pairs; ++s) {
-            if (s + kAhead < pairs) { arrived<(kAhead - 1) * kTailLoads>(); fetch_tails(free, s + kAhead); }
-            else                    { arrived<0>(); }
-            char const *const from = lds + buffer * kTailStage + lane * 16;
-            DenseHalf8 u[TM][2], v[TN][2];
+            for (int s = 0; s < pairs; ++s) {
+                if (s + kAhead < pairs) { arrived<(kAhead - 1) * kThirdLoads>(); fetch_two(free, s + kAhead); }
+                else                    { arrived<0>(); }
+                char const *const from = lds + buffer * kThirdStage + lane * 16;
+                DenseHalf8 u[TM][2], v[TN][2];
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
+                for (int q = 0; q < 2; ++q) {
 #pragma unroll
-                for (int j = 0; j < TN; ++j) { v[j][q] = *reinterpret_cast<DenseHalf8 const *>(from + (kBM + wn * TN + j) * 2048 + q * 1024); }
+                    for (int j = 0; j < TN; ++j) { v[j][q] = *reinterpret_cast<DenseHalf8 const *>(from + (kBM + wn * TN + j) * 2048 + q * 1024); }
 #pragma unroll
-                for (int i = 0; i < TM; ++i) { u[i][q] = *reinterpret_cast<DenseHalf8 const *>(from + (wm * TM + i) * 2048 + q * 1024); }
-            }
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                if (q == 1 && 2 * s + 1 >= stages) { break; }
-#pragma unroll
-                for (int i = 0; i < TM; ++i) {
-#pragma unroll
-                    for (int j = 0; j < TN; ++j) { acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(u[i][q], v[j][q], acc[i][j], 0, 0, 0); }
+                    for (int i = 0; i < TM; ++i) { u[i][q] = *reinterpret_cast<DenseHalf8 const *>(from + (wm * TM + i) * 2048 + q * 1024); }
                 }
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    if (q == 1 && 2 * s + 1 >= stages) { break; }
+#pragma unroll
+                    for (int i = 0; i < TM; ++i) {
+#pragma unroll
+                        for (int j = 0; j < TN; ++j) { acc[i][j] = product_of<true>(u[i][q], v[j][q], acc[i][j]); }
+                    }
+                }
+                free = buffer;
+                buffer = buffer + 1 == BUFFERS ? 0 : buffer + 1;
             }
-            free = buffer;
-            buffer = buffer + 1 == BUFFERS ? 0 : buffer + 1;
-        }
-        __syncthreads();                        // (nobody reads LDS any more, where the first stages go)
-#pragma unroll
-        for (int i = 0; i < TM; ++i) {
-#pragma unroll
-            for (int j = 0; j < TN; ++j) { acc[i][j] *= 1.0f / kTailScale; }
-        }
+            __syncthreads();                    // (nobody reads LDS any more, where the next loads go)
+        };
+        thirds(std::true_type{});
+        if constexpr (PB == 2) { thirds(std::false_type{}); }
     }
     struct Halves { DenseHalf8 a[TM][2], b[TN][PB]; };
     auto const read = [&](int buffer, Halves &h) {
@@ -697,23 +724,27 @@ __device__ __forceinline__ void packed_tile(PackedProduct const &p, int id, char
     auto const multiply = [&](Halves const &h) {
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
+            if constexpr (TRIPLE && PB == 2) {
 #pragma unroll
-            for (int j = 0; j < TN; ++j) { acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(h.a[i][1], h.b[j][0], acc[i][j], 0, 0, 0); }
-            if constexpr (PB == 2) {
-#pragma unroll
-                for (int j = 0; j < TN; ++j) { acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(h.a[i][0], h.b[j][1], acc[i][j], 0, 0, 0); }
+                for (int j = 0; j < TN; ++j) { acc[i][j] = product_of<TRIPLE>(h.a[i][1], h.b[j][1], acc[i][j]); }
             }
 #pragma unroll
-            for (int j = 0; j < TN; ++j) { acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(h.a[i][0], h.b[j][0], acc[i][j], 0, 0, 0); }
+            for (int j = 0; j < TN; ++j) { acc[i][j] = product_of<TRIPLE>(h.a[i][1], h.b[j][0], acc[i][j]); }
+            if constexpr (PB == 2) {
+#pragma unroll
+                for (int j = 0; j < TN; ++j) { acc[i][j] = product_of<TRIPLE>(h.a[i][0], h.b[j][1], acc[i][j]); }
+            }
+#pragma unroll
+            for (int j = 0; j < TN; ++j) { acc[i][j] = product_of<TRIPLE>(h.a[i][0], h.b[j][0], acc[i][j]); }
             __builtin_amdgcn_sched_barrier(0);
         }
     };
     // Of each element whether its sum has not been as large as its limit yet, bit 16 j + r; later whether it is formed again.  Looked at up to eight times on the way, every 1024 k or more: with
-    // fewer a sum is seldom that small at the end, but for gradients of a softmax, every 256.  Nor where the limits are below 2^12 (sums of scaled values are 2^27 and more): all rows of a wavefront have that in common.
+    // fewer a sum is seldom that small at the end.  Nor where the limits are below 2^12 (sums of scaled values are 2^27 and more): all rows of a wavefront have that in common.
     uint32_t again[TM];
 #pragma unroll
     for (int i = 0; i < TM; ++i) { again[i] = 0xffffffffu; }
-    int const look_every = max(TAILS ? 16 : 64, (stages / 8 + 1) & ~1);
+    int const look_every = max(64, (stages / 8 + 1) & ~1);
     int look = look_every;
     auto const look_at_sums = [&] {
         look += look_every;
@@ -914,18 +945,18 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void dense_packed_kernel(PackedPro
     __shared__ int scales[(TM * WM + 2 * WN) * 32];
     __shared__ float limits[(TM * WM + 2 * WN) * 32];
     __shared__ float bias[TM * WM * 32];
-    packed_tile<USE, kRows, PB == 1 ? kBitColumns : kColumns, 0, TM, WM, WN, PB, BUFFERS>(p, blockIdx.x, lds, scales, limits, bias);
+    packed_tile<USE, kRows, PB == 1 ? kBitColumns : kColumns, false, TM, WM, WN, PB, BUFFERS>(p, blockIdx.x, lds, scales, limits, bias);
 }
 
 // the weights' gradient, and behind it the input's (either may have no workgroups)
-template <bool TAILS, int TM, int WM, int WN, int PB, int BUFFERS>
+template <bool TRIPLE, int TM, int WM, int WN, int PB, int BUFFERS>
 __global__ __launch_bounds__(WM * WN * 64, 2) void dense_packed_pair_kernel(PackedProduct p, PackedProduct q)
 {
     __shared__ __attribute__((aligned(1024))) char lds[packed_lds<TM, WM, WN, BUFFERS>()];
     __shared__ int scales[(TM * WM + 2 * WN) * 32];
     __shared__ float limits[(TM * WM + 2 * WN) * 32];
-    if ((int)blockIdx.x < p.workgroups) { packed_tile<kUseStore, kGradRows, PB == 1 ? kBitRows : kRows, TAILS ? 1 : 0, TM, WM, WN, PB, BUFFERS>(p, blockIdx.x, lds, scales, limits, nullptr); }
-    else                                { packed_tile<kUseStore, kColumns, kGradColumns, TAILS ? 2 : 0, TM, WM, WN, 2, BUFFERS>(q, blockIdx.x - p.workgroups, lds, scales, limits, nullptr); }
+    if ((int)blockIdx.x < p.workgroups) { packed_tile<kUseStore, kGradRows, PB == 1 ? kBitRows : kRows, TRIPLE, TM, WM, WN, PB, BUFFERS>(p, blockIdx.x, lds, scales, limits, nullptr); }
+    else                                { packed_tile<kUseStore, kColumns, kGradColumns, TRIPLE, TM, WM, WN, 2, BUFFERS>(q, blockIdx.x - p.workgroups, lds, scales, limits, nullptr); }
 }
 
 // `top`: the largest magnitude of the sums
@@ -947,7 +978,8 @@ __device__ __forceinline__ float sum_of_slabs(PackedProduct const &p, int m, int
 // as the tiles have it, with the scales off
 __device__ __forceinline__ float limit_at(PackedProduct const &p, int m, int n)
 {
-    return p.b_pieces == 2 ? ldexpf(limit_of<2>(p.lost_a[m] + p.lost_b[n]), -(p.ea[m] + p.eb[n])) : ldexpf(limit_of<1>(p.lost_a[m] + p.lost_b[n]), -p.ea[m]);
+    float const lost = p.lost_a[m] + p.lost_b[n];
+    return p.b_pieces == 2 ? ldexpf(p.triple ? limit_of<2, true>(lost) : limit_of<2, false>(lost), -(p.ea[m] + p.eb[n])) : ldexpf(limit_of<1, false>(lost), -p.ea[m]);
 }
 
 // The slabs' sums of a product, in order, and what becomes of them: a wavefront takes 64 neighbours of a row.

@@ -74,7 +74,7 @@ inline bool backward_packed(int inputs, int outputs, int frames)
            volume(inputs, outputs, frames) >= 2.9e8 + 48.0 * (2.0 * outputs * frames + (double)inputs * frames + (double)inputs * outputs);
 }
 
-// A loss, with its gradients or alone (a frame's loss has the same bits either way); packed gradients have tails.  With gradients, inputs x channels x frames: 512 x 512 x 1024 47 and 66,
+// A loss, with its gradients or alone (a frame's loss has the same bits either way); packed gradients are triples.  With gradients, inputs x channels x frames: 512 x 512 x 1024 47 and 66,
 // 784 x 512 x 1024 51 and 71, 777 x 1001 x 500 60 and 70, 512 x 1000 x 1000 63 and 78, 256 x 2048 x 1024 77 and 79, 1024 x 1001 x 700 87 and 91, 777 x 1001 x 1000 105 and 86, 64 x 8192 x 1024 103
 // and 139, 128 x 8192 x 1024 156 and 151, 64 x 4096 x 4096 187 and 203, 4096 x 64 x 1024 61 and 82, 4096 x 4096 x 32 97 and 186, x 64 127 and 191.
 inline bool loss_packed(int inputs, int channels, int frames)

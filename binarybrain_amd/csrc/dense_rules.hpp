@@ -74,13 +74,14 @@ inline bool backward_packed(int inputs, int outputs, int frames)
            volume(inputs, outputs, frames) >= 2.9e8 + 48.0 * (2.0 * outputs * frames + (double)inputs * frames + (double)inputs * outputs);
 }
 
-// A loss, with its gradients or alone (a frame's loss has the same bits either way); packed gradients are triples.  With gradients, inputs x channels x frames: 512 x 512 x 1024 47 and 66,
-// 784 x 512 x 1024 51 and 71, 777 x 1001 x 500 60 and 70, 512 x 1000 x 1000 63 and 78, 256 x 2048 x 1024 77 and 79, 1024 x 1001 x 700 87 and 91, 777 x 1001 x 1000 105 and 86, 64 x 8192 x 1024 103
-// and 139, 128 x 8192 x 1024 156 and 151, 64 x 4096 x 4096 187 and 203, 4096 x 64 x 1024 61 and 82, 4096 x 4096 x 32 97 and 186, x 64 127 and 191.
+// A loss, with its gradients or alone (a frame's loss has the same bits either way); packed gradients are triples.  With gradients, inputs x channels x frames, straight and
+// packed: 256 x 2048 x 1024 77 us and 82, 1024 x 1001 x 700 87 and 99, 777 x 1001 x 1000 107 and 94, 1024 x 1024 x 1024 118 and 106, 512 x 2048 x 1024 111 and 99, 128 x 8192 x 1024 156 and 157,
+// 128 x 2048 x 4096 159 and 128, 64 x 4096 x 4096 187 and 220, 64 x 8192 x 2048 176 and 243, 4096 x 256 x 1024 127 and 109, 4096 x 4096 x 64 127 and 213, x 128 225 and 243, 784 x 1000 x 2048 164
+// and 122; over packed bits 1024 x 1024 x 1024 89 and 97, 784 x 1000 x 2048 128 and 114; the loss alone 777 x 1001 x 1000 44 and 33, 1024 x 1024 x 1024 34 and 40.
 inline bool loss_packed(int inputs, int channels, int frames)
 {
     return long_enough(inputs, channels, frames) &&
-           volume(inputs, channels, frames) >= (1 << 29) + 25.0 * ((double)channels * frames + 4.0 * inputs * ((double)channels + frames));
+           volume(inputs, channels, frames) >= (1 << 29) + 50.0 * channels * frames + 100.0 * inputs * ((double)channels + frames);
 }
 
 // Tiles of a packed product: 256 x 256 by eight wavefronts, 256 x 128 or 128 x 128 by four (two such workgroups on a compute unit); stages that lie in LDS.  Large, middle and small tiles, us:

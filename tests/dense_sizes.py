@@ -26,9 +26,9 @@ BACKWARD = {
 # (more than 64 Mi logits: pieces, the last one shorter and no multiple of 32)
 LOSS = {
     (24, 701, 100000): "straight pieces 2 last 189",
-    (64, 701, 100000): "packed pieces 2 last 189 logits large slabs 1",
-    (40, 9001, 9000): "packed pieces 2 last 1577 logits large slabs 1",
-    (67, 3097, 4890): "packed pieces 1 last 3097 logits middle slabs 1",
-    (395, 1378, 1260): "packed pieces 1 last 1378 logits small slabs 1",
+    (128, 701, 100000): "packed pieces 2 last 189 logits large slabs 1",
+    (80, 9001, 9000): "packed pieces 2 last 1577 logits large slabs 1",
+    (131, 3097, 4890): "packed pieces 1 last 3097 logits middle slabs 1",
+    (470, 1378, 1260): "packed pieces 1 last 1378 logits small slabs 1",
     (2000, 700, 700): "packed pieces 1 last 700 logits small slabs 6",
 }
